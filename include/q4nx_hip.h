@@ -298,6 +298,118 @@ int q4nx_gqa_decode_records(const uint16_t *q, const uint16_t *k_cache,
                             void *ws, size_t ws_bytes, const q4nx_policy *policy,
                             void *stream);
 
+/* ---------------------------------------------------------------- paged 4-bit K/V cache
+ * K and V of one layer in pages of 4-bit codes, 10 D bytes per 8 positions and kv head instead of
+ * 32 D (bf16). No reference counterpart: its cache is one dense bf16 buffer per sequence
+ * (designs/granite_gemv/granite_attention.h:28-34).
+ * A row's channels are quantised in groups of 32: m = the least value, d = bf16((max - m) / 15),
+ * code = rint((x - m) / d) held to 0..15 (every step rounded to fp32, to nearest even; 0 where
+ * d = 0); it stands for d * code + m. A group that holds a NaN or an infinity, or whose range
+ * overflows, stands for NaN in all 32 channels.
+ * A page holds page_len positions: per kv head page_len/32 tiles of 40 D bytes, then bf16 lo[D],
+ * hi[D], each channel's least and greatest K since the page's first position was written (NaN for a
+ * group that had a NaN). A tile: K codes, V codes (16 D bytes each), then bf16 (d, m) of the 32
+ * positions x D/32 groups for K, then for V. Codes lie as the matrix cores take them, D/64 x 64
+ * lanes x 4 dwords; lane 16 kg + n, chunk c:
+ *   K dword 2 tt + g: position 16 tt + n, channels 64 c + 32 g + 8 kg + i, nibbles from the lowest
+ *     i = 0, 2, 4, 6, 1, 3, 5, 7
+ *   V dword t: channel 64 c + 16 t + n, nibbles from the lowest positions 4 kg + 0..3 and
+ *     16 + 4 kg + 0..3
+ * A sequence's pages are a row of the table (logical page p holds positions p * page_len ..). An
+ * entry outside [0, n_pages) names no page: writes to it are dropped, reads of its positions give
+ * NaN. Positions at or past table_len * page_len are not in the cache. */
+typedef struct q4nx_kv4 {
+  uint8_t *pages;       /* page 0, 16-byte aligned                                          */
+  int64_t page_stride;  /* bytes from page to page, a multiple of 16, >= q4nx_kv4_page_bytes */
+  int32_t *table;       /* [n_seqs][table_stride]                                           */
+  int64_t table_stride;
+  int n_pages;
+  int page_len;         /* 32, 64 or 128                                                    */
+  int n_kv_heads;       /* 1..1024                                                          */
+  int head_dim;         /* 64 or 128                                                        */
+  int n_seqs;           /* 1..8192                                                          */
+  int table_len;        /* entries of a row in use                                          */
+} q4nx_kv4;
+/* Bytes of a page; 0 for an invalid shape. */
+size_t q4nx_kv4_page_bytes(int page_len, int n_kv_heads, int head_dim);
+
+/* Quantises new rows of K and V into positions pos[b], pos[b] + 1, .. of every sequence b < n_seqs.
+ * cu (NULL: one row per sequence): int32 [n_seqs + 1], sequence b's rows are cu[b] .. cu[b+1] - 1;
+ * max_new: at least the most rows of one sequence (rows past it may stay unwritten).
+ * The row of position p = pos[b] + i is at k + h * head_stride +
+ *   by_position == 0: (cu[b] + i) * row_stride                (new rows, packed)
+ *   by_position == 1: b * seq_stride + p * row_stride         (a cache as q4nx_qkv_rope writes it)
+ * (elements, multiples of 8; k and v 16-byte aligned; v alike). Rows with an index outside
+ * [0, src_rows) and positions outside the cache are skipped. Everything else in the pages is left
+ * as it is, the other positions of a tile included. Writing into a page that another sequence
+ * shares changes it for both. */
+int q4nx_kv4_append(const q4nx_kv4 *cache, const uint16_t *k, const uint16_t *v, int by_position,
+                    int64_t src_rows, int64_t row_stride, int64_t head_stride, int64_t seq_stride,
+                    const int32_t *pos, const int32_t *cu, int max_new, void *stream);
+/* What the rows at those positions stand for, packed [out_rows][Hkv][D]: bf16 or, with out_f32, fp32.
+ * Rows at positions outside the cache are NaN; rows at or past out_rows are not written. */
+int q4nx_kv4_read(const q4nx_kv4 *cache, void *k_out, void *v_out, int out_f32, int64_t out_rows,
+                  const int32_t *pos, const int32_t *cu, int max_new, void *stream);
+
+/* GQA attention over the cache: q bf16 [total][q_stride] holding [Hq][D] (q_stride a multiple of 8),
+ * out bf16 and / or fp32 [total][Hq][D]. Query head h reads kv head h / (Hq/Hkv), Hq/Hkv <= 16.
+ * Without cu, one token per sequence (total = n_seqs): positions [0, lens[b]). With cu, sequence b's
+ * tokens are rows cu[b] .. cu[b+1] - 1, the last of them at position lens[b] - 1: token i of n sees
+ * positions [0, lens[b] - n + 1 + i). A row that sees nothing gives zeros; lens[b] > max_len reads
+ * max_len positions; rows behind the last sequence are not written; max_new: at least the most
+ * tokens of one sequence. A NaN in the cache makes NaN of at least its channels in every row that
+ * sees it.
+ * sel (one token per sequence only): int32 [n_seqs][Hkv][n_sel], the logical pages to read, as
+ * q4nx_kv4_select gives them; entries outside the sequence are none, a page named twice counts twice.
+ * n_split = 0 chooses how many workgroups share a sequence. ws: q4nx_kv4_attn_ws_bytes(...). */
+size_t q4nx_kv4_attn_ws_bytes(const q4nx_kv4 *cache, int n_q_heads, int max_new, int max_len,
+                              int n_sel, int n_split);
+int q4nx_kv4_attn(const q4nx_kv4 *cache, const uint16_t *q, int64_t q_stride, uint16_t *out,
+                  float *out_f32, int n_q_heads, const int32_t *cu, int total, int max_new,
+                  const int32_t *lens, int max_len, float scale, const int32_t *sel, int n_sel,
+                  int n_split, void *ws, size_t ws_bytes, void *stream);
+
+/* The pages a token's attention reads: for every sequence and kv head the n_sel pages of the highest
+ * score sum over the group's heads and channels of max(q lo, q hi) (fp64; ties to the lowest page),
+ * the first n_first and the last n_last pages among them whatever their score, then pages whose
+ * score is NaN. sel int32 [n_seqs][Hkv][n_sel]: ascending, -1 behind the last. lens[b] > max_len
+ * counts as max_len; at most 16384 pages per sequence. ws: q4nx_kv4_select_ws_bytes(...). */
+size_t q4nx_kv4_select_ws_bytes(const q4nx_kv4 *cache, int max_len);
+int q4nx_kv4_select(const q4nx_kv4 *cache, const uint16_t *q, int64_t q_stride, int n_q_heads,
+                    const int32_t *lens, int max_len, int n_sel, int n_first, int n_last, int32_t *sel,
+                    void *ws, size_t ws_bytes, void *stream);
+
+/* Page bookkeeping on the device. refs int32 [n_pages]: how many table entries name a page (0: free).
+ * A sequence's row holds its pages from the front and -1 behind them. layer l's page p is at
+ * cache->pages + l * layer_stride + p * page_stride; layers share tables and counts. status
+ * (optional): the number of sequences (or pairs) that were not done; those change nothing.
+ * ws: q4nx_kv4_pages_ws_bytes(cache, n).
+ *
+ * reserve: sequence b gets the pages it lacks for want[b] positions, the lowest free ones, sequences
+ * in order. One that wants more than its row holds gets none; where the free pages end, the sequence
+ * whose pages do not all fit gets none, nor do those after it. */
+size_t q4nx_kv4_pages_ws_bytes(const q4nx_kv4 *cache, int n);
+int q4nx_kv4_reserve(const q4nx_kv4 *cache, int32_t *refs, const int32_t *want, int32_t *status,
+                     void *ws, size_t ws_bytes, void *stream);
+/* fork: sequence dst[i] goes on from src[i]: its full pages are shared, the last, partly filled one is
+ * copied (in every layer) into the lowest free page, in the order of the pairs; lens[dst] = lens[src].
+ * A pair is not done if an index is outside the sequences, dst is a source or an earlier pair's dst or
+ * has pages, or no page is free. */
+int q4nx_kv4_fork(const q4nx_kv4 *cache, int64_t layer_stride, int n_layers, int32_t *lens,
+                  int32_t *refs, const int32_t *src, const int32_t *dst, int n, int32_t *status,
+                  void *ws, size_t ws_bytes, void *stream);
+/* free: the sequences' entries become -1, their pages' counts go down, lens 0. */
+int q4nx_kv4_free(const q4nx_kv4 *cache, int32_t *lens, int32_t *refs, const int32_t *seqs, int n,
+                  int32_t *status, void *stream);
+/* compact: pages in use move below `live` (int32 [1], optional: their number): the i-th one at or
+ * behind it to the i-th free one before it, in every layer, table and counts with them. */
+int q4nx_kv4_compact(const q4nx_kv4 *cache, int64_t layer_stride, int n_layers, int32_t *refs,
+                     int32_t *live, void *ws, size_t ws_bytes, void *stream);
+/* Page src_pages[i] copied to dst_pages[i] in every layer; pairs outside the pool are skipped. No page
+ * may be written that another pair reads or writes. */
+int q4nx_kv4_copy_pages(const q4nx_kv4 *cache, int64_t layer_stride, int n_layers,
+                        const int32_t *src_pages, const int32_t *dst_pages, int n, void *stream);
+
 /* ---------------------------------------------------------------- weight-stream floors
  * The null GEMV: exactly the grid, workgroup size and per-lane loads of the batch-1 q4 GEMV
  * (q4nx_gemv_q4 at batch 1 under the default policy: the row-block kernel) and its 16

@@ -52,6 +52,16 @@ class Policy(C.Structure):
 
 c_pol = C.POINTER(Policy)
 
+
+class Kv4(C.Structure):
+    """q4nx_kv4: one layer's pages of a 4-bit K/V cache and its sequences' table."""
+    _fields_ = [("pages", c_p), ("page_stride", c_i64), ("table", c_p), ("table_stride", c_i64),
+                ("n_pages", c_i), ("page_len", c_i), ("n_kv_heads", c_i), ("head_dim", c_i),
+                ("n_seqs", c_i), ("table_len", c_i)]
+
+
+c_kv4 = C.POINTER(Kv4)
+
 # name -> (restype, argtypes); mirrors include/q4nx_hip.h
 SIGNATURES: dict[str, tuple] = {
     "q4nx_abi_version": (c_i, []),
@@ -91,6 +101,20 @@ SIGNATURES: dict[str, tuple] = {
     "q4nx_gqa_decode_records": (c_i, [c_p, c_p, c_p, c_i, c_i, c_i, c_i, c_p, c_i, c_i64,
                                       c_i64, c_f, c_i, c_p, c_sz, c_pol, c_p]),
     "q4nx_gemv_attn_q4": (c_i, [c_p, c_i, c_p, c_i, c_i, c_i, c_p, c_p, c_p, c_p]),
+    "q4nx_kv4_page_bytes": (c_sz, [c_i, c_i, c_i]),
+    "q4nx_kv4_append": (c_i, [c_kv4, c_p, c_p, c_i, c_i64, c_i64, c_i64, c_i64, c_p, c_p, c_i, c_p]),
+    "q4nx_kv4_read": (c_i, [c_kv4, c_p, c_p, c_i, c_i64, c_p, c_p, c_i, c_p]),
+    "q4nx_kv4_attn_ws_bytes": (c_sz, [c_kv4, c_i, c_i, c_i, c_i, c_i]),
+    "q4nx_kv4_attn": (c_i, [c_kv4, c_p, c_i64, c_p, c_p, c_i, c_p, c_i, c_i, c_p, c_i, c_f, c_p, c_i,
+                            c_i, c_p, c_sz, c_p]),
+    "q4nx_kv4_select_ws_bytes": (c_sz, [c_kv4, c_i]),
+    "q4nx_kv4_select": (c_i, [c_kv4, c_p, c_i64, c_i, c_p, c_i, c_i, c_i, c_i, c_p, c_p, c_sz, c_p]),
+    "q4nx_kv4_pages_ws_bytes": (c_sz, [c_kv4, c_i]),
+    "q4nx_kv4_reserve": (c_i, [c_kv4, c_p, c_p, c_p, c_p, c_sz, c_p]),
+    "q4nx_kv4_fork": (c_i, [c_kv4, c_i64, c_i, c_p, c_p, c_p, c_p, c_i, c_p, c_p, c_sz, c_p]),
+    "q4nx_kv4_free": (c_i, [c_kv4, c_p, c_p, c_p, c_i, c_p, c_p]),
+    "q4nx_kv4_compact": (c_i, [c_kv4, c_i64, c_i, c_p, c_p, c_p, c_sz, c_p]),
+    "q4nx_kv4_copy_pages": (c_i, [c_kv4, c_i64, c_i, c_p, c_p, c_i, c_p]),
     "q4nx_gemv_q4_null": (c_i, [c_p, c_p, c_p, c_i, c_i, c_p]),
     "q4nx_stream_read": (c_i, [c_p, c_sz, c_p, c_p]),
     "q4nx_round_bf16": (c_i, [c_p, c_p, c_i64, c_p]),
