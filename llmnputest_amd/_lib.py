@@ -104,7 +104,7 @@ SIGNATURES: dict[str, tuple] = {
     "q4nx_kv4_page_bytes": (c_sz, [c_i, c_i, c_i]),
     "q4nx_kv4_append": (c_i, [c_kv4, c_p, c_p, c_i, c_i64, c_i64, c_i64, c_i64, c_p, c_p, c_i, c_p]),
     "q4nx_kv4_read": (c_i, [c_kv4, c_p, c_p, c_i, c_i64, c_p, c_p, c_i, c_p]),
-    "q4nx_kv4_attn_ws_bytes": (c_sz, [c_kv4, c_i, c_i, c_i, c_i, c_i]),
+    "q4nx_kv4_attn_ws_bytes": (c_sz, [c_kv4, c_i, c_i, c_i, c_i, c_i, c_i]),
     "q4nx_kv4_attn": (c_i, [c_kv4, c_p, c_i64, c_p, c_p, c_i, c_p, c_i, c_i, c_p, c_i, c_f, c_p, c_i,
                             c_i, c_p, c_sz, c_p]),
     "q4nx_kv4_select_ws_bytes": (c_sz, [c_kv4, c_i]),

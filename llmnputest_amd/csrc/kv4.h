@@ -44,9 +44,13 @@ __device__ __forceinline__ int kv4_page(const Kv4& c, int b, int lp) {
   return id >= 0 && id < c.n_pages ? id : -1;
 }
 
-// Two codes as the bf16 pair (128 + code, 128 + code).
+// Two codes as the bf16 pair (128 + code, 128 + code): a shift and v_and_or_b32, which takes one
+// constant from a scalar register and needs the other in a vector register.
 __device__ __forceinline__ uint32_t kv4_pair(uint32_t w, int r) {
-  return ((w >> (4 * r)) & 0x000F000Fu) | 0x43004300u;
+  uint32_t mask = 0x000F000Fu, bias = 0x43004300u;
+  asm("" : "+s"(mask));
+  asm("" : "+v"(bias));
+  return ((w >> (4 * r)) & mask) | bias;
 }
 __device__ __forceinline__ u32x4_t kv4_operand(uint32_t w) {
   return u32x4_t{kv4_pair(w, 0), kv4_pair(w, 1), kv4_pair(w, 2), kv4_pair(w, 3)};

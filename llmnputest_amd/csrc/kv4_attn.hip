@@ -5,9 +5,9 @@
 //   S^T[pos][row]  = sum_g d_g[pos] (c . q)_g + m_g[pos] (sum of q)_g
 //   O^T[dim][row] += sum_pos (p d_g(dim))[pos] c[pos][dim] + sum_pos p m_g(dim)
 // so the codes enter the matrix cores as they are stored, as the bf16 numbers 128 + c (exact), and
-// the scales stay in fp32. The 128 is taken out exactly where it can be: the score's accumulator
-// starts at -128 (sum of q)_g, and the values' sum is joined by an operand of -128s. p d_g enters as
-// two bf16 terms, which carry it to 2^-17.
+// the scales stay in fp32. The 128 is taken out again: the score's accumulator starts at
+// -128 (sum of q)_g, and m_g - 128 d_g takes m_g's place in the values. p d_g enters as two bf16 terms,
+// which carry it to 2^-18, so that a value is off by at most 143 2^-18 of its step.
 #include <math.h>
 
 #include "kv4.h"
@@ -23,7 +23,9 @@ struct Kv4AttnArgs {
   const int32_t* cu;
   const int32_t* lens;
   const int32_t* sel;
-  int n_sel, hq, group, total, row_tiles, n_split;
+  int n_sel, hq, group, total, row_tiles;
+  int n_split, chunk;   // blocks: workgroups per row tile, tiles for each of them
+  int unit;             // one token: tiles per part of a (sequence, kv head), 0: by what there is
   float scale_l2;
   float* partial;
   uint32_t partial_bytes;
@@ -33,12 +35,516 @@ struct Kv4AttnArgs {
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 constexpr int kWaves = 4;
+constexpr int kLineTiles = 16384;   // tiles of a call above which its workgroups share one line of them
+// Those workgroups: what the chip holds at once (three waves per SIMD at D = 64, two at 128).
+__host__ __device__ constexpr int kv4_line(int d) { return d == 64 ? 768 : 512; }
+constexpr int kMergeParts = 64;   // records of an item merged per pass
+constexpr int kMergeBatch = 8;    // of them in flight per thread
+
+// x - bf16 (the lo or hi half of pair) in one instruction; the difference of a number and its bf16
+// rounding is exact. The pair (-1, 0) comes from a register: as an inline constant -1.0 the
+// instruction takes it for (0, -1).
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+typedef short s16x2_t __attribute__((ext_vector_type(2)));
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+struct Kv4Minus {
+  uint32_t lo = 0x0000BF80u, hi = 0xBF800000u;
+  __device__ Kv4Minus() { asm volatile("" : "+v"(lo), "+v"(hi)); }
+  static __device__ __forceinline__ float dot(float x, uint32_t pair, uint32_t one) {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(s16x2_t, pair),
+                                           __builtin_bit_cast(s16x2_t, one), x, false);
+  }
+};
 
 template <int NG>
-__global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4AttnArgs a) {
-  constexpr int D = 32 * NG, C = D / 64, NT = D / 16, REC = D + 4;
-  __shared__ __attribute__((aligned(16))) float s_o[kWaves][16][REC];
-  __shared__ __attribute__((aligned(16))) float s_fin[16][REC];
+struct Kv4TileRegs {
+  u32x4_t k[NG / 2], v[NG / 2];
+  uint32_t s[NG];
+};
+
+// The waves' states of `used` rows in s_o ([wave][row][dims, m, l]) -> s_fin, then the records of the
+// item's parts in their order by whichever workgroup arrives last, and the rows out.
+template <int D, int TH, int NW, int ROWS, typename Rec>
+__device__ __forceinline__ void kv4_finish(const Kv4AttnArgs& a, float (*s_o)[ROWS][D + 4],
+                                           float (*s_fin)[D + 4], int* s_last, int item, int part,
+                                           int parts, Rec&& rec_of, int used, int c0, int row0, int h) {
+  constexpr int REC = D + 4;
+  const int tid = threadIdx.x;
+  __syncthreads();
+  for (int e = tid; e < used * D; e += TH) {
+    const int r = e / D, d = e % D;
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) M = fmaxf(M, s_o[w][r][D]);
+    const float Mb = M == -INFINITY ? 0.f : M;
+    float L = 0.f, A = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float f = ex2(s_o[w][r][D] - Mb);
+      L = fmaf(s_o[w][r][D + 1], f, L);
+      A = fmaf(s_o[w][r][d], f, A);
+    }
+    s_fin[r][d] = A;
+    if (d < 4) s_fin[r][D + d] = d == 0 ? M : (d == 1 ? L : 0.f);
+  }
+  __syncthreads();
+  if (parts > 1) {
+    const __amdgpu_buffer_rsrc_t pr = make_rsrc(a.partial, a.partial_bytes);
+    const uint32_t rec = (uint32_t)rec_of(part) * (ROWS * REC * 4);
+    for (int e = tid; e < used * REC / 4; e += TH)
+      st16_sys(pr, rec + e * 16, ((const uint4*)s_fin)[e]);
+    wait_vm();
+    __syncthreads();
+    if (tid == 0) *s_last = ticket(&a.counters[item], parts) ? 1 : 0;
+    __syncthreads();
+    if (!*s_last) return;
+    // 16 lanes of a row find the parts' weights; a thread sums four channels over every ng-th part, its
+    // first records on their way meanwhile; ng sums meet in LDS
+    constexpr int KC = (ROWS * D / 4 + TH - 1) / TH;
+    __shared__ float s_f[kMergeParts][ROWS], s_c[ROWS];
+    const int cols = used * D / 4, ng = max(1, min(NW, TH / cols));
+    const int grp = cols < TH ? tid / cols : 0, c0_ = tid - grp * cols;
+    float4 A[KC];
+    float M = -INFINITY, L = 0.f;   // of row tid / 16, in its 16 lanes
+#pragma unroll
+    for (int k = 0; k < KC; ++k) A[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p0 = 0; p0 < parts; p0 += kMergeParts) {
+      const int cnt = min(kMergeParts, parts - p0);
+      uint4 x[KC][kMergeBatch];
+      auto fetch = [&](int k0) {
+#pragma unroll
+        for (int k = 0; k < KC; ++k) {
+          const int c = min(c0_ + k * TH, cols - 1);
+#pragma unroll
+          for (int i = 0; i < kMergeBatch; ++i)
+            x[k][i] = ld16_sys(pr, (uint32_t)rec_of(p0 + min(grp + ng * (k0 + i), cnt - 1)) *
+                                           (ROWS * REC * 4) +
+                                       (c / (D / 4)) * (REC * 4) + (c % (D / 4)) * 16);
+        }
+      };
+      if (grp < ng) fetch(0);
+      const int r = tid >> 4, j = tid & 15;
+      if (r < used) {
+        float mi[4], li[4], top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool in = j + 16 * i < cnt;
+          const float* p = a.partial + ((size_t)rec_of(p0 + (in ? j + 16 * i : 0)) * ROWS + r) * REC + D;
+          mi[i] = in ? load_sys(p) : -INFINITY;
+          li[i] = in ? load_sys(p + 1) : 0.f;
+          top = fmaxf(top, mi[i]);
+        }
+        const float Mn = fmaxf(M, group16_max(top)), Mb = Mn == -INFINITY ? 0.f : Mn;
+        const float f = ex2(M - Mb);
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float g = ex2(mi[i] - Mb);
+          s_f[j + 16 * i][r] = g;
+          sum = fmaf(li[i], g, sum);
+        }
+        L = fmaf(L, f, group16_sum(sum));
+        M = Mn;
+        if (j == 0) s_c[r] = f;
+      }
+      __syncthreads();
+      if (grp < ng) {
+#pragma unroll
+        for (int k = 0; k < KC; ++k) {
+          const float f = s_c[min(c0_ + k * TH, cols - 1) / (D / 4)];
+          A[k].x *= f;
+          A[k].y *= f;
+          A[k].z *= f;
+          A[k].w *= f;
+        }
+        for (int k0 = 0; grp + ng * k0 < cnt; k0 += kMergeBatch) {
+          if (k0) fetch(k0);
+#pragma unroll
+          for (int k = 0; k < KC; ++k) {
+            const int row = min(c0_ + k * TH, cols - 1) / (D / 4);
+#pragma unroll
+            for (int i = 0; i < kMergeBatch; ++i) {
+              const int p = grp + ng * (k0 + i);
+              if (p < cnt) {
+                const float g = s_f[p][row];
+                A[k].x = fmaf(__uint_as_float(x[k][i].x), g, A[k].x);
+                A[k].y = fmaf(__uint_as_float(x[k][i].y), g, A[k].y);
+                A[k].z = fmaf(__uint_as_float(x[k][i].z), g, A[k].z);
+                A[k].w = fmaf(__uint_as_float(x[k][i].w), g, A[k].w);
+              }
+            }
+          }
+        }
+      }
+      __syncthreads();
+    }
+    if (tid < 16 * used && (tid & 15) == 0) s_fin[tid >> 4][D + 1] = L;
+#pragma unroll
+    for (int k = 0; k < KC; ++k) {
+      const int c = c0_ + k * TH;
+      if (grp < ng && c < cols) *(float4*)&s_o[grp][c / (D / 4)][c % (D / 4) * 4] = A[k];
+    }
+    __syncthreads();
+    for (int e = tid; e < used * D; e += TH) {
+      float y = 0.f;
+      for (int g = 0; g < ng; ++g) y += s_o[g][e / D][e % D];
+      s_fin[e / D][e % D] = y;
+    }
+    __syncthreads();
+  }
+  for (int e = tid; e < used * D; e += TH) {
+    const int r = e / D, d = e % D;
+    const float L = s_fin[r][D + 1];
+    const float y = L == 0.f ? 0.f : attn_div(s_fin[r][d], L);   // nothing seen: 0; a NaN stays
+    const int row = row0 + r;
+    const int64_t at = ((int64_t)(c0 + row / a.group) * a.hq + h * a.group + row % a.group) * D + d;
+    if (a.out) a.out[at] = f32_to_bf16(y);
+    if (a.out_f32) a.out_f32[at] = y;
+  }
+}
+
+// One token per sequence. The group's heads are the rows of a score tile, spread so that a lane holds
+// R = ceil(heads / 4) of them for one position (head 4 i + kg in register i), and all that belongs to a
+// position, its scales and the exponentials, is done once per head and position:
+//   S[head][pos] = d_g (c . q)_g + m_g (sum of q)_g, summed over g;   C starts at -128 (sum of q)_g
+//   O^T[dim][head] += c^T[dim][pos] . (p d_g)^T[pos][head];  sum p (m_g - 128 d_g) apart, per lane
+// p d_g goes through LDS from rows to columns: a lane's pair (position n, 16 + n) is an operand
+// register as it is, so the writes are consecutive dwords and an operand one 16-byte read. The scales
+// are one load of 4 NG bytes a lane (K's positions in lanes 0..31, V's in 32..63), spread by lane swaps.
+// A wave takes every fourth tile of its part; a lane finds the page of one of the wave's next 64
+// tiles, so table and list are read ahead, and two tiles are in flight while one is computed.
+//
+// Who does what is decided here, from the lengths as they are: of W tiles in all a part has
+//   8 (W < 1024), 16 (W < 8192), 32 (W <= 16384) or W / 768 (D = 64; 512 at 128)
+// tiles. Up to 32 a (sequence, kv head) is cut into parts of its own (a short call, where a second
+// segment would be waited for); beyond that the W tiles are one line that the workgroups cut evenly,
+// so that lengths however unlike load the chip alike, and a workgroup's stretch may end one
+// (sequence, kv head) and begin the next.
+
+// x / y for quotients below 2^20 or so: the reciprocal is off by less than one in them.
+__device__ __forceinline__ int div_few(int x, int y) {
+  int q = (int)((float)x * __builtin_amdgcn_rcpf((float)y));
+  q -= q * y > x;
+  q += (q + 1) * y <= x;
+  return q;
+}
+
+// Inclusive sum over the lanes of a wave.
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);   // row_shr 1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);   // lane 15 to the next row
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);   // lane 31 to the upper half
+  return x;
+}
+
+template <int NG, int R>
+__global__ __launch_bounds__(256) void kv4_decode_kernel(Kv4AttnArgs a) {
+  constexpr int D = 32 * NG, C = D / 64, NT = D / 16, PF = 2, H = 4 * R;
+  constexpr int kLine = kv4_line(D);
+  __shared__ __attribute__((aligned(16))) float s_o[kWaves][H][D + 4];
+  __shared__ __attribute__((aligned(16))) float s_fin[H][D + 4];
+  __shared__ __attribute__((aligned(16))) uint32_t s_p[kWaves][NG][2][H * 16];
+  __shared__ float s_x[kWaves][NG + 1][H];   // sums of p (m - 128 d), and a move of the reference
+  __shared__ int s_last;
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, kg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int tpp = a.c.tiles, nb = a.c.n_seqs, hkv = a.c.hkv;
+  auto len_of = [&](int b) { return b < nb ? max(0, min(a.lens[b], a.c.cap)) : 0; };
+  auto tiles_of = [&](int len) {
+    return a.sel ? a.n_sel * tpp : max(1, (len + kKv4Tile - 1) / kKv4Tile);
+  };
+  const int len0 = len_of(lane);   // of the first 64 sequences, the only ones as a rule
+  // x(tiles) summed over the sequences up to the one whose hkv shares hold `target`: that sequence,
+  // what lies before it, its x and length (no such one: all sequences)
+  struct Where {
+    int b, before, x, len;
+  };
+  auto find = [&](int target, auto&& x) {
+    Where r{nb, 0, 0, 0};
+    for (int c = 0; c < nb; c += 64) {
+      const int len = c ? len_of(c + lane) : len0;
+      const int mine = c + lane < nb ? x(tiles_of(len)) : 0;
+      const int sum = wave_scan(mine);
+      const unsigned long long hit = __ballot(c + lane < nb && (r.before + sum) * hkv > target);
+      if (hit) {
+        const int l0 = __builtin_ctzll(hit);
+        r.b = c + l0;
+        r.x = __builtin_amdgcn_readlane(mine, l0);
+        r.len = __builtin_amdgcn_readlane(len, l0);
+        r.before += __builtin_amdgcn_readlane(sum, l0) - r.x;
+        return r;
+      }
+      r.before += __builtin_amdgcn_readlane(sum, 63);
+    }
+    return r;
+  };
+  const int W = find(0x7FFFFFFF, [](int x) { return x; }).before * hkv;
+  const bool line = a.unit == 0 && W > kLineTiles;
+  // parts of their own have 8, 16 or 32 tiles (or as many as asked for)
+  const int sh = W < 1024 ? 3 : W < 8192 ? 4 : 5;
+  const int unit = a.unit ? a.unit : line ? (W + kLine - 1) / kLine : 1 << sh;
+  auto share = [&](int x) {
+    return line ? x : a.unit ? div_few(x + unit - 1, unit) : (x + unit - 1) >> sh;
+  };
+
+  for (int at = blockIdx.x * (line ? unit : 1), left = line ? unit : 1;;) {
+  const Where f = find(at, share);
+  if (f.b == nb) return;
+  const int b = f.b, end = f.len, nt = tiles_of(f.len);
+  const int rem = at - f.before * hkv;
+  const int h = div_few(rem, f.x), in = rem - h * f.x;
+  const int take = line ? min(left, f.x - in) : 1;
+  // the item's parts, this one, its tiles, the workgroup of its first part
+  const int off = at - in, rec0 = line ? off / unit : off;
+  const int part = line ? (int)blockIdx.x - rec0 : in;
+  const int parts = line ? (off + f.x - 1) / unit - rec0 + 1 : f.x;
+  const int first = line ? in : in * unit, stop = line ? in + take : min(nt, (in + 1) * unit);
+  const int item = b * hkv + h;
+
+  // q (of the negative scale's sign) as the rows of a tile: row 4 kg + i is head 4 i + kg
+  u32x4_t q[NG];
+  f32x4_t z[NG];
+  float qs[NG][R];
+  {
+    const int head = 4 * (n & 3) + (n >> 2);
+    const bool live = (n & 3) < R && head < a.group;
+    const uint16_t* p = a.q + (int64_t)b * a.q_stride + (h * a.group + (live ? head : 0)) * D + 8 * kg;
+    const uint32_t sign = a.scale_l2 < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      q[g] = *(const u32x4_t*)(p + 32 * g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) q[g][i] = live ? q[g][i] ^ sign : 0u;
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s += bf16lo(q[g][i]) + bf16hi(q[g][i]);
+      s = xor32_sum(xor16_sum(s));
+      z[g] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        qs[g][i] = __shfl(s, 4 * kg + i);
+        z[g][i] = -128.f * qs[g][i];
+      }
+    }
+  }
+  const float scale = fabsf(a.scale_l2);
+  f32x4_t o[NT];
+  float ms[NG][R], m[R], mb[R], lim[R], l[R];
+#pragma unroll
+  for (int u = 0; u < NT; ++u) o[u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    m[i] = lim[i] = -INFINITY;
+    mb[i] = l[i] = 0.f;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) ms[g][i] = 0.f;
+  }
+  const Kv4Minus neg;
+  const int t0 = first + wave, t1 = stop;
+  const int64_t head_off = (int64_t)h * kv4_head_bytes(a.c.page_len, D);
+  // the operand this lane reads: row n of s_p (rows past H again the first ones)
+  const uint32_t p_at = (uint32_t)((n % H) * 16 + 4 * kg);
+
+  for (int i0 = 0; t0 + kWaves * i0 < t1; i0 += 64) {
+    const int count = min(64, (t1 - t0 - kWaves * i0 + kWaves - 1) / kWaves);
+    // this lane's tile: its page, and its first position (past every length when there is none)
+    int id = 0, pos = 1 << 30;
+    if (lane < count) {
+      const int t = t0 + kWaves * (i0 + lane);
+      const int e = t / tpp, sub = t % tpp;
+      const int lp = a.sel ? a.sel[(int64_t)item * a.n_sel + e] : e;
+      if (lp >= 0 && lp < a.c.table_len) {
+        id = kv4_page(a.c, b, lp) * 4 + sub;   // negative: no page
+        pos = lp * a.c.page_len + sub * kKv4Tile;
+      }
+    }
+    Kv4TileRegs<NG> buf[PF];
+    auto load = [&](Kv4TileRegs<NG>& r, int i) {
+      const int x = __builtin_amdgcn_readlane(id, i);
+      const uint8_t* tile = a.c.pages + (int64_t)(x < 0 ? 0 : x >> 2) * a.c.page_stride + head_off +
+                            (x < 0 ? 0 : x & 3) * kv4_tile_bytes(D);
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        r.k[c] = *(const u32x4_t*)(tile + (c * 64 + lane) * 16);
+        r.v[c] = *(const u32x4_t*)(tile + 16 * D + (c * 64 + lane) * 16);
+      }
+      if constexpr (NG == 2) {
+        const uint2 s = *(const uint2*)(tile + 32 * D + lane * 8);
+        r.s[0] = s.x;
+        r.s[1] = s.y;
+      } else {
+        const u32x4_t s = *(const u32x4_t*)(tile + 32 * D + lane * 16);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) r.s[g] = s[g];
+      }
+    };
+    auto compute = [&](const Kv4TileRegs<NG>& r, int i0_) {
+      const int base = __builtin_amdgcn_readlane(pos, i0_);
+      const bool none = __builtin_amdgcn_readlane(id, i0_) < 0;
+      const bool part = base + kKv4Tile > end || none;
+      uint32_t w[NG], sc[2][2][NG];   // [K, V][tt]: this lane's position's scales
+#pragma unroll
+      for (int g = 0; g < NG; ++g) w[g] = r.s[g];
+      if (part) {
+        // masked positions' scales may be anything (the page's older bytes)
+        const bool seen = base + (lane & 31) < end;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) w[g] = seen ? (none ? kKv4NaN : w[g]) : 0u;
+      }
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const auto x = __builtin_amdgcn_permlane16_swap(w[g], w[g], false, false);
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) {
+          const auto y = __builtin_amdgcn_permlane32_swap(x[tt], x[tt], false, false);
+          sc[0][tt][g] = y[0];
+          sc[1][tt][g] = y[1];
+        }
+      }
+      float s[2][R];
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) s[tt][i] = 0.f;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          const f32x4_t y = mfma_bf16(q[g], kv4_operand(r.k[g >> 1][2 * tt + (g & 1)]), z[g]);
+          const float d = bf16lo(sc[0][tt][g]), mm = bf16hi(sc[0][tt][g]);
+#pragma unroll
+          for (int i = 0; i < R; ++i) s[tt][i] = fmaf(d, y[i], fmaf(mm, qs[g][i], s[tt][i]));
+        }
+      }
+      if (part) {
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+          if (base + 16 * tt + n >= end)
+#pragma unroll
+            for (int i = 0; i < R; ++i) s[tt][i] = -INFINITY;
+      }
+      // a head's reference moves only when a score has passed it by 2^8: sums stay far from overflow
+      float top[R];
+      bool move = false;
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        top[i] = fmaxf(s[0][i], s[1][i]) * scale;
+        move |= top[i] > lim[i];
+      }
+      if (__any(move)) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          const float mn = fmaxf(m[i], group16_max(top[i]));
+          const float nb_ = mn == -INFINITY ? 0.f : mn;
+          const float f_ = ex2(m[i] - nb_);
+          m[i] = mn;
+          mb[i] = nb_;
+          lim[i] = mn + 8.f;
+          l[i] *= f_;
+#pragma unroll
+          for (int g = 0; g < NG; ++g) ms[g][i] *= f_;
+          if (n == 0) s_x[wave][NG][4 * i + kg] = f_;
+        }
+        __builtin_amdgcn_wave_barrier();
+        const float f_ = s_x[wave][NG][n % H];
+#pragma unroll
+        for (int u = 0; u < NT; ++u) o[u] *= f_;
+        __builtin_amdgcn_wave_barrier();
+      }
+      float p[2][R];
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+        for (int i = 0; i < R; ++i) p[tt][i] = ex2(fmaf(s[tt][i], scale, -mb[i]));
+      if (part) {
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+          if (base + 16 * tt + n >= end)
+#pragma unroll
+            for (int i = 0; i < R; ++i) p[tt][i] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < R; ++i) l[i] += p[0][i] + p[1][i];
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const float d0 = bf16lo(sc[1][0][g]), d1 = bf16lo(sc[1][1][g]);
+        const float m0 = fmaf(-128.f, d0, bf16hi(sc[1][0][g]));
+        const float m1 = fmaf(-128.f, d1, bf16hi(sc[1][1][g]));
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          const float x0 = p[0][i] * d0, x1 = p[1][i] * d1;
+          ms[g][i] = fmaf(p[0][i], m0, fmaf(p[1][i], m1, ms[g][i]));
+          const uint32_t hi = pack_bf16x2_op(x0, x1);
+          s_p[wave][g][0][64 * i + lane] = hi;
+          s_p[wave][g][1][64 * i + lane] =
+              pack_bf16x2_op(Kv4Minus::dot(x0, hi, neg.lo), Kv4Minus::dot(x1, hi, neg.hi));
+        }
+      }
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const u32x4_t hi = *(const u32x4_t*)&s_p[wave][g][0][p_at];
+        const u32x4_t lo = *(const u32x4_t*)&s_p[wave][g][1][p_at];
+#pragma unroll
+        for (int u = 2 * g; u < 2 * g + 2; ++u) {
+          const u32x4_t v = kv4_operand(r.v[u >> 2][u & 3]);
+          o[u] = mfma_bf16(v, hi, o[u]);
+          o[u] = mfma_bf16(v, lo, o[u]);
+        }
+      }
+      __builtin_amdgcn_wave_barrier();
+    };
+    // loads stand outside every branch (the last tile again behind the end): the wait for a tile then
+    // leaves the younger loads in flight
+#pragma unroll
+    for (int j = 0; j < PF; ++j) load(buf[j], min(j, count - 1));
+    for (int i = 0; i < count; i += PF) {
+#pragma unroll
+      for (int j = 0; j < PF; ++j) {
+        if (i + j < count) compute(buf[j], i + j);
+        load(buf[j], min(i + j + PF, count - 1));
+      }
+    }
+  }
+
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    l[i] = group16_sum(l[i]);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      ms[g][i] = group16_sum(ms[g][i]);
+      if (n == 0) s_x[wave][g][4 * i + kg] = ms[g][i];
+    }
+    if (n == 0) {
+      s_o[wave][4 * i + kg][D] = m[i];
+      s_o[wave][4 * i + kg][D + 1] = l[i];
+    }
+  }
+  __builtin_amdgcn_wave_barrier();
+  if (n < H) {
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      const float y = s_x[wave][u >> 1][n];
+      *(float4*)&s_o[wave][n][16 * u + 4 * kg] =
+          make_float4(o[u][0] + y, o[u][1] + y, o[u][2] + y, o[u][3] + y);
+    }
+  }
+  // a workgroup has at most one part that another began and one that another goes on with
+  auto rec_of = [&](int p) { return line ? 2 * (rec0 + p) + (p == 0) : rec0 + p; };
+  kv4_finish<D, 256, kWaves, H>(a, s_o, s_fin, &s_last, item, part, parts, rec_of, a.group, b, 0, h);
+  at += take;
+  left -= take;
+  if (left <= 0) return;
+  __syncthreads();
+  }
+}
+
+template <int NG>
+__global__ __launch_bounds__(256) void kv4_block_kernel(Kv4AttnArgs a) {
+  constexpr int D = 32 * NG, C = D / 64, NT = D / 16;
+  __shared__ __attribute__((aligned(16))) float s_o[kWaves][16][D + 4];
+  __shared__ __attribute__((aligned(16))) float s_fin[16][D + 4];
   __shared__ int s_last;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, kg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -61,6 +567,10 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4AttnArgs a) {
   const int tok = live ? row / a.group : 0, qh = live ? row % a.group : 0;
   const int end = live ? max(0, min(a.lens[b] - nq + tok + 1, a.c.cap)) : 0;   // positions this row sees
   const int top = max(0, min(a.lens[b] - nq + min(rt * 16 + 15, rows - 1) / a.group + 1, a.c.cap));
+
+  const int nt = (top + kKv4Tile - 1) / kKv4Tile;
+  const int parts = max(1, (nt + a.chunk - 1) / a.chunk);
+  if (split >= parts) return;
 
   // q, and its sums by group
   u32x4_t q[NG];
@@ -88,16 +598,11 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4AttnArgs a) {
   const u32x4_t minus = {0xC300C300u, 0xC300C300u, 0xC300C300u, 0xC300C300u};
 
   const int tpp = a.c.tiles;
-  const int nt = a.sel ? a.n_sel * tpp : (top + kKv4Tile - 1) / kKv4Tile;
-  const int chunk = (nt + a.n_split - 1) / a.n_split;
-  const int t_end = min(nt, (split + 1) * chunk);
-  for (int t = split * chunk + wave; t < t_end; t += kWaves) {
+  const int t_end = min(nt, (split + 1) * a.chunk);
+  for (int t = split * a.chunk + wave; t < t_end; t += kWaves) {
     const int e = t / tpp, sub = t % tpp;
-    int lp = e;
-    if (a.sel) lp = a.sel[((int64_t)b * a.c.hkv + h) * a.n_sel + e];
-    if (lp < 0 || (int64_t)lp * a.c.page_len + sub * kKv4Tile >= top) continue;
-    const int base = lp * a.c.page_len + sub * kKv4Tile;
-    const int id = kv4_page(a.c, b, lp);
+    const int base = t * kKv4Tile;
+    const int id = kv4_page(a.c, b, e);
     const uint8_t* tile = a.c.pages + (int64_t)max(id, 0) * a.c.page_stride +
                           (int64_t)h * kv4_head_bytes(a.c.page_len, D) + sub * kv4_tile_bytes(D);
     u32x4_t kc[C], vc[C];
@@ -194,66 +699,8 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4AttnArgs a) {
     s_o[wave][n][D] = m;
     s_o[wave][n][D + 1] = l;
   }
-  __syncthreads();
-  const int used = min(16, rows - rt * 16);
-  for (int e = tid; e < used * D; e += 256) {
-    const int r = e / D, d = e % D;
-    float M = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) M = fmaxf(M, s_o[w][r][D]);
-    const float Mb = M == -INFINITY ? 0.f : M;
-    float L = 0.f, A = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const float f = ex2(s_o[w][r][D] - Mb);
-      L = fmaf(s_o[w][r][D + 1], f, L);
-      A = fmaf(s_o[w][r][d], f, A);
-    }
-    s_fin[r][d] = A;
-    if (d < 4) s_fin[r][D + d] = d == 0 ? M : (d == 1 ? L : 0.f);
-  }
-  __syncthreads();
-  if (a.n_split > 1) {
-    const __amdgpu_buffer_rsrc_t pr = make_rsrc(a.partial, a.partial_bytes);
-    const uint32_t rec = ((uint32_t)bk * a.n_split + split) * (16 * REC * 4);
-    for (int e = tid; e < used * REC / 4; e += 256)
-      st16_sys(pr, rec + e * 16, ((const uint4*)&s_fin[0][0])[e]);
-    wait_vm();
-    __syncthreads();
-    if (tid == 0) s_last = ticket(&a.counters[bk], a.n_split) ? 1 : 0;
-    __syncthreads();
-    if (!s_last) return;
-    const float* recs = a.partial + (size_t)bk * a.n_split * 16 * REC;
-    for (int e = tid; e < used * D; e += 256) {
-      const int r = e / D, d = e % D;
-      float M = -INFINITY, L = 0.f, A = 0.f;
-      for (int sp = 0; sp < a.n_split; ++sp) {
-        const float* p = recs + ((size_t)sp * 16 + r) * REC;
-        const float mi = load_sys(p + D), li = load_sys(p + D + 1), ai = load_sys(p + d);
-        const float Mn = fmaxf(M, mi), Mb = Mn == -INFINITY ? 0.f : Mn;
-        const float f0 = ex2(M - Mb), f1 = ex2(mi - Mb);
-        L = L * f0 + li * f1;
-        A = A * f0 + ai * f1;
-        M = Mn;
-      }
-      s_fin[r][d] = A;
-      if (d == 0) s_fin[r][D + 1] = L;
-    }
-    __syncthreads();
-  }
-  for (int e = tid; e < used * D; e += 256) {
-    const int r = e / D, d = e % D;
-    const float L = s_fin[r][D + 1];
-    const float y = L == 0.f ? 0.f : attn_div(s_fin[r][d], L);   // nothing seen: 0; a NaN stays
-    const int row_ = rt * 16 + r;
-    const int64_t at = ((int64_t)(c0 + row_ / a.group) * a.hq + h * a.group + row_ % a.group) * D + d;
-    if (a.out) a.out[at] = f32_to_bf16(y);
-    if (a.out_f32) a.out_f32[at] = y;
-  }
-}
-
-static size_t kv4_partial_bytes(int64_t items, int n_split, int d) {
-  return (size_t)items * n_split * 16 * (d + 4) * 4;
+  kv4_finish<D, 256, kWaves, 16>(a, s_o, s_fin, &s_last, bk, split, parts,
+                                [&](int p) { return bk * a.n_split + p; }, min(16, rows - rt * 16), c0, rt * 16, h);
 }
 
 static int kv4_row_tiles(int max_new, int group) { return (int)(((int64_t)max_new * group + 15) / 16); }
@@ -267,21 +714,42 @@ static int kv4_auto_split(int64_t items, int tiles) {
 }
 
 struct Kv4Plan {
-  int64_t items;
-  int n_split;
+  int64_t items, grid;
+  int n_split, chunk, unit;
+  bool shared;   // whether an item may be of several parts
   size_t bytes;
 };
-static Kv4Plan kv4_plan(const q4nx_kv4* c, int n_q_heads, int max_new, int max_len, int n_sel,
-                        int n_split) {
-  Kv4Plan p;
-  const int rt = kv4_row_tiles(max_new, n_q_heads / c->n_kv_heads);
-  p.items = (int64_t)c->n_seqs * c->n_kv_heads * rt;
+static Kv4Plan kv4_plan(const q4nx_kv4* c, int n_q_heads, bool block, int max_new, int max_len,
+                        int n_sel, int n_split) {
+  Kv4Plan p{};
+  const int group = n_q_heads / c->n_kv_heads;
   const int64_t cap = (int64_t)c->table_len * c->page_len;
   const int64_t len = n_sel ? (int64_t)n_sel * c->page_len : (max_len < cap ? max_len : cap);
-  p.n_split = n_split > 0 ? n_split : kv4_auto_split(p.items, (int)((len + kKv4Tile - 1) / kKv4Tile));
-  p.bytes = p.n_split > 1 ? (size_t)Q4NX_WS_COUNTER_BYTES +
-                                kv4_partial_bytes(p.items, p.n_split, c->head_dim)
-                          : 0;
+  const int tiles = (int)((len + kKv4Tile - 1) / kKv4Tile);
+  int64_t recs;
+  int rows = 16;
+  if (block) {
+    p.items = (int64_t)c->n_seqs * c->n_kv_heads * kv4_row_tiles(max_new, group);
+    const int want = n_split > 0 ? n_split : kv4_auto_split(p.items, tiles);
+    p.chunk = (tiles + want - 1) / want;
+    p.n_split = (tiles + p.chunk - 1) / p.chunk;   // every split has work at the longest length
+    p.grid = recs = p.items * p.n_split;
+    p.shared = p.n_split > 1;
+  } else {
+    p.items = (int64_t)c->n_seqs * c->n_kv_heads;
+    rows = (group + 3) / 4 * 4;
+    if (n_split > 0) p.unit = (tiles + n_split - 1) / n_split;
+    else if (p.items * 4 > Q4NX_WS_COUNTER_BYTES) p.unit = tiles;   // no counter for each
+    // by what there is: at most kLineTiles in parts of 8 and more, or one line
+    const int line = kv4_line(c->head_dim);
+    const int64_t all = p.items * tiles, some = all < kLineTiles ? all : kLineTiles;
+    p.grid = p.unit ? p.items * ((tiles + p.unit - 1) / p.unit) : p.items + some / 8;
+    if (!p.unit && p.items * ((tiles + 7) / 8) < p.grid) p.grid = p.items * ((tiles + 7) / 8);
+    if (!p.unit && all > kLineTiles && p.grid < line) p.grid = line;
+    recs = p.grid > 2 * line ? p.grid : 2 * line;
+    p.shared = p.unit ? p.unit < tiles : tiles > 8;
+  }
+  p.bytes = p.shared ? (size_t)Q4NX_WS_COUNTER_BYTES + (size_t)recs * rows * (c->head_dim + 4) * 4 : 0;
   return p;
 }
 
@@ -297,13 +765,13 @@ using namespace q4nx;
 
 extern "C" {
 
-size_t q4nx_kv4_attn_ws_bytes(const q4nx_kv4* cache, int n_q_heads, int max_new, int max_len,
-                              int n_sel, int n_split) {
+size_t q4nx_kv4_attn_ws_bytes(const q4nx_kv4* cache, int n_q_heads, int block, int max_new,
+                              int max_len, int n_sel, int n_split) {
   Kv4 c;
   if (kv4_resolve(cache, &c, "q4nx_kv4_attn_ws_bytes") != Q4NX_OK ||
       !kv4_attn_shape(cache, n_q_heads, max_new, max_len, n_sel) || n_split < 0 || n_split > 1024)
     return 0;
-  return kv4_plan(cache, n_q_heads, max_new, max_len, n_sel, n_split).bytes;
+  return kv4_plan(cache, n_q_heads, block != 0, max_new, max_len, n_sel, n_split).bytes;
 }
 
 int q4nx_kv4_attn(const q4nx_kv4* cache, const uint16_t* q, int64_t q_stride, uint16_t* out,
@@ -323,17 +791,20 @@ int q4nx_kv4_attn(const q4nx_kv4* cache, const uint16_t* q, int64_t q_stride, ui
   Q4NX_REQUIRE(cu ? total >= 1 : (max_new == 1 && total == cache->n_seqs), Q4NX_ERR_SHAPE,
                "%s: total=%d, max_new=%d (without cu one token for each of %d sequences)", what, total,
                max_new, cache->n_seqs);
-  Q4NX_REQUIRE(n_sel == 0 || max_new == 1, Q4NX_ERR_SHAPE,
-               "%s: a page list is for one token per sequence, max_new=%d", what, max_new);
+  Q4NX_REQUIRE(n_sel == 0 || cu == nullptr, Q4NX_ERR_SHAPE,
+               "%s: a page list is for one token per sequence, without cu", what);
   Q4NX_REQUIRE(q_stride >= (int64_t)n_q_heads * cache->head_dim && q_stride % 8 == 0, Q4NX_ERR_SHAPE,
                "%s: q_stride=%lld must hold Hq * D and be a multiple of 8", what, (long long)q_stride);
-  const Kv4Plan p = kv4_plan(cache, n_q_heads, max_new, max_len, n_sel, n_split);
-  Q4NX_REQUIRE(p.items * p.n_split <= (int64_t)1 << 30, Q4NX_ERR_SHAPE,
-               "%s: %lld workgroups", what, (long long)(p.items * p.n_split));
-  if (p.n_split > 1) {
+  const Kv4Plan p = kv4_plan(cache, n_q_heads, cu != nullptr, max_new, max_len, n_sel, n_split);
+  const int64_t longest = n_sel ? (int64_t)n_sel * cache->page_len : max_len;
+  Q4NX_REQUIRE(p.grid <= (int64_t)1 << 30 && p.items * (longest / kKv4Tile + 1) < (int64_t)1 << 31,
+               Q4NX_ERR_SHAPE, "%s: %lld rows of up to %lld positions", what, (long long)p.items,
+               (long long)longest);
+  if (p.shared) {
     Q4NX_REQUIRE(p.bytes - Q4NX_WS_COUNTER_BYTES < (size_t)1 << 31 &&
                      p.items * 4 <= Q4NX_WS_COUNTER_BYTES,
-                 Q4NX_ERR_SHAPE, "%s: too many rows for %d splits", what, p.n_split);
+                 Q4NX_ERR_SHAPE, "%s: %lld rows to be shared by several workgroups", what,
+                 (long long)p.items);
     Q4NX_REQUIRE(ws != nullptr && ws_bytes >= p.bytes && Q4NX_ALIGNED(ws, 256), Q4NX_ERR_WS,
                  "%s: workspace of %zu bytes (256-aligned) needed, %zu given", what, p.bytes, ws_bytes);
     a.counters = (unsigned*)ws;
@@ -353,13 +824,24 @@ int q4nx_kv4_attn(const q4nx_kv4* cache, const uint16_t* q, int64_t q_stride, ui
   a.total = total;
   a.row_tiles = kv4_row_tiles(max_new, a.group);
   a.n_split = p.n_split;
+  a.chunk = p.chunk;
+  a.unit = p.unit;
   if (max_len < a.c.cap) a.c.cap = max_len;
   a.scale_l2 = (float)((double)scale * 1.4426950408889634);
-  const dim3 grid((unsigned)(p.items * p.n_split));
-  if (cache->head_dim == 64)
-    hipLaunchKernelGGL(kv4_attn_kernel<2>, grid, dim3(256), 0, (hipStream_t)stream, a);
-  else
-    hipLaunchKernelGGL(kv4_attn_kernel<4>, grid, dim3(256), 0, (hipStream_t)stream, a);
+  const dim3 grid((unsigned)p.grid);
+  const bool d64 = cache->head_dim == 64;
+  hipStream_t s = (hipStream_t)stream;
+  if (cu == nullptr) {
+    auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a); };
+    switch ((a.group + 3) / 4) {   // heads per lane
+      case 1: d64 ? run(kv4_decode_kernel<2, 1>) : run(kv4_decode_kernel<4, 1>); break;
+      case 2: d64 ? run(kv4_decode_kernel<2, 2>) : run(kv4_decode_kernel<4, 2>); break;
+      case 3: d64 ? run(kv4_decode_kernel<2, 3>) : run(kv4_decode_kernel<4, 3>); break;
+      default: d64 ? run(kv4_decode_kernel<2, 4>) : run(kv4_decode_kernel<4, 4>); break;
+    }
+  }
+  else if (d64) hipLaunchKernelGGL(kv4_block_kernel<2>, grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL(kv4_block_kernel<4>, grid, dim3(256), 0, s, a);
   return check_launch(what);
 }
 

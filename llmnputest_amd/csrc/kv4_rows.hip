@@ -333,8 +333,10 @@ int kv4_resolve(const q4nx_kv4* c, Kv4* out, const char* what) {
                "%s: head_dim=%d, 64 and 128 are built", what, c->head_dim);
   Q4NX_REQUIRE(c->page_len == 32 || c->page_len == 64 || c->page_len == 128, Q4NX_ERR_SHAPE,
                "%s: page_len=%d, not 32, 64 or 128", what, c->page_len);
-  Q4NX_REQUIRE(c->n_kv_heads >= 1 && c->n_kv_heads <= 1024 && c->n_pages >= 1, Q4NX_ERR_SHAPE,
-               "%s: n_kv_heads=%d (1..1024), n_pages=%d", what, c->n_kv_heads, c->n_pages);
+  Q4NX_REQUIRE(c->n_kv_heads >= 1 && c->n_kv_heads <= 1024 && c->n_pages >= 1 &&
+                   c->n_pages <= 1 << 28,
+               Q4NX_ERR_SHAPE,
+               "%s: n_kv_heads=%d (1..1024), n_pages=%d (1..2^28)", what, c->n_kv_heads, c->n_pages);
   Q4NX_REQUIRE(c->n_seqs >= 1 && c->n_seqs <= 8192 && c->table_len >= 1 &&
                    c->table_stride >= c->table_len &&
                    (int64_t)c->table_len * c->page_len <= (int64_t)1 << 30,

@@ -245,7 +245,7 @@ class Kv4Cache:
             sp, ns = sel.data_ptr(), sel.shape[2]
         new = 1 if cu is None else max_new or n
         most = min(self.max_len if table is None else c.table_len * self.page_len, max_len or 1 << 30)
-        need = self._need(c, "q4nx_kv4_attn_ws_bytes", hq, new, most, ns, n_split)
+        need = self._need(c, "q4nx_kv4_attn_ws_bytes", hq, int(cu is not None), new, most, ns, n_split)
         ws, wp, wn, stream = ops._scratch(ws, need)
         _lib.call("q4nx_kv4_attn", c, q.data_ptr(), stride, out.data_ptr(), ops._ptr(of), hq, u, n, new,
                   lp, most, d ** -0.5 if scale is None else float(scale), sp, ns, int(n_split), wp, wn,

@@ -62,7 +62,7 @@ def test_bad_caches_are_refused(bad):
                   call("q4nx_kv4_compact", c, 0, 1, P, None, P, 1 << 20, None),
                   call("q4nx_kv4_copy_pages", c, 0, 1, P, P, 1, None)):
         assert rc in (ERR_ARG, ERR_SHAPE)
-    assert _lib.lib().q4nx_kv4_attn_ws_bytes(c, 40, 1, 1000, 0, 4) == 0
+    assert _lib.lib().q4nx_kv4_attn_ws_bytes(c, 40, 0, 1, 1000, 0, 4) == 0
     assert _lib.lib().q4nx_kv4_select_ws_bytes(c, 1000) == 0
     assert _lib.lib().q4nx_kv4_pages_ws_bytes(c, 1) == 0
 
