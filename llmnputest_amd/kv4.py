@@ -77,6 +77,8 @@ class Kv4Cache:
         self.n_kv_heads, self.head_dim, self.page_len = n_kv_heads, head_dim, page_len
         self.max_len = self.table_len * page_len
         self.device = pool.device
+        self._index = pool.get_device()
+        self._lib = _lib.lib()
         self.status = torch.zeros(1, dtype=torch.int32, device=pool.device)
         self._layers = [_lib.Kv4(pool.data_ptr() + i * pool.stride(0), pool.stride(1), table.data_ptr(),
                                  table.stride(0), self.n_pages, page_len, n_kv_heads, head_dim,
@@ -88,7 +90,7 @@ class Kv4Cache:
         """The C view of a layer, and its sequences: those of `table` when one is given."""
         if not 0 <= layer < self.n_layers:
             raise IndexError(f"layer {layer} of {self.n_layers}")
-        if self.device.index != torch.cuda.current_device():
+        if self._index != torch.cuda.current_device():
             raise ValueError(f"the cache is on {self.device}, the current device is "
                              f"cuda:{torch.cuda.current_device()}")
         c = self._layers[layer]
@@ -103,16 +105,22 @@ class Kv4Cache:
         return v, v.n_seqs
 
     def _tensor(self, t: torch.Tensor, name: str, dtype) -> None:
-        if t.device != self.device:
+        if t.get_device() != self._index:
             raise ValueError(f"{name} must be on {self.device}, got {t.device}")
         if t.dtype != dtype:
             raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
 
     def _ints(self, t: torch.Tensor, name: str, n: int) -> int:
-        self._tensor(t, name, torch.int32)
-        if t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        if t.get_device() != self._index or t.dtype != torch.int32:
+            self._tensor(t, name, torch.int32)
+        if t.shape != (n,) or not t.is_contiguous():
             raise ValueError(f"{name} must be {n} contiguous values")
         return t.data_ptr()
+
+    def _call(self, name: str, *args) -> None:
+        rc = getattr(self._lib, name)(*args)
+        if rc:
+            _lib.check(rc)
 
     def _list(self, x, name: str) -> torch.Tensor:
         t = torch.as_tensor(x, dtype=torch.int32, device=self.device) if not torch.is_tensor(x) else x
@@ -127,13 +135,16 @@ class Kv4Cache:
             raise ValueError(f"{name} must be [rows, {heads}, {self.head_dim}], channels contiguous")
         return t
 
-    def _query(self, q: torch.Tensor) -> int:
-        self._tensor(q, "q", torch.bfloat16)
-        if q.dim() != 3 or q.shape[2] != self.head_dim or q.stride(2) != 1 \
-                or (q.shape[1] > 1 and q.stride(1) != self.head_dim):
+    def _query(self, q: torch.Tensor) -> tuple[int, int, int]:
+        """Rows, heads and row stride of q."""
+        if q.get_device() != self._index or q.dtype != torch.bfloat16:
+            self._tensor(q, "q", torch.bfloat16)
+        shape, stride = q.shape, q.stride()
+        if len(shape) != 3 or shape[2] != self.head_dim or stride[2] != 1 \
+                or (shape[1] > 1 and stride[1] != self.head_dim):
             raise ValueError(f"q must be [rows, Hq, {self.head_dim}], heads contiguous")
         # a single row's stride says nothing
-        return q.stride(0) if q.shape[0] > 1 else q.shape[1] * self.head_dim
+        return shape[0], shape[1], stride[0] if shape[0] > 1 else shape[1] * self.head_dim
 
     def _need(self, c, fn: str, *args) -> int:
         key = (fn, c.n_seqs, c.table_len, *args)
@@ -183,7 +194,7 @@ class Kv4Cache:
         self._call_append(c, k_cache, v_cache, 1, n, row, head, seq, pos, cu, max_new or n)
 
     def _call_append(self, c, k, v, by_position, rows, row, head, seq, pos, cu, max_new):
-        _lib.call("q4nx_kv4_append", c, k.data_ptr(), v.data_ptr(), by_position, rows, row, head, seq,
+        self._call("q4nx_kv4_append", c, k.data_ptr(), v.data_ptr(), by_position, rows, row, head, seq,
                   self._ints(pos, "pos", c.n_seqs),
                   None if cu is None else self._ints(cu, "cu", c.n_seqs + 1),
                   1 if cu is None else max_new, ops._stream())
@@ -201,9 +212,9 @@ class Kv4Cache:
         u = None if cu is None else self._ints(cu, "cu", b + 1)
         n = b if cu is None else int(cu[-1]) if total is None else total
         shape = (max(n, 0), self.n_kv_heads, self.head_dim)
-        k, v = torch.empty((2, *shape), dtype=dtype, device=self.device)
+        k, v = torch.empty((2, *shape), dtype=dtype, device=self.device).unbind(0)
         if n > 0:
-            _lib.call("q4nx_kv4_read", c, k.data_ptr(), v.data_ptr(), int(dtype == torch.float32), n, p,
+            self._call("q4nx_kv4_read", c, k.data_ptr(), v.data_ptr(), int(dtype == torch.float32), n, p,
                       u, 1 if cu is None else max_new or n, ops._stream())
         return k, v
 
@@ -221,14 +232,14 @@ class Kv4Cache:
         default D ** -0.5. sel: `select`'s pages, for one token per sequence. out: rows behind the
         last sequence are left as they are."""
         c, b = self._layer(layer, table)
-        stride = self._query(q)
-        n, hq, d = q.shape
+        n, hq, stride = self._query(q)
+        d = self.head_dim
         lp = self._ints(self.lens if lens is None else lens, "lens", b)
         u = None if cu is None else self._ints(cu, "cu", b + 1)
         if cu is None and n != b:
             raise ValueError(f"{n} rows for {b} sequences (give cu for other numbers of rows)")
         if out is None:
-            out = torch.empty((n, hq, d), dtype=torch.bfloat16, device=self.device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         else:
             self._tensor(out, "out", torch.bfloat16)
             if out.shape != q.shape or not out.is_contiguous():
@@ -246,10 +257,15 @@ class Kv4Cache:
         new = 1 if cu is None else max_new or n
         most = min(self.max_len if table is None else c.table_len * self.page_len, max_len or 1 << 30)
         need = self._need(c, "q4nx_kv4_attn_ws_bytes", hq, int(cu is not None), new, most, ns, n_split)
-        ws, wp, wn, stream = ops._scratch(ws, need)
-        _lib.call("q4nx_kv4_attn", c, q.data_ptr(), stride, out.data_ptr(), ops._ptr(of), hq, u, n, new,
-                  lp, most, d ** -0.5 if scale is None else float(scale), sp, ns, int(n_split), wp, wn,
-                  stream)
+        wp = wn = 0
+        if need:
+            ws, wp, wn, stream = ops._scratch(ws, need)
+        else:
+            stream = ops._stream()
+        self._call("q4nx_kv4_attn", c, q.data_ptr(), stride, out.data_ptr(),
+                   None if of is None else of.data_ptr(), hq, u, n, new, lp, most,
+                   d ** -0.5 if scale is None else float(scale), sp, ns, int(n_split), wp or None, wn,
+                   stream)
         return (out, of) if want_f32 else out
 
     def select(self, layer: int, q: torch.Tensor, lens: torch.Tensor | None = None, n_sel: int = 64,
@@ -260,9 +276,9 @@ class Kv4Cache:
         highest, int32 [n_seqs, Hkv, n_sel], ascending, -1 behind the last; the first n_first and the
         last n_last of a sequence are always among them."""
         c, b = self._layer(layer, table)
-        stride = self._query(q)
-        if q.shape[0] != b:
-            raise ValueError(f"{q.shape[0]} rows for {b} sequences")
+        n, hq, stride = self._query(q)
+        if n != b:
+            raise ValueError(f"{n} rows for {b} sequences")
         lp = self._ints(self.lens if lens is None else lens, "lens", b)
         if out is None:
             out = torch.empty((b, self.n_kv_heads, n_sel), dtype=torch.int32, device=self.device)
@@ -272,8 +288,8 @@ class Kv4Cache:
                 raise ValueError(f"out must be contiguous [{b}, {self.n_kv_heads}, {n_sel}]")
         most = min(self.max_len if table is None else c.table_len * self.page_len, max_len or 1 << 30)
         ws, wp, wn, stream = ops._scratch(ws, self._need(c, "q4nx_kv4_select_ws_bytes", most))
-        _lib.call("q4nx_kv4_select", c, q.data_ptr(), stride, q.shape[1], lp, most, n_sel, n_first,
-                  n_last, out.data_ptr(), wp, wn, stream)
+        self._call("q4nx_kv4_select", c, q.data_ptr(), stride, hq, lp, most, n_sel, n_first, n_last,
+                   out.data_ptr(), wp, wn, stream)
         return out
 
     # ------------------------------------------------------------ pages
@@ -289,7 +305,7 @@ class Kv4Cache:
         if want.shape[0] != self.n_seqs:
             raise ValueError(f"want needs {self.n_seqs} values")
         c, ws, wp, wn, stream = self._pages_ws(0, ws)
-        _lib.call("q4nx_kv4_reserve", c, self.refs.data_ptr(), want.data_ptr(), self.status.data_ptr(),
+        self._call("q4nx_kv4_reserve", c, self.refs.data_ptr(), want.data_ptr(), self.status.data_ptr(),
                   wp, wn, stream)
 
     def fork(self, src, dst, ws: ops.Workspace | None = None) -> None:
@@ -302,7 +318,7 @@ class Kv4Cache:
         if n == 0:
             return
         c, ws, wp, wn, stream = self._pages_ws(n, ws)
-        _lib.call("q4nx_kv4_fork", c, self.pool.stride(0), self.n_layers, self.lens.data_ptr(),
+        self._call("q4nx_kv4_fork", c, self.pool.stride(0), self.n_layers, self.lens.data_ptr(),
                   self.refs.data_ptr(), src.data_ptr(), dst.data_ptr(), n, self.status.data_ptr(), wp, wn,
                   stream)
 
@@ -315,7 +331,7 @@ class Kv4Cache:
         if n == 0:
             return
         c, _ = self._layer(0, None)
-        _lib.call("q4nx_kv4_free", c, self.lens.data_ptr(), self.refs.data_ptr(), seqs.data_ptr(), n,
+        self._call("q4nx_kv4_free", c, self.lens.data_ptr(), self.refs.data_ptr(), seqs.data_ptr(), n,
                   self.status.data_ptr(), ops._stream())
 
     def compact(self, ws: ops.Workspace | None = None) -> torch.Tensor:
@@ -323,7 +339,7 @@ class Kv4Cache:
         on the device (pages from there on are free)."""
         live = torch.empty(1, dtype=torch.int32, device=self.device)
         c, ws, wp, wn, stream = self._pages_ws(0, ws)
-        _lib.call("q4nx_kv4_compact", c, self.pool.stride(0), self.n_layers, self.refs.data_ptr(),
+        self._call("q4nx_kv4_compact", c, self.pool.stride(0), self.n_layers, self.refs.data_ptr(),
                   live.data_ptr(), wp, wn, stream)
         return live
 
@@ -336,5 +352,5 @@ class Kv4Cache:
         if src.shape[0] == 0:
             return
         c, _ = self._layer(0, None)
-        _lib.call("q4nx_kv4_copy_pages", c, self.pool.stride(0), self.n_layers, src.data_ptr(),
+        self._call("q4nx_kv4_copy_pages", c, self.pool.stride(0), self.n_layers, src.data_ptr(),
                   dst.data_ptr(), src.shape[0], ops._stream())
