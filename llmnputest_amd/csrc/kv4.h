@@ -26,6 +26,7 @@ struct Kv4 {
   int32_t* table;
   int64_t table_stride;
   int n_pages, page_len, tiles, hkv, n_seqs, table_len;
+  int shift;   // log2 of tiles, the tiles of a page
   int cap;   // positions a sequence can hold: table_len * page_len
 };
 

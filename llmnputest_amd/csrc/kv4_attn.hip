@@ -1,13 +1,13 @@
-// Attention over the paged 4-bit K/V cache, on the matrix cores.
+// Attention over the paged 4-bit K/V cache, on the matrix cores: single tokens (codes enter the products
+// as they are stored, bound by memory and the exponentials), and blocks of new tokens (tiles taken apart
+// once for 128 rows). Scores, their maxima and sums, and the outputs are fp32 until they are written.
 //
-// A query row is (new token i, query head of the group); 16 rows are the columns of every tile.
 // With x = d_g c + m_g per group g of 32 channels,
-//   S^T[pos][row]  = sum_g d_g[pos] (c . q)_g + m_g[pos] (sum of q)_g
-//   O^T[dim][row] += sum_pos (p d_g(dim))[pos] c[pos][dim] + sum_pos p m_g(dim)
-// so the codes enter the matrix cores as they are stored, as the bf16 numbers 128 + c (exact), and
-// the scales stay in fp32. The 128 is taken out again: the score's accumulator starts at
-// -128 (sum of q)_g, and m_g - 128 d_g takes m_g's place in the values. p d_g enters as two bf16 terms,
-// which carry it to 2^-18, so that a value is off by at most 143 2^-18 of its step.
+//   score = sum_g d_g (c . q)_g + m_g (sum of q)_g,    out = sum_pos p d_g c + sum_pos p m_g
+// so a code is an operand as it is, the bf16 number 128 + c (exact), and the scales stay in fp32. The
+// 128 is taken out again: a score's accumulator starts at -128 (sum of q)_g, and m_g - 128 d_g takes
+// m_g's place in the values. p d_g enters as two bf16 terms, which carry it to 2^-18, so that a value is
+// off by at most 143 2^-18 of its step.
 #include <math.h>
 
 #include "kv4.h"
@@ -23,7 +23,7 @@ struct Kv4AttnArgs {
   const int32_t* cu;
   const int32_t* lens;
   const int32_t* sel;
-  int n_sel, hq, group, total, row_tiles;
+  int n_sel, hq, group, total, row_tiles;   // row_tiles: row blocks per sequence
   int n_split, chunk;   // blocks: workgroups per row tile, tiles for each of them
   int unit;             // one token: tiles per part of a (sequence, kv head), 0: by what there is
   float scale_l2;
@@ -111,7 +111,7 @@ __device__ __forceinline__ void kv4_finish(const Kv4AttnArgs& a, float (*s_o)[RO
     for (int p0 = 0; p0 < parts; p0 += kMergeParts) {
       const int cnt = min(kMergeParts, parts - p0);
       uint4 x[KC][kMergeBatch];
-      auto fetch = [&](int k0) {
+      auto fetch = [&](int k0) __attribute__((always_inline)) {
 #pragma unroll
         for (int k = 0; k < KC; ++k) {
           const int c = min(c0_ + k * TH, cols - 1);
@@ -354,7 +354,7 @@ __global__ __launch_bounds__(256) void kv4_decode_kernel(Kv4AttnArgs a) {
     int id = 0, pos = 1 << 30;
     if (lane < count) {
       const int t = t0 + kWaves * (i0 + lane);
-      const int e = t / tpp, sub = t % tpp;
+      const int e = t >> a.c.shift, sub = t & (tpp - 1);
       const int lp = a.sel ? a.sel[(int64_t)item * a.n_sel + e] : e;
       if (lp >= 0 && lp < a.c.table_len) {
         id = kv4_page(a.c, b, lp) * 4 + sub;   // negative: no page
@@ -362,7 +362,7 @@ __global__ __launch_bounds__(256) void kv4_decode_kernel(Kv4AttnArgs a) {
       }
     }
     Kv4TileRegs<NG> buf[PF];
-    auto load = [&](Kv4TileRegs<NG>& r, int i) {
+    auto load = [&](Kv4TileRegs<NG>& r, int i) __attribute__((always_inline)) {
       const int x = __builtin_amdgcn_readlane(id, i);
       const uint8_t* tile = a.c.pages + (int64_t)(x < 0 ? 0 : x >> 2) * a.c.page_stride + head_off +
                             (x < 0 ? 0 : x & 3) * kv4_tile_bytes(D);
@@ -381,7 +381,7 @@ __global__ __launch_bounds__(256) void kv4_decode_kernel(Kv4AttnArgs a) {
         for (int g = 0; g < 4; ++g) r.s[g] = s[g];
       }
     };
-    auto compute = [&](const Kv4TileRegs<NG>& r, int i0_) {
+    auto compute = [&](const Kv4TileRegs<NG>& r, int i0_) __attribute__((always_inline)) {
       const int base = __builtin_amdgcn_readlane(pos, i0_);
       const bool none = __builtin_amdgcn_readlane(id, i0_) < 0;
       const bool part = base + kKv4Tile > end || none;
@@ -540,176 +540,384 @@ __global__ __launch_bounds__(256) void kv4_decode_kernel(Kv4AttnArgs a) {
   }
 }
 
+// Blocks of new tokens. A workgroup has RB = 16 CT NW query rows (token, head of the group) of one
+// (sequence, kv head), a wave CT tiles of 16; all of them share each tile of the cache, which the waves
+// take apart together, once, into operands in LDS:
+//   K = (d c + m) scale log2(e) and V = d c + m, each as two bf16 terms (2^-18 of the value)
+//   S^T[pos][row] = K . Q^T - reference,  O^T[dim][row] += V^T . P^T with P as two terms (hi hi, lo hi,
+//   hi lo: 20 products of 16 x 16 x 32 for 32 positions, 16 rows and D = 64)
+// The reference is the accumulator's start, so an exponential is one instruction a score. A score tile's
+// lanes hold rows as columns and positions 4 kg + e and 16 + 4 kg + e, the order of V's operand, so P
+// goes from registers to registers. While a tile is computed the next one's bytes are on their way, and
+// its operands are written to the other buffer: one barrier a tile.
+// The exponentials and the splitting of P bound it (60 instruction slots a product pair against 20 x 4
+// of the matrix cores, and taking the tile apart).
+// Poison: in tiles that some rows do not see, V's groups of NaN are left out of the product (0 times
+// NaN) and given to the rows that see them.
+template <int D>
+constexpr int kv4_block_waves() { return 4; }
+constexpr int kBlockCt = 2;   // at 4 long prompts take 2 % less, short ones 40 % more
+template <int D>
+constexpr int kv4_block_rows() { return 16 * kBlockCt * kv4_block_waves<D>(); }
+
 template <int NG>
-__global__ __launch_bounds__(256) void kv4_block_kernel(Kv4AttnArgs a) {
-  constexpr int D = 32 * NG, C = D / 64, NT = D / 16;
-  __shared__ __attribute__((aligned(16))) float s_o[kWaves][16][D + 4];
-  __shared__ __attribute__((aligned(16))) float s_fin[16][D + 4];
+__global__ __launch_bounds__(64 * kv4_block_waves<32 * NG>()) void kv4_block_kernel(Kv4AttnArgs a) {
+  constexpr int D = 32 * NG, NT = D / 16, CT = kBlockCt, NW = kv4_block_waves<D>();
+  constexpr int RB = 16 * CT * NW, REC = D + 4, C = NG / 2, KJ = 2 * NG;
+  static_assert(NW == 4 && CT == 2, "a wave takes one dword of four; its row tiles are 2, 1 or 0");
+  __shared__ __attribute__((aligned(16))) u32x4_t s_op[2][4 * NG][2][64];   // [buffer][K, V dwords][term][lane]
+  __shared__ uint32_t s_bad[2][NG];
   __shared__ int s_last;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, kg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int split = blockIdx.x % a.n_split;
-  const int bk = blockIdx.x / a.n_split;        // (b * hkv + h) * row_tiles + rt
-  const int rt = bk % a.row_tiles;
-  const int h = (bk / a.row_tiles) % a.c.hkv;
-  const int b = bk / a.row_tiles / a.c.hkv;
-  int c0 = b, nq = 1;
-  if (a.cu) {
-    c0 = a.cu[b];
-    nq = a.cu[b + 1] - c0;
-    if (c0 < 0 || nq < 0) nq = 0;
-    nq = min(nq, a.total - c0);
-  }
-  const int rows = nq * a.group;
-  if (rt * 16 >= rows) return;   // uniform, and in every split of it
-  const int row = rt * 16 + n;
-  const bool live = row < rows;
-  const int tok = live ? row / a.group : 0, qh = live ? row % a.group : 0;
-  const int end = live ? max(0, min(a.lens[b] - nq + tok + 1, a.c.cap)) : 0;   // positions this row sees
-  const int top = max(0, min(a.lens[b] - nq + min(rt * 16 + 15, rows - 1) / a.group + 1, a.c.cap));
-
+  // the rows that see most first
+  int x = blockIdx.x;
+  const int split = x % a.n_split;
+  x /= a.n_split;
+  const int h = x % a.c.hkv;
+  x /= a.c.hkv;
+  const int b = x % a.c.n_seqs, rb = a.row_tiles - 1 - x / a.c.n_seqs;
+  const int c0 = a.cu[b];
+  int nq = a.cu[b + 1] - c0;
+  if (c0 < 0 || nq < 0) nq = 0;
+  nq = min(nq, a.total - c0);
+  const int rows = nq * a.group, row0 = rb * RB;
+  if (row0 >= rows) return;   // uniform, and in every split of it
+  const int first_tok = row0 / a.group, last_tok = (min(row0 + RB, rows) - 1) / a.group;
+  auto sees = [&](int tok) { return max(0, min(a.lens[b] - nq + tok + 1, a.c.cap)); };
+  const int top = sees(last_tok), all_see = sees(first_tok);
   const int nt = (top + kKv4Tile - 1) / kKv4Tile;
   const int parts = max(1, (nt + a.chunk - 1) / a.chunk);
   if (split >= parts) return;
+  const int t_begin = split * a.chunk, t_end = min(nt, (split + 1) * a.chunk);
 
-  // q, and its sums by group
-  u32x4_t q[NG];
-  float qs[NG];
-  {
+  u32x4_t q[CT][NG];
+  int end[CT], tiles_w = 0;   // positions a row sees; this wave's tiles of rows
+#pragma unroll
+  for (int c = 0; c < CT; ++c) {
+    const int r0 = row0 + (c * NW + wave) * 16, row = r0 + n;
+    if (r0 < rows) tiles_w = c + 1;
+    const bool live = row < rows;
+    const int tok = live ? row / a.group : 0, qh = live ? row % a.group : 0;
+    end[c] = live ? sees(tok) : 0;
     const uint16_t* p = a.q + (int64_t)(c0 + tok) * a.q_stride + (h * a.group + qh) * D + 8 * kg;
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      q[g] = live ? *(const u32x4_t*)(p + 32 * g) : u32x4_t{0, 0, 0, 0};
-      float s = 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s += bf16lo(q[g][i]) + bf16hi(q[g][i]);
-      qs[g] = xor32_sum(xor16_sum(s));
+      q[c][g] = *(const u32x4_t*)(p + 32 * g);
+      if (!live) q[c][g] = u32x4_t{0, 0, 0, 0};
     }
   }
-  f32x4_t o[NT], off[NG];
-  float ms[NG], m = -INFINITY, l = 0.f;
+  f32x4_t o[CT][NT], nref[CT];   // the negative reference, four times; 0 while there is none
+  int lim[CT];                   // the word of 8, what a score may pass it by; while there is none, the least
+  float l[CT];
+  constexpr int kLimit = 0x41000000;
 #pragma unroll
-  for (int u = 0; u < NT; ++u) o[u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int c = 0; c < CT; ++c) {
+    nref[c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    lim[c] = INT32_MIN;
+    l[c] = 0.f;
 #pragma unroll
-  for (int g = 0; g < NG; ++g) {
-    off[g] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    ms[g] = 0.f;
+    for (int u = 0; u < NT; ++u) o[c][u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
-  const u32x4_t minus = {0xC300C300u, 0xC300C300u, 0xC300C300u, 0xC300C300u};
+  const Kv4Minus neg;
 
-  const int tpp = a.c.tiles;
-  const int t_end = min(nt, (split + 1) * a.chunk);
-  for (int t = split * a.chunk + wave; t < t_end; t += kWaves) {
-    const int e = t / tpp, sub = t % tpp;
-    const int base = t * kKv4Tile;
-    const int id = kv4_page(a.c, b, e);
+  // ---- taking a tile apart: dword `wave` of every lane's four of K and of V
+  const int ktt = wave >> 1, kgg = wave & 1;
+  uint32_t kc[C], ks[C], vc[C], vs[C][8];
+  int id_now = 0, id_next = 0;
+  auto page = [&](int t) __attribute__((always_inline)) { return kv4_page(a.c, b, t >> a.c.shift); };
+  auto fetch = [&](int t, int id) __attribute__((always_inline)) {
     const uint8_t* tile = a.c.pages + (int64_t)max(id, 0) * a.c.page_stride +
-                          (int64_t)h * kv4_head_bytes(a.c.page_len, D) + sub * kv4_tile_bytes(D);
-    u32x4_t kc[C], vc[C];
+                          (int64_t)h * kv4_head_bytes(a.c.page_len, D) +
+                          (t & (a.c.tiles - 1)) * kv4_tile_bytes(D);
+    const uint8_t* pc = tile + lane * 16 + wave * 4;
+    const uint8_t* pk = tile + 32 * D + ((16 * ktt + n) * NG + kgg) * 4;
+    const uint8_t* pv = tile + 32 * D + 128 * NG + kg * 16 * NG + (wave >> 1) * 4;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      kc[c] = *(const u32x4_t*)(tile + (c * 64 + lane) * 16);
-      vc[c] = *(const u32x4_t*)(tile + 16 * D + (c * 64 + lane) * 16);
+      kc[c] = *(const uint32_t*)(pc + c * 1024);
+      vc[c] = *(const uint32_t*)(pc + 16 * D + c * 1024);
+      ks[c] = *(const uint32_t*)(pk + c * 8);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        vs[c][e] = *(const uint32_t*)(pv + c * 8 + (16 * (e >> 2) + (e & 3)) * NG * 4);
     }
-    uint32_t ks[2][4][NG], vs[2][4][NG];
+  };
+  // x as two bf16 terms, pairs (x0, x1)
+  auto split2 = [&](float x0, float x1, uint32_t& hi, uint32_t& lo) __attribute__((always_inline)) {
+    hi = pack_bf16x2_op(x0, x1);
+    lo = pack_bf16x2_op(Kv4Minus::dot(x0, hi, neg.lo), Kv4Minus::dot(x1, hi, neg.hi));
+  };
+  auto spread = [&](int t, int id, int buf) __attribute__((always_inline)) {
+    const bool part = (t + 1) * kKv4Tile > all_see;
+    if (id < 0) {
 #pragma unroll
-    for (int tt = 0; tt < 2; ++tt)
+      for (int c = 0; c < C; ++c) {
+        ks[c] = kKv4NaN;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+        for (int e = 0; e < 8; ++e) vs[c][e] = kKv4NaN;
+      }
+    }
+    if (part) {
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          const int at = ((16 * tt + 4 * kg + i) * NG + g) * 4;
-          ks[tt][i][g] = *(const uint32_t*)(tile + 32 * D + at);
-          vs[tt][i][g] = *(const uint32_t*)(tile + 32 * D + 128 * NG + at);
-          if (id < 0) ks[tt][i][g] = kKv4NaN;
+      for (int c = 0; c < C; ++c) {
+        uint32_t bad = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int p = 16 * (e >> 2) + 4 * kg + (e & 3);
+          const float y = bf16lo(vs[c][e]) + bf16hi(vs[c][e]);
+          // a position that no row sees may hold anything (the page's older bytes)
+          const bool out = t * kKv4Tile + p >= top, nan = !(fabsf(y) < INFINITY);
+          if (!out && nan) bad |= 1u << p;
+          if (out || nan) vs[c][e] = 0u;
         }
-    float s[2][4];
-    bool ok[2][4];
-#pragma unroll
-    for (int tt = 0; tt < 2; ++tt) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[tt][i] = 0.f;
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        const float z = -128.f * qs[g];
-        const f32x4_t r = mfma_bf16(kv4_operand(kc[g >> 1][2 * tt + (g & 1)]), q[g], f32x4_t{z, z, z, z});
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          s[tt][i] += bf16lo(ks[tt][i][g]) * r[i] + bf16hi(ks[tt][i][g]) * qs[g];
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        ok[tt][i] = base + 16 * tt + 4 * kg + i < end;
-        s[tt][i] = ok[tt][i] ? s[tt][i] * a.scale_l2 : -INFINITY;
+        bad |= (uint32_t)__shfl_xor((int)bad, 16);
+        bad |= (uint32_t)__shfl_xor((int)bad, 32);
+        if (lane == 0 && (wave & 1) == 0) s_bad[buf][2 * c + (wave >> 1)] = bad;
       }
     }
-    float mr = s[0][0];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) mr = fmaxf(mr, s[i >> 2][i & 3]);
-    mr = xor32_max(xor16_max(mr));
-    const float mn = fmaxf(m, mr);
-    const float mb = mn == -INFINITY ? 0.f : mn;
-    const float corr = ex2(m - mb);
-    m = mn;
-    l *= corr;
-#pragma unroll
-    for (int u = 0; u < NT; ++u) o[u] *= corr;
-    float p[2][4];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      p[i >> 2][i & 3] = ex2(s[i >> 2][i & 3] - mb);
-      l += p[i >> 2][i & 3];
-    }
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      ms[g] *= corr;
-      off[g] *= corr;
+    for (int c = 0; c < C; ++c) {
+      const float d = bf16lo(ks[c]) * a.scale_l2, m = bf16hi(ks[c]) * a.scale_l2;
       u32x4_t hi, lo;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        // a masked position's scale may be anything (the page's older bytes): not 0 * NaN
-        const float x0 = ok[0][i] ? p[0][i] * bf16lo(vs[0][i][g]) : 0.f;
-        const float x1 = ok[1][i] ? p[1][i] * bf16lo(vs[1][i][g]) : 0.f;
-        ms[g] += ok[0][i] ? p[0][i] * bf16hi(vs[0][i][g]) : 0.f;
-        ms[g] += ok[1][i] ? p[1][i] * bf16hi(vs[1][i][g]) : 0.f;
-        hi[i] = pack_bf16x2_op(x0, x1);
-        lo[i] = pack_bf16x2_op(x0 - bf16lo(hi[i]), x1 - bf16hi(hi[i]));
+      for (int r = 0; r < 4; ++r) {
+        uint32_t y0, y1;
+        split2(fmaf((float)((kc[c] >> (4 * r)) & 15u), d, m),
+               fmaf((float)((kc[c] >> (4 * r + 16)) & 15u), d, m), y0, y1);
+        hi[r] = y0;
+        lo[r] = y1;
       }
-      off[g] = mfma_bf16(minus, hi, off[g]);
-      off[g] = mfma_bf16(minus, lo, off[g]);
+      s_op[buf][4 * c + wave][0][lane] = hi;
+      s_op[buf][4 * c + wave][1][lane] = lo;
 #pragma unroll
-      for (int u = 2 * g; u < 2 * g + 2; ++u) {
-        const u32x4_t v = kv4_operand(vc[u >> 2][u & 3]);
-        o[u] = mfma_bf16(v, hi, o[u]);
-        o[u] = mfma_bf16(v, lo, o[u]);
+      for (int r = 0; r < 4; ++r) {
+        uint32_t y0, y1;
+        split2(fmaf((float)((vc[c] >> (4 * r)) & 15u), bf16lo(vs[c][r]), bf16hi(vs[c][r])),
+               fmaf((float)((vc[c] >> (4 * r + 16)) & 15u), bf16lo(vs[c][4 + r]), bf16hi(vs[c][4 + r])),
+               y0, y1);
+        hi[r] = y0;
+        lo[r] = y1;
+      }
+      s_op[buf][KJ + 4 * c + wave][0][lane] = hi;
+      s_op[buf][KJ + 4 * c + wave][1][lane] = lo;
+    }
+  };
+  // one tile for the first N of this wave's row tiles; part: some rows do not see all of it (the empty
+  // asm keeps what follows from being done for every tile and selected)
+  auto compute = [&](auto n_tiles, int t, int buf) __attribute__((always_inline)) {
+    constexpr int N = decltype(n_tiles)::value;
+    const int base = t * kKv4Tile;
+    const bool part = base + kKv4Tile > all_see;
+    f32x4_t s[N][2];
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt) {
+        const int j = 4 * (g >> 1) + 2 * tt + (g & 1);
+        const u32x4_t hi = s_op[buf][j][0][lane], lo = s_op[buf][j][1][lane];
+#pragma unroll
+        for (int c = 0; c < N; ++c) s[c][tt] = mfma_bf16(hi, q[c][g], g == 0 ? nref[c] : s[c][tt]);
+#pragma unroll
+        for (int c = 0; c < N; ++c) s[c][tt] = mfma_bf16(lo, q[c][g], s[c][tt]);
+      }
+    if (part) {
+      asm volatile("");
+#pragma unroll
+      for (int c = 0; c < N; ++c)
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (base + 16 * tt + 4 * kg + e >= end[c]) s[c][tt][e] = -INFINITY;
+    }
+    // The reference moves only when a score has passed it by 2^8: sums stay far from overflow. As signed
+    // words, floats compare alike where one is positive, which is all that is asked here (a NaN's word is
+    // greater than any), and take no canonicalising step.
+    bool move = false;
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      int y = __float_as_int(s[c][0][0]);
+#pragma unroll
+      for (int e = 1; e < 8; ++e) y = max(y, __float_as_int(s[c][e >> 2][e & 3]));
+      move |= y > lim[c];
+    }
+    if (__any(move)) {
+#pragma unroll
+      for (int c = 0; c < N; ++c) {
+        float y = s[c][0][0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) y = fmaxf(y, s[c][e >> 2][e & 3]);
+        y = xor32_max(xor16_max(y));
+        const bool first = lim[c] != kLimit, now = y > (first ? -INFINITY : 0.f);
+        const float by = now ? y : 0.f, f = now && first ? 0.f : ex2(-by);
+        if (now) lim[c] = kLimit;
+        l[c] *= f;
+#pragma unroll
+        for (int u = 0; u < NT; ++u) o[c][u] *= f;
+        nref[c] -= by;
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) s[c][tt] -= by;
       }
     }
-  }
+    u32x4_t ph[N], pl[N];
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float p0 = ex2(s[c][0][e]), p1 = ex2(s[c][1][e]);
+        l[c] += p0 + p1;
+        uint32_t y0, y1;
+        split2(p0, p1, y0, y1);
+        ph[c][e] = y0;
+        pl[c][e] = y1;
+      }
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      const u32x4_t hi = s_op[buf][KJ + u][0][lane], lo = s_op[buf][KJ + u][1][lane];
+#pragma unroll
+      for (int c = 0; c < N; ++c) o[c][u] = mfma_bf16(hi, ph[c], o[c][u]);
+#pragma unroll
+      for (int c = 0; c < N; ++c) o[c][u] = mfma_bf16(hi, pl[c], o[c][u]);
+#pragma unroll
+      for (int c = 0; c < N; ++c) o[c][u] = mfma_bf16(lo, ph[c], o[c][u]);
+    }
+    if (part) {
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const uint32_t bad = s_bad[buf][g];
+        if (bad == 0) continue;
+#pragma unroll
+        for (int c = 0; c < N; ++c) {
+          // the row's positions of this tile are the first end - base
+          const int k = end[c] - base;
+          const uint32_t mine = k >= 32 ? bad : k <= 0 ? 0u : bad & ((1u << k) - 1u);
+          if (mine) {
+#pragma unroll
+            for (int u = 2 * g; u < 2 * g + 2; ++u) o[c][u] += NAN;
+          }
+        }
+      }
+    }
+  };
 
-  // ---- the waves' states through LDS: s_o[wave][row][dim], m and l behind the dims
-  l = xor32_sum(xor16_sum(l));
-#pragma unroll
-  for (int g = 0; g < NG; ++g) ms[g] = xor32_sum(xor16_sum(ms[g]));
-#pragma unroll
-  for (int u = 0; u < NT; ++u)
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      s_o[wave][n][16 * u + 4 * kg + i] = o[u][i] + off[u >> 1][i] + ms[u >> 1];
-  if (kg == 0) {
-    s_o[wave][n][D] = m;
-    s_o[wave][n][D + 1] = l;
+  if (t_begin < t_end) {
+    id_now = page(t_begin);
+    fetch(t_begin, id_now);
+    id_next = page(min(t_begin + 1, t_end - 1));
+    spread(t_begin, id_now, 0);
   }
-  kv4_finish<D, 256, kWaves, 16>(a, s_o, s_fin, &s_last, bk, split, parts,
-                                [&](int p) { return bk * a.n_split + p; }, min(16, rows - rt * 16), c0, rt * 16, h);
+  __syncthreads();
+  auto run = [&](auto n_tiles) __attribute__((always_inline)) {
+    for (int t = t_begin; t < t_end; ++t) {
+      const int buf = (t - t_begin) & 1;
+      id_now = id_next;
+      fetch(min(t + 1, t_end - 1), id_now);
+      id_next = page(min(t + 2, t_end - 1));
+      if constexpr (decltype(n_tiles)::value > 0) compute(n_tiles, t, buf);
+      if (t + 1 < t_end) spread(t + 1, id_now, buf ^ 1);
+      __syncthreads();
+    }
+  };
+  if (tiles_w == 2) run(std::integral_constant<int, 2>{});
+  else if (tiles_w == 1) run(std::integral_constant<int, 1>{});
+  else run(std::integral_constant<int, 0>{});
+
+  // ---- rows out: a lane has four channels of its row in each o[u]
+#pragma unroll
+  for (int c = 0; c < CT; ++c) l[c] = xor32_sum(xor16_sum(l[c]));
+  if (parts == 1) {
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+      const int row = row0 + (c * NW + wave) * 16 + n;
+      if (row >= rows) continue;
+      const int64_t at = ((int64_t)(c0 + row / a.group) * a.hq + h * a.group + row % a.group) * D + 4 * kg;
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = l[c] == 0.f ? 0.f : attn_div(o[c][u][e], l[c]);
+        if (a.out)
+          *(uint2*)(a.out + at + 16 * u) = make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
+        if (a.out_f32) *(float4*)(a.out_f32 + at + 16 * u) = make_float4(y[0], y[1], y[2], y[3]);
+      }
+    }
+    return;
+  }
+  const int item = blockIdx.x / a.n_split;
+  const __amdgpu_buffer_rsrc_t pr = make_rsrc(a.partial, a.partial_bytes);
+  const uint32_t rec0 = (uint32_t)item * a.n_split * (RB * REC * 4);
+#pragma unroll
+  for (int c = 0; c < CT; ++c) {
+    const int r = (c * NW + wave) * 16 + n;
+    if (row0 + r >= rows) continue;
+    const uint32_t at = rec0 + (uint32_t)(split * RB + r) * (REC * 4);
+#pragma unroll
+    for (int u = 0; u < NT; ++u)
+      st16_sys(pr, at + (16 * u + 4 * kg) * 4,
+               make_uint4(__float_as_uint(o[c][u][0]), __float_as_uint(o[c][u][1]),
+                          __float_as_uint(o[c][u][2]), __float_as_uint(o[c][u][3])));
+    if (kg == 0)
+      st16_sys(pr, at + D * 4, make_uint4(__float_as_uint(lim[c] != kLimit ? -INFINITY : -nref[c][0]),
+                                          __float_as_uint(l[c]), 0u, 0u));
+  }
+  wait_vm();
+  __syncthreads();
+  if (tid == 0) s_last = ticket(&a.counters[item], parts) ? 1 : 0;
+  __syncthreads();
+  if (!s_last) return;
+  for (int e = tid; e < min(RB, rows - row0) * (D / 4); e += 64 * NW) {
+    const int r = e / (D / 4), d = e % (D / 4) * 4;
+    float M = -INFINITY, L = 0.f;
+    float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p0 = 0; p0 < parts; p0 += 4) {
+      uint4 v[4], ml[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t at = rec0 + (uint32_t)(min(p0 + i, parts - 1) * RB + r) * (REC * 4);
+        v[i] = ld16_sys(pr, at + d * 4);
+        ml[i] = ld16_sys(pr, at + D * 4);
+      }
+      float Mn = M;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) Mn = fmaxf(Mn, __uint_as_float(ml[i].x));
+      const float Mb = Mn == -INFINITY ? 0.f : Mn, f = ex2(M - Mb);
+      L *= f;
+      A.x *= f;
+      A.y *= f;
+      A.z *= f;
+      A.w *= f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (p0 + i < parts) {
+          const float g = ex2(__uint_as_float(ml[i].x) - Mb);
+          L = fmaf(__uint_as_float(ml[i].y), g, L);
+          A.x = fmaf(__uint_as_float(v[i].x), g, A.x);
+          A.y = fmaf(__uint_as_float(v[i].y), g, A.y);
+          A.z = fmaf(__uint_as_float(v[i].z), g, A.z);
+          A.w = fmaf(__uint_as_float(v[i].w), g, A.w);
+        }
+      M = Mn;
+    }
+    float y[4] = {A.x, A.y, A.z, A.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = L == 0.f ? 0.f : attn_div(y[i], L);
+    const int row = row0 + r;
+    const int64_t at = ((int64_t)(c0 + row / a.group) * a.hq + h * a.group + row % a.group) * D + d;
+    if (a.out) *(uint2*)(a.out + at) = make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
+    if (a.out_f32) *(float4*)(a.out_f32 + at) = make_float4(y[0], y[1], y[2], y[3]);
+  }
 }
 
-static int kv4_row_tiles(int max_new, int group) { return (int)(((int64_t)max_new * group + 15) / 16); }
-
-// Splits per row tile, by the positions a sequence may have.
-static int kv4_auto_split(int64_t items, int tiles) {
-  int64_t s = 1024 / (items < 1 ? 1 : items);
-  const int64_t by_len = (tiles + 2 * kWaves - 1) / (2 * kWaves);
-  s = s < by_len ? s : by_len;
+// Row blocks of a sequence, and workgroups that share one: enough of them to fill the chip, eight tiles
+// each at least.
+static int kv4_row_blocks(int max_new, int group, int d) {
+  const int rb = d == 64 ? kv4_block_rows<64>() : kv4_block_rows<128>();
+  return (int)(((int64_t)max_new * group + rb - 1) / rb);
+}
+static int kv4_block_split(int64_t items, int tiles) {
+  int64_t s = 768 / (items < 1 ? 1 : items);
+  s = s < tiles / 8 ? s : tiles / 8;
   return (int)(s < 1 ? 1 : (s > 64 ? 64 : s));
 }
 
@@ -729,8 +937,9 @@ static Kv4Plan kv4_plan(const q4nx_kv4* c, int n_q_heads, bool block, int max_ne
   int64_t recs;
   int rows = 16;
   if (block) {
-    p.items = (int64_t)c->n_seqs * c->n_kv_heads * kv4_row_tiles(max_new, group);
-    const int want = n_split > 0 ? n_split : kv4_auto_split(p.items, tiles);
+    p.items = (int64_t)c->n_seqs * c->n_kv_heads * kv4_row_blocks(max_new, group, c->head_dim);
+    rows = c->head_dim == 64 ? kv4_block_rows<64>() : kv4_block_rows<128>();
+    const int want = n_split > 0 ? n_split : kv4_block_split(p.items, tiles);
     p.chunk = (tiles + want - 1) / want;
     p.n_split = (tiles + p.chunk - 1) / p.chunk;   // every split has work at the longest length
     p.grid = recs = p.items * p.n_split;
@@ -797,7 +1006,8 @@ int q4nx_kv4_attn(const q4nx_kv4* cache, const uint16_t* q, int64_t q_stride, ui
                "%s: q_stride=%lld must hold Hq * D and be a multiple of 8", what, (long long)q_stride);
   const Kv4Plan p = kv4_plan(cache, n_q_heads, cu != nullptr, max_new, max_len, n_sel, n_split);
   const int64_t longest = n_sel ? (int64_t)n_sel * cache->page_len : max_len;
-  Q4NX_REQUIRE(p.grid <= (int64_t)1 << 30 && p.items * (longest / kKv4Tile + 1) < (int64_t)1 << 31,
+  Q4NX_REQUIRE(p.grid <= (int64_t)1 << 30 &&
+                   (cu != nullptr || p.items * (longest / kKv4Tile + 1) < (int64_t)1 << 31),
                Q4NX_ERR_SHAPE, "%s: %lld rows of up to %lld positions", what, (long long)p.items,
                (long long)longest);
   if (p.shared) {
@@ -822,7 +1032,7 @@ int q4nx_kv4_attn(const q4nx_kv4* cache, const uint16_t* q, int64_t q_stride, ui
   a.hq = n_q_heads;
   a.group = n_q_heads / cache->n_kv_heads;
   a.total = total;
-  a.row_tiles = kv4_row_tiles(max_new, a.group);
+  a.row_tiles = kv4_row_blocks(max_new, a.group, cache->head_dim);
   a.n_split = p.n_split;
   a.chunk = p.chunk;
   a.unit = p.unit;
@@ -840,8 +1050,8 @@ int q4nx_kv4_attn(const q4nx_kv4* cache, const uint16_t* q, int64_t q_stride, ui
       default: d64 ? run(kv4_decode_kernel<2, 4>) : run(kv4_decode_kernel<4, 4>); break;
     }
   }
-  else if (d64) hipLaunchKernelGGL(kv4_block_kernel<2>, grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL(kv4_block_kernel<4>, grid, dim3(256), 0, s, a);
+  else if (d64) hipLaunchKernelGGL(kv4_block_kernel<2>, grid, dim3(64 * kv4_block_waves<64>()), 0, s, a);
+  else hipLaunchKernelGGL(kv4_block_kernel<4>, grid, dim3(64 * kv4_block_waves<128>()), 0, s, a);
   return check_launch(what);
 }
 
