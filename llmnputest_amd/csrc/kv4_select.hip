@@ -21,10 +21,18 @@ struct Kv4SelArgs {
   unsigned* counters;
 };
 
-constexpr int kSelPages = 64;   // pages scored by a workgroup
+// Pages scored by a workgroup, and its threads, all of which work on the list in the last one to arrive.
+// 2048 pages, one sequence (8 kv heads): 14.0 us; 64 pages and 256 threads 16.6, 64 and 512 14.7, 128 and
+// 1024 15.6. Eight sequences of up to 938 pages: 15.7, against 15.4, 17.5 and 20.0 us. The bounds of
+// scattered pages are what takes long: 64 pages in all take 6.3 us.
+constexpr int kSelPages = 128;
+constexpr int kSelThreads = 512;
+constexpr int kSelWaves = kSelThreads / 64;
 
+// Keys from here on: a NaN score (its page is read, so that it shows), above it the pages always read.
+constexpr unsigned long long kSpecial = ~1ull;
 __device__ __forceinline__ unsigned long long f64_key(double x) {
-  if (x != x) return ~1ull;   // a NaN's page is read, so that it shows; those always read are ~0
+  if (x != x) return kSpecial;
   const unsigned long long u = (unsigned long long)__double_as_longlong(x);
   return (u >> 63) ? ~u : (u | 0x8000000000000000ull);
 }
@@ -34,33 +42,12 @@ __device__ __forceinline__ unsigned long long load_sys64(const unsigned long lon
                            __HIP_MEMORY_SCOPE_SYSTEM);
 }
 
-// Sum over the 256 threads of the values before this one's, and of all.
-__device__ __forceinline__ int scan256(int v, int* s_scan, int* total) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  int x = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(x, o);
-    if (lane >= o) x += y;
-  }
-  __syncthreads();
-  if (lane == 63) s_scan[wave] = x;
-  __syncthreads();
-  int before = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    if (w < wave) before += s_scan[w];
-    all += s_scan[w];
-  }
-  *total = all;
-  return before + x - v;
-}
-
 template <int NG>
-__global__ __launch_bounds__(256) void kv4_select_kernel(Kv4SelArgs a) {
+__global__ __launch_bounds__(kSelThreads) void kv4_select_kernel(Kv4SelArgs a) {
   constexpr int D = 32 * NG, L = D / 4, PW = 64 / L;   // lanes per page, pages per wave step
   extern __shared__ unsigned long long s_key[];
-  __shared__ int s_hist[256], s_scan[4], s_pick[2];
+  __shared__ int s_hist[256], s_pick[3], s_count[kSelWaves][2], s_special[kSelWaves];
+  __shared__ unsigned long long s_range[kSelWaves][2], s_out[kSelPages];
   __shared__ int s_last;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -76,35 +63,57 @@ __global__ __launch_bounds__(256) void kv4_select_kernel(Kv4SelArgs a) {
   const int ch = (sub % (L / 2)) * 8;
   if (part * kSelPages < np) {
     double w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    for (int g = 0; g < a.group; ++g) {
-      const u32x4_t x = *(const u32x4_t*)(a.q + (int64_t)b * a.q_stride + (h * a.group + g) * D + ch);
+    constexpr int HEADS = 8;   // loads in flight
+    for (int g0 = 0; g0 < a.group; g0 += HEADS) {
+      u32x4_t y[HEADS];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float f = (i & 1) ? bf16hi(x[i >> 1]) : bf16lo(x[i >> 1]);
-        if (f != f || (f > 0.f) == high) w[i] += (double)f;   // a zero adds nothing to either
+      for (int g = 0; g < HEADS; ++g)
+        y[g] = *(const u32x4_t*)(a.q + (int64_t)b * a.q_stride +
+                                 (h * a.group + min(g0 + g, a.group - 1)) * D + ch);
+#pragma unroll
+      for (int g = 0; g < HEADS; ++g) {
+        if (g0 + g >= a.group) break;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float f = (i & 1) ? bf16hi(y[g][i >> 1]) : bf16lo(y[g][i >> 1]);
+          if (f != f || (f > 0.f) == high) w[i] += (double)f;   // a zero adds nothing to either
+        }
       }
     }
-    for (int p = part * kSelPages + wave * PW + lane / L; p < (part + 1) * kSelPages; p += 4 * PW) {
-      double s = 0;
-      const int id = p < np ? kv4_page(a.c, b, p) : -1;
-      if (id >= 0) {
-        const uint8_t* at = a.c.pages + (int64_t)id * a.c.page_stride +
-                            (int64_t)h * kv4_head_bytes(a.c.page_len, D) +
-                            a.c.tiles * kv4_tile_bytes(D) + sub * 16;
-        const u32x4_t x = *(const u32x4_t*)at;
+    constexpr int STEPS = kSelPages / (kSelWaves * PW);
+    const int p0 = part * kSelPages + wave * PW + lane / L;
+    int id[STEPS];
+    u32x4_t x[STEPS];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          s = fma(w[i], (double)((i & 1) ? bf16hi(x[i >> 1]) : bf16lo(x[i >> 1])), s);
-      }
+    for (int i = 0; i < STEPS; ++i) {
+      const int p = p0 + kSelWaves * PW * i;
+      id[i] = p < np ? kv4_page(a.c, b, p) : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i)
+      x[i] = *(const u32x4_t*)(a.c.pages + (int64_t)max(id[i], 0) * a.c.page_stride +
+                               (int64_t)h * kv4_head_bytes(a.c.page_len, D) +
+                               a.c.tiles * kv4_tile_bytes(D) + sub * 16);
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      const int p = p0 + kSelWaves * PW * i;
+      double s = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        s = fma(w[j], (double)((j & 1) ? bf16hi(x[i][j >> 1]) : bf16lo(x[i][j >> 1])), s);
 #pragma unroll
       for (int o = 1; o < L; o <<= 1) s += __shfl_xor(s, o);
-      if (sub == 0 && p < np) {
-        const bool always = p < a.n_first || p >= np - a.n_last || id < 0;
-        __hip_atomic_store(keys + p, always ? ~0ull : f64_key(s), __ATOMIC_RELAXED,
-                           __HIP_MEMORY_SCOPE_SYSTEM);
+      if (sub == 0) {
+        const bool always = p < a.n_first || p >= np - a.n_last;
+        s_out[p - part * kSelPages] = always ? ~0ull : id[i] < 0 ? kSpecial : f64_key(s);
       }
     }
   }
+  // published together: single keys written through cost more than the scores
+  __syncthreads();
+  for (int e = tid; e < kSelPages && part * kSelPages + e < np; e += kSelThreads)
+    __hip_atomic_store(keys + part * kSelPages + e, s_out[e], __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_SYSTEM);
   wait_vm();
   __syncthreads();
   if (tid == 0) s_last = ticket(&a.counters[bk], a.parts) ? 1 : 0;
@@ -113,53 +122,126 @@ __global__ __launch_bounds__(256) void kv4_select_kernel(Kv4SelArgs a) {
 
   // ---- the last part to arrive: the n_sel greatest keys, the lowest page first among equals
   int32_t* out = a.sel + (size_t)bk * a.n_sel;
-  for (int e = min(np, a.n_sel) + tid; e < a.n_sel; e += 256) out[e] = -1;
+  for (int e = min(np, a.n_sel) + tid; e < a.n_sel; e += kSelThreads) out[e] = -1;
   if (np <= a.n_sel) {
-    for (int e = tid; e < np; e += 256) out[e] = e;
+    for (int e = tid; e < np; e += kSelThreads) out[e] = e;
     return;
   }
-  for (int e = tid; e < np; e += 256) s_key[e] = load_sys64(keys + e);
-  // digit by digit from the top: the digit at which the n_sel-th key lies, until a whole bucket fits
-  unsigned long long prefix = 0;
-  int want = a.n_sel, shift = 64;
+  // the keys, their range and how many are always read or NaN (those lie above every score)
+  unsigned long long lo = kSpecial, hi = 0;
+  int special = 0;
+  constexpr int kBatch = 4;   // loads in flight: they go past the caches
+  for (int e0 = tid; e0 < np; e0 += kSelThreads * kBatch) {
+    unsigned long long k[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) k[i] = load_sys64(keys + min(e0 + kSelThreads * i, np - 1));
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (e0 + kSelThreads * i >= np) break;
+      s_key[e0 + kSelThreads * i] = k[i];
+      if (k[i] >= kSpecial) ++special;
+      else {
+        lo = k[i] < lo ? k[i] : lo;
+        hi = k[i] > hi ? k[i] : hi;
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const unsigned long long l2 = __shfl_xor(lo, o), h2 = __shfl_xor(hi, o);
+    lo = l2 < lo ? l2 : lo;
+    hi = h2 > hi ? h2 : hi;
+    special += __shfl_xor(special, o);
+  }
+  if (lane == 0) {
+    s_range[wave][0] = lo;
+    s_range[wave][1] = hi;
+    s_special[wave] = special;
+  }
+  if (tid < 256) s_hist[tid] = 0;
+  __syncthreads();
+  special = 0;
+#pragma unroll
+  for (int w = 0; w < kSelWaves; ++w) {
+    lo = s_range[w][0] < lo ? s_range[w][0] : lo;
+    hi = s_range[w][1] > hi ? s_range[w][1] : hi;
+    special += s_special[w];
+  }
+  // Digit by digit from the first bit in which the scores differ: the digit at which the n_sel-th key
+  // lies, until a whole bucket fits (two or three digits as a rule). Where the special keys alone are
+  // too many, from the top over all of them.
+  const bool all = special >= a.n_sel;
+  int shift = all ? 64 : lo == hi ? 0 : 64 - __builtin_clzll(lo ^ hi);
+  unsigned long long prefix = shift == 64 ? 0 : lo >> shift;
+  int want = all ? a.n_sel : a.n_sel - special;
   bool whole = false;
   while (shift > 0 && !whole) {
-    shift -= 8;
-    s_hist[tid] = 0;
-    __syncthreads();
-    for (int e = tid; e < np; e += 256) {
+    const int next = shift > 8 ? shift - 8 : 0, digits = (1 << (shift - next)) - 1;
+    for (int e = tid; e < np; e += kSelThreads) {
       const unsigned long long k = s_key[e];
-      if (shift == 56 || (k >> (shift + 8)) == prefix) atomicAdd(&s_hist[(int)(k >> shift) & 255], 1);
+      if ((all || k < kSpecial) && (shift == 64 || (k >> shift) == prefix))
+        atomicAdd(&s_hist[(int)(k >> next) & digits], 1);
     }
     __syncthreads();
-    int all;
-    const int mine = s_hist[255 - tid];
-    const int above = scan256(mine, s_scan, &all);   // keys of greater digits
-    if (above < want && above + mine >= want) {
-      s_pick[0] = 255 - tid;
-      s_pick[1] = above;
+    if (wave == 0) {   // lane l: digits 255 - 4 l .. 252 - 4 l, the greater first
+      int c[4], sum = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        c[i] = s_hist[255 - 4 * lane - i];
+        sum += c[i];
+      }
+      int before = sum;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(before, o);
+        if (lane >= o) before += y;
+      }
+      before -= sum;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (before < want && before + c[i] >= want) {
+          s_pick[0] = 255 - 4 * lane - i;
+          s_pick[1] = before;
+          s_pick[2] = c[i];
+        }
+        before += c[i];
+      }
     }
     __syncthreads();
-    prefix = (prefix << 8) | (unsigned)s_pick[0];
+    prefix = (prefix << (shift - next)) | (unsigned)s_pick[0];
     want -= s_pick[1];
-    whole = s_hist[s_pick[0]] == want;
+    whole = s_pick[2] == want;
+    shift = next;
+    if (tid < 256) s_hist[tid] = 0;
     __syncthreads();
   }
-  // pages in order: a thread's run of them, what lies before it by a sum over the threads
-  const int seg = (np + 255) / 256, e0 = tid * seg, e1 = min(np, e0 + seg);
-  int gt = 0, eq = 0, all;
-  for (int e = e0; e < e1; ++e) {
-    const unsigned long long k = s_key[e] >> shift;
-    gt += k > prefix;
-    eq += k == prefix;
+  // the pages in order: a wave's stretch of them, 64 at a time
+  const int span = (np + kSelThreads - 1) / kSelThreads * 64, e0 = wave * span, e1 = min(np, e0 + span);
+  auto is_gt = [&](int e) { return e < e1 && ((s_key[e] >> shift) > prefix); };
+  auto is_eq = [&](int e) { return e < e1 && ((s_key[e] >> shift) == prefix); };
+  int gt = 0, eq = 0;
+  for (int e = e0; e < e1; e += 64) {
+    gt += __popcll(__ballot(is_gt(e + lane)));
+    eq += __popcll(__ballot(is_eq(e + lane)));
   }
-  int g0 = scan256(gt, s_scan, &all);
-  int q0 = scan256(eq, s_scan, &all);
-  for (int e = e0; e < e1; ++e) {
-    const unsigned long long k = s_key[e] >> shift;
-    if (k > prefix || (k == prefix && q0 < want)) out[g0 + min(q0, want)] = e;
-    g0 += k > prefix;
-    q0 += k == prefix;
+  if (lane == 0) {
+    s_count[wave][0] = gt;
+    s_count[wave][1] = eq;
+  }
+  __syncthreads();
+  int g0 = 0, q0 = 0;
+  for (int w = 0; w < wave; ++w) {
+    g0 += s_count[w][0];
+    q0 += s_count[w][1];
+  }
+  const unsigned long long below = (1ull << lane) - 1;
+  for (int e = e0; e < e1; e += 64) {
+    const bool g = is_gt(e + lane), q = is_eq(e + lane);
+    const unsigned long long bg = __ballot(g), bq = __ballot(q);
+    const int gi = g0 + __popcll(bg & below), qi = q0 + __popcll(bq & below);
+    if (g || (q && qi < want)) out[gi + min(qi, want)] = e + lane;
+    g0 += __popcll(bg);
+    q0 += __popcll(bq);
   }
 }
 
@@ -225,9 +307,9 @@ int q4nx_kv4_select(const q4nx_kv4* cache, const uint16_t* q, int64_t q_stride, 
   const dim3 grid((unsigned)(items * a.parts));
   const size_t lds = (size_t)mp * 8;
   if (cache->head_dim == 64)
-    hipLaunchKernelGGL(kv4_select_kernel<2>, grid, dim3(256), lds, (hipStream_t)stream, a);
+    hipLaunchKernelGGL(kv4_select_kernel<2>, grid, dim3(kSelThreads), lds, (hipStream_t)stream, a);
   else
-    hipLaunchKernelGGL(kv4_select_kernel<4>, grid, dim3(256), lds, (hipStream_t)stream, a);
+    hipLaunchKernelGGL(kv4_select_kernel<4>, grid, dim3(kSelThreads), lds, (hipStream_t)stream, a);
   return check_launch(what);
 }
 

@@ -37,6 +37,7 @@ import numpy as np
 import torch
 
 from . import ops
+from .kv4 import Kv4Cache
 from .ops import Policy
 from .q4nx import Q4_TILE_BYTES, Q8_TILE_BYTES, Q4NX, TILE_BYTES, check_stored_shape, projection_shape
 
@@ -203,11 +204,18 @@ class GraniteDecoder:
     """Decode state for up to `max_batch` sequences of up to `max_len` positions.
 
     `step()` runs one token for every sequence at its own position; `generate()` runs the
-    greedy loop on the device from HIP graphs of GRAPH_STEPS steps and of one step."""
+    greedy loop on the device from HIP graphs of GRAPH_STEPS steps and of one step.
+
+    kv="q4" keeps K and V in pages of 4-bit codes (`kv`, a Kv4Cache with pages for max_len positions
+    of every sequence): 2048 bytes a layer and position of 8 kv heads become 672. The fused q/k/v
+    launch then writes a bf16 row into one cache that all layers share, from where it is quantised;
+    two launches more a layer than kv="bf16". sparse_pages > 0: attention reads that many pages of
+    each (sequence, kv head), chosen by every token's query, the first and the newest among them."""
 
     def __init__(self, weights: GraniteWeights, max_batch: int = 1, max_len: int = 4096,
                  device="cuda", fused_attn_o: bool = True, attn_splits: int = 0,
-                 policy: Policy | None = None):
+                 policy: Policy | None = None, kv: str = "bf16", page_len: int = 64,
+                 sparse_pages: int = 0):
         c = weights.cfg
         self.cfg, self.w = c, weights
         # the launch policy of every kernel this decoder issues (its own copy: other
@@ -221,9 +229,23 @@ class GraniteDecoder:
         self.max_batch = max_batch
         self.max_len = (max_len + 63) // 64 * 64
         b, dev = max_batch, self.dev
+        if kv not in ("bf16", "q4"):
+            raise ValueError(f'kv must be "bf16" or "q4", not {kv!r}')
+        if sparse_pages and (kv != "q4" or sparse_pages < 2):
+            raise ValueError('sparse_pages needs kv="q4" and at least 2 pages')
         kv_shape = (b, c.n_kv, self.max_len, c.head_dim)
-        self.k_cache = [torch.zeros(kv_shape, dtype=torch.bfloat16, device=dev) for _ in range(c.n_layers)]
-        self.v_cache = [torch.zeros(kv_shape, dtype=torch.bfloat16, device=dev) for _ in range(c.n_layers)]
+        # kv="q4": the rows of one layer at a time, on their way into its pages
+        own = c.n_layers if kv == "bf16" else 1
+        self.k_cache, self.v_cache = (
+            [torch.zeros(kv_shape, dtype=torch.bfloat16, device=dev) for _ in range(own)] * (c.n_layers // own)
+            for _ in range(2))
+        self.kv: Kv4Cache | None = None
+        self.sparse_pages = sparse_pages
+        if kv == "q4":
+            self.kv = Kv4Cache(c.n_layers, b * -(-self.max_len // page_len), b, self.max_len, c.n_kv,
+                               c.head_dim, page_len, device=dev)
+            self.kv.reserve([self.max_len] * b)
+            self.sel = torch.full((b, c.n_kv, max(1, sparse_pages)), -1, dtype=torch.int32, device=dev)
         self.rope = ops.rope_table(self.max_len, c.head_dim, c.theta, device=dev)
         self.h = torch.zeros((b, c.hidden), dtype=torch.float32, device=dev)
         # sums of h^2 per 16 entries, written by each producer of h for the next RMSNorm
@@ -295,7 +317,13 @@ class GraniteDecoder:
             ops.qkv_rope(L["q"], L["k"], L["v"], c.n_q, c.n_kv, kt_h, h, self.pos[:b], self.rope,
                          kc, vc, q_out=q, norm_w=L["norm_in"], eps=c.eps, ws=self.ws,
                          ssq_in=ssq, policy=pol, raw_out=tr and tr["raw"], xn_out=tr and tr["xn"])
-            if fuse_o:
+            if self.kv is not None:
+                self._attn_q4(li, b, q, attn)
+                ops.gemv_ex(L["o"], "q4", attn.view(b, c.q_dim), c.hidden // 32, kt_q,
+                            residual=h, out=h, ssq_out=ssq, ws=self.ws, policy=pol)
+                if tr is not None:
+                    tr["attn"].copy_(attn)
+            elif fuse_o:
                 rec = ops.gqa_decode_records(q.view(b, c.n_q, c.head_dim), kc, vc, self.lens[:b],
                                              n_split, c.scale, max_len=self.max_len, ws=self.ws,
                                              policy=pol)
@@ -323,6 +351,42 @@ class GraniteDecoder:
         ops.gemv_ex(w.lm_head, w.lm_head_kind, h, c.vocab // 32, kt_h, norm_w=w.norm_final,
                     eps=c.eps, out=self.logits[:b], argmax_keys=self.keys[:b], ssq_in=ssq,
                     ws=self.ws, policy=pol)
+
+    def _attn_q4(self, li: int, b: int, q: torch.Tensor, attn: torch.Tensor) -> None:
+        """The layer's new rows into its pages, then attention over them."""
+        kv, c = self.kv, self.cfg
+        table = None if b == kv.n_seqs else kv.table[:b]
+        kv.append_cached(li, self.k_cache[li], self.v_cache[li], self.pos[:b], table=table)
+        q3, lens, sel = q.view(b, c.n_q, c.head_dim), self.lens[:b], None
+        if self.sparse_pages:
+            sel = kv.select(li, q3, lens, self.sparse_pages, max_len=self.max_len, out=self.sel[:b],
+                            ws=self.ws, table=table)
+        kv.attn(li, q3, lens, max_len=self.max_len, scale=c.scale, sel=sel, n_split=self.attn_splits,
+                out=attn, ws=self.ws, table=table)
+
+    def fork(self, src, dst, lens) -> None:
+        """Sequences dst go on from the first lens[i] positions of src[i] (kv="q4"): full pages are shared,
+        the last one is copied, what dst held is given up. The tokens that follow go on from there
+        through step() or generate() with start positions >= lens. A sequence with shared pages must
+        not be wound back into them."""
+        if self.kv is None:
+            raise ValueError('fork needs kv="q4"')
+        src, dst, lens = [int(x) for x in src], [int(x) for x in dst], [int(x) for x in lens]
+        n = self.max_batch
+        if not len(src) == len(dst) == len(lens) or len(set(dst)) != len(dst) or set(src) & set(dst) \
+                or not all(0 <= x < n for x in src + dst) or not all(0 <= x <= self.max_len for x in lens) \
+                or any(lens[i] != lens[src.index(s)] for i, s in enumerate(src)):
+            raise ValueError("src and dst must be distinct sequences, each dst once, each src with one length")
+        if not src:
+            return
+        kv = self.kv
+        kv.free(dst)
+        for s, x in zip(src, lens):
+            kv.lens[s] = x
+        kv.fork(src, dst)
+        kv.reserve([self.max_len] * n)
+        if int(kv.status):
+            raise RuntimeError("the pool has no pages left for the forked sequences")
 
     def _trace_layer(self, tr: dict, li: int, b: int, pos_host, mlp) -> dict:
         """Host copies of one layer's bf16 narrowing points (uint16 bits): the normalised
@@ -444,7 +508,10 @@ class GraniteDecoder:
         context; no prefill runs through the model)."""
         g = torch.Generator(device=self.dev)
         g.manual_seed(seed)
-        for kc, vc in zip(self.k_cache, self.v_cache):
+        rows = torch.arange(self.max_batch + 1, dtype=torch.int32, device=self.dev) * ctx
+        for li, (kc, vc) in enumerate(zip(self.k_cache, self.v_cache)):
             for t in (kc, vc):
                 t.zero_()
                 t[:, :, :ctx] = torch.randn(t[:, :, :ctx].shape, device=self.dev, generator=g).to(torch.bfloat16)
+            if self.kv is not None and ctx:
+                self.kv.append_cached(li, kc, vc, torch.zeros_like(rows[1:]), rows, max_new=ctx)
