@@ -363,9 +363,9 @@ int q4nx_kv4_read(const q4nx_kv4 *cache, void *k_out, void *v_out, int out_f32, 
  * q4nx_kv4_select gives them; entries outside the sequence are none, a page named twice counts twice.
  * n_split = 0 shares the work by the lengths as the kernel finds them (which positions are summed
  * together, so the last bits, then hang on all of them); n_split >= 1 cuts the longest length into so
- * many parts and every sequence into parts of that size. ws: q4nx_kv4_attn_ws_bytes(...), block = 1
- * for a call with cu. */
-size_t q4nx_kv4_attn_ws_bytes(const q4nx_kv4 *cache, int n_q_heads, int block, int max_new,
+ * many parts and every sequence into parts of that size. ws: q4nx_kv4_attn_ws_bytes(...), with total = 0
+ * for a call without cu; where many rows share a sequence's tiles they are taken apart there first. */
+size_t q4nx_kv4_attn_ws_bytes(const q4nx_kv4 *cache, int n_q_heads, int total, int max_new,
                               int max_len, int n_sel, int n_split);
 int q4nx_kv4_attn(const q4nx_kv4 *cache, const uint16_t *q, int64_t q_stride, uint16_t *out,
                   float *out_f32, int n_q_heads, const int32_t *cu, int total, int max_new,

@@ -23,10 +23,13 @@ struct Kv4AttnArgs {
   const int32_t* cu;
   const int32_t* lens;
   const int32_t* sel;
-  int n_sel, hq, group, total, row_tiles;   // row_tiles: row blocks per sequence
+  int n_sel, hq, group, total;
   int n_split, chunk;   // blocks: workgroups per row tile, tiles for each of them
   int unit;             // one token: tiles per part of a (sequence, kv head), 0: by what there is
   float scale_l2;
+  u32x4_t* ops;         // blocks: tiles taken apart beforehand, [seq * hkv][ops_tiles][4 NG][2][64]
+  uint32_t* bad;        // their V's NaN groups, [..][ops_tiles][NG]: a bit per position
+  int ops_tiles;
   float* partial;
   uint32_t partial_bytes;
   unsigned* counters;
@@ -53,6 +56,11 @@ struct Kv4Minus {
   static __device__ __forceinline__ float dot(float x, uint32_t pair, uint32_t one) {
     return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(s16x2_t, pair),
                                            __builtin_bit_cast(s16x2_t, one), x, false);
+  }
+  // a pair as two bf16 terms each: 2^-18 of a value is left out
+  __device__ __forceinline__ void split(float x0, float x1, uint32_t& hi_, uint32_t& lo_) const {
+    hi_ = pack_bf16x2_op(x0, x1);
+    lo_ = pack_bf16x2_op(dot(x0, hi_, lo), dot(x1, hi_, hi));
   }
 };
 
@@ -560,29 +568,144 @@ constexpr int kBlockCt = 2;   // at 4 long prompts take 2 % less, short ones 40 
 template <int D>
 constexpr int kv4_block_rows() { return 16 * kBlockCt * kv4_block_waves<D>(); }
 
+// A tile taken apart: a wave's dword of every lane's four of K and of V (C chunks of 64 channels).
 template <int NG>
+struct Kv4Apart {
+  static constexpr int D = 32 * NG, C = NG / 2, KJ = 2 * NG;
+  uint32_t kc[C], ks[C], vc[C], vs[C][8];
+
+  __device__ __forceinline__ void fetch(const uint8_t* tile, int wave, int lane) {
+    const int n = lane & 15, kg = lane >> 4, ktt = wave >> 1, kgg = wave & 1;
+    const uint8_t* pc = tile + lane * 16 + wave * 4;
+    const uint8_t* pk = tile + 32 * D + ((16 * ktt + n) * NG + kgg) * 4;
+    const uint8_t* pv = tile + 32 * D + 128 * NG + kg * 16 * NG + (wave >> 1) * 4;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      kc[c] = *(const uint32_t*)(pc + c * 1024);
+      vc[c] = *(const uint32_t*)(pc + 16 * D + c * 1024);
+      ks[c] = *(const uint32_t*)(pk + c * 8);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        vs[c][e] = *(const uint32_t*)(pv + c * 8 + (16 * (e >> 2) + (e & 3)) * NG * 4);
+    }
+  }
+  __device__ __forceinline__ void poison() {   // an entry that names no page
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      ks[c] = kKv4NaN;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) vs[c][e] = kKv4NaN;
+    }
+  }
+  // V without its NaN groups, and without positions from `seen` (of this tile's 32) on, which may hold
+  // anything (the page's older bytes); f(group, NaN positions) once for each group
+  template <typename F>
+  __device__ __forceinline__ void clean(int seen, int wave, int lane, F&& f) {
+    const int kg = lane >> 4;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      uint32_t bad = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int p = 16 * (e >> 2) + 4 * kg + (e & 3);
+        const bool out = p >= seen, nan = !(fabsf(bf16lo(vs[c][e]) + bf16hi(vs[c][e])) < INFINITY);
+        if (!out && nan) bad |= 1u << p;
+        if (out || nan) vs[c][e] = 0u;
+      }
+      bad |= (uint32_t)__shfl_xor((int)bad, 16);
+      bad |= (uint32_t)__shfl_xor((int)bad, 32);
+      if (lane == 0 && (wave & 1) == 0) f(2 * c + (wave >> 1), bad);
+    }
+  }
+  // out(dword, high terms, low terms): K's 2 NG, then V's
+  template <typename F>
+  __device__ __forceinline__ void spread(float scale, int wave, const Kv4Minus& neg, F&& out) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const float d = bf16lo(ks[c]) * scale, m = bf16hi(ks[c]) * scale;
+      u32x4_t hi, lo;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        uint32_t y0, y1;
+        neg.split(fmaf((float)((kc[c] >> (4 * r)) & 15u), d, m),
+                  fmaf((float)((kc[c] >> (4 * r + 16)) & 15u), d, m), y0, y1);
+        hi[r] = y0;
+        lo[r] = y1;
+      }
+      out(4 * c + wave, hi, lo);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        uint32_t y0, y1;
+        neg.split(fmaf((float)((vc[c] >> (4 * r)) & 15u), bf16lo(vs[c][r]), bf16hi(vs[c][r])),
+                  fmaf((float)((vc[c] >> (4 * r + 16)) & 15u), bf16lo(vs[c][4 + r]), bf16hi(vs[c][4 + r])),
+                  y0, y1);
+        hi[r] = y0;
+        lo[r] = y1;
+      }
+      out(KJ + 4 * c + wave, hi, lo);
+    }
+  }
+};
+
+// Tiles taken apart beforehand, one per workgroup, for calls in which many row blocks read each: 16 KB
+// (D = 64) written once in place of some 110 instructions a wave and row block.
+template <int NG>
+__global__ __launch_bounds__(256) void kv4_apart_kernel(Kv4AttnArgs a) {
+  constexpr int D = 32 * NG;
+  const int t = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+  const int end = max(0, min(a.lens[b], a.c.cap)), lane = threadIdx.x & 63;
+  if (t * kKv4Tile >= end) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int id = kv4_page(a.c, b, t >> a.c.shift);
+  Kv4Apart<NG> x;
+  x.fetch(a.c.pages + (int64_t)max(id, 0) * a.c.page_stride +
+              (int64_t)h * kv4_head_bytes(a.c.page_len, D) + (t & (a.c.tiles - 1)) * kv4_tile_bytes(D),
+          wave, lane);
+  if (id < 0) x.poison();
+  const int64_t at = ((int64_t)b * a.c.hkv + h) * a.ops_tiles + t;
+  x.clean(end - t * kKv4Tile, wave, lane, [&](int g, uint32_t bad) { a.bad[at * NG + g] = bad; });
+  u32x4_t* out = a.ops + at * (4 * NG * 128) + lane;
+  const Kv4Minus neg;
+  x.spread(a.scale_l2, wave, neg, [&](int j, const u32x4_t& hi, const u32x4_t& lo) {
+    out[j * 128] = hi;
+    out[j * 128 + 64] = lo;
+  });
+}
+
+// PRE: the tiles come from kv4_apart_kernel, straight into LDS.
+template <int NG, bool PRE>
 __global__ __launch_bounds__(64 * kv4_block_waves<32 * NG>()) void kv4_block_kernel(Kv4AttnArgs a) {
   constexpr int D = 32 * NG, NT = D / 16, CT = kBlockCt, NW = kv4_block_waves<D>();
-  constexpr int RB = 16 * CT * NW, REC = D + 4, C = NG / 2, KJ = 2 * NG;
+  constexpr int RB = 16 * CT * NW, REC = D + 4, KJ = 2 * NG;
   static_assert(NW == 4 && CT == 2, "a wave takes one dword of four; its row tiles are 2, 1 or 0");
   __shared__ __attribute__((aligned(16))) u32x4_t s_op[2][4 * NG][2][64];   // [buffer][K, V dwords][term][lane]
   __shared__ uint32_t s_bad[2][NG];
   __shared__ int s_last;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, kg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  // the rows that see most first
-  int x = blockIdx.x;
-  const int split = x % a.n_split;
-  x /= a.n_split;
-  const int h = x % a.c.hkv;
-  x /= a.c.hkv;
-  const int b = x % a.c.n_seqs, rb = a.row_tiles - 1 - x / a.c.n_seqs;
-  const int c0 = a.cu[b];
-  int nq = a.cu[b + 1] - c0;
-  if (c0 < 0 || nq < 0) nq = 0;
-  nq = min(nq, a.total - c0);
+  // the row block: of the sequences' blocks in order, in each the rows that see most first
+  const int item = blockIdx.x / a.n_split, split = blockIdx.x - item * a.n_split;
+  const int h = item % a.c.hkv, index = item / a.c.hkv;
+  auto tokens_of = [&](int b) {
+    const int from = a.cu[b], n = a.cu[b + 1] - from;
+    return from < 0 || n < 0 ? 0 : min(n, a.total - from);
+  };
+  int b = -1, rb = 0;
+  for (int s0 = 0, before = 0; s0 < a.c.n_seqs && b < 0; s0 += 64) {
+    const bool in = s0 + lane < a.c.n_seqs;
+    const int mine = in ? (max(0, tokens_of(s0 + lane)) * a.group + RB - 1) / RB : 0;
+    const int sum = before + wave_scan(mine);
+    const unsigned long long hit = __ballot(in && sum > index);
+    if (hit) {
+      const int l0 = __builtin_ctzll(hit);
+      b = s0 + l0;
+      rb = __builtin_amdgcn_readlane(sum, l0) - 1 - index;
+    }
+    before = __builtin_amdgcn_readlane(sum, 63);
+  }
+  if (b < 0) return;
+  const int c0 = a.cu[b], nq = tokens_of(b);
   const int rows = nq * a.group, row0 = rb * RB;
-  if (row0 >= rows) return;   // uniform, and in every split of it
   const int first_tok = row0 / a.group, last_tok = (min(row0 + RB, rows) - 1) / a.group;
   auto sees = [&](int tok) { return max(0, min(a.lens[b] - nq + tok + 1, a.c.cap)); };
   const int top = sees(last_tok), all_see = sees(first_tok);
@@ -621,87 +744,36 @@ __global__ __launch_bounds__(64 * kv4_block_waves<32 * NG>()) void kv4_block_ker
   }
   const Kv4Minus neg;
 
-  // ---- taking a tile apart: dword `wave` of every lane's four of K and of V
-  const int ktt = wave >> 1, kgg = wave & 1;
-  uint32_t kc[C], ks[C], vc[C], vs[C][8];
+  // ---- a tile's operands into a buffer: taken apart here, or copied
+  Kv4Apart<NG> x_;
   int id_now = 0, id_next = 0;
+  uint32_t bad_now[NG], bad_next[NG];
+  const int64_t ops0 = ((int64_t)b * a.c.hkv + h) * a.ops_tiles;
   auto page = [&](int t) __attribute__((always_inline)) { return kv4_page(a.c, b, t >> a.c.shift); };
   auto fetch = [&](int t, int id) __attribute__((always_inline)) {
-    const uint8_t* tile = a.c.pages + (int64_t)max(id, 0) * a.c.page_stride +
-                          (int64_t)h * kv4_head_bytes(a.c.page_len, D) +
-                          (t & (a.c.tiles - 1)) * kv4_tile_bytes(D);
-    const uint8_t* pc = tile + lane * 16 + wave * 4;
-    const uint8_t* pk = tile + 32 * D + ((16 * ktt + n) * NG + kgg) * 4;
-    const uint8_t* pv = tile + 32 * D + 128 * NG + kg * 16 * NG + (wave >> 1) * 4;
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      kc[c] = *(const uint32_t*)(pc + c * 1024);
-      vc[c] = *(const uint32_t*)(pc + 16 * D + c * 1024);
-      ks[c] = *(const uint32_t*)(pk + c * 8);
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        vs[c][e] = *(const uint32_t*)(pv + c * 8 + (16 * (e >> 2) + (e & 3)) * NG * 4);
-    }
-  };
-  // x as two bf16 terms, pairs (x0, x1)
-  auto split2 = [&](float x0, float x1, uint32_t& hi, uint32_t& lo) __attribute__((always_inline)) {
-    hi = pack_bf16x2_op(x0, x1);
-    lo = pack_bf16x2_op(Kv4Minus::dot(x0, hi, neg.lo), Kv4Minus::dot(x1, hi, neg.hi));
+    x_.fetch(a.c.pages + (int64_t)max(id, 0) * a.c.page_stride +
+                 (int64_t)h * kv4_head_bytes(a.c.page_len, D) +
+                 (t & (a.c.tiles - 1)) * kv4_tile_bytes(D),
+             wave, lane);
   };
   auto spread = [&](int t, int id, int buf) __attribute__((always_inline)) {
-    const bool part = (t + 1) * kKv4Tile > all_see;
-    if (id < 0) {
+    if (id < 0) x_.poison();
+    if ((t + 1) * kKv4Tile > all_see)
+      x_.clean(top - t * kKv4Tile, wave, lane, [&](int g, uint32_t bad) { s_bad[buf][g] = bad; });
+    x_.spread(a.scale_l2, wave, neg, [&](int j, const u32x4_t& hi, const u32x4_t& lo) {
+      s_op[buf][j][0][lane] = hi;
+      s_op[buf][j][1][lane] = lo;
+    });
+  };
+  auto copy = [&](int t, int buf) __attribute__((always_inline)) {
+    const u32x4_t* from = a.ops + (ops0 + t) * (4 * NG * 128) + wave * (2 * NG * 64) + lane;
+    u32x4_t* to = &s_op[buf][wave * NG][0][0];
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        ks[c] = kKv4NaN;
+    for (int i = 0; i < 2 * NG; ++i)
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + 64 * i),
+                                       (__attribute__((address_space(3))) void*)(to + 64 * i), 16, 0, 0);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) vs[c][e] = kKv4NaN;
-      }
-    }
-    if (part) {
-#pragma unroll
-      for (int c = 0; c < C; ++c) {
-        uint32_t bad = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int p = 16 * (e >> 2) + 4 * kg + (e & 3);
-          const float y = bf16lo(vs[c][e]) + bf16hi(vs[c][e]);
-          // a position that no row sees may hold anything (the page's older bytes)
-          const bool out = t * kKv4Tile + p >= top, nan = !(fabsf(y) < INFINITY);
-          if (!out && nan) bad |= 1u << p;
-          if (out || nan) vs[c][e] = 0u;
-        }
-        bad |= (uint32_t)__shfl_xor((int)bad, 16);
-        bad |= (uint32_t)__shfl_xor((int)bad, 32);
-        if (lane == 0 && (wave & 1) == 0) s_bad[buf][2 * c + (wave >> 1)] = bad;
-      }
-    }
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      const float d = bf16lo(ks[c]) * a.scale_l2, m = bf16hi(ks[c]) * a.scale_l2;
-      u32x4_t hi, lo;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        uint32_t y0, y1;
-        split2(fmaf((float)((kc[c] >> (4 * r)) & 15u), d, m),
-               fmaf((float)((kc[c] >> (4 * r + 16)) & 15u), d, m), y0, y1);
-        hi[r] = y0;
-        lo[r] = y1;
-      }
-      s_op[buf][4 * c + wave][0][lane] = hi;
-      s_op[buf][4 * c + wave][1][lane] = lo;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        uint32_t y0, y1;
-        split2(fmaf((float)((vc[c] >> (4 * r)) & 15u), bf16lo(vs[c][r]), bf16hi(vs[c][r])),
-               fmaf((float)((vc[c] >> (4 * r + 16)) & 15u), bf16lo(vs[c][4 + r]), bf16hi(vs[c][4 + r])),
-               y0, y1);
-        hi[r] = y0;
-        lo[r] = y1;
-      }
-      s_op[buf][KJ + 4 * c + wave][0][lane] = hi;
-      s_op[buf][KJ + 4 * c + wave][1][lane] = lo;
-    }
+    for (int g = 0; g < NG; ++g) bad_next[g] = a.bad[(ops0 + t) * NG + g];
   };
   // one tile for the first N of this wave's row tiles; part: some rows do not see all of it (the empty
   // asm keeps what follows from being done for every tile and selected)
@@ -768,7 +840,7 @@ __global__ __launch_bounds__(64 * kv4_block_waves<32 * NG>()) void kv4_block_ker
         const float p0 = ex2(s[c][0][e]), p1 = ex2(s[c][1][e]);
         l[c] += p0 + p1;
         uint32_t y0, y1;
-        split2(p0, p1, y0, y1);
+        neg.split(p0, p1, y0, y1);
         ph[c][e] = y0;
         pl[c][e] = y1;
       }
@@ -782,10 +854,10 @@ __global__ __launch_bounds__(64 * kv4_block_waves<32 * NG>()) void kv4_block_ker
 #pragma unroll
       for (int c = 0; c < N; ++c) o[c][u] = mfma_bf16(lo, ph[c], o[c][u]);
     }
-    if (part) {
+    if (PRE || part) {
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        const uint32_t bad = s_bad[buf][g];
+        const uint32_t bad = PRE ? bad_now[g] : s_bad[buf][g];
         if (bad == 0) continue;
 #pragma unroll
         for (int c = 0; c < N; ++c) {
@@ -802,20 +874,33 @@ __global__ __launch_bounds__(64 * kv4_block_waves<32 * NG>()) void kv4_block_ker
   };
 
   if (t_begin < t_end) {
-    id_now = page(t_begin);
-    fetch(t_begin, id_now);
-    id_next = page(min(t_begin + 1, t_end - 1));
-    spread(t_begin, id_now, 0);
+    if constexpr (PRE) {
+      copy(t_begin, 0);
+      wait_vm();
+    } else {
+      id_now = page(t_begin);
+      fetch(t_begin, id_now);
+      id_next = page(min(t_begin + 1, t_end - 1));
+      spread(t_begin, id_now, 0);
+    }
   }
   __syncthreads();
   auto run = [&](auto n_tiles) __attribute__((always_inline)) {
     for (int t = t_begin; t < t_end; ++t) {
       const int buf = (t - t_begin) & 1;
-      id_now = id_next;
-      fetch(min(t + 1, t_end - 1), id_now);
-      id_next = page(min(t + 2, t_end - 1));
-      if constexpr (decltype(n_tiles)::value > 0) compute(n_tiles, t, buf);
-      if (t + 1 < t_end) spread(t + 1, id_now, buf ^ 1);
+      if constexpr (PRE) {
+#pragma unroll
+        for (int g = 0; g < NG; ++g) bad_now[g] = bad_next[g];
+        if (t + 1 < t_end) copy(t + 1, buf ^ 1);
+        if constexpr (decltype(n_tiles)::value > 0) compute(n_tiles, t, buf);
+        wait_vm();
+      } else {
+        id_now = id_next;
+        fetch(min(t + 1, t_end - 1), id_now);
+        id_next = page(min(t + 2, t_end - 1));
+        if constexpr (decltype(n_tiles)::value > 0) compute(n_tiles, t, buf);
+        if (t + 1 < t_end) spread(t + 1, id_now, buf ^ 1);
+      }
       __syncthreads();
     }
   };
@@ -844,7 +929,6 @@ __global__ __launch_bounds__(64 * kv4_block_waves<32 * NG>()) void kv4_block_ker
     }
     return;
   }
-  const int item = blockIdx.x / a.n_split;
   const __amdgpu_buffer_rsrc_t pr = make_rsrc(a.partial, a.partial_bytes);
   const uint32_t rec0 = (uint32_t)item * a.n_split * (RB * REC * 4);
 #pragma unroll
@@ -909,26 +993,34 @@ __global__ __launch_bounds__(64 * kv4_block_waves<32 * NG>()) void kv4_block_ker
   }
 }
 
-// Row blocks of a sequence, and workgroups that share one: enough of them to fill the chip, eight tiles
-// each at least.
-static int kv4_row_blocks(int max_new, int group, int d) {
-  const int rb = d == 64 ? kv4_block_rows<64>() : kv4_block_rows<128>();
-  return (int)(((int64_t)max_new * group + rb - 1) / rb);
+// Row blocks of a call, at most, and workgroups that share one: enough to fill the chip where there are
+// few blocks, eight tiles each at least.
+static int64_t kv4_row_blocks(int n_seqs, int total, int group, int rows) {
+  return n_seqs + (int64_t)total * group / rows;
 }
-static int kv4_block_split(int64_t items, int tiles) {
-  int64_t s = 768 / (items < 1 ? 1 : items);
+static int kv4_block_split(int64_t blocks, int tiles) {
+  if (blocks >= 512) return 1;
+  int64_t s = (768 + blocks - 1) / blocks;
   s = s < tiles / 8 ? s : tiles / 8;
-  return (int)(s < 1 ? 1 : (s > 64 ? 64 : s));
+  return (int)(s < 1 ? 1 : (s > 32 ? 32 : s));
 }
+
+// Tiles are taken apart beforehand from so many row blocks per sequence (as a mean) on, if that takes no
+// more than so many bytes (a default workspace's limit).
+constexpr int kApartBlocks = 4;
+constexpr int64_t kApartBytes = 192 << 20;
 
 struct Kv4Plan {
   int64_t items, grid;
   int n_split, chunk, unit;
   bool shared;   // whether an item may be of several parts
-  size_t bytes;
+  size_t bytes;  // workspace, `ops` of it before the tiles taken apart beforehand (0: none are)
+  size_t ops;
+  int ops_tiles;
 };
-static Kv4Plan kv4_plan(const q4nx_kv4* c, int n_q_heads, bool block, int max_new, int max_len,
-                        int n_sel, int n_split) {
+static Kv4Plan kv4_plan(const q4nx_kv4* c, int n_q_heads, int total, int max_len, int n_sel,
+                        int n_split) {
+  const bool block = total > 0;   // the rows of blocks, 0: one token per sequence
   Kv4Plan p{};
   const int group = n_q_heads / c->n_kv_heads;
   const int64_t cap = (int64_t)c->table_len * c->page_len;
@@ -937,9 +1029,12 @@ static Kv4Plan kv4_plan(const q4nx_kv4* c, int n_q_heads, bool block, int max_ne
   int64_t recs;
   int rows = 16;
   if (block) {
-    p.items = (int64_t)c->n_seqs * c->n_kv_heads * kv4_row_blocks(max_new, group, c->head_dim);
     rows = c->head_dim == 64 ? kv4_block_rows<64>() : kv4_block_rows<128>();
-    const int want = n_split > 0 ? n_split : kv4_block_split(p.items, tiles);
+    p.items = c->n_kv_heads * kv4_row_blocks(c->n_seqs, total, group, rows);
+    int64_t blocks = ((int64_t)total * group + rows - 1) / rows;   // as a rule: full blocks
+    blocks = c->n_kv_heads * (blocks > c->n_seqs ? blocks : c->n_seqs);
+    const int want = n_split > 0 ? n_split
+                     : p.items * 4 > Q4NX_WS_COUNTER_BYTES ? 1 : kv4_block_split(blocks, tiles);
     p.chunk = (tiles + want - 1) / want;
     p.n_split = (tiles + p.chunk - 1) / p.chunk;   // every split has work at the longest length
     p.grid = recs = p.items * p.n_split;
@@ -959,6 +1054,13 @@ static Kv4Plan kv4_plan(const q4nx_kv4* c, int n_q_heads, bool block, int max_ne
     p.shared = p.unit ? p.unit < tiles : tiles > 8;
   }
   p.bytes = p.shared ? (size_t)Q4NX_WS_COUNTER_BYTES + (size_t)recs * rows * (c->head_dim + 4) * 4 : 0;
+  const int64_t heads = (int64_t)c->n_seqs * c->n_kv_heads;
+  const int64_t ops = heads * tiles * (256 * c->head_dim + c->head_dim / 8);
+  if (block && (int64_t)total * group >= (int64_t)kApartBlocks * rows * c->n_seqs && ops <= kApartBytes) {
+    p.ops = (p.bytes ? p.bytes + 255 : Q4NX_WS_COUNTER_BYTES) & ~(size_t)255;
+    p.ops_tiles = tiles;
+    p.bytes = p.ops + (size_t)ops;
+  }
   return p;
 }
 
@@ -974,13 +1076,14 @@ using namespace q4nx;
 
 extern "C" {
 
-size_t q4nx_kv4_attn_ws_bytes(const q4nx_kv4* cache, int n_q_heads, int block, int max_new,
+size_t q4nx_kv4_attn_ws_bytes(const q4nx_kv4* cache, int n_q_heads, int total, int max_new,
                               int max_len, int n_sel, int n_split) {
   Kv4 c;
   if (kv4_resolve(cache, &c, "q4nx_kv4_attn_ws_bytes") != Q4NX_OK ||
-      !kv4_attn_shape(cache, n_q_heads, max_new, max_len, n_sel) || n_split < 0 || n_split > 1024)
+      !kv4_attn_shape(cache, n_q_heads, max_new, max_len, n_sel) || n_split < 0 || n_split > 1024 ||
+      total < 0)
     return 0;
-  return kv4_plan(cache, n_q_heads, block != 0, max_new, max_len, n_sel, n_split).bytes;
+  return kv4_plan(cache, n_q_heads, total, max_len, n_sel, n_split).bytes;
 }
 
 int q4nx_kv4_attn(const q4nx_kv4* cache, const uint16_t* q, int64_t q_stride, uint16_t* out,
@@ -1004,22 +1107,28 @@ int q4nx_kv4_attn(const q4nx_kv4* cache, const uint16_t* q, int64_t q_stride, ui
                "%s: a page list is for one token per sequence, without cu", what);
   Q4NX_REQUIRE(q_stride >= (int64_t)n_q_heads * cache->head_dim && q_stride % 8 == 0, Q4NX_ERR_SHAPE,
                "%s: q_stride=%lld must hold Hq * D and be a multiple of 8", what, (long long)q_stride);
-  const Kv4Plan p = kv4_plan(cache, n_q_heads, cu != nullptr, max_new, max_len, n_sel, n_split);
+  const Kv4Plan p = kv4_plan(cache, n_q_heads, cu ? total : 0, max_len, n_sel, n_split);
   const int64_t longest = n_sel ? (int64_t)n_sel * cache->page_len : max_len;
   Q4NX_REQUIRE(p.grid <= (int64_t)1 << 30 &&
                    (cu != nullptr || p.items * (longest / kKv4Tile + 1) < (int64_t)1 << 31),
                Q4NX_ERR_SHAPE, "%s: %lld rows of up to %lld positions", what, (long long)p.items,
                (long long)longest);
-  if (p.shared) {
-    Q4NX_REQUIRE(p.bytes - Q4NX_WS_COUNTER_BYTES < (size_t)1 << 31 &&
-                     p.items * 4 <= Q4NX_WS_COUNTER_BYTES,
-                 Q4NX_ERR_SHAPE, "%s: %lld rows to be shared by several workgroups", what,
-                 (long long)p.items);
+  if (p.bytes)
     Q4NX_REQUIRE(ws != nullptr && ws_bytes >= p.bytes && Q4NX_ALIGNED(ws, 256), Q4NX_ERR_WS,
                  "%s: workspace of %zu bytes (256-aligned) needed, %zu given", what, p.bytes, ws_bytes);
+  if (p.shared) {
+    const size_t recs = (p.ops ? p.ops : p.bytes) - Q4NX_WS_COUNTER_BYTES;
+    Q4NX_REQUIRE(recs < (size_t)1 << 31 && p.items * 4 <= Q4NX_WS_COUNTER_BYTES, Q4NX_ERR_SHAPE,
+                 "%s: %lld rows to be shared by several workgroups", what, (long long)p.items);
     a.counters = (unsigned*)ws;
     a.partial = (float*)((uint8_t*)ws + Q4NX_WS_COUNTER_BYTES);
-    a.partial_bytes = (uint32_t)(p.bytes - Q4NX_WS_COUNTER_BYTES);
+    a.partial_bytes = (uint32_t)recs;
+  }
+  if (p.ops) {
+    const int64_t tiles = (int64_t)a.c.n_seqs * a.c.hkv * p.ops_tiles;
+    a.ops = (u32x4_t*)((uint8_t*)ws + p.ops);
+    a.bad = (uint32_t*)((uint8_t*)a.ops + tiles * 256 * cache->head_dim);
+    a.ops_tiles = p.ops_tiles;
   }
   a.q = q;
   a.q_stride = q_stride;
@@ -1032,7 +1141,6 @@ int q4nx_kv4_attn(const q4nx_kv4* cache, const uint16_t* q, int64_t q_stride, ui
   a.hq = n_q_heads;
   a.group = n_q_heads / cache->n_kv_heads;
   a.total = total;
-  a.row_tiles = kv4_row_blocks(max_new, a.group, cache->head_dim);
   a.n_split = p.n_split;
   a.chunk = p.chunk;
   a.unit = p.unit;
@@ -1050,8 +1158,17 @@ int q4nx_kv4_attn(const q4nx_kv4* cache, const uint16_t* q, int64_t q_stride, ui
       default: d64 ? run(kv4_decode_kernel<2, 4>) : run(kv4_decode_kernel<4, 4>); break;
     }
   }
-  else if (d64) hipLaunchKernelGGL(kv4_block_kernel<2>, grid, dim3(64 * kv4_block_waves<64>()), 0, s, a);
-  else hipLaunchKernelGGL(kv4_block_kernel<4>, grid, dim3(64 * kv4_block_waves<128>()), 0, s, a);
+  else {
+    auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a); };
+    if (p.ops) {
+      const dim3 tiles((unsigned)p.ops_tiles, (unsigned)a.c.hkv, (unsigned)a.c.n_seqs);
+      if (d64) hipLaunchKernelGGL(kv4_apart_kernel<2>, tiles, dim3(256), 0, s, a);
+      else hipLaunchKernelGGL(kv4_apart_kernel<4>, tiles, dim3(256), 0, s, a);
+      d64 ? run(kv4_block_kernel<2, true>) : run(kv4_block_kernel<4, true>);
+    } else {
+      d64 ? run(kv4_block_kernel<2, false>) : run(kv4_block_kernel<4, false>);
+    }
+  }
   return check_launch(what);
 }
 

@@ -256,7 +256,7 @@ class Kv4Cache:
             sp, ns = sel.data_ptr(), sel.shape[2]
         new = 1 if cu is None else max_new or n
         most = min(self.max_len if table is None else c.table_len * self.page_len, max_len or 1 << 30)
-        need = self._need(c, "q4nx_kv4_attn_ws_bytes", hq, int(cu is not None), new, most, ns, n_split)
+        need = self._need(c, "q4nx_kv4_attn_ws_bytes", hq, 0 if cu is None else n, new, most, ns, n_split)
         wp = wn = 0
         if need:
             ws, wp, wn, stream = ops._scratch(ws, need)
