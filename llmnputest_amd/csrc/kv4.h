@@ -10,7 +10,8 @@
 //            positions 4 kg .. 4 kg + 3 and 16 + 4 kg .. 16 + 4 kg + 3
 //   K scales bf16 (d, m) [32][D/32], V scales the same
 // so one 16-byte load per lane is a whole operand set, and (dword >> 4 r) & 0x000f000f are the codes
-// of operand elements 2 r and 2 r + 1: or-ed into 0x4300 each is the bf16 number 128 + code.
+// of operand elements 2 r and 2 r + 1: or-ed into 0x4300 each is the bf16 number 128 + code
+// (three bits higher, into 0x4180: 16 + code).
 #pragma once
 
 #include "common.h"
@@ -55,6 +56,16 @@ __device__ __forceinline__ uint32_t kv4_pair(uint32_t w, int r) {
 }
 __device__ __forceinline__ u32x4_t kv4_operand(uint32_t w) {
   return u32x4_t{kv4_pair(w, 0), kv4_pair(w, 1), kv4_pair(w, 2), kv4_pair(w, 3)};
+}
+
+// The same as (16 + code, 16 + code): one shift more, and an eighth of what is left of a rounding of the
+// other operand when the 16 is taken out of a sum again.
+__device__ __forceinline__ u32x4_t kv4_operand16(uint32_t w) {
+  uint32_t mask = 0x00780078u, bias = 0x41804180u;
+  asm("" : "+s"(mask));
+  asm("" : "+v"(bias));
+  return u32x4_t{((w << 3) & mask) | bias, ((w >> 1) & mask) | bias, ((w >> 5) & mask) | bias,
+                 ((w >> 9) & mask) | bias};
 }
 
 }  // namespace q4nx

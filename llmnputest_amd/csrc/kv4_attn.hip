@@ -4,10 +4,10 @@
 //
 // With x = d_g c + m_g per group g of 32 channels,
 //   score = sum_g d_g (c . q)_g + m_g (sum of q)_g,    out = sum_pos p d_g c + sum_pos p m_g
-// so a code is an operand as it is, the bf16 number 128 + c (exact), and the scales stay in fp32. The
-// 128 is taken out again: a score's accumulator starts at -128 (sum of q)_g, and m_g - 128 d_g takes
-// m_g's place in the values. p d_g enters as two bf16 terms, which carry it to 2^-18, so that a value is
-// off by at most 143 2^-18 of its step.
+// so a code is an operand as it is, the bf16 number 128 + c for K and 16 + c for V (exact), and the scales
+// stay in fp32. The offsets are taken out again: a score's accumulator starts at -128 (sum of q)_g, and
+// m_g - 16 d_g takes m_g's place in the values. p d_g enters as two bf16 terms, which carry it to 2^-18,
+// so that a value is off by at most 31 2^-18 of its step.
 #include <math.h>
 
 #include "kv4.h"
@@ -215,7 +215,7 @@ __device__ __forceinline__ void kv4_finish(const Kv4AttnArgs& a, float (*s_o)[RO
 // R = ceil(heads / 4) of them for one position (head 4 i + kg in register i), and all that belongs to a
 // position, its scales and the exponentials, is done once per head and position:
 //   S[head][pos] = d_g (c . q)_g + m_g (sum of q)_g, summed over g;   C starts at -128 (sum of q)_g
-//   O^T[dim][head] += c^T[dim][pos] . (p d_g)^T[pos][head];  sum p (m_g - 128 d_g) apart, per lane
+//   O^T[dim][head] += c^T[dim][pos] . (p d_g)^T[pos][head];  sum p (m_g - 16 d_g) apart, per lane
 // p d_g goes through LDS from rows to columns: a lane's pair (position n, 16 + n) is an operand
 // register as it is, so the writes are consecutive dwords and an operand one 16-byte read. The scales
 // are one load of 4 NG bytes a lane (K's positions in lanes 0..31, V's in 32..63), spread by lane swaps.
@@ -255,7 +255,7 @@ __global__ __launch_bounds__(256) void kv4_decode_kernel(Kv4AttnArgs a) {
   __shared__ __attribute__((aligned(16))) float s_o[kWaves][H][D + 4];
   __shared__ __attribute__((aligned(16))) float s_fin[H][D + 4];
   __shared__ __attribute__((aligned(16))) uint32_t s_p[kWaves][NG][2][H * 16];
-  __shared__ float s_x[kWaves][NG + 1][H];   // sums of p (m - 128 d), and a move of the reference
+  __shared__ float s_x[kWaves][NG + 1][H];   // sums of p (m - 16 d), and a move of the reference
   __shared__ int s_last;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, kg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -477,8 +477,8 @@ __global__ __launch_bounds__(256) void kv4_decode_kernel(Kv4AttnArgs a) {
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         const float d0 = bf16lo(sc[1][0][g]), d1 = bf16lo(sc[1][1][g]);
-        const float m0 = fmaf(-128.f, d0, bf16hi(sc[1][0][g]));
-        const float m1 = fmaf(-128.f, d1, bf16hi(sc[1][1][g]));
+        const float m0 = fmaf(-16.f, d0, bf16hi(sc[1][0][g]));
+        const float m1 = fmaf(-16.f, d1, bf16hi(sc[1][1][g]));
 #pragma unroll
         for (int i = 0; i < R; ++i) {
           const float x0 = p[0][i] * d0, x1 = p[1][i] * d1;
@@ -496,7 +496,7 @@ __global__ __launch_bounds__(256) void kv4_decode_kernel(Kv4AttnArgs a) {
         const u32x4_t lo = *(const u32x4_t*)&s_p[wave][g][1][p_at];
 #pragma unroll
         for (int u = 2 * g; u < 2 * g + 2; ++u) {
-          const u32x4_t v = kv4_operand(r.v[u >> 2][u & 3]);
+          const u32x4_t v = kv4_operand16(r.v[u >> 2][u & 3]);
           o[u] = mfma_bf16(v, hi, o[u]);
           o[u] = mfma_bf16(v, lo, o[u]);
         }
