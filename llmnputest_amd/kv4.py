@@ -33,6 +33,12 @@ def page_bytes(page_len: int = 64, n_kv_heads: int = 8, head_dim: int = 64) -> i
     return n
 
 
+def _row_stride(table: torch.Tensor) -> int:
+    """Entries from row to row of a page table; a single row's stride says nothing. Rows that overlap
+    (an expanded row) keep their stride, which the library refuses."""
+    return table.stride(0) if table.shape[0] > 1 else table.shape[1]
+
+
 class Kv4Cache:
     """Pages of every layer (`pool` uint8 [n_layers, n_pages, page bytes]), the sequences' page table
     (`table` int32 [n_seqs, table_len], -1: none), their lengths (`lens` int32 [n_seqs]) and how many
@@ -81,7 +87,7 @@ class Kv4Cache:
         self._lib = _lib.lib()
         self.status = torch.zeros(1, dtype=torch.int32, device=pool.device)
         self._layers = [_lib.Kv4(pool.data_ptr() + i * pool.stride(0), pool.stride(1), table.data_ptr(),
-                                 table.stride(0), self.n_pages, page_len, n_kv_heads, head_dim,
+                                 _row_stride(table), self.n_pages, page_len, n_kv_heads, head_dim,
                                  self.n_seqs, self.table_len) for i in range(self.n_layers)]
         self._needs: dict = {}   # workspace bytes by the sizes that set them
 
@@ -100,7 +106,7 @@ class Kv4Cache:
         if table.dim() != 2 or table.stride(1) != 1 or table.numel() == 0:
             raise ValueError("table must be [sequences, pages], rows contiguous")
         v = _lib.Kv4.from_buffer_copy(c)
-        v.table, v.table_stride = table.data_ptr(), max(table.stride(0), table.shape[1])
+        v.table, v.table_stride = table.data_ptr(), _row_stride(table)
         v.n_seqs, v.table_len = table.shape
         return v, v.n_seqs
 

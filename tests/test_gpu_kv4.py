@@ -788,3 +788,15 @@ def test_python_refusals(dev):
         kv4.Kv4Cache.over(c.pool, c.table, c.lens, c.refs, n_kv_heads=1, page_len=32)
     c.append(0, z(0, 2, 64), z(0, 2, 64), one, cu=ints([0, 0, 0], dev))   # nothing to do
     assert c.attn(0, z(0, 4, 64), one, cu=ints([0, 0, 0], dev)).shape == (0, 4, 64)
+
+
+def test_a_row_shown_twice_is_refused(dev):
+    c = kv4.Kv4Cache(1, 8, 2, 128, n_kv_heads=2, page_len=32, device=dev)
+    twice = c.table[:1].expand(2, 4)
+    one, q = ints([0, 0], dev), torch.zeros((2, 4, 64), dtype=torch.bfloat16, device=dev)
+    for f in (lambda: c.attn(0, q, one, table=twice), lambda: c.select(0, q, one, n_sel=2, table=twice),
+              lambda: c.append(0, q[:, :2], q[:, :2], one, table=twice), lambda: c.read(0, one, table=twice)):
+        with pytest.raises(ops._lib.Q4NXError, match="stride"):
+            f()
+    with pytest.raises(ops._lib.Q4NXError, match="stride"):
+        kv4.Kv4Cache.over(c.pool, twice, c.lens, c.refs, n_kv_heads=2, page_len=32).read(0, one)

@@ -147,6 +147,18 @@ def test_python_refuses_before_the_library():
                           t(2, dtype=torch.int32), t(4, dtype=torch.int32))
 
 
+def test_a_table_view_keeps_its_stride():
+    """Rows of a wider table, a single row of any stride, and one row shown twice: its stride 0 has to
+    reach the library, which refuses it (with the width in its place row 1 would be read behind row 0)."""
+    import torch
+    t = torch.zeros((6, 10), dtype=torch.int32)
+    assert kv4._row_stride(t[1:5, :4]) == 10 and kv4._row_stride(t[::2]) == 20
+    assert kv4._row_stride(t[2:3, :4]) == 4 and kv4._row_stride(t[:1].expand(1, 10)) == 10
+    assert kv4._row_stride(t[:1].expand(3, 10)) == 0
+    for f in (append, read, attn, select):
+        assert f(cache(table_stride=0))[0] == ERR_SHAPE
+
+
 def test_page_bytes():
     f = _lib.lib().q4nx_kv4_page_bytes
     assert f(64, 8, 64) == 8 * (2 * 2560 + 256) and f(32, 1, 128) == 5120 + 512
