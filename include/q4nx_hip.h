@@ -308,7 +308,7 @@ int q4nx_gqa_decode_records(const uint16_t *q, const uint16_t *k_cache,
  * overflows, stands for NaN in all 32 channels.
  * A page holds page_len positions: per kv head page_len/32 tiles of 40 D bytes, then bf16 lo[D],
  * hi[D], each channel's least and greatest K since the page's first position was written (NaN for a
- * group that had a NaN). A tile: K codes, V codes (16 D bytes each), then bf16 (d, m) of the 32
+ * group that had one that stands for NaN). A tile: K codes, V codes (16 D bytes each), then bf16 (d, m) of the 32
  * positions x D/32 groups for K, then for V. Codes lie as the matrix cores take them, D/64 x 64
  * lanes x 4 dwords; lane 16 kg + n, chunk c:
  *   K dword 2 tt + g: position 16 tt + n, channels 64 c + 32 g + 8 kg + i, nibbles from the lowest
@@ -342,7 +342,7 @@ size_t q4nx_kv4_page_bytes(int page_len, int n_kv_heads, int head_dim);
  * (elements, multiples of 8; k and v 16-byte aligned; v alike). Rows with an index outside
  * [0, src_rows) and positions outside the cache are skipped. Everything else in the pages is left
  * as it is, the other positions of a tile included. Writing into a page that another sequence
- * shares changes it for both. */
+ * shares changes it for both; two sequences of one call must not write into one page. */
 int q4nx_kv4_append(const q4nx_kv4 *cache, const uint16_t *k, const uint16_t *v, int by_position,
                     int64_t src_rows, int64_t row_stride, int64_t head_stride, int64_t seq_stride,
                     const int32_t *pos, const int32_t *cu, int max_new, void *stream);
@@ -352,13 +352,14 @@ int q4nx_kv4_read(const q4nx_kv4 *cache, void *k_out, void *v_out, int out_f32, 
                   const int32_t *pos, const int32_t *cu, int max_new, void *stream);
 
 /* GQA attention over the cache: q bf16 [total][q_stride] holding [Hq][D] (q_stride a multiple of 8),
- * out bf16 and / or fp32 [total][Hq][D]. Query head h reads kv head h / (Hq/Hkv), Hq/Hkv <= 16.
+ * out bf16 (8-byte aligned) and / or fp32 (16) [total][Hq][D]; total * Hq < 2^30. Query head h reads kv head h / (Hq/Hkv), Hq/Hkv <= 16.
  * Without cu, one token per sequence (total = n_seqs): positions [0, lens[b]). With cu, sequence b's
  * tokens are rows cu[b] .. cu[b+1] - 1, the last of them at position lens[b] - 1: token i of n sees
  * positions [0, lens[b] - n + 1 + i). A row that sees nothing gives zeros; lens[b] > max_len reads
  * max_len positions; rows behind the last sequence are not written; max_new: at least the most
  * tokens of one sequence. A NaN in the cache makes NaN of at least its channels in every row that
- * sees it.
+ * sees it. Sums are taken of unnormalised exponentials of up to 2^8: |v| times the positions seen has
+ * to stay below 2^112.
  * sel (one token per sequence only): int32 [n_seqs][Hkv][n_sel], the logical pages to read, as
  * q4nx_kv4_select gives them; entries outside the sequence are none, a page named twice counts twice.
  * n_split = 0 shares the work by the lengths as the kernel finds them (which positions are summed
@@ -373,7 +374,8 @@ int q4nx_kv4_attn(const q4nx_kv4 *cache, const uint16_t *q, int64_t q_stride, ui
                   int n_split, void *ws, size_t ws_bytes, void *stream);
 
 /* The pages a token's attention reads: for every sequence and kv head the n_sel pages of the highest
- * score sum over the group's heads and channels of max(q lo, q hi) (fp64; ties to the lowest page),
+ * score sum over the group's heads and channels of max(q lo, q hi) (fp64; ties to the lowest page; a
+ * bound of q . k, so for a positive scale),
  * the first n_first and the last n_last pages among them whatever their score, then pages whose
  * score is NaN. sel int32 [n_seqs][Hkv][n_sel]: ascending, -1 behind the last. lens[b] > max_len
  * counts as max_len; at most 16384 pages per sequence. ws: q4nx_kv4_select_ws_bytes(...). */

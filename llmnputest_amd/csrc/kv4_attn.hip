@@ -291,6 +291,7 @@ __global__ __launch_bounds__(256) void kv4_decode_kernel(Kv4AttnArgs a) {
   };
   const int W = find(0x7FFFFFFF, [](int x) { return x; }).before * hkv;
   const bool line = a.unit == 0 && W > kLineTiles;
+  if (line && (int)blockIdx.x >= kLine) return;
   // parts of their own have 8, 16 or 32 tiles (or as many as asked for)
   const int sh = W < 1024 ? 3 : W < 8192 ? 4 : 5;
   const int unit = a.unit ? a.unit : line ? (W + kLine - 1) / kLine : 1 << sh;
@@ -695,7 +696,7 @@ __global__ __launch_bounds__(64 * kv4_block_waves<32 * NG>()) void kv4_block_ker
     const bool in = s0 + lane < a.c.n_seqs;
     const int mine = in ? (max(0, tokens_of(s0 + lane)) * a.group + RB - 1) / RB : 0;
     const int sum = before + wave_scan(mine);
-    const unsigned long long hit = __ballot(in && sum > index);
+    const unsigned long long hit = __ballot(in && sum > index && sum - mine <= index);
     if (hit) {
       const int l0 = __builtin_ctzll(hit);
       b = s0 + l0;
@@ -707,7 +708,7 @@ __global__ __launch_bounds__(64 * kv4_block_waves<32 * NG>()) void kv4_block_ker
   const int c0 = a.cu[b], nq = tokens_of(b);
   const int rows = nq * a.group, row0 = rb * RB;
   const int first_tok = row0 / a.group, last_tok = (min(row0 + RB, rows) - 1) / a.group;
-  auto sees = [&](int tok) { return max(0, min(a.lens[b] - nq + tok + 1, a.c.cap)); };
+  auto sees = [&](int tok) { return max(0, min(max(a.lens[b], 0) - nq + tok + 1, a.c.cap)); };
   const int top = sees(last_tok), all_see = sees(first_tok);
   const int nt = (top + kKv4Tile - 1) / kKv4Tile;
   const int parts = max(1, (nt + a.chunk - 1) / a.chunk);
@@ -1051,7 +1052,8 @@ static Kv4Plan kv4_plan(const q4nx_kv4* c, int n_q_heads, int total, int max_len
     if (!p.unit && p.items * ((tiles + 7) / 8) < p.grid) p.grid = p.items * ((tiles + 7) / 8);
     if (!p.unit && all > kLineTiles && p.grid < line) p.grid = line;
     recs = p.grid > 2 * line ? p.grid : 2 * line;
-    p.shared = p.unit ? p.unit < tiles : tiles > 8;
+    // on a line any item of two tiles may end one workgroup's stretch and begin the next
+    p.shared = p.unit ? p.unit < tiles : tiles > 8 || (all > kLineTiles && tiles > 1);
   }
   p.bytes = p.shared ? (size_t)Q4NX_WS_COUNTER_BYTES + (size_t)recs * rows * (c->head_dim + 4) * 4 : 0;
   const int64_t heads = (int64_t)c->n_seqs * c->n_kv_heads;
@@ -1095,6 +1097,8 @@ int q4nx_kv4_attn(const q4nx_kv4* cache, const uint16_t* q, int64_t q_stride, ui
   if (int rc = kv4_resolve(cache, &a.c, what)) return rc;
   Q4NX_REQUIRE(q && lens && (out || out_f32) && Q4NX_ALIGNED(q, 16), Q4NX_ERR_ARG,
                "%s: q (16-byte aligned), lens and an output are required", what);
+  Q4NX_REQUIRE(Q4NX_ALIGNED(out, 8) && Q4NX_ALIGNED(out_f32, 16), Q4NX_ERR_ARG,
+               "%s: out must be 8-byte, out_f32 16-byte aligned", what);
   Q4NX_REQUIRE((sel != nullptr) == (n_sel > 0) && n_split >= 0 && n_split <= 1024, Q4NX_ERR_ARG,
                "%s: sel and n_sel=%d go together; n_split=%d outside 0..1024", what, n_sel, n_split);
   Q4NX_REQUIRE(kv4_attn_shape(cache, n_q_heads, max_new, max_len, n_sel), Q4NX_ERR_SHAPE,
@@ -1107,6 +1111,8 @@ int q4nx_kv4_attn(const q4nx_kv4* cache, const uint16_t* q, int64_t q_stride, ui
                "%s: a page list is for one token per sequence, without cu", what);
   Q4NX_REQUIRE(q_stride >= (int64_t)n_q_heads * cache->head_dim && q_stride % 8 == 0, Q4NX_ERR_SHAPE,
                "%s: q_stride=%lld must hold Hq * D and be a multiple of 8", what, (long long)q_stride);
+  Q4NX_REQUIRE((int64_t)total * n_q_heads < (int64_t)1 << 30, Q4NX_ERR_SHAPE,
+               "%s: total=%d rows of %d heads, fewer than 2^30 in all", what, total, n_q_heads);
   const Kv4Plan p = kv4_plan(cache, n_q_heads, cu ? total : 0, max_len, n_sel, n_split);
   const int64_t longest = n_sel ? (int64_t)n_sel * cache->page_len : max_len;
   Q4NX_REQUIRE(p.grid <= (int64_t)1 << 30 &&

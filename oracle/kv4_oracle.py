@@ -183,8 +183,8 @@ def attention(pages: Pages, table, q, ends, scale, keep=None):
                 # the exponent's own rounding; values: p d in two bf16 terms (2^-18 of a code of up to
                 # 31), and sums of up to 31 p d over the tiles, joined over at most 64 splits of 4 waves;
                 # blocks: k, v and p are two bf16 terms each, 2^-18 of them left out
-                es = (scale * ((143 * dk[see] + mk[see]) @ np.abs(x)) * 40 + 4 * np.abs(s)) * 2.0 ** -24
-                es += scale * ((15 * dk[see] + mk[see]) @ np.abs(x)) * 2.0 ** -18
+                es = (abs(scale) * ((143 * dk[see] + mk[see]) @ np.abs(x)) * 40 + 4 * np.abs(s)) * 2.0 ** -24
+                es += abs(scale) * ((15 * dk[see] + mk[see]) @ np.abs(x)) * 2.0 ** -18
                 tiles = len(pos) / 32 + 80
                 bound[i, h * group + g] = (2 * es.max() + 2.0 ** -20 + 3 * 2.0 ** -18) * (p @ (15 * dv[see] + mv[see])) \
                     + (p @ dv[see]) * (31 * 2.0 ** -18 + 31 * tiles * 2.0 ** -24) \

@@ -379,6 +379,107 @@ def test_prompt_rows_before_the_cache_are_zero(dev):
     assert not got[:10].any() and got[10].any()
 
 
+def test_lengths_of_the_lowest_value(dev):
+    """lens of -2^31: nothing is seen, by single tokens and by blocks."""
+    x = Case(dev, 27, 2, 64, 32, [40, 40])
+    x.fill([40, 40])
+    low = ints([-2 ** 31, 40], dev)
+    out = x.c.attn(0, up(x.q(2, 4), dev), low)
+    assert not out[0].any() and out[1].any()
+    for n_split in (0, 2):
+        out = x.c.attn(0, up(x.q(300, 4), dev), low, cu=ints([0, 260, 300], dev), n_split=n_split)
+        assert not out[:260].any() and out[260:].any()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("scale", [0.0, -0.7])
+def test_scales_of_any_sign(dev, d, scale):
+    x = Case(dev, 28, 1, d, 64, [130, 33])
+    x.fill([130, 33])
+    q = x.q(2, 5)
+    got = x.c.attn(0, up(q, dev), ints([130, 33], dev), scale=scale, want_f32=True)
+    check(*got, *x.want(q, [(0, [130]), (1, [33])], scale))
+    q = x.q(60, 5)
+    got = x.c.attn(0, up(q, dev), ints([130, 33], dev), cu=ints([0, 50, 60], dev), scale=scale, want_f32=True)
+    check(*got, *x.want(q, [(0, range(81, 131)), (50, range(24, 34))], scale))
+
+
+@pytest.mark.parametrize("n_seqs,d", [(65, 64), (700, 128), (2100, 64)])
+def test_many_sequences(dev, n_seqs, d):
+    """More sequences than a wave has lanes, and (2100 x 8 kv heads) more than there are counters."""
+    hkv = 8 if n_seqs == 2100 else 1
+    lens = np.random.default_rng(3).integers(0, 70, n_seqs)
+    lens[:3] = [0, 69, 64]
+    x = Case(dev, 29, hkv, d, 32, lens)
+    some = [0, 1, 2, 62, 63, 64] + ([127, 128, n_seqs - 2, n_seqs - 1] if n_seqs > 65 else [])
+    at = np.concatenate([[0], np.cumsum(lens)])
+    k, v = x.rows(at[-1]), x.rows(at[-1])
+    x.c.append(0, up(k, dev), up(v, dev), ints([0] * n_seqs, dev), ints(at, dev), max_new=69)
+    x.o.append(x.table[some], [0] * len(some), [range(at[b], at[b + 1]) for b in some], k, v)
+    q = x.q(n_seqs, 2 * hkv)
+    got = x.c.attn(0, up(q, dev), ints(lens, dev), want_f32=True)
+    new = np.minimum(lens, np.random.default_rng(4).integers(0, 6, n_seqs))
+    cu = np.concatenate([[0], np.cumsum(new)])
+    qb = x.q(cu[-1], 2 * hkv)
+    block = x.c.attn(0, up(qb, dev), ints(lens, dev), cu=ints(cu, dev), max_new=5, want_f32=True)
+    for b in some:
+        want, bound = ko.attention(x.o, x.table[b], q[b:b + 1].astype(np.float64), [int(lens[b])], d ** -0.5)
+        check(got[0][b:b + 1], got[1][b:b + 1], want, bound)
+        if new[b]:
+            rows = slice(cu[b], cu[b + 1])
+            want, bound = ko.attention(x.o, x.table[b], qb[rows].astype(np.float64),
+                                       range(int(lens[b] - new[b]) + 1, int(lens[b]) + 1), d ** -0.5)
+            check(block[0][rows], block[1][rows], want, bound)
+
+
+@pytest.mark.parametrize("n_seqs,tiles,d", [(1024, 8, 64), (1100, 2, 128), (2040, 4, 64)])
+def test_many_short_sequences_share_a_line(dev, n_seqs, tiles, d):
+    """More than 16384 tiles in (sequence, kv head)s of at most eight: some end one workgroup's stretch and
+    begin the next. All sequences name the same pages and ask the same, so that those of one length are
+    alike."""
+    x = Case(dev, 32, 8, d, 32, [32 * tiles], spare=0)
+    x.fill([32 * tiles])
+    lens = np.random.default_rng(6).integers(32 * tiles - 40, 32 * tiles + 1, n_seqs)
+    table = x.c.table.expand(n_seqs, tiles).contiguous()
+    q = np.repeat(x.q(1, 8), n_seqs, 0)
+    out, out32 = x.c.attn(0, up(q, dev), ints(lens, dev), table=table, want_f32=True)
+    for n in np.unique(lens)[::13]:
+        want, bound = ko.attention(x.o, x.table[0], q[:1].astype(np.float64), [int(n)], d ** -0.5)
+        rows = torch.from_numpy(np.flatnonzero(lens == n)).to(dev)
+        check(out[rows], out32[rows], want, bound)
+
+
+def test_more_tiles_than_workgroups_times_words(dev):
+    """2048 sequences x 8 kv heads over 2^18 positions each, all of them one page again and again: the
+    launch has more workgroups than share the line of tiles, and a workgroup's place times its share
+    passes 2^31. What is seen is the page's 128 positions, 2048 times each: the page's own attention. The
+    bound grows with the tiles summed, 8192 + 80 of them for the oracle's 4 + 80."""
+    x = Case(dev, 30, 8, 64, 128, [128], spare=0)
+    x.fill([128])
+    n, pages = 2048, 2048
+    c = kv4.Kv4Cache.over(x.c.pool, torch.zeros((n, pages), dtype=torch.int32, device=dev),
+                          ints([pages * 128] * n, dev), x.c.refs, n_kv_heads=8, head_dim=64, page_len=128)
+    q = x.q(n, 8)
+    out, out32 = c.attn(0, up(q, dev), want_f32=True)
+    for b in (0, 1, 700, 1023, 1024, n - 1):
+        want, bound = ko.attention(x.o, x.table[0], q[b:b + 1].astype(np.float64), [128], 0.125)
+        check(out[b:b + 1], out32[b:b + 1], want, bound * (8272 / 84))
+    assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("d,n_split", [(64, 0), (64, 3), (128, 0)])
+def test_blocks_are_the_same_every_time(dev, d, n_split):
+    """Neither the order in which workgroups end nor what runs beside them changes a bit."""
+    x = Case(dev, 31, 2, d, 64, [700, 1500])
+    x.fill([700, 1500])
+    cu, lens, q = ints([0, 300, 1000], dev), ints([700, 1500], dev), up(x.q(1000, 10), dev)
+    one = up(x.q(2, 10), dev)
+    first, token = x.c.attn(0, q, lens, cu=cu, n_split=n_split), x.c.attn(0, one, lens)
+    for _ in range(30):
+        assert torch.equal(x.c.attn(0, q, lens, cu=cu, n_split=n_split), first)
+        assert torch.equal(x.c.attn(0, one, lens), token)
+
+
 def test_prompt_poison_is_causal(dev):
     """A NaN at a position shows in the tokens that see it, not in those before it."""
     x = Case(dev, 22, 1, 64, 32, [90, 90])

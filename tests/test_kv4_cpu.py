@@ -12,6 +12,7 @@ from oracle import kv4_oracle as ko
 ERR_ARG, ERR_SHAPE, ERR_WS = -1, -2, -3
 P = C.c_void_p(0x10000)      # aligned, never dereferenced
 ODD = C.c_void_p(0x10008)
+ODD4 = C.c_void_p(0x10004)
 
 
 def cache(**kw):
@@ -94,7 +95,8 @@ def test_read_refusals(kw, code):
     (dict(stride=2552), ERR_SHAPE), (dict(stride=2564), ERR_SHAPE), (dict(most=0), ERR_SHAPE),
     (dict(sel=P), ERR_ARG), (dict(n_sel=4), ERR_ARG), (dict(sel=P, n_sel=4, cu=P, new=2), ERR_SHAPE),
     (dict(split=-1), ERR_ARG), (dict(split=1025), ERR_ARG), (dict(split=2), ERR_WS),
-    (dict(split=2, ws=P, n=1000), ERR_WS)], ids=str)
+    (dict(split=2, ws=P, n=1000), ERR_WS), (dict(out=ODD4), ERR_ARG),
+    (dict(cu=P, total=1 << 25), ERR_SHAPE)], ids=str)
 def test_attn_refusals(kw, code):
     assert attn(cache(), **kw)[0] == code
 
@@ -157,6 +159,52 @@ def test_a_table_view_keeps_its_stride():
     assert kv4._row_stride(t[:1].expand(3, 10)) == 0
     for f in (append, read, attn, select):
         assert f(cache(table_stride=0))[0] == ERR_SHAPE
+
+
+def shares(lens, hkv, cap, line_groups):
+    """The parts that single tokens are cut into, as the kernel finds them from the lengths: a list of
+    (item, part, parts, record) for the calls without n_split and with a counter for each item."""
+    tiles = [max(1, -(-min(max(int(n), 0), cap) // 32)) for n in lens]
+    total = sum(tiles) * hkv
+    out = []
+    if total <= 16384:
+        unit = 8 if total < 1024 else 16 if total < 8192 else 32
+        at = 0
+        for b, n in enumerate(tiles):
+            for h in range(hkv):
+                parts = -(-n // unit)
+                out += [(b * hkv + h, p, parts, at + p) for p in range(parts)]
+                at += parts
+        return out
+    unit, off = -(-total // line_groups), 0
+    for b, n in enumerate(tiles):
+        for h in range(hkv):
+            first, last = off // unit, (off + n - 1) // unit
+            out += [(b * hkv + h, g - first, last - first + 1, 2 * g + (g == first)) for g in range(first, last + 1)]
+            off += n
+    return out
+
+
+@pytest.mark.parametrize("d,groups", [(64, 768), (128, 512)])
+def test_the_workspace_holds_every_share(d, groups):
+    """Wherever the lengths cut an item in parts, the call had to ask for a workspace, and its records lie
+    within it, each written by one workgroup."""
+    rng = np.random.default_rng(5)
+    cases = [(1024, 8, 8), (2040, 8, 4), (512, 8, 16), (2048, 8, 2), (2048, 8, 1), (1, 1, 1), (1, 8, 17), (64, 8, 512),
+             (3, 2, 9000), (1, 1, 20000), (256, 64, 9)]
+    cases += [(int(rng.integers(1, 400)), int(rng.integers(1, 40)), int(rng.integers(1, 60))) for _ in range(60)]
+    for n_seqs, hkv, tiles in cases:
+        c = cache(n_seqs=n_seqs, n_kv_heads=hkv, head_dim=d, page_len=32, table_len=tiles, table_stride=tiles,
+                  page_stride=1 << 24)
+        group = int(rng.integers(1, 17))
+        size = _lib.lib().q4nx_kv4_attn_ws_bytes(C.byref(c), group * hkv, 0, 1, 1 << 30, 0, 0)
+        records = (size - 65536) // (-(-group // 4) * 4 * (d + 4) * 4) if size else 0
+        for lens in ([tiles * 32] * n_seqs, [0] * n_seqs, rng.integers(0, tiles * 32 + 40, n_seqs)):
+            cut = [x for x in shares(lens, hkv, tiles * 32, groups) if x[2] > 1]
+            assert not cut or size, (n_seqs, hkv, tiles)
+            places = [x[3] for x in cut]
+            assert len(set(places)) == len(places) and max(places, default=-1) < records
+            assert max((x[0] for x in cut), default=0) * 4 < 65536
 
 
 def test_page_bytes():
