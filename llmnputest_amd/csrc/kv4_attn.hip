@@ -26,6 +26,7 @@ struct Kv4AttnArgs {
   int n_sel, hq, group, total;
   int n_split, chunk;   // blocks: workgroups per row tile, tiles for each of them
   int unit;             // one token: tiles per part of a (sequence, kv head), 0: by what there is
+  bool whole;           // one token: every (sequence, kv head) is one part
   float scale_l2;
   u32x4_t* ops;         // blocks: tiles taken apart beforehand, [seq * hkv][ops_tiles][4 NG][2][64]
   uint32_t* bad;        // their V's NaN groups, [..][ops_tiles][NG]: a bit per position
@@ -38,7 +39,12 @@ struct Kv4AttnArgs {
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 constexpr int kWaves = 4;
-constexpr int kLineTiles = 16384;   // tiles of a call above which its workgroups share one line of them
+// Tiles of a call above which its workgroups share one line of them, and how many there have to be for
+// each (sequence, kv head) as a mean.
+constexpr int kLineTiles = 16384;
+// From so many (sequence, kv head)s of at most so many tiles on, each is one part.
+constexpr int kWholeItems = 1024, kWholeTiles = 64;
+__host__ __device__ constexpr int kv4_line_mean(int d) { return d == 64 ? 256 : 64; }
 // Those workgroups: what the chip holds at once (three waves per SIMD at D = 64, two at 128).
 __host__ __device__ constexpr int kv4_line(int d) { return d == 64 ? 768 : 512; }
 constexpr int kMergeParts = 64;   // records of an item merged per pass
@@ -223,11 +229,14 @@ __device__ __forceinline__ void kv4_finish(const Kv4AttnArgs& a, float (*s_o)[RO
 // tiles, so table and list are read ahead, and two tiles are in flight while one is computed.
 //
 // Who does what is decided here, from the lengths as they are: of W tiles in all a part has
-//   8 (W < 1024), 16 (W < 8192), 32 (W <= 16384) or W / 768 (D = 64; 512 at 128)
-// tiles. Up to 32 a (sequence, kv head) is cut into parts of its own (a short call, where a second
-// segment would be waited for); beyond that the W tiles are one line that the workgroups cut evenly,
-// so that lengths however unlike load the chip alike, and a workgroup's stretch may end one
-// (sequence, kv head) and begin the next.
+//   8 (W < 1024), 16 (W < 8192), 32 (W <= 32768) or 64 tiles of one (sequence, kv head);
+// from 16384 tiles on, if that is more than 256 (D = 64; 64 at 128) for each (sequence, kv head), the W
+// tiles are one line that 768 (512) workgroups cut evenly, so that lengths however unlike load the chip
+// alike, and a workgroup's stretch may end one (sequence, kv head) and begin the next. Times in us with
+// 40 heads of 8 kv heads, line / parts of 64: b8 x 65536 45.6 / 50.2, b1 x 131072 34 / 38, b32 x 8192
+// 38 / 31, b64 x 4096 48 / 31; 64 heads of D = 128, b32 x 8192 56 / 63. From 1024 (sequence, kv head)s of
+// at most 64 tiles on, known from the call's sizes, each is one part and nothing is looked for: b2040 x
+// 128 109 (292 with the search), b256 x 512 25 (33).
 
 // x / y for quotients below 2^20 or so: the reciprocal is off by less than one in them.
 __device__ __forceinline__ int div_few(int x, int y) {
@@ -272,36 +281,63 @@ __global__ __launch_bounds__(256) void kv4_decode_kernel(Kv4AttnArgs a) {
   };
   auto find = [&](int target, auto&& x) {
     Where r{nb, 0, 0, 0};
-    for (int c = 0; c < nb; c += 64) {
-      const int len = c ? len_of(c + lane) : len0;
-      const int mine = c + lane < nb ? x(tiles_of(len)) : 0;
-      const int sum = wave_scan(mine);
-      const unsigned long long hit = __ballot(c + lane < nb && (r.before + sum) * hkv > target);
+    if (nb <= 64) {
+      const int mine = lane < nb ? x(tiles_of(len0)) : 0, sum = wave_scan(mine);
+      const unsigned long long hit = __ballot(lane < nb && sum * hkv > target);
       if (hit) {
+        r.b = __builtin_ctzll(hit);
+        r.x = __builtin_amdgcn_readlane(mine, r.b);
+        r.len = __builtin_amdgcn_readlane(len0, r.b);
+        r.before = __builtin_amdgcn_readlane(sum, r.b) - r.x;
+      } else {
+        r.before = __builtin_amdgcn_readlane(sum, 63);
+      }
+      return r;
+    }
+    for (int c = 0; c < nb; c += 256) {   // four sequences a lane
+      int len[4], mine[4], all = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) len[j] = len_of(c + 4 * lane + j);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        mine[j] = c + 4 * lane + j < nb ? x(tiles_of(len[j])) : 0;
+        all += mine[j];
+      }
+      const int sum = wave_scan(all);
+      const unsigned long long hit = __ballot((r.before + sum) * hkv > target);
+      if (hit) {   // the first lane that passes the target does so at one of its sequences
         const int l0 = __builtin_ctzll(hit);
-        r.b = c + l0;
-        r.x = __builtin_amdgcn_readlane(mine, l0);
-        r.len = __builtin_amdgcn_readlane(len, l0);
-        r.before += __builtin_amdgcn_readlane(sum, l0) - r.x;
+        r.before += __builtin_amdgcn_readlane(sum - all, l0);
+        r.b = c + 4 * l0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          r.x = __builtin_amdgcn_readlane(mine[j], l0);
+          r.len = __builtin_amdgcn_readlane(len[j], l0);
+          if ((r.before + r.x) * hkv > target) break;
+          r.before += r.x;
+          ++r.b;
+        }
         return r;
       }
       r.before += __builtin_amdgcn_readlane(sum, 63);
     }
     return r;
   };
-  const int W = find(0x7FFFFFFF, [](int x) { return x; }).before * hkv;
-  const bool line = a.unit == 0 && W > kLineTiles;
+  const int W = a.unit ? 0 : find(0x7FFFFFFF, [](int x) { return x; }).before * hkv;
+  const bool line = a.unit == 0 && W > kLineTiles && W > (int64_t)kv4_line_mean(D) * nb * hkv;
   if (line && (int)blockIdx.x >= kLine) return;
-  // parts of their own have 8, 16 or 32 tiles (or as many as asked for)
-  const int sh = W < 1024 ? 3 : W < 8192 ? 4 : 5;
+  // parts of their own have 8, 16, 32 or 64 tiles (or as many as asked for)
+  const int sh = W < 1024 ? 3 : W < 8192 ? 4 : W <= 2 * kLineTiles ? 5 : 6;
   const int unit = a.unit ? a.unit : line ? (W + kLine - 1) / kLine : 1 << sh;
   auto share = [&](int x) {
     return line ? x : a.unit ? div_few(x + unit - 1, unit) : (x + unit - 1) >> sh;
   };
 
   for (int at = blockIdx.x * (line ? unit : 1), left = line ? unit : 1;;) {
-  const Where f = find(at, share);
-  if (f.b == nb) return;
+  Where f{at / hkv, at / hkv, 1, 0};
+  if (a.whole) f.len = len_of(f.b);
+  else f = find(at, share);
+  if (f.b >= nb) return;
   const int b = f.b, end = f.len, nt = tiles_of(f.len);
   const int rem = at - f.before * hkv;
   const int h = div_few(rem, f.x), in = rem - h * f.x;
@@ -1006,15 +1042,16 @@ static int kv4_block_split(int64_t blocks, int tiles) {
   return (int)(s < 1 ? 1 : (s > 32 ? 32 : s));
 }
 
-// Tiles are taken apart beforehand from so many row blocks per sequence (as a mean) on, if that takes no
-// more than so many bytes (a default workspace's limit).
+// Bytes that a choice made here asks for, at most: within a default workspace.
+constexpr int64_t kMostBytes = 192 << 20;
+// Tiles are taken apart beforehand from so many row blocks per sequence (as a mean) on.
 constexpr int kApartBlocks = 4;
-constexpr int64_t kApartBytes = 192 << 20;
 
 struct Kv4Plan {
   int64_t items, grid;
   int n_split, chunk, unit;
   bool shared;   // whether an item may be of several parts
+  bool whole;    // every item is one part
   size_t bytes;  // workspace, `ops` of it before the tiles taken apart beforehand (0: none are)
   size_t ops;
   int ops_tiles;
@@ -1044,11 +1081,16 @@ static Kv4Plan kv4_plan(const q4nx_kv4* c, int n_q_heads, int total, int max_len
     p.items = (int64_t)c->n_seqs * c->n_kv_heads;
     rows = (group + 3) / 4 * 4;
     if (n_split > 0) p.unit = (tiles + n_split - 1) / n_split;
-    else if (p.items * 4 > Q4NX_WS_COUNTER_BYTES) p.unit = tiles;   // no counter for each
-    // by what there is: at most kLineTiles in parts of 8 and more, or one line
+    // no counter for each, or so many short ones that they fill the chip and end together
+    else if (p.items * 4 > Q4NX_WS_COUNTER_BYTES || (p.items >= kWholeItems && tiles <= kWholeTiles))
+      p.unit = tiles;
+    // by what there is: parts of 8 tiles and more, of 64 where they are many but few for each item, or
+    // one line
     const int line = kv4_line(c->head_dim);
     const int64_t all = p.items * tiles, some = all < kLineTiles ? all : kLineTiles;
-    p.grid = p.unit ? p.items * ((tiles + p.unit - 1) / p.unit) : p.items + some / 8;
+    const int64_t few = kv4_line_mean(c->head_dim) * p.items, mean = (all < few ? all : few) / 64;
+    p.grid = p.unit ? p.items * ((tiles + p.unit - 1) / p.unit)
+                    : p.items + (some / 8 > mean ? some / 8 : mean);
     if (!p.unit && p.items * ((tiles + 7) / 8) < p.grid) p.grid = p.items * ((tiles + 7) / 8);
     if (!p.unit && all > kLineTiles && p.grid < line) p.grid = line;
     recs = p.grid > 2 * line ? p.grid : 2 * line;
@@ -1056,9 +1098,16 @@ static Kv4Plan kv4_plan(const q4nx_kv4* c, int n_q_heads, int total, int max_len
     p.shared = p.unit ? p.unit < tiles : tiles > 8 || (all > kLineTiles && tiles > 1);
   }
   p.bytes = p.shared ? (size_t)Q4NX_WS_COUNTER_BYTES + (size_t)recs * rows * (c->head_dim + 4) * 4 : 0;
+  if (!block && n_split == 0 && (int64_t)p.bytes > kMostBytes) {   // thousands of items: one part each
+    p.unit = tiles;
+    p.grid = p.items;
+    p.shared = false;
+    p.bytes = 0;
+  }
+  p.whole = p.unit >= tiles;
   const int64_t heads = (int64_t)c->n_seqs * c->n_kv_heads;
   const int64_t ops = heads * tiles * (256 * c->head_dim + c->head_dim / 8);
-  if (block && (int64_t)total * group >= (int64_t)kApartBlocks * rows * c->n_seqs && ops <= kApartBytes) {
+  if (block && (int64_t)total * group >= (int64_t)kApartBlocks * rows * c->n_seqs && ops <= kMostBytes) {
     p.ops = (p.bytes ? p.bytes + 255 : Q4NX_WS_COUNTER_BYTES) & ~(size_t)255;
     p.ops_tiles = tiles;
     p.bytes = p.ops + (size_t)ops;
@@ -1150,6 +1199,7 @@ int q4nx_kv4_attn(const q4nx_kv4* cache, const uint16_t* q, int64_t q_stride, ui
   a.n_split = p.n_split;
   a.chunk = p.chunk;
   a.unit = p.unit;
+  a.whole = p.whole;
   if (max_len < a.c.cap) a.c.cap = max_len;
   a.scale_l2 = (float)((double)scale * 1.4426950408889634);
   const dim3 grid((unsigned)p.grid);

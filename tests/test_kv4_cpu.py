@@ -161,14 +161,14 @@ def test_a_table_view_keeps_its_stride():
         assert f(cache(table_stride=0))[0] == ERR_SHAPE
 
 
-def shares(lens, hkv, cap, line_groups):
+def shares(lens, hkv, cap, line_groups, mean):
     """The parts that single tokens are cut into, as the kernel finds them from the lengths: a list of
     (item, part, parts, record) for the calls without n_split and with a counter for each item."""
     tiles = [max(1, -(-min(max(int(n), 0), cap) // 32)) for n in lens]
     total = sum(tiles) * hkv
     out = []
-    if total <= 16384:
-        unit = 8 if total < 1024 else 16 if total < 8192 else 32
+    if total <= 16384 or total <= mean * len(lens) * hkv:
+        unit = 8 if total < 1024 else 16 if total < 8192 else 32 if total <= 32768 else 64
         at = 0
         for b, n in enumerate(tiles):
             for h in range(hkv):
@@ -185,13 +185,13 @@ def shares(lens, hkv, cap, line_groups):
     return out
 
 
-@pytest.mark.parametrize("d,groups", [(64, 768), (128, 512)])
-def test_the_workspace_holds_every_share(d, groups):
+@pytest.mark.parametrize("d,groups,mean", [(64, 768, 256), (128, 512, 64)])
+def test_the_workspace_holds_every_share(d, groups, mean):
     """Wherever the lengths cut an item in parts, the call had to ask for a workspace, and its records lie
     within it, each written by one workgroup."""
     rng = np.random.default_rng(5)
     cases = [(1024, 8, 8), (2040, 8, 4), (512, 8, 16), (2048, 8, 2), (2048, 8, 1), (1, 1, 1), (1, 8, 17), (64, 8, 512),
-             (3, 2, 9000), (1, 1, 20000), (256, 64, 9)]
+             (3, 2, 9000), (1, 1, 20000), (256, 64, 9), (2048, 8, 100), (300, 8, 70), (100, 8, 300)]
     cases += [(int(rng.integers(1, 400)), int(rng.integers(1, 40)), int(rng.integers(1, 60))) for _ in range(60)]
     for n_seqs, hkv, tiles in cases:
         c = cache(n_seqs=n_seqs, n_kv_heads=hkv, head_dim=d, page_len=32, table_len=tiles, table_stride=tiles,
@@ -199,8 +199,13 @@ def test_the_workspace_holds_every_share(d, groups):
         group = int(rng.integers(1, 17))
         size = _lib.lib().q4nx_kv4_attn_ws_bytes(C.byref(c), group * hkv, 0, 1, 1 << 30, 0, 0)
         records = (size - 65536) // (-(-group // 4) * 4 * (d + 4) * 4) if size else 0
+        if n_seqs * hkv >= 1024 and tiles <= 64:
+            assert size == 0   # one part each
+            continue
         for lens in ([tiles * 32] * n_seqs, [0] * n_seqs, rng.integers(0, tiles * 32 + 40, n_seqs)):
-            cut = [x for x in shares(lens, hkv, tiles * 32, groups) if x[2] > 1]
+            cut = [x for x in shares(lens, hkv, tiles * 32, groups, mean) if x[2] > 1]
+            if not size and 5 * n_seqs * hkv * -(-group // 4) * 16 * (d + 4) > 192 << 20:
+                continue   # records of thousands of items would not fit: one part each
             assert not cut or size, (n_seqs, hkv, tiles)
             places = [x[3] for x in cut]
             assert len(set(places)) == len(places) and max(places, default=-1) < records
