@@ -987,59 +987,107 @@ __global__ __launch_bounds__(64 * kv4_block_waves<32 * NG>()) void kv4_block_ker
   if (tid == 0) s_last = ticket(&a.counters[item], parts) ? 1 : 0;
   __syncthreads();
   if (!s_last) return;
-  for (int e = tid; e < min(RB, rows - row0) * (D / 4); e += 64 * NW) {
-    const int r = e / (D / 4), d = e % (D / 4) * 4;
-    float M = -INFINITY, L = 0.f;
-    float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int p0 = 0; p0 < parts; p0 += 4) {
-      uint4 v[4], ml[4];
+  // Two threads a row find the parts' weights, then a thread sums four channels of eight rows at a time,
+  // sixteen records in flight. The operands' buffers hold the weights.
+  constexpr int PB = 32, RT = 64 * NW * 4 / D, E = 8;   // parts per pass, rows per step, steps
+  static_assert(RB % (RT * E) == 0 && sizeof(s_op) >= PB * RB * 4, "the weights fit, rows come out even");
+  float(*s_w)[RB] = (float(*)[RB])s_op;
+  const int used = min(RB, rows - row0), mine = min(tid >> 1, used - 1);
+  float M = -INFINITY, L = 0.f;
+  for (int p0 = 0; p0 < parts; p0 += 16) {
+    uint4 ml[8];
+    float Mn = M;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t at = rec0 + (uint32_t)(min(p0 + i, parts - 1) * RB + r) * (REC * 4);
-        v[i] = ld16_sys(pr, at + d * 4);
-        ml[i] = ld16_sys(pr, at + D * 4);
-      }
-      float Mn = M;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) Mn = fmaxf(Mn, __uint_as_float(ml[i].x));
-      const float Mb = Mn == -INFINITY ? 0.f : Mn, f = ex2(M - Mb);
-      L *= f;
-      A.x *= f;
-      A.y *= f;
-      A.z *= f;
-      A.w *= f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (p0 + i < parts) {
-          const float g = ex2(__uint_as_float(ml[i].x) - Mb);
-          L = fmaf(__uint_as_float(ml[i].y), g, L);
-          A.x = fmaf(__uint_as_float(v[i].x), g, A.x);
-          A.y = fmaf(__uint_as_float(v[i].y), g, A.y);
-          A.z = fmaf(__uint_as_float(v[i].z), g, A.z);
-          A.w = fmaf(__uint_as_float(v[i].w), g, A.w);
-        }
-      M = Mn;
+    for (int i = 0; i < 8; ++i) {
+      const int p = p0 + 2 * i + (tid & 1);
+      ml[i] = ld16_sys(pr, rec0 + (uint32_t)(min(p, parts - 1) * RB + mine) * (REC * 4) + D * 4);
+      if (p >= parts) ml[i].x = __float_as_uint(-INFINITY);
     }
-    float y[4] = {A.x, A.y, A.z, A.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = L == 0.f ? 0.f : attn_div(y[i], L);
-    const int row = row0 + r;
-    const int64_t at = ((int64_t)(c0 + row / a.group) * a.hq + h * a.group + row % a.group) * D + d;
-    if (a.out) *(uint2*)(a.out + at) = make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
-    if (a.out_f32) *(float4*)(a.out_f32 + at) = make_float4(y[0], y[1], y[2], y[3]);
+    for (int i = 0; i < 8; ++i) Mn = fmaxf(Mn, __uint_as_float(ml[i].x));
+    Mn = fmaxf(Mn, __shfl_xor(Mn, 1));
+    const float Mb = Mn == -INFINITY ? 0.f : Mn;
+    L *= ex2(M - Mb);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int p = p0 + 2 * i + (tid & 1);
+      if (p < parts) L = fmaf(__uint_as_float(ml[i].y), ex2(__uint_as_float(ml[i].x) - Mb), L);
+      if (p < min(parts, PB)) s_w[p][tid >> 1] = __uint_as_float(ml[i].x);
+    }
+    M = Mn;
+  }
+  L += __shfl_xor(L, 1);
+  const float Mb = M == -INFINITY ? 0.f : M;
+  __shared__ float s_l[RB];
+  if ((tid & 1) == 0) s_l[tid >> 1] = L;
+  const int r0 = tid / (D / 4), d = tid % (D / 4) * 4;
+  for (int k0 = 0; k0 < used; k0 += RT * E) {   // once at D = 64, twice at 128
+    float4 A[E];
+#pragma unroll
+    for (int k = 0; k < E; ++k) A[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int g0 = 0; g0 < parts; g0 += PB) {
+      const int cnt = min(PB, parts - g0);
+      __syncthreads();
+      if (k0 == 0 || parts > PB) {   // the first ones' references lie there already
+        const bool have = k0 == 0 && g0 == 0;
+        for (int i = tid & 1; i < cnt; i += 2) {
+          const float m = have ? s_w[i][tid >> 1]
+                               : __uint_as_float(ld16_sys(pr, rec0 + (uint32_t)((g0 + i) * RB + mine) *
+                                                                         (REC * 4) + D * 4).x);
+          s_w[i][tid >> 1] = ex2(m - Mb);
+        }
+      }
+      __syncthreads();
+      for (int p0 = 0; p0 < cnt; p0 += 2) {
+        uint4 v[2][E];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int k = 0; k < E; ++k)
+            v[i][k] = ld16_sys(pr, rec0 + (uint32_t)((g0 + min(p0 + i, cnt - 1)) * RB +
+                                                     min(k0 + RT * k + r0, used - 1)) * (REC * 4) + d * 4);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (p0 + i < cnt)
+#pragma unroll
+            for (int k = 0; k < E; ++k) {
+              const float g = s_w[p0 + i][k0 + RT * k + r0];
+              A[k].x = fmaf(__uint_as_float(v[i][k].x), g, A[k].x);
+              A[k].y = fmaf(__uint_as_float(v[i][k].y), g, A[k].y);
+              A[k].z = fmaf(__uint_as_float(v[i][k].z), g, A[k].z);
+              A[k].w = fmaf(__uint_as_float(v[i][k].w), g, A[k].w);
+            }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+      const int r = k0 + RT * k + r0, row = row0 + r;
+      if (r >= used) continue;
+      const float sum = s_l[r];
+      float y[4] = {A[k].x, A[k].y, A[k].z, A[k].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = sum == 0.f ? 0.f : attn_div(y[i], sum);
+      const int64_t at = ((int64_t)(c0 + row / a.group) * a.hq + h * a.group + row % a.group) * D + d;
+      if (a.out) *(uint2*)(a.out + at) = make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
+      if (a.out_f32) *(float4*)(a.out_f32 + at) = make_float4(y[0], y[1], y[2], y[3]);
+    }
   }
 }
 
-// Row blocks of a call, at most, and workgroups that share one: enough to fill the chip where there are
-// few blocks, eight tiles each at least.
+// Row blocks of a call, at most, and workgroups that share one: what the chip holds at once where there are
+// few blocks, of eight tiles each at least, and no more of them than each has tiles (a tile takes 1.3 us,
+// and a part as long to merge). 64 tokens over 8000 positions, 40 heads of 8 kv heads: 49 us in 15 parts,
+// 59 in 8, 65 in 32; 256 tokens 94 in 9, 101 in 10 (a second round of workgroups), 113 in 16.
 static int64_t kv4_row_blocks(int n_seqs, int total, int group, int rows) {
   return n_seqs + (int64_t)total * group / rows;
 }
 static int kv4_block_split(int64_t blocks, int tiles) {
   if (blocks >= 512) return 1;
-  int64_t s = (768 + blocks - 1) / blocks;
+  int64_t s = 768 / blocks;
   s = s < tiles / 8 ? s : tiles / 8;
-  return (int)(s < 1 ? 1 : (s > 32 ? 32 : s));
+  if (s > 32) s = 32;
+  while (s > 1 && s * s > tiles) --s;
+  return (int)(s < 1 ? 1 : s);
 }
 
 // Bytes that a choice made here asks for, at most: within a default workspace.

@@ -379,6 +379,25 @@ def test_prompt_rows_before_the_cache_are_zero(dev):
     assert not got[:10].any() and got[10].any()
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n_split", [5, 17, 32, 63])
+def test_blocks_merged_from_many_parts(dev, d, n_split):
+    """Parts by the dozen (more than are weighed at a time among them), some of which some rows do not see
+    at all, row blocks that end in the middle, and a sequence that is one part beside one of many."""
+    x = Case(dev, 33, 1, d, 64, [2010, 40])
+    x.fill([2010, 40])
+    q, cu = x.q(53, 3, 3.0), [0, 50, 53]
+    want, bound = x.want(q, [(0, range(1961, 2011)), (50, range(38, 41))], d ** -0.5)
+    check(*x.c.attn(0, up(q, dev), ints([2010, 40], dev), cu=ints(cu, dev), n_split=n_split, want_f32=True),
+          want, bound)
+    q = x.q(2010, 3)
+    rows = [0, 1, 31, 32, 500, 1279, 1999, 2009]
+    got, got32 = x.c.attn(0, up(q, dev), ints([2010, 0], dev), cu=ints([0, 2010, 2010], dev), n_split=n_split,
+                          want_f32=True)
+    want, bound = ko.attention(x.o, x.table[0], q[rows].astype(np.float64), [r + 1 for r in rows], d ** -0.5)
+    check(got[rows], got32[rows], want, bound)
+
+
 def test_lengths_of_the_lowest_value(dev):
     """lens of -2^31: nothing is seen, by single tokens and by blocks."""
     x = Case(dev, 27, 2, 64, 32, [40, 40])
