@@ -1074,20 +1074,27 @@ __global__ __launch_bounds__(64 * kv4_block_waves<32 * NG>()) void kv4_block_ker
   }
 }
 
-// Row blocks of a call, at most, and workgroups that share one: what the chip holds at once where there are
-// few blocks, of eight tiles each at least, and no more of them than each has tiles (a tile takes 1.3 us,
-// and a part as long to merge). 64 tokens over 8000 positions, 40 heads of 8 kv heads: 49 us in 15 parts,
-// 59 in 8, 65 in 32; 256 tokens 94 in 9, 101 in 10 (a second round of workgroups), 113 in 16.
+// Row blocks of a call, at most.
 static int64_t kv4_row_blocks(int n_seqs, int total, int group, int rows) {
   return n_seqs + (int64_t)total * group / rows;
 }
+// Workgroups that share a row block's tiles: the number that takes least by what was measured (us at
+// D = 64; both terms are twice as long at 128). A tile takes 1.3 where a CU has one workgroup, 1.8 with two
+// and 2.2 with the three it can hold; merging 3, 0.5 for each part, and 0.0175 for each record. 64 tokens over
+// 8000 positions, 40 heads of 8 kv heads: 49 us in 15 parts, 59 in 8, 65 in 32; 256 tokens 90 in 9,
+// 101 in 10 (a second round of workgroups), 311 in one; 4 tokens over 1000 15 in 8, 20 in 3.
 static int kv4_block_split(int64_t blocks, int tiles) {
-  if (blocks >= 512) return 1;
-  int64_t s = 768 / blocks;
-  s = s < tiles / 8 ? s : tiles / 8;
-  if (s > 32) s = 32;
-  while (s > 1 && s * s > tiles) --s;
-  return (int)(s < 1 ? 1 : s);
+  int best = 1;
+  float least = 0.f;
+  for (int s = 1; s <= 32 && s <= tiles && (s == 1 || blocks * s <= 768); ++s) {
+    const float tile = blocks * s <= 256 ? 1.3f : blocks * s <= 512 ? 1.8f : 2.2f;
+    const float cost = (float)((tiles + s - 1) / s) * tile + (s == 1 ? 0.f : 3.f + s * (0.5f + 0.0175f * (float)blocks));
+    if (s == 1 || cost < 0.97f * least) {
+      best = s;
+      least = cost;
+    }
+  }
+  return best;
 }
 
 // Bytes that a choice made here asks for, at most: within a default workspace.
