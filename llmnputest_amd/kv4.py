@@ -135,11 +135,18 @@ class Kv4Cache:
             raise ValueError(f"{name} must be a contiguous list")
         return t
 
-    def _rows(self, t: torch.Tensor, name: str, heads: int) -> torch.Tensor:
-        self._tensor(t, name, torch.bfloat16)
-        if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != self.head_dim or t.stride(2) != 1:
-            raise ValueError(f"{name} must be [rows, {heads}, {self.head_dim}], channels contiguous")
-        return t
+    def _rows(self, k: torch.Tensor, v: torch.Tensor) -> tuple[int, int, int]:
+        """Rows of k and v, their row and head strides."""
+        for t, name in ((k, "k"), (v, "v")):
+            if t.get_device() != self._index or t.dtype != torch.bfloat16:
+                self._tensor(t, name, torch.bfloat16)
+        shape, stride = k.shape, k.stride()
+        if len(shape) != 3 or shape[1] != self.n_kv_heads or shape[2] != self.head_dim or stride[2] != 1:
+            raise ValueError(f"k must be [rows, {self.n_kv_heads}, {self.head_dim}], channels contiguous")
+        if v.shape != shape or v.stride() != stride:
+            raise ValueError("k and v must have one shape and one layout")
+        # strides of one row or one head say nothing
+        return shape[0], stride[0] if shape[0] > 1 else 0, stride[1] if shape[1] > 1 else 0
 
     def _query(self, q: torch.Tensor) -> tuple[int, int, int]:
         """Rows, heads and row stride of q."""
@@ -169,18 +176,12 @@ class Kv4Cache:
         positions pos[b], pos[b] + 1, .. of every sequence: one row each, or rows cu[b] .. cu[b+1] - 1
         (int32 [n_seqs + 1]); max_new: at least the most rows of one sequence (default: all rows)."""
         c, b = self._layer(layer, table)
-        self._rows(k, "k", self.n_kv_heads)
-        self._rows(v, "v", self.n_kv_heads)
-        n = k.shape[0]
-        if k.shape != v.shape or k.stride() != v.stride():
-            raise ValueError("k and v must have one shape and one layout")
+        n, row, head = self._rows(k, v)
         if cu is None and n != b:
             raise ValueError(f"{n} rows for {b} sequences (give cu for other numbers of rows)")
         if n == 0:
             return
-        # strides of one row or one head say nothing
-        self._call_append(c, k, v, 0, n, k.stride(0) if n > 1 else 0,
-                          k.stride(1) if k.shape[1] > 1 else 0, 0, pos, cu, max_new or n)
+        self._call_append(c, k, v, 0, n, row, head, 0, pos, cu, max_new or n)
 
     def append_cached(self, layer: int, k_cache: torch.Tensor, v_cache: torch.Tensor, pos: torch.Tensor,
                       cu: torch.Tensor | None = None, max_new: int | None = None,
@@ -218,7 +219,8 @@ class Kv4Cache:
         u = None if cu is None else self._ints(cu, "cu", b + 1)
         n = b if cu is None else int(cu[-1]) if total is None else total
         shape = (max(n, 0), self.n_kv_heads, self.head_dim)
-        k, v = torch.empty((2, *shape), dtype=dtype, device=self.device).unbind(0)
+        k = torch.empty(shape, dtype=dtype, device=self.device)
+        v = torch.empty_like(k)
         if n > 0:
             self._call("q4nx_kv4_read", c, k.data_ptr(), v.data_ptr(), int(dtype == torch.float32), n, p,
                       u, 1 if cu is None else max_new or n, ops._stream())
