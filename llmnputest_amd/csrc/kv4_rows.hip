@@ -221,6 +221,13 @@ __global__ __launch_bounds__(512) void kv4_append_kernel(Kv4RowArgs a) {
   const int64_t src = (a.by_position ? s.b * a.seq_stride : 0) + s.h * a.head_stride;
   const uint16_t* rows = is_v ? a.v : a.k;
   const bool any = t0 < t1;
+  // the page's bounds so far, on their way while rows are quantised: with 128 threads and more, two of the
+  // 2 D for each
+  uint16_t* bounds = (uint16_t*)(head + a.c.tiles * kv4_tile_bytes(D));
+  const bool begins = s.first == s.page * a.c.page_len;
+  uint32_t bound0[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) bound0[i] = bounds[min(tid + i * (int)blockDim.x, 2 * D - 1)];
 
   u32x4_t x[2][NG], old[C];
   uint32_t keep = 0;   // nibbles of V's dwords whose positions are not new
@@ -342,16 +349,16 @@ __global__ __launch_bounds__(512) void kv4_append_kernel(Kv4RowArgs a) {
   }
   __syncthreads();
   // ---- the page's bounds: of this call's rows, with the older ones' unless the page begins here
-  uint16_t* bounds = (uint16_t*)(head + a.c.tiles * kv4_tile_bytes(D));
-  const bool begins = s.first == s.page * a.c.page_len;
-  for (int e = tid; e < 2 * D; e += (int)blockDim.x) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int e = tid + i * (int)blockDim.x;
+    if (e >= 2 * D) break;
     const int side = e / D, ch = e % D;
     short x = s_b[0][side][ch];
     for (int w = 1; w < a.c.tiles; ++w) x = bound_of(x, s_b[w][side][ch], side);
     if (!begins) {
-      const uint32_t y = bounds[e];
-      const bool nan = (y & 0x7FFFu) > 0x7F80u;
-      x = bound_of(x, nan ? (short)0x7FC0 : order(y)[0], side);
+      const bool nan = (bound0[i] & 0x7FFFu) > 0x7F80u;
+      x = bound_of(x, nan ? (short)0x7FC0 : order(bound0[i])[0], side);
     }
     bounds[e] = x == 0x7FC0 ? (uint16_t)0x7FC0 : (uint16_t)as_u32(order((uint32_t)(uint16_t)x));
   }
