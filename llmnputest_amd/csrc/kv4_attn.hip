@@ -42,8 +42,10 @@ constexpr int kWaves = 4;
 // Tiles of a call above which its workgroups share one line of them, and how many there have to be for
 // each (sequence, kv head) as a mean.
 constexpr int kLineTiles = 16384;
-// From so many (sequence, kv head)s of at most so many tiles on, each is one part.
-constexpr int kWholeItems = 1024, kWholeTiles = 64;
+constexpr int kMostTiles = 128, kMostParts = 32;   // of a part and of an item (a mean) that are not on a line
+// A (sequence, kv head) is one part where it has at most kShortTiles, and from kWholeItems of them of at
+// most kWholeTiles on.
+constexpr int kShortTiles = 32, kWholeItems = 512, kWholeTiles = 64;
 __host__ __device__ constexpr int kv4_line_mean(int d) { return d == 64 ? 256 : 64; }
 // Those workgroups: what the chip holds at once (three waves per SIMD at D = 64, two at 128).
 __host__ __device__ constexpr int kv4_line(int d) { return d == 64 ? 768 : 512; }
@@ -231,15 +233,17 @@ __device__ __forceinline__ void kv4_finish(const Kv4AttnArgs& a, float (*s_o)[RO
 // A wave takes every fourth tile of its part; a lane finds the page of one of the wave's next 64
 // tiles, so table and list are read ahead, and two tiles are in flight while one is computed.
 //
-// Who does what is decided here, from the lengths as they are: of W tiles in all a part has
-//   8 (W < 1024), 16 (W < 8192), 32 (W <= 32768) or 64 tiles of one (sequence, kv head);
-// from 16384 tiles on, if that is more than 256 (D = 64; 64 at 128) for each (sequence, kv head), the W
-// tiles are one line that 768 (512) workgroups cut evenly, so that lengths however unlike load the chip
-// alike, and a workgroup's stretch may end one (sequence, kv head) and begin the next. Times in us with
-// 40 heads of 8 kv heads, line / parts of 64: b8 x 65536 45.6 / 50.2, b1 x 131072 34 / 38, b32 x 8192
-// 38 / 31, b64 x 4096 48 / 31; 64 heads of D = 128, b32 x 8192 56 / 63. From 1024 (sequence, kv head)s of
-// at most 64 tiles on, known from the call's sizes, each is one part and nothing is looked for: b2040 x
-// 128 109 (292 with the search), b256 x 512 25 (33).
+// Who does what is decided here, from the lengths as they are. Of W tiles in all a part has W / 768 (D = 64;
+// 512 at 128: what the chip holds at once, less half a part for each item) of one (sequence, kv head), at
+// least 8 (W < 1024) or 16, at most 128 and no more than 32 parts an item as a mean; from 16384 tiles on, if
+// that is more than 256 (64 at 128) for each item, the W tiles are one line that 768 (512) workgroups cut
+// evenly, so that lengths however unlike load the chip alike, and a workgroup's stretch may end one item
+// and begin the next. Times in us with 40 heads of 8 kv heads, line / parts: b8 x 65536 45.6 / 50.2,
+// b1 x 131072 34 / 38, b32 x 8192 38 / 28, b64 x 4096 48 / 32; 64 heads of D = 128, b32 x 8192 56 / 63. In
+// parts of 32 tiles as against W / 512, 32 heads of D = 128, b16 x 5003: 22.3 / 20.4.
+// Known from the call's sizes, items of at most 32 tiles are one part each, and from 512 items on of at
+// most 64, and nothing is looked for: b1 x 513 7.9 (9.1 in three parts), b64 x 1024 12.0 (15.8), b64 x 2048
+// 19.2 (21.6), b2040 x 128 107 (292); but b1 x 1300 12.0 (9.4 in parts), b16 x 2048 15.6 (12.4).
 
 // x / y for quotients below 2^20 or so: the reciprocal is off by less than one in them.
 __device__ __forceinline__ int div_few(int x, int y) {
@@ -329,12 +333,13 @@ __global__ __launch_bounds__(256) void kv4_decode_kernel(Kv4AttnArgs a) {
   const int W = a.unit ? 0 : find(0x7FFFFFFF, [](int x) { return x; }).before * hkv;
   const bool line = a.unit == 0 && W > kLineTiles && W > (int64_t)kv4_line_mean(D) * nb * hkv;
   if (line && (int)blockIdx.x >= kLine) return;
-  // parts of their own have 8, 16, 32 or 64 tiles (or as many as asked for)
-  const int sh = W < 1024 ? 3 : W < 8192 ? 4 : W <= 2 * kLineTiles ? 5 : 6;
-  const int unit = a.unit ? a.unit : line ? (W + kLine - 1) / kLine : 1 << sh;
-  auto share = [&](int x) {
-    return line ? x : a.unit ? div_few(x + unit - 1, unit) : (x + unit - 1) >> sh;
-  };
+  // parts of their own: as many as the chip holds at once (half of an item's last part is empty as a mean)
+  const int room = max(kLine - nb * hkv / 2, kLine / 2);
+  const int unit = a.unit ? a.unit
+                   : line ? (W + kLine - 1) / kLine
+                          : min(max(max((W + room - 1) / room, W / (kMostParts * nb * hkv)),
+                                    W < 1024 ? 8 : 16), kMostTiles);
+  auto share = [&](int x) { return line ? x : div_few(x + unit - 1, unit); };
 
   for (int at = blockIdx.x * (line ? unit : 1), left = line ? unit : 1;;) {
   Where f{at / hkv, at / hkv, 1, 0};
@@ -1143,16 +1148,17 @@ static Kv4Plan kv4_plan(const q4nx_kv4* c, int n_q_heads, int total, int max_len
     p.items = (int64_t)c->n_seqs * c->n_kv_heads;
     rows = (group + 3) / 4 * 4;
     if (n_split > 0) p.unit = (tiles + n_split - 1) / n_split;
-    // no counter for each, or so many short ones that they fill the chip and end together
-    else if (p.items * 4 > Q4NX_WS_COUNTER_BYTES || (p.items >= kWholeItems && tiles <= kWholeTiles))
+    // no counter for each, or short ones (so many of them that they fill the chip and end together)
+    else if (p.items * 4 > Q4NX_WS_COUNTER_BYTES || tiles <= kShortTiles ||
+             (p.items >= kWholeItems && tiles <= kWholeTiles))
       p.unit = tiles;
-    // by what there is: parts of 8 tiles and more, of 64 where they are many but few for each item, or
-    // one line
+    // by what there is: parts of 8 tiles and more, as many as there is room for besides one for each item
+    // (or of kMostTiles), or one line
     const int line = kv4_line(c->head_dim);
-    const int64_t all = p.items * tiles, some = all < kLineTiles ? all : kLineTiles;
-    const int64_t few = kv4_line_mean(c->head_dim) * p.items, mean = (all < few ? all : few) / 64;
+    const int64_t all = p.items * tiles, room = all / 8 < line ? all / 8 : line;
+    const int64_t few = kv4_line_mean(c->head_dim) * p.items, most = (all < few ? all : few) / kMostTiles;
     p.grid = p.unit ? p.items * ((tiles + p.unit - 1) / p.unit)
-                    : p.items + (some / 8 > mean ? some / 8 : mean);
+                    : p.items + (room > most ? room : most);
     if (!p.unit && p.items * ((tiles + 7) / 8) < p.grid) p.grid = p.items * ((tiles + 7) / 8);
     if (!p.unit && all > kLineTiles && p.grid < line) p.grid = line;
     recs = p.grid > 2 * line ? p.grid : 2 * line;

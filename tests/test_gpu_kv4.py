@@ -451,7 +451,7 @@ def test_many_sequences(dev, n_seqs, d):
             check(block[0][rows], block[1][rows], want, bound)
 
 
-@pytest.mark.parametrize("n_seqs,tiles,d", [(1024, 8, 64), (1100, 2, 128), (120, 20, 64),
+@pytest.mark.parametrize("n_seqs,tiles,d", [(1024, 8, 64), (1100, 2, 128), (120, 20, 64), (100, 35, 64),
                                             (80, 260, 64), (70, 70, 128)])
 def test_many_short_sequences_share_a_line(dev, n_seqs, tiles, d):
     """More than 16384 tiles in (sequence, kv head)s of at most eight: some end one workgroup's stretch and

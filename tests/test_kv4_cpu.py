@@ -168,7 +168,8 @@ def shares(lens, hkv, cap, line_groups, mean):
     total = sum(tiles) * hkv
     out = []
     if total <= 16384 or total <= mean * len(lens) * hkv:
-        unit = 8 if total < 1024 else 16 if total < 8192 else 32 if total <= 32768 else 64
+        room = max(line_groups - len(lens) * hkv // 2, line_groups // 2)
+        unit = min(max(-(-total // room), total // (32 * len(lens) * hkv), 8 if total < 1024 else 16), 128)
         at = 0
         for b, n in enumerate(tiles):
             for h in range(hkv):
@@ -199,11 +200,17 @@ def test_the_workspace_holds_every_share(d, groups, mean):
         group = int(rng.integers(1, 17))
         size = _lib.lib().q4nx_kv4_attn_ws_bytes(C.byref(c), group * hkv, 0, 1, 1 << 30, 0, 0)
         records = (size - 65536) // (-(-group // 4) * 4 * (d + 4) * 4) if size else 0
-        if n_seqs * hkv >= 1024 and tiles <= 64:
+        if tiles <= 32 or (n_seqs * hkv >= 512 and tiles <= 64):
             assert size == 0   # one part each
             continue
         for lens in ([tiles * 32] * n_seqs, [0] * n_seqs, rng.integers(0, tiles * 32 + 40, n_seqs)):
-            cut = [x for x in shares(lens, hkv, tiles * 32, groups, mean) if x[2] > 1]
+            all_ = shares(lens, hkv, tiles * 32, groups, mean)
+            cut = [x for x in all_ if x[2] > 1]
+            items, most = n_seqs * hkv, n_seqs * hkv * tiles
+            grid = items + max(min(most // 8, groups), min(most, mean * items) // 128)   # as launched
+            line = sum(max(1, -(-min(int(n), tiles * 32) // 32)) for n in lens) * hkv
+            if not (line > 16384 and line > mean * items):
+                assert len(all_) <= min(grid, items * -(-tiles // 8)) or most > 16384 and len(all_) <= max(grid, groups)
             if not size and 5 * n_seqs * hkv * -(-group // 4) * 16 * (d + 4) > 192 << 20:
                 continue   # records of thousands of items would not fit: one part each
             assert not cut or size, (n_seqs, hkv, tiles)
