@@ -228,8 +228,8 @@ __device__ __forceinline__ void kv4_finish(const Kv4AttnArgs& a, float (*s_o)[RO
 // register as it is, so the writes are consecutive dwords and an operand one 16-byte read. The scales
 // are one load of 4 NG bytes a lane (K's positions in lanes 0..31, V's in 32..63), spread by lane swaps.
 // Bound by its instructions, some 165 of the VALU and 12 of the matrix cores a tile (a third of them takes
-// the codes apart): 8 sequences of up to 65536 positions, 180 MB, in 45.8 us, 3.9 TB/s of the 6.5 that a
-// plain read reaches. Short calls are a chain of latencies: 1 x 513 takes 8.7.
+// the codes apart): 8 sequences of up to 65536 positions, 180 MB, in 45.4 us, 4.0 TB/s of the 6.5 that a
+// plain read reaches. Short calls are a chain of latencies: 1 x 513 takes 7.9.
 // A wave takes every fourth tile of its part; a lane finds the page of one of the wave's next 64
 // tiles, so table and list are read ahead, and two tiles are in flight while one is computed.
 //
