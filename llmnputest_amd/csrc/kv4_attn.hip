@@ -55,9 +55,7 @@ constexpr int kMergeBatch = 8;    // of them in flight per thread
 // x - bf16 (the lo or hi half of pair) in one instruction; the difference of a number and its bf16
 // rounding is exact. The pair (-1, 0) comes from a register: as an inline constant -1.0 the
 // instruction takes it for (0, -1).
-typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 typedef short s16x2_t __attribute__((ext_vector_type(2)));
-typedef short s16x4_t __attribute__((ext_vector_type(4)));
 struct Kv4Minus {
   uint32_t lo = 0x0000BF80u, hi = 0xBF800000u;
   __device__ Kv4Minus() { asm volatile("" : "+v"(lo), "+v"(hi)); }
