@@ -215,10 +215,12 @@ __global__ __launch_bounds__(kSelThreads) void kv4_select_kernel(Kv4SelArgs a) {
     if (tid < 256) s_hist[tid] = 0;
     __syncthreads();
   }
-  // the pages in order: a wave's stretch of them, 64 at a time
+  // the pages in order: a wave's stretch of them, 64 at a time; special keys lie above every score, also
+  // where a score of +inf has their leading digits
   const int span = (np + kSelThreads - 1) / kSelThreads * 64, e0 = wave * span, e1 = min(np, e0 + span);
-  auto is_gt = [&](int e) { return e < e1 && ((s_key[e] >> shift) > prefix); };
-  auto is_eq = [&](int e) { return e < e1 && ((s_key[e] >> shift) == prefix); };
+  auto above = [&](unsigned long long k) { return !all && k >= kSpecial; };
+  auto is_gt = [&](int e) { return e < e1 && (above(s_key[e]) || (s_key[e] >> shift) > prefix); };
+  auto is_eq = [&](int e) { return e < e1 && !above(s_key[e]) && (s_key[e] >> shift) == prefix; };
   int gt = 0, eq = 0;
   for (int e = e0; e < e1; e += 64) {
     gt += __popcll(__ballot(is_gt(e + lane)));

@@ -1,0 +1,54 @@
+"""Edges of the paged 4-bit K/V cache: infinities in a query, counts past one wave, lengths of zero,
+positions at the ends of 32 bits, strides that say nothing."""
+
+import numpy as np
+import pytest
+import torch
+
+from llmnputest_amd import kv4
+from oracle import kv4_oracle as ko
+from tests.test_gpu_kv4 import Case, bf16, ints, up
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------ selection
+
+def signed_pages(dev, d, page, n, infinite, ch, hkv=1):
+    """n pages whose channel `ch` of K is positive in the pages `infinite` and negative in the others."""
+    x = Case(dev, 50, hkv, d, page, [n * page])
+    k, v = x.rows(n * page), x.rows(n * page)
+    k[..., ch] = -bf16(1 + np.abs(k[..., ch]))
+    for p in infinite:
+        k[p * page:(p + 1) * page, :, ch] *= -1
+    x.c.append(0, up(k, dev), up(v, dev), ints([0], dev), ints([0, n * page], dev))
+    x.o.append(x.table, [0], [range(n * page)], k, v)
+    return x
+
+
+@pytest.mark.parametrize("d,page", [(64, 32), (128, 64)])
+@pytest.mark.parametrize("infinite", [[4, 9], [4], [1, 2, 3, 5, 8, 12], [0, 13], list(range(14)), []], ids=str)
+@pytest.mark.parametrize("n_sel,first,last", [(4, 1, 1), (3, 0, 1), (2, 0, 0), (6, 3, 1), (2, 1, 1)])
+def test_select_with_an_infinity_in_q(dev, d, page, infinite, n_sel, first, last):
+    """Scores of +inf and -inf: the pages always read are there, then the infinite ones, the lowest first,
+    and every entry is written, however many of them the list holds."""
+    x = signed_pages(dev, d, page, 14, infinite, 5)
+    q = x.q(1, 3)
+    q[0, 1, 5] = np.inf
+    out = torch.full((1, 1, n_sel), -77, dtype=torch.int32, device=dev)
+    x.c.select(0, up(q, dev), ints([14 * page], dev), n_sel, first, last, out=out)
+    want = ko.select(x.o, x.table[0], q[0].astype(np.float64), 14 * page, n_sel, first, last)
+    assert np.array_equal(out[0].cpu().numpy(), want)
+
+
+def test_select_with_infinities_of_both_signs(dev):
+    """-inf in q, and +inf in one channel against -inf in another (scores that are NaN): as many lists as
+    there are kv heads, each with its own."""
+    x = signed_pages(dev, 64, 32, 20, [2, 7, 11], 40, hkv=2)
+    q = x.q(1, 4)
+    q[0, 0, 40], q[0, 3, 40], q[0, 3, 41] = -np.inf, np.inf, -np.inf
+    for n_sel, first, last in ((5, 1, 1), (3, 1, 1), (17, 2, 3), (19, 0, 0)):
+        with np.errstate(invalid="ignore"):
+            want = ko.select(x.o, x.table[0], q[0].astype(np.float64), 640, n_sel, first, last)
+        got = x.c.select(0, up(q, dev), ints([640], dev), n_sel, first, last)
+        assert np.array_equal(got[0].cpu().numpy(), want), n_sel
