@@ -212,6 +212,7 @@ __global__ __launch_bounds__(kPlan) void kv4_reserve_kernel(Kv4PoolArgs a) {
   __shared__ int s_w[kPlan / 64], s_bad;
   const int tid = threadIdx.x;
   if (tid == 0) s_bad = 0;
+  __syncthreads();   // before any wave counts
   int need = 0;
   for (int b0 = 0; b0 < a.c.n_seqs; b0 += kPlan) {
     const int b = b0 + tid;

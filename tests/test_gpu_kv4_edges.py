@@ -52,3 +52,24 @@ def test_select_with_infinities_of_both_signs(dev):
             want = ko.select(x.o, x.table[0], q[0].astype(np.float64), 640, n_sel, first, last)
         got = x.c.select(0, up(q, dev), ints([640], dev), n_sel, first, last)
         assert np.array_equal(got[0].cpu().numpy(), want), n_sel
+
+
+# ------------------------------------------------------------------ bookkeeping
+
+@pytest.mark.parametrize("n_seqs,n_pages", [(700, 1000), (3000, 20000), (65, 400)])
+def test_reserve_counts_what_every_wave_refuses(dev, n_seqs, n_pages):
+    """Hundreds of sequences that want more than their row holds, in every wave of the launch and in more
+    than one round of it: `status` counts each."""
+    rng = np.random.default_rng(n_seqs)
+    for turn in range(6):
+        c = kv4.Kv4Cache(1, n_pages, n_seqs, 4 * 32, n_kv_heads=1, page_len=32, device=dev)
+        book = ko.Book(n_seqs, 4, n_pages, 32)
+        want = rng.integers(0, 4 * 32 + 1, n_seqs)
+        over = rng.random(n_seqs) < 0.5
+        over[64:] |= turn == 0          # all of them but the first wave's
+        want[over] += 4 * 32 + 1
+        c.reserve(want.tolist())
+        bad = book.reserve(want)
+        assert int(c.status) == bad >= over.sum(), turn
+        assert np.array_equal(c.table.cpu().numpy(), book.table)
+        assert np.array_equal(c.refs.cpu().numpy(), book.refs)
