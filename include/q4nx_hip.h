@@ -399,7 +399,7 @@ int q4nx_kv4_reserve(const q4nx_kv4 *cache, int32_t *refs, const int32_t *want, 
 /* fork: sequence dst[i] goes on from src[i]: its full pages are shared, the last, partly filled one is
  * copied (in every layer) into the lowest free page, in the order of the pairs; lens[dst] = lens[src].
  * A pair is not done if an index is outside the sequences, dst is a source or an earlier pair's dst or
- * has pages, or no page is free. */
+ * has pages, src does not have the page of its position lens[src] - 1, or no page is free. */
 int q4nx_kv4_fork(const q4nx_kv4 *cache, int64_t layer_stride, int n_layers, int32_t *lens,
                   int32_t *refs, const int32_t *src, const int32_t *dst, int n, int32_t *status,
                   void *ws, size_t ws_bytes, void *stream);

@@ -102,9 +102,10 @@ __global__ __launch_bounds__(kPlan) void kv4_fork_plan(Kv4PoolArgs a) {
       const int s = a.src[i], d = a.dst[i];
       if (s >= 0 && s < a.c.n_seqs && d >= 0 && d < a.c.n_seqs && s_owner[d] == i &&
           !((s_src[d >> 5] >> (d & 31)) & 1) && a.c.table[(int64_t)d * a.c.table_stride] < 0) {
+        // rows hold their pages from the front: with its last one a source has all that its length needs
         const int len = max(0, min(a.lens[s], a.c.cap));
-        if (len % a.c.page_len == 0) state = -1;
-        else if (kv4_page(a.c, s, len / a.c.page_len) >= 0) state = 0;
+        if (len == 0 || kv4_page(a.c, s, (len - 1) / a.c.page_len) >= 0)
+          state = len % a.c.page_len == 0 ? -1 : 0;
       }
       bad += state == -2;
     }

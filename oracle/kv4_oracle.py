@@ -255,7 +255,11 @@ class Book:
             if not first or d in sources or self.table[d, 0] >= 0:
                 bad += 1
                 continue
-            full, rest = divmod(int(self.lens[s]), self.page)
+            length = int(self.lens[s])
+            full, rest = divmod(length, self.page)
+            if length and not 0 <= self.table[s, (length - 1) // self.page] < len(self.refs):
+                bad += 1
+                continue
             if rest and not free:
                 bad += 1
                 continue

@@ -73,3 +73,33 @@ def test_reserve_counts_what_every_wave_refuses(dev, n_seqs, n_pages):
         assert int(c.status) == bad >= over.sum(), turn
         assert np.array_equal(c.table.cpu().numpy(), book.table)
         assert np.array_equal(c.refs.cpu().numpy(), book.refs)
+
+
+def test_fork_of_a_source_without_its_pages(dev):
+    """A source's length past the pages it has, a multiple of the page among them, is not done and changes
+    nothing; at its last page it is done; a length of zero shares nothing."""
+    for extra, done in ((0, True), (1, False), (31, False), (32, False), (64, False), (-1, True), (-64, True)):
+        c = kv4.Kv4Cache(1, 9, 3, 6 * 32, n_kv_heads=1, page_len=32, device=dev)
+        book = ko.Book(3, 6, 9, 32)
+        c.reserve([64, 0, 20])
+        book.reserve([64, 0, 20])
+        book.lens[:] = [64 + extra, 0, 20]
+        c.lens.copy_(torch.from_numpy(book.lens))
+        c.fork([0, 2], [1, 1])       # the second pair's dst is taken either way
+        assert book.fork([0, 2], [1, 1]) == 2 - done
+        assert int(c.status) == 2 - done, extra
+        assert np.array_equal(c.table.cpu().numpy(), book.table), extra
+        assert np.array_equal(c.refs.cpu().numpy(), book.refs), extra
+        assert np.array_equal(c.lens.cpu().numpy(), book.lens), extra
+        assert (c.table[1, 0] >= 0).item() == (done and extra > -64)
+
+
+def test_fork_of_a_row_that_names_no_page(dev):
+    """The last full page's entry lies outside the pool: not done, and no entry of it is handed on."""
+    c = kv4.Kv4Cache(1, 9, 2, 6 * 32, n_kv_heads=1, page_len=32, device=dev)
+    c.reserve([64, 0])
+    c.table[0, 1] = 1 << 20
+    c.lens.copy_(ints([64, 0], dev))
+    c.fork([0], [1])
+    assert int(c.status) == 1 and (c.table[1] == -1).all() and c.lens.tolist() == [64, 0]
+    assert c.refs.tolist() == [1, 1] + [0] * 7
