@@ -384,7 +384,10 @@ class GraniteDecoder:
         for s, x in zip(src, lens):
             kv.lens[s] = x
         kv.fork(src, dst)
+        undone = kv.status.clone()   # reserve() reports there too
         kv.reserve([self.max_len] * n)
+        if int(undone):
+            raise RuntimeError("a source lacks pages of its prefix, or the pool has none left for the copies")
         if int(kv.status):
             raise RuntimeError("the pool has no pages left for the forked sequences")
 
