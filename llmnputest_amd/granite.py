@@ -391,6 +391,21 @@ class GraniteDecoder:
         if int(kv.status):
             raise RuntimeError("the pool has no pages left for the forked sequences")
 
+    def reset(self, seqs) -> None:
+        """The sequences give up their pages, shared ones too, for pages of their own; what they held is
+        gone (kv="q4")."""
+        if self.kv is None:
+            raise ValueError('reset needs kv="q4"')
+        seqs = sorted({int(x) for x in seqs})
+        if not all(0 <= x < self.max_batch for x in seqs):
+            raise ValueError(f"sequences must be in [0, {self.max_batch})")
+        if not seqs:
+            return
+        self.kv.free(seqs)
+        self.kv.reserve([self.max_len] * self.max_batch)
+        if int(self.kv.status):
+            raise RuntimeError("the pool has no pages left for the sequences")
+
     def _trace_layer(self, tr: dict, li: int, b: int, pos_host, mlp) -> dict:
         """Host copies of one layer's bf16 narrowing points (uint16 bits): the normalised
         inputs, q and k narrowed before the rotation (from the fp32 GEMV outputs), q after
@@ -509,6 +524,8 @@ class GraniteDecoder:
     def seed_cache(self, ctx: int, seed: int = 0) -> None:
         """Fill positions [0, ctx) of every layer's K/V cache with bf16 N(0,1) (a synthetic
         context; no prefill runs through the model)."""
+        if self.kv is not None:   # every sequence writes its own rows
+            self.reset(range(self.max_batch))
         g = torch.Generator(device=self.dev)
         g.manual_seed(seed)
         rows = torch.arange(self.max_batch + 1, dtype=torch.int32, device=self.dev) * ctx
