@@ -246,6 +246,8 @@ class GraniteDecoder:
                                c.head_dim, page_len, device=dev)
             self.kv.reserve([self.max_len] * b)
             self.sel = torch.full((b, c.n_kv, max(1, sparse_pages)), -1, dtype=torch.int32, device=dev)
+        # per sequence, where pages begin that no other one can have (on a page's border)
+        self._own_from = [0] * b
         self.rope = ops.rope_table(self.max_len, c.head_dim, c.theta, device=dev)
         self.h = torch.zeros((b, c.hidden), dtype=torch.float32, device=dev)
         # sums of h^2 per 16 entries, written by each producer of h for the next RMSNorm
@@ -367,8 +369,8 @@ class GraniteDecoder:
     def fork(self, src, dst, lens) -> None:
         """Sequences dst go on from the first lens[i] positions of src[i] (kv="q4"): full pages are shared,
         the last one is copied, what dst held is given up. The tokens that follow go on from there
-        through step() or generate() with start positions >= lens. A sequence with shared pages must
-        not be wound back into them."""
+        through step() or generate() with start positions >= lens: positions in pages that another
+        sequence still has are refused there (reset() gives a sequence pages of its own again)."""
         if self.kv is None:
             raise ValueError('fork needs kv="q4"')
         src, dst, lens = [int(x) for x in src], [int(x) for x in dst], [int(x) for x in lens]
@@ -390,6 +392,9 @@ class GraniteDecoder:
             raise RuntimeError("a source lacks pages of its prefix, or the pool has none left for the copies")
         if int(kv.status):
             raise RuntimeError("the pool has no pages left for the forked sequences")
+        for s, d, x in zip(src, dst, lens):
+            self._own_from[d] = x // kv.page_len * kv.page_len
+            self._own_from[s] = max(self._own_from[s], self._own_from[d])
 
     def reset(self, seqs) -> None:
         """The sequences give up their pages, shared ones too, for pages of their own; what they held is
@@ -403,8 +408,26 @@ class GraniteDecoder:
             return
         self.kv.free(seqs)
         self.kv.reserve([self.max_len] * self.max_batch)
+        for x in seqs:
+            self._own_from[x] = 0
         if int(self.kv.status):
             raise RuntimeError("the pool has no pages left for the sequences")
+
+    def _check_own(self, positions, n: int = 1) -> None:
+        """Refuses n positions from positions[i] of sequence i on where a page of them is another's too.
+        Only sequences that were forked, and only positions before that, look at the device."""
+        if self.kv is None:
+            return
+        page = self.kv.page_len
+        for i, p in enumerate(positions):
+            end = min(p + n, self._own_from[i])
+            if p >= end:
+                continue
+            first, last = p // page, -(-end // page)
+            if int(self.kv.refs[self.kv.table[i, first:last].long()].max()) > 1:
+                raise ValueError(f"position {p} of sequence {i} lies in a page that another sequence shares")
+            if last * page == self._own_from[i]:   # the others have ended
+                self._own_from[i] = first * page
 
     def _trace_layer(self, tr: dict, li: int, b: int, pos_host, mlp) -> dict:
         """Host copies of one layer's bf16 narrowing points (uint16 bits): the normalised
@@ -442,6 +465,7 @@ class GraniteDecoder:
             raise ValueError("batch exceeds max_batch or positions do not match tokens")
         if int(positions.max()) >= self.max_len or int(positions.min()) < 0:
             raise ValueError(f"positions must be in [0, {self.max_len})")
+        self._check_own(positions.tolist())
         self.tokens[:b].copy_(tokens)
         self.pos[:b].copy_(positions)
         self.lens[:b].copy_(positions + 1)
@@ -466,6 +490,8 @@ class GraniteDecoder:
         generate()). A second graph holds GRAPH_STEPS such steps back to back: the same
         launches in the same order, so replaying it once equals GRAPH_STEPS replays of the
         first."""
+        if self.kv is not None and any(self._own_from):
+            self._check_own(self.pos[:b].tolist())   # the warm step below writes there
         snap = (self.tokens.clone(), self.pos.clone(), self.lens.clone(), self.step_ctr.clone())
         self._launch_step(b)                       # warm: sizes every workspace
         self._advance(b)
@@ -495,6 +521,7 @@ class GraniteDecoder:
             raise ValueError("start positions must be >= 0, one per sequence")
         if b != self.max_batch:
             raise ValueError("generate() runs all max_batch sequences; size the decoder to them")
+        self._check_own(start.tolist(), n_new)
         # tokens, positions, lengths and the step counter in one copy: four of them, three waited
         # for, added 15 to 30 us to a one-token call
         state = torch.zeros(self._state.shape, dtype=torch.int32, device=first.device)

@@ -60,3 +60,66 @@ def test_reset_gives_pages_of_ones_own(weights):
             dec.reset(bad)
     with pytest.raises(ValueError, match="reset"):
         GraniteDecoder(weights, max_batch=2, max_len=64).reset([0])
+
+
+def pools(dec):
+    return [t.clone() for t in (dec.kv.pool, dec.kv.table, dec.kv.refs)]
+
+
+@pytest.mark.parametrize("page", [32, 64])
+def test_no_row_goes_into_a_shared_page(weights, page):
+    """After a fork: positions in the shared prefix are refused by step(), generate() and capture(), with
+    nothing written, whichever sequence they belong to; positions behind it are taken."""
+    dec = decoder(weights, 3, page_len=page)
+    dec.seed_cache(150, seed=6)
+    dec.fork([0], [1], [140])
+    full = 140 // page * page
+    before = pools(dec)
+    for bad in ([full - 1, 150, 150], [150, 0, 150], [0, 0, 150], [150, full - 1, 150]):
+        with pytest.raises(ValueError, match="shares"):
+            dec.step([1, 2, 3], bad)
+        with pytest.raises(ValueError, match="shares"):
+            dec.generate([1, 2, 3], bad, 40)
+    with pytest.raises(ValueError, match="shares"):
+        dec.step([1], [5])
+    with pytest.raises(ValueError, match="shares"):
+        dec.capture(3)               # its warm step would write at positions 0
+    assert all(torch.equal(a, b) for a, b in zip(before, pools(dec)))
+    dec.step([1, 2, 3], [full, 150, 0])
+    dec.generate([1, 2, 3], [150, full, 17], 5)
+    dec.step([1, 2, 3], [140, 140, 3])
+
+
+def test_a_shared_page_is_ones_own_when_the_others_have_ended(weights):
+    """The source may be wound back once both copies have other pages; a copy after reset(); what a fork
+    from a fork shares is refused in all three."""
+    dec = decoder(weights, 3)
+    dec.seed_cache(150, seed=6)
+    dec.fork([0], [1], [130])
+    dec.fork([1], [2], [70])
+    for bad in ([63, 200, 200], [200, 63, 200], [200, 200, 63], [64, 200, 200], [200, 127, 200]):
+        with pytest.raises(ValueError, match="shares"):
+            dec.step([1, 1, 1], bad)
+    dec.step([1, 1, 1], [128, 128, 64])
+    dec.reset([1])
+    with pytest.raises(ValueError, match="shares"):
+        dec.step([1, 1, 1], [63, 0, 200])
+    dec.step([1, 1, 1], [64, 0, 64])          # the pages from 64 on were shared with sequence 1 alone
+    with pytest.raises(ValueError, match="shares"):
+        dec.generate([1, 1, 1], [60, 0, 200], 10)
+    dec.fork([1], [2], [0])
+    dec.step([1, 1, 1], [0, 0, 0])
+    new = decoder(weights, 3)
+    for d in (dec, new):
+        d.seed_cache(64, seed=2)
+    assert (dec.generate([5, 6, 7], [10, 64, 3], 9)[0] == new.generate([5, 6, 7], [10, 64, 3], 9)[0]).all()
+
+
+def test_a_sequence_wound_back_is_as_new(weights):
+    """A copy that was given up and its source, both started over: the logits of a decoder never forked."""
+    dec, new = decoder(weights, 2, 128), decoder(weights, 2, 128)
+    dec.seed_cache(100, seed=6)
+    dec.fork([0], [1], [100])
+    dec.reset([0, 1])
+    for i in range(3):
+        assert torch.equal(dec.step([9 + i, 3], [i, i]), new.step([9 + i, 3], [i, i]))
