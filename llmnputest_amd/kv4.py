@@ -159,6 +159,11 @@ class Kv4Cache:
         # a single row's stride says nothing
         return shape[0], shape[1], stride[0] if shape[0] > 1 else shape[1] * self.head_dim
 
+    def _most(self, c, max_len: int | None) -> int:
+        """The positions a sequence may have in a call."""
+        cap = c.table_len * self.page_len
+        return cap if max_len is None else min(cap, max_len)
+
     def _need(self, c, fn: str, *args) -> int:
         key = (fn, c.n_seqs, c.table_len, *args)
         n = self._needs.get(key)
@@ -263,7 +268,10 @@ class Kv4Cache:
                 raise ValueError(f"sel must be [{b}, {self.n_kv_heads}, pages]")
             sp, ns = sel.data_ptr(), sel.shape[2]
         new = 1 if cu is None else max_new or n
-        most = min(self.max_len if table is None else c.table_len * self.page_len, max_len or 1 << 30)
+        most = self._most(c, max_len)
+        if most == 0:   # the library wants one position at least: the lengths are zeros instead
+            none = torch.zeros(b, dtype=torch.int32, device=self.device)
+            most, lp = 1, none.data_ptr()
         need = self._need(c, "q4nx_kv4_attn_ws_bytes", hq, 0 if cu is None else n, new, most, ns, n_split)
         wp = wn = 0
         if need:
@@ -294,7 +302,10 @@ class Kv4Cache:
             self._tensor(out, "out", torch.int32)
             if out.shape != (b, self.n_kv_heads, n_sel) or not out.is_contiguous():
                 raise ValueError(f"out must be contiguous [{b}, {self.n_kv_heads}, {n_sel}]")
-        most = min(self.max_len if table is None else c.table_len * self.page_len, max_len or 1 << 30)
+        most = self._most(c, max_len)
+        if most == 0:   # the library wants one position at least: the lengths are zeros instead
+            none = torch.zeros(b, dtype=torch.int32, device=self.device)
+            most, lp = 1, none.data_ptr()
         ws, wp, wn, stream = ops._scratch(ws, self._need(c, "q4nx_kv4_select_ws_bytes", most))
         self._call("q4nx_kv4_select", c, q.data_ptr(), stride, hq, lp, most, n_sel, n_first, n_last,
                    out.data_ptr(), wp, wn, stream)

@@ -103,3 +103,29 @@ def test_fork_of_a_row_that_names_no_page(dev):
     c.fork([0], [1])
     assert int(c.status) == 1 and (c.table[1] == -1).all() and c.lens.tolist() == [64, 0]
     assert c.refs.tolist() == [1, 1] + [0] * 7
+
+
+# ------------------------------------------------------------------ arguments
+
+def test_max_len_of_zero_reads_nothing(dev):
+    """max_len=0 is a bound like any other: zeros, no pages, and rows behind the last sequence as they were."""
+    x = Case(dev, 51, 2, 64, 32, [100, 70])
+    x.fill([100, 70])
+    lens, q = ints([100, 70], dev), up(x.q(2, 6), dev)
+    out = torch.full_like(q, 3.0)
+    got, got32 = x.c.attn(0, q, lens, max_len=0, out=out, want_f32=True)
+    assert got is out and not got.any() and not got32.any()
+    assert not x.c.attn(0, q, lens, max_len=0, n_split=4).any()
+    block = up(x.q(40, 6), dev)
+    out = torch.full_like(block, 3.0)
+    for n_split in (0, 3):
+        x.c.attn(0, block, lens, cu=ints([0, 30, 33], dev), max_len=0, out=out.fill_(3.0), n_split=n_split)
+        assert not out[:33].any() and (out[33:] == 3).all()
+    sel = x.c.select(0, q, lens, n_sel=3, max_len=0)
+    assert (sel == -1).all() and not x.c.attn(0, q, lens, sel=sel).any()
+    assert lens.tolist() == [100, 70]
+    assert x.c.attn(0, q, lens, max_len=1).any()
+    from llmnputest_amd import ops
+    for call in (lambda: x.c.attn(0, q, lens, max_len=-1), lambda: x.c.select(0, q, lens, n_sel=3, max_len=-1)):
+        with pytest.raises(ops._lib.Q4NXError, match="max_len"):
+            call()
