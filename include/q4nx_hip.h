@@ -356,8 +356,8 @@ int q4nx_kv4_read(const q4nx_kv4 *cache, void *k_out, void *v_out, int out_f32, 
  * Without cu, one token per sequence (total = n_seqs): positions [0, lens[b]). With cu, sequence b's
  * tokens are rows cu[b] .. cu[b+1] - 1, the last of them at position lens[b] - 1: token i of n sees
  * positions [0, lens[b] - n + 1 + i). A row that sees nothing gives zeros; lens[b] > max_len reads
- * max_len positions; rows behind the last sequence are not written; max_new: at least the most
- * tokens of one sequence. A NaN in the cache makes NaN of at least its channels in every row that
+ * max_len positions; rows behind the last sequence are not written; max_new: the most tokens of one
+ * sequence (at least 1; no result hangs on it). A NaN in the cache makes NaN of at least its channels in every row that
  * sees it. Sums are taken of unnormalised exponentials of up to 2^8: |v| times the positions seen has
  * to stay below 2^112.
  * sel (one token per sequence only): int32 [n_seqs][Hkv][n_sel], the logical pages to read, as

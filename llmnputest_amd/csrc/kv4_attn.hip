@@ -1183,7 +1183,7 @@ static Kv4Plan kv4_plan(const q4nx_kv4* c, int n_q_heads, int total, int max_len
 
 static bool kv4_attn_shape(const q4nx_kv4* c, int n_q_heads, int max_new, int max_len, int n_sel) {
   return n_q_heads >= 1 && n_q_heads % c->n_kv_heads == 0 && n_q_heads / c->n_kv_heads <= 16 &&
-         max_new >= 1 && max_new <= 1 << 20 && max_len >= 1 && n_sel >= 0 &&
+         max_new >= 1 && max_len >= 1 && n_sel >= 0 &&
          (int64_t)n_sel * c->page_len <= (int64_t)1 << 30;
 }
 

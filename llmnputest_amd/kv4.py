@@ -239,8 +239,8 @@ class Kv4Cache:
              table: torch.Tensor | None = None):
         """GQA attention of q (bf16 [rows, Hq, D]) over the cache, bf16 [rows, Hq, D] (and the fp32
         copy when want_f32). One token per sequence, at position lens[b] - 1; or, with cu (int32
-        [n_seqs + 1]), a block of new tokens each, causal, the last at lens[b] - 1 (max_new: at least
-        the most of one sequence; default: all rows). lens counts the new tokens, whose rows the cache
+        [n_seqs + 1]), a block of new tokens each, causal, the last at lens[b] - 1 (max_new: the most
+        of one sequence; no result hangs on it). lens counts the new tokens, whose rows the cache
         holds already. max_len: at least the longest length (fewer read fewer positions). scale:
         default D ** -0.5. sel: `select`'s pages, for one token per sequence. out: rows behind the
         last sequence are left as they are."""

@@ -7,7 +7,7 @@ import torch
 
 from llmnputest_amd import kv4
 from oracle import kv4_oracle as ko
-from tests.test_gpu_kv4 import Case, bf16, ints, up
+from tests.test_gpu_kv4 import Case, bf16, check, ints, up
 
 pytestmark = pytest.mark.gpu
 
@@ -129,3 +129,16 @@ def test_max_len_of_zero_reads_nothing(dev):
     for call in (lambda: x.c.attn(0, q, lens, max_len=-1), lambda: x.c.select(0, q, lens, n_sel=3, max_len=-1)):
         with pytest.raises(ops._lib.Q4NXError, match="max_len"):
             call()
+
+
+def test_a_block_of_more_than_a_million_tokens(dev):
+    """All but the last rows stand before the cache's first position and see nothing."""
+    x = Case(dev, 55, 1, 64, 64, [70])
+    x.fill([70])
+    n = (1 << 20) + 77
+    q = x.q(100, 1)
+    many = torch.ones((n, 1, 64), dtype=torch.bfloat16, device=dev)
+    many[-100:] = up(q, dev)
+    got, got32 = x.c.attn(0, many, ints([70], dev), cu=ints([0, n], dev), want_f32=True)
+    assert not got[:-70].any() and not got32[:-70].any()
+    check(got[-70:], got32[-70:], *x.want(q[30:], [(0, range(1, 71))], 0.125))
