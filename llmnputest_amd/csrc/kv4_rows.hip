@@ -80,7 +80,9 @@ struct Kv4Span {
 __device__ __forceinline__ bool kv4_span(const Kv4RowArgs& a, Kv4Span* s) {
   s->h = blockIdx.x % a.c.hkv;
   s->b = blockIdx.x / a.c.hkv;
-  const int64_t p0 = a.pos[s->b];
+  // a position past either of these is as far outside the cache as they are: a table holds at most 2^30, and
+  // a launch covers fewer rows of a sequence
+  const int64_t p0 = max(-(1 << 30), min(a.pos[s->b], 1 << 30));
   int64_t c0 = s->b, n = 1;
   if (a.cu) {
     c0 = a.cu[s->b];

@@ -142,3 +142,26 @@ def test_a_block_of_more_than_a_million_tokens(dev):
     got, got32 = x.c.attn(0, many, ints([70], dev), cu=ints([0, n], dev), want_f32=True)
     assert not got[:-70].any() and not got32[:-70].any()
     check(got[-70:], got32[-70:], *x.want(q[30:], [(0, range(1, 71))], 0.125))
+
+
+@pytest.mark.parametrize("d,page", [(64, 32), (128, 128)])
+def test_read_at_the_ends_of_32_bits(dev, d, page):
+    """Positions outside the cache are NaN, the furthest an int32 names among them; rows that a sequence
+    does not have stay as they were, and a row inside is still found."""
+    x = Case(dev, 52, 2, d, page, [300, 300, 300, 300])
+    k, _ = x.rows(300), x.rows(300)
+    x.c.append(0, up(k, dev), up(k, dev), ints([0] * 4, dev), ints([0, 300, 300, 300, 300], dev))
+    one = x.c.read(0, ints([299] * 4, dev), dtype=torch.float32)[0][0]
+    assert torch.isfinite(one).all()
+    for far in (2 ** 31 - 1, 2 ** 31 - 300, 2 ** 30, -2 ** 31, -2 ** 31 + 5, -2 ** 30, 1 << 20, -1 << 20):
+        kk, vv = x.c.read(0, ints([299, far, far, far], dev), dtype=torch.float32)
+        for y in (kk, vv):
+            assert torch.equal(y[0], one) and torch.isnan(y[1:]).all(), far
+        kk, vv = x.c.read(0, ints([299, far, far, -1], dev), ints([0, 1, 151, 401, 402], dev), total=405)
+        for y in (kk, vv):
+            assert torch.equal(y[0], one.to(torch.bfloat16)) and torch.isnan(y[1:402]).all(), far
+    # the same positions are dropped by a write
+    before = x.pool()
+    for far in (2 ** 31 - 1, -2 ** 31, 2 ** 30, -2 ** 30):
+        x.c.append(0, up(k, dev), up(k, dev), ints([far] * 4, dev), ints([0, 100, 150, 299, 300], dev))
+        assert np.array_equal(x.pool(), before), far
