@@ -39,6 +39,11 @@ def _row_stride(table: torch.Tensor) -> int:
     return table.stride(0) if table.shape[0] > 1 else table.shape[1]
 
 
+def _strides(t: torch.Tensor) -> tuple:
+    """Strides, 0 where a dimension has one entry and its stride says nothing."""
+    return tuple(x if n > 1 else 0 for n, x in zip(t.shape, t.stride()))
+
+
 class Kv4Cache:
     """Pages of every layer (`pool` uint8 [n_layers, n_pages, page bytes]), the sequences' page table
     (`table` int32 [n_seqs, table_len], -1: none), their lengths (`lens` int32 [n_seqs]) and how many
@@ -143,9 +148,8 @@ class Kv4Cache:
         shape, stride = k.shape, k.stride()
         if len(shape) != 3 or shape[1] != self.n_kv_heads or shape[2] != self.head_dim or stride[2] != 1:
             raise ValueError(f"k must be [rows, {self.n_kv_heads}, {self.head_dim}], channels contiguous")
-        if v.shape != shape or v.stride() != stride:
+        if v.shape != shape or (v.stride() != stride and _strides(v) != _strides(k)):
             raise ValueError("k and v must have one shape and one layout")
-        # strides of one row or one head say nothing
         return shape[0], stride[0] if shape[0] > 1 else 0, stride[1] if shape[1] > 1 else 0
 
     def _query(self, q: torch.Tensor) -> tuple[int, int, int]:
@@ -199,10 +203,10 @@ class Kv4Cache:
             if t.dim() != 4 or t.shape[0] < b or t.shape[1] != self.n_kv_heads \
                     or t.shape[3] != self.head_dim or t.stride(3) != 1 or t.numel() == 0:
                 raise ValueError(f"{name} must be [{b}, {self.n_kv_heads}, L, {self.head_dim}]")
-        if k_cache.shape != v_cache.shape or k_cache.stride() != v_cache.stride():
+        seq, head, row, _ = strides = _strides(k_cache)
+        if k_cache.shape != v_cache.shape or _strides(v_cache) != strides:
             raise ValueError("k_cache and v_cache must have one shape and one layout")
         n = k_cache.shape[2]
-        seq, head, row = (k_cache.stride(i) if k_cache.shape[i] > 1 else 0 for i in range(3))
         self._call_append(c, k_cache, v_cache, 1, n, row, head, seq, pos, cu, max_new or n)
 
     def _call_append(self, c, k, v, by_position, rows, row, head, seq, pos, cu, max_new):

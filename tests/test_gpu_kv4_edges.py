@@ -165,3 +165,28 @@ def test_read_at_the_ends_of_32_bits(dev, d, page):
     for far in (2 ** 31 - 1, -2 ** 31, 2 ** 30, -2 ** 30):
         x.c.append(0, up(k, dev), up(k, dev), ints([far] * 4, dev), ints([0, 100, 150, 299, 300], dev))
         assert np.array_equal(x.pool(), before), far
+
+
+def test_strides_of_single_rows_and_heads_say_nothing(dev):
+    """K out of a fused projection's output and V alone: with one row, or one kv head, the strides that
+    differ are never used."""
+    x, y = (Case(dev, 53, 1, 64, 32, [40]) for _ in range(2))
+    k, v = x.rows(1), x.rows(1)
+    fused = torch.zeros((1, 3, 64), dtype=torch.bfloat16, device=dev)
+    fused[:, 1:2] = up(k, dev)
+    apart = up(v, dev).as_strided((1, 1, 64), (8, 8, 1))
+    assert fused[:, 1:2].stride() != apart.stride()
+    x.c.append(0, fused[:, 1:2], apart, ints([3], dev))
+    y.c.append(0, up(k, dev), up(v, dev), ints([3], dev))
+    assert np.array_equal(x.pool(), y.pool())
+    dense = torch.zeros((1, 1, 40, 64), dtype=torch.bfloat16, device=dev)
+    dense[0, 0, 9] = up(k, dev)[0, 0]
+    wide = torch.zeros((1, 3, 40, 64), dtype=torch.bfloat16, device=dev)
+    wide[0, 1, 9] = up(v, dev)[0, 0]
+    x.c.append_cached(0, dense, wide[:, 1:2], ints([9], dev))
+    y.c.append(0, up(k, dev), up(v, dev), ints([9], dev))
+    assert np.array_equal(x.pool(), y.pool())
+    z = Case(dev, 54, 2, 64, 32, [40])   # two kv heads: the head stride counts
+    k = up(z.rows(2), dev)
+    with pytest.raises(ValueError, match="layout"):
+        z.c.append(0, k, k.transpose(0, 1).contiguous().transpose(0, 1), ints([0], dev), ints([0, 2], dev))
