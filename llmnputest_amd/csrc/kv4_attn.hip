@@ -1160,8 +1160,8 @@ static Kv4Plan kv4_plan(const q4nx_kv4* c, int n_q_heads, int total, int max_len
     if (!p.unit && p.items * ((tiles + 7) / 8) < p.grid) p.grid = p.items * ((tiles + 7) / 8);
     if (!p.unit && all > kLineTiles && p.grid < line) p.grid = line;
     recs = p.grid > 2 * line ? p.grid : 2 * line;
-    // on a line any item of two tiles may end one workgroup's stretch and begin the next
-    p.shared = p.unit ? p.unit < tiles : tiles > 8 || (all > kLineTiles && tiles > 1);
+    // cut by the lengths as they are, any item may be of several parts
+    p.shared = p.unit < tiles;
   }
   p.bytes = p.shared ? (size_t)Q4NX_WS_COUNTER_BYTES + (size_t)recs * rows * (c->head_dim + 4) * 4 : 0;
   if (!block && n_split == 0 && (int64_t)p.bytes > kMostBytes) {   // thousands of items: one part each
