@@ -392,7 +392,8 @@ int q4nx_kv4_select(const q4nx_kv4 *cache, const uint16_t *q, int64_t q_stride, 
  *
  * reserve: sequence b gets the pages it lacks for want[b] positions, the lowest free ones, sequences
  * in order. One that wants more than its row holds gets none; where the free pages end, the sequence
- * whose pages do not all fit gets none, nor do those after it. */
+ * whose pages do not all fit gets none, nor do those after it. n_seqs * (n_pages + 1) and
+ * n_seqs * table_len stay below 2^31. */
 size_t q4nx_kv4_pages_ws_bytes(const q4nx_kv4 *cache, int n);
 int q4nx_kv4_reserve(const q4nx_kv4 *cache, int32_t *refs, const int32_t *want, int32_t *status,
                      void *ws, size_t ws_bytes, void *stream);

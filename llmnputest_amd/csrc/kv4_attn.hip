@@ -1,6 +1,5 @@
 // Attention over the paged 4-bit K/V cache, on the matrix cores: single tokens (codes enter the products
-// as they are stored, bound by memory and the exponentials), and blocks of new tokens (tiles taken apart
-// once for 128 rows). Scores, their maxima and sums, and the outputs are fp32 until they are written.
+// as they are stored), and blocks of new tokens (tiles taken apart once for 128 rows). Scores, their maxima and sums, and the outputs are fp32 until they are written.
 //
 // With x = d_g c + m_g per group g of 32 channels,
 //   score = sum_g d_g (c . q)_g + m_g (sum of q)_g,    out = sum_pos p d_g c + sum_pos p m_g
@@ -225,9 +224,12 @@ __device__ __forceinline__ void kv4_finish(const Kv4AttnArgs& a, float (*s_o)[RO
 // p d_g goes through LDS from rows to columns: a lane's pair (position n, 16 + n) is an operand
 // register as it is, so the writes are consecutive dwords and an operand one 16-byte read. The scales
 // are one load of 4 NG bytes a lane (K's positions in lanes 0..31, V's in 32..63), spread by lane swaps.
-// Bound by its instructions, some 165 of the VALU and 12 of the matrix cores a tile (a third of them takes
-// the codes apart): 8 sequences of up to 65536 positions, 180 MB, in 45.4 us, 4.0 TB/s of the 6.5 that a
-// plain read reaches. Short calls are a chain of latencies: 1 x 513 takes 7.9.
+// A tile is 169 instructions of the VALU and 12 of the matrix cores (315 and 24 at D = 128), a third of them to
+// take the codes apart. 8 sequences of up to 65536 positions, 180 MB, take 43 to 46 us, 4.0 to 4.2 TB/s of the
+// 6.5 that a plain read reaches: the VALU is active in 0.77 of the busy cycles (what is found before the tiles
+// and merged behind them makes it 222 instructions a tile), the matrix cores in 0.16, and the 2.4 waves a SIMD
+// wait 0.30 of their time. 16 of up to 5003 at D = 128, 52 MB, take 20 us: VALU 0.50, matrix cores 0.10; 1.8 waves
+// a SIMD, which wait half of their time, are too few. Short calls are a chain of latencies: 1 x 513 takes 8.0.
 // A wave takes every fourth tile of its part; a lane finds the page of one of the wave's next 64
 // tiles, so table and list are read ahead, and two tiles are in flight while one is computed.
 //
@@ -240,8 +242,9 @@ __device__ __forceinline__ void kv4_finish(const Kv4AttnArgs& a, float (*s_o)[RO
 // b1 x 131072 34 / 38, b32 x 8192 38 / 28, b64 x 4096 48 / 32; 64 heads of D = 128, b32 x 8192 56 / 63. In
 // parts of 32 tiles as against W / 512, 32 heads of D = 128, b16 x 5003: 22.3 / 20.4.
 // Known from the call's sizes, items of at most 32 tiles are one part each, and from 512 items on of at
-// most 64, and nothing is looked for: b1 x 513 7.9 (9.1 in three parts), b64 x 1024 12.0 (15.8), b64 x 2048
-// 19.2 (21.6), b2040 x 128 107 (292); but b1 x 1300 12.0 (9.4 in parts), b16 x 2048 15.6 (12.4).
+// most 64, and nothing is looked for: b1 x 513 8.0 (9.0 in three parts), b1 x 640 8.1 (9.0), b64 x 1024 12.0
+// (15.8), b64 x 2048 19.2 (21.6), b2040 x 128 107 (292); but b1 x 1300 11.9 (9.3 in parts), b16 x 2048 15.6
+// (12.4). Near the line few items lose a little: b1 x 770 9.3 (9.0 in four parts), x 1024 10.0 (9.1), b8 alike.
 
 // x / y for quotients below 2^20 or so: the reciprocal is off by less than one in them.
 __device__ __forceinline__ int div_few(int x, int y) {
@@ -602,9 +605,10 @@ __global__ __launch_bounds__(256) void kv4_decode_kernel(Kv4AttnArgs a) {
 // goes from registers to registers. While a tile is computed the next one's bytes are on their way, and
 // its operands are written to the other buffer: one barrier a tile.
 // A wave's tile is 640 cycles of the matrix cores and 650 of the VALU (exponentials, P's terms). 8192 tokens,
-// 40 heads of 8 kv heads: 770 us, 446 TFLOP/s of the attention's own and 1.1 PFLOP/s of products, the matrix
-// cores busy 0.57 of the time and the VALU 0.59 at three waves a SIMD (a library's bf16 product reaches 1.28).
-// 2048 tokens: 88 us, 0.34, bound by the longest row block's 64 tiles of 1.3 us.
+// 40 heads of 8 kv heads: 720 us, 478 TFLOP/s of the attention's own and 1.2 PFLOP/s of products, the matrix
+// cores busy in 0.57 of the busy cycles and the VALU in 0.59 at three waves a SIMD (a library's bf16 product
+// reaches 1.24 to 1.28); 32 heads of D = 128 1056 us, 520 TFLOP/s, 0.58 and 0.39 at two waves.
+// 2048 tokens: 87 us, 0.34, bound by the longest row block's 64 tiles of 1.3 us.
 // Poison: in tiles that some rows do not see, V's groups of NaN are left out of the product (0 times
 // NaN) and given to the rows that see them.
 template <int D>
@@ -693,8 +697,9 @@ struct Kv4Apart {
 };
 
 // Tiles taken apart beforehand, one per workgroup, for calls in which many row blocks read each: 16 KB
-// (D = 64) written once in place of some 110 instructions a wave and row block. 8192 tokens: 950 us without,
-// 770 with, 35 of them here; 2048 tokens 95 and 88.
+// (D = 64) written once in place of some 110 instructions a wave and row block. 8192 tokens: 908 us without,
+// 720 with, 16 of them here (1537 and 1056 at D = 128, 32 heads); 2048 tokens 101 and 87; 3 x up to 509 over
+// 8191 208 and 163; 512 tokens 27.6 and 26.1.
 template <int NG>
 __global__ __launch_bounds__(256) void kv4_apart_kernel(Kv4AttnArgs a) {
   constexpr int D = 32 * NG;

@@ -7,8 +7,9 @@
 // the lane and two lane swaps (16, 32), and K's dword is made where it is stored. V's dwords run along
 // positions: its codes go through LDS as words of four bytes, channels n, 16 + n, 32 + n and 48 + n of
 // a position, made by a lane swap and a 4 x 4 transpose of bytes in registers on either side.
-// Bound by the quantising arithmetic (some 20 instructions a value) and one tile's chain of latencies: 9k
-// rows of 8 kv heads x 64 append in 16 us (21.5 MB, 1.3 TB/s) and read in 10 (2.1 TB/s); one row of each of 8
+// Bound by instructions (26 of the VALU a value in all to append, 13 to read) and one tile's chain of latencies:
+// 9k rows of 8 kv heads x 64 append in 16 us (21.5 MB, 1.3 TB/s), the VALU active in 0.68 of the busy cycles
+// and the waves waiting 0.40 of their time, and read in 11 (2.0 TB/s), 0.54 and 0.43; one row of each of 8
 // sequences in 5.5 and 3.6. With one wave for K and V in turn, and V's bytes through LDS one by one, the
 // appends took 27.
 #include <math.h>

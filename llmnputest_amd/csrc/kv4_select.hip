@@ -4,6 +4,9 @@
 // with Q+ and Q- the sums over the heads of q's positive and negative parts: one product per bound,
 // however many heads share the pages. Products and sums are fp64, so that which pages are chosen does
 // not hang on the order of a sum. Bounds are 4 D bytes per page and kv head, read once.
+// Bound by a chain of loads: a head's row of q is waited for before the next one's, then the four table
+// entries of a lane likewise; only the bounds are in flight together. With 2048 pages, one sequence and five
+// heads a kv head the waves wait 0.68 of their time, and the VALU is active in 0.25 of the busy cycles.
 #include <math.h>
 
 #include "kv4.h"
@@ -22,9 +25,9 @@ struct Kv4SelArgs {
 };
 
 // Pages scored by a workgroup, and its threads, all of which work on the list in the last one to arrive.
-// 2048 pages, one sequence (8 kv heads): 14.0 us; 64 pages and 256 threads 16.6, 64 and 512 14.7, 128 and
-// 1024 15.6. Eight sequences of up to 938 pages: 15.7, against 15.4, 17.5 and 20.0 us. The bounds of
-// scattered pages are what takes long: 64 pages in all take 6.3 us.
+// 2048 pages, one sequence (8 kv heads): 14.1 us; 64 pages and 256 threads 16.6, 64 and 512 14.7, 128 and
+// 1024 15.6. Eight sequences of up to 938 pages: 15.4, against 15.4, 17.5 and 20.0 us. 64 pages in all take
+// 6.3 us.
 constexpr int kSelPages = 128;
 constexpr int kSelThreads = 512;
 constexpr int kSelWaves = kSelThreads / 64;
@@ -63,7 +66,7 @@ __global__ __launch_bounds__(kSelThreads) void kv4_select_kernel(Kv4SelArgs a) {
   const int ch = (sub % (L / 2)) * 8;
   if (part * kSelPages < np) {
     double w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    constexpr int HEADS = 8;   // loads in flight
+    constexpr int HEADS = 8;   // to a round
     for (int g0 = 0; g0 < a.group; g0 += HEADS) {
       u32x4_t y[HEADS];
 #pragma unroll
