@@ -398,7 +398,8 @@ size_t q4nx_kv4_pages_ws_bytes(const q4nx_kv4 *cache, int n);
 int q4nx_kv4_reserve(const q4nx_kv4 *cache, int32_t *refs, const int32_t *want, int32_t *status,
                      void *ws, size_t ws_bytes, void *stream);
 /* fork: sequence dst[i] goes on from src[i]: its full pages are shared, the last, partly filled one is
- * copied (in every layer) into the lowest free page, in the order of the pairs; lens[dst] = lens[src].
+ * copied (in every layer) into the lowest free page, in the order of the pairs; lens[dst] = lens[src],
+ * held to what a row can hold.
  * A pair is not done if an index is outside the sequences, dst is a source or an earlier pair's dst or
  * has pages, src does not have the page of its position lens[src] - 1, or no page is free. */
 int q4nx_kv4_fork(const q4nx_kv4 *cache, int64_t layer_stride, int n_layers, int32_t *lens,

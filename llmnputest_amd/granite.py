@@ -388,10 +388,9 @@ class GraniteDecoder:
         kv.fork(src, dst)
         undone = kv.status.clone()   # reserve() reports there too
         kv.reserve([self.max_len] * n)
-        if int(undone):
-            raise RuntimeError("a source lacks pages of its prefix, or the pool has none left for the copies")
-        if int(kv.status):
-            raise RuntimeError("the pool has no pages left for the forked sequences")
+        if int(undone) or int(kv.status):
+            self.reset(dst)   # pairs that were done share pages
+            raise RuntimeError("a source lacks pages of its prefix, or the pool has none left: nothing is forked")
         for s, d, x in zip(src, dst, lens):
             self._own_from[d] = x // kv.page_len * kv.page_len
             self._own_from[s] = max(self._own_from[s], self._own_from[d])

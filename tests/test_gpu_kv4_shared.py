@@ -123,3 +123,15 @@ def test_a_sequence_wound_back_is_as_new(weights):
     dec.reset([0, 1])
     for i in range(3):
         assert torch.equal(dec.step([9 + i, 3], [i, i]), new.step([9 + i, 3], [i, i]))
+
+
+def test_nothing_stays_shared_after_a_fork_that_failed(weights):
+    """One of two pairs cannot be done: the other's pages are not left shared without a guard."""
+    dec = decoder(weights, 4)
+    dec.seed_cache(150, seed=6)
+    dec.kv.free([2])
+    with pytest.raises(RuntimeError, match="prefix"):
+        dec.fork([0, 2], [1, 3], [130, 130])
+    refs, table = dec.kv.refs.cpu(), dec.kv.table.cpu()
+    assert int(refs.max()) == 1 and (table >= 0).all() and int(refs.sum()) == table.numel()
+    dec.step([1, 2, 3, 4], [0, 0, 0, 0])
