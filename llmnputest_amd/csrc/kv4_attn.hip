@@ -1,5 +1,6 @@
 // Attention over the paged 4-bit K/V cache, on the matrix cores: single tokens (codes enter the products
-// as they are stored), and blocks of new tokens (tiles taken apart once for 128 rows). Scores, their maxima and sums, and the outputs are fp32 until they are written.
+// as they are stored), and blocks of new tokens (tiles taken apart once for 128 rows). Scores, their maxima
+// and sums, and the outputs are fp32 until they are written.
 //
 // With x = d_g c + m_g per group g of 32 channels,
 //   score = sum_g d_g (c . q)_g + m_g (sum of q)_g,    out = sum_pos p d_g c + sum_pos p m_g
