@@ -298,6 +298,30 @@ int q4nx_gqa_decode_records(const uint16_t *q, const uint16_t *k_cache,
                             void *ws, size_t ws_bytes, const q4nx_policy *policy,
                             void *stream);
 
+/* ---------------------------------------------------------------- shared prefixes
+ * One token per sequence over a prefix that many sequences share and over each one's own cache:
+ * out[b][h] = softmax(scale * [Kpre; Kown] q) [Vpre; Vown]. Prefix p's rows are
+ * k_prefix + p * prefix_stride + kv_head * prefix_h_stride + l * head_dim for l < prefix_lens[p]
+ * (at most max_prefix); they are read once for all sequences cu[p] .. cu[p+1] - 1 (int32
+ * [n_prefixes + 1], not falling; NULL: one prefix for all). A sequence in no such range has no prefix.
+ * Own rows as in q4nx_qkv_rope, l < lens[b] (at most max_len; 0: none, the caches may be NULL). Query
+ * head h reads kv head h / (Hq/Hkv), Hq/Hkv <= 16; head_dim 64 or 128; scale >= 0. A sequence that sees
+ * nothing gives zeros. q, out: [batch][Hq][head_dim]; caches bf16, 16-byte aligned, strides in elements,
+ * multiples of 8. Softmax weights of a prefix with more than 16 rows (members * Hq/Hkv) enter the product
+ * rounded to bf16 (their sum is that of the rounded ones), all others with 17 bits. |v| times the
+ * positions seen has to stay below 2^112. No reference counterpart: its attention reads one sequence's cache
+ * (designs/granite_gemv/granite_attention.h:221-237).
+ * ws: q4nx_gqa_prefix_decode_ws_bytes(...) bytes (0: a shape that is not taken). */
+size_t q4nx_gqa_prefix_decode_ws_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim,
+                                       int n_prefixes, int max_prefix, int max_len);
+int q4nx_gqa_prefix_decode(const uint16_t *q, const uint16_t *k_prefix, const uint16_t *v_prefix,
+                           int64_t prefix_stride, int64_t prefix_h_stride,
+                           const int32_t *prefix_lens, const int32_t *cu, int n_prefixes,
+                           int max_prefix, const uint16_t *k_cache, const uint16_t *v_cache,
+                           int64_t kv_b_stride, int64_t kv_h_stride, const int32_t *lens, int max_len,
+                           uint16_t *out, float *out_f32, int batch, int n_q_heads, int n_kv_heads,
+                           int head_dim, float scale, void *ws, size_t ws_bytes, void *stream);
+
 /* ---------------------------------------------------------------- paged 4-bit K/V cache
  * K and V of one layer in pages of 4-bit codes, 10 D bytes per 8 positions and kv head instead of
  * 32 D (bf16). No reference counterpart: its cache is one dense bf16 buffer per sequence

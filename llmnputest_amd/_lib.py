@@ -101,6 +101,9 @@ SIGNATURES: dict[str, tuple] = {
     "q4nx_gqa_decode_records": (c_i, [c_p, c_p, c_p, c_i, c_i, c_i, c_i, c_p, c_i, c_i64,
                                       c_i64, c_f, c_i, c_p, c_sz, c_pol, c_p]),
     "q4nx_gemv_attn_q4": (c_i, [c_p, c_i, c_p, c_i, c_i, c_i, c_p, c_p, c_p, c_p]),
+    "q4nx_gqa_prefix_decode_ws_bytes": (c_sz, [c_i, c_i, c_i, c_i, c_i, c_i, c_i]),
+    "q4nx_gqa_prefix_decode": (c_i, [c_p, c_p, c_p, c_i64, c_i64, c_p, c_p, c_i, c_i, c_p, c_p, c_i64,
+                                     c_i64, c_p, c_i, c_p, c_p, c_i, c_i, c_i, c_i, c_f, c_p, c_sz, c_p]),
     "q4nx_kv4_page_bytes": (c_sz, [c_i, c_i, c_i]),
     "q4nx_kv4_append": (c_i, [c_kv4, c_p, c_p, c_i, c_i64, c_i64, c_i64, c_i64, c_p, c_p, c_i, c_p]),
     "q4nx_kv4_read": (c_i, [c_kv4, c_p, c_p, c_i, c_i64, c_p, c_p, c_i, c_p]),

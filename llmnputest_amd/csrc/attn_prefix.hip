@@ -1,0 +1,469 @@
+// Attention of one token per sequence over a prefix that many sequences share and over each one's own
+// cache. No reference counterpart: its attention reads one sequence's cache per query head
+// (designs/granite_gemv/granite_attention.h:221-237).
+//
+//   out[b][h] = softmax(scale q[b][h] . [Kpre; Kown]^T) [Vpre; Vown]
+//
+// The rows of a prefix are read once for all members of its group: per kv head the members' query heads
+// of the group are the rows of one product, R = members * Hq/Hkv of them, and the exact (m, l, acc) merge
+// joins what the prefix's parts and the own cache's parts give. Two launches: the parts, and the merge.
+//
+// Parts, all in one grid (the prefix's first, which take longest; the own cache's, which wait for memory,
+// run beside them):
+//   own caches      (sequence, kv head, part): part_narrow
+//   prefix, R > 16  (kv head, 64 NR rows, part): part_wide below
+//   prefix, R <= 16 (kv head, part): part_narrow over the members' rows
+
+#include "attn_parts.h"
+
+namespace q4nx {
+
+struct PrefixArgs {
+  const uint16_t* q;
+  const uint16_t* k;      // own rows, [batch][hkv][..][D]
+  const uint16_t* v;
+  const uint16_t* kp;     // the prefixes', [n_prefixes][hkv][..][D]
+  const uint16_t* vp;
+  const int32_t* lens;
+  const int32_t* plens;
+  const int32_t* cu;      // nullptr: one prefix, all sequences
+  uint16_t* out;
+  float* out_f32;
+  float* rec;             // [batch * hkv][slots][G][kRec<D>], own parts first
+  int64_t b_stride, h_stride, pp_stride, ph_stride;
+  int batch, hq, hkv, G, n_prefixes, max_prefix, max_len;
+  int ns_pre, chunk_pre, tiles, ns_own, chunk_own;
+  float scale_l2;
+};
+
+// The group of prefix p: sequences [first, first + members).
+struct Group {
+  int p, first, members;
+};
+__device__ __forceinline__ int cu_at(const PrefixArgs& a, int p) {
+  return a.cu == nullptr ? (p > 0 ? a.batch : 0) : min(max(a.cu[p], 0), a.batch);
+}
+// 16-row-tile counting for a prefix of so many members: tiles of RT rows.
+__device__ __forceinline__ int tiles_of(int members, int G, int RT) { return (members * G + RT - 1) / RT; }
+
+// Which prefix row tile t belongs to, 64 prefixes at a time; t becomes its index there. p = -1: none.
+__device__ __forceinline__ Group find_tile(const PrefixArgs& a, int RT, int lane, int& t) {
+  for (int p0 = 0; p0 < a.n_prefixes; p0 += 64) {
+    const int p = p0 + lane;
+    int first = 0, members = 0;
+    if (p < a.n_prefixes) {
+      first = cu_at(a, p);
+      members = max(cu_at(a, p + 1) - first, 0);
+    }
+    const int n = tiles_of(members, a.G, RT);
+    int upto = n;   // inclusive scan
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int x = __shfl_up(upto, d);
+      if (lane >= d) upto += x;
+    }
+    const uint64_t past = __ballot(upto > t);
+    if (past != 0) {
+      const int w = __builtin_ctzll(past);
+      t -= __builtin_amdgcn_readlane(upto - n, w);
+      return {p0 + w, __builtin_amdgcn_readlane(first, w), __builtin_amdgcn_readlane(members, w)};
+    }
+    t -= __builtin_amdgcn_readlane(upto, 63);
+  }
+  return {-1, 0, 0};
+}
+
+// 64 NR query rows (16 NR a wave) over cache rows [0, end): tiles of 64 positions of K and V go through
+// LDS, loaded one tile ahead, read by all four waves. V^T comes out of the transposing LDS read. P is
+// rounded to bf16 once (2^-9 of a weight; the same rounded weights are summed to l, by a product with
+// ones, so they still add up to one). The running maximum moves only when a row's tile exceeds it by 2^8
+// (weights stay below 2^8 then), which leaves out nearly every rescaling of the accumulators.
+// 16-byte pieces of a row are swizzled by the row, so that 16 rows' pieces lie in different banks.
+template <int D>
+__device__ __forceinline__ int swz_k(int row, int c) {
+  return row * (D / 8) + (c ^ (D == 64 ? (row >> 1) & 7 : row & 15));
+}
+template <int D>
+__device__ __forceinline__ int swz_v(int row, int c) {
+  return row * (D / 8) + (c ^ (D == 64 ? row & 7 : (row & 7) * 2));
+}
+
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4_t lds_s16x4_t;
+
+template <int D, int NR, typename RowAt, typename RecOf>
+__device__ __forceinline__ void part_wide(const PrefixArgs& a, const uint16_t* kbase, const uint16_t* vbase,
+                                          int end, int row0, int R, uint4* lds, RowAt row_at, RecOf rec_of) {
+  constexpr int KC = D / 32, C = D / 8, LD = 64 * C / 256;
+  uint4* const sk = lds;                  // [2][64 * C]
+  uint4* const sv = lds + 2 * 64 * C;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int j = lane & 15, g = lane >> 4;
+  const int r0 = row0 + wave * 16 * NR;
+
+  u32x4_t q[NR][KC];
+#pragma unroll
+  for (int n = 0; n < NR; ++n)
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+      const int r = r0 + 16 * n + j;
+      q[n][c] = r < R ? *(const u32x4_t*)(row_at(r) + 32 * c + 8 * g) : u32x4_t{0u, 0u, 0u, 0u};
+    }
+  f32x4_t o[NR][D / 16], l[NR];
+  float m[NR];
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    m[n] = -INFINITY;
+    l[n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < D / 16; ++u) o[n][u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+
+  uint4 gk[LD], gv[LD];
+  auto fetch = [&](int p0) {   // rows past the end: the last one again, whose weight is masked to 0
+#pragma unroll
+    for (int i = 0; i < LD; ++i) {
+      const int id = tid + 256 * i;
+      const size_t at = (size_t)min(p0 + id / C, end - 1) * D + id % C * 8;
+      gk[i] = *(const uint4*)(kbase + at);
+      gv[i] = *(const uint4*)(vbase + at);
+    }
+  };
+  auto put = [&](int b) {
+#pragma unroll
+    for (int i = 0; i < LD; ++i) {
+      const int id = tid + 256 * i;
+      sk[b * 64 * C + swz_k<D>(id / C, id % C)] = gk[i];
+      sv[b * 64 * C + swz_v<D>(id / C, id % C)] = gv[i];
+    }
+  };
+  const bool busy = r0 < R;   // waves without rows only load
+  const uint32_t one2 = 0x3F803F80u;
+  const u32x4_t ones = {one2, one2, one2, one2};
+  const int nt = (end + 63) / 64;
+  fetch(0);
+  put(0);
+  __syncthreads();
+  for (int t = 0; t < nt; ++t) {
+    const int b = t & 1;
+    if (t + 1 < nt) fetch((t + 1) * 64);
+    if (busy) {
+      const uint4* const kt = sk + b * 64 * C;
+      const uint4* const vt = sv + b * 64 * C;
+      f32x4_t s[NR][4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+#pragma unroll
+        for (int n = 0; n < NR; ++n) s[n][x] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+          const u32x4_t kk = *(const u32x4_t*)(kt + swz_k<D>(16 * x + j, 4 * c + g));
+#pragma unroll
+          for (int n = 0; n < NR; ++n) s[n][x] = mfma_bf16(kk, q[n][c], s[n][x]);
+        }
+      }
+      if ((t + 1) * 64 > end) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (t * 64 + 16 * x + 4 * g + e >= end)
+#pragma unroll
+              for (int n = 0; n < NR; ++n) s[n][x][e] = -INFINITY;
+      }
+      float mx[NR];
+      bool up = false;
+#pragma unroll
+      for (int n = 0; n < NR; ++n) {
+        float v = s[n][0][0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) v = fmaxf(v, s[n][i >> 2][i & 3]);
+        mx[n] = xor32_max(xor16_max(v)) * a.scale_l2;
+        up |= mx[n] > m[n] + 8.f;
+      }
+      if (__any(up)) {
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+          const float mn = fmaxf(m[n], mx[n]);
+          const float corr = mn == -INFINITY ? 0.f : exp2_hw(m[n] - mn);
+          m[n] = mn;
+          l[n] *= corr;
+#pragma unroll
+          for (int u = 0; u < D / 16; ++u) o[n][u] *= corr;
+        }
+      }
+      u32x4_t pp[NR][2];
+#pragma unroll
+      for (int n = 0; n < NR; ++n) {
+        const float mb = m[n] == -INFINITY ? 0.f : m[n];
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+          for (int w = 0; w < 2; ++w)
+            pp[n][x >> 1][2 * (x & 1) + w] =
+                pack_bf16x2_op(exp2_hw(fmaf(s[n][x][2 * w], a.scale_l2, -mb)),
+                               exp2_hw(fmaf(s[n][x][2 * w + 1], a.scale_l2, -mb)));
+      }
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+#pragma unroll
+        for (int n = 0; n < NR; ++n) l[n] = mfma_bf16(ones, pp[n][x], l[n]);
+#pragma unroll
+        for (int u = 0; u < D / 16; ++u) {
+          uint2 h[2];
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const int row = 32 * x + 16 * y + 4 * g + (j >> 2);
+            const char* p = (const char*)(vt + swz_v<D>(row, 2 * u + ((j & 3) >> 1))) + 8 * (j & 1);
+            h[y] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)p));
+          }
+          const u32x4_t vv = {h[0].x, h[0].y, h[1].x, h[1].y};
+#pragma unroll
+          for (int n = 0; n < NR; ++n) o[n][u] = mfma_bf16(vv, pp[n][x], o[n][u]);
+        }
+      }
+    }
+    if (t + 1 < nt) put(b ^ 1);   // its readers left it before the last barrier
+    __syncthreads();
+  }
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    const int r = r0 + 16 * n + j;
+    if (r >= R) continue;
+    float* to = a.rec + rec_of(r);
+#pragma unroll
+    for (int u = 0; u < D / 16; ++u)
+      *(float4*)(to + 16 * u + 4 * g) = make_float4(o[n][u][0], o[n][u][1], o[n][u][2], o[n][u][3]);
+    if (g == 0) *(float2*)(to + D) = make_float2(m[n], l[n][0]);
+  }
+}
+
+template <int D, int NR>
+__global__ __launch_bounds__(256, 2) void prefix_parts_kernel(PrefixArgs a) {
+  constexpr int kNarrow = (kPartWaves * 16 * D + 8 * 16) * 4;
+  constexpr int kWide = 4 * 64 * D * 2;
+  __shared__ __attribute__((aligned(16))) uint4 lds[(kNarrow > kWide ? kNarrow : kWide) / 16];
+  const int lane = threadIdx.x & 63;
+  const int slots = a.ns_own + a.ns_pre;
+  int blk = blockIdx.x;
+  const int n_pre = a.hkv * a.tiles * a.ns_pre;
+  if (blk < n_pre) {
+    // the kv head fastest: with 8 of them an XCD's L2 holds one head's rows for all of its row tiles
+    const int kvh = blk % a.hkv;
+    blk /= a.hkv;
+    int t = blk % a.tiles;
+    const int part = blk / a.tiles;
+    const Group gr = find_tile(a, 64 * NR, lane, t);
+    if (gr.p < 0) return;
+    const int len = min(max(a.plens[gr.p], 0), a.max_prefix);
+    const int start = part * a.chunk_pre;
+    if (start >= len) return;
+    const int end = min(a.chunk_pre, len - start);
+    const int R = gr.members * a.G;
+    const size_t at = (size_t)gr.p * a.pp_stride + (size_t)kvh * a.ph_stride + (size_t)start * D;
+    auto row_at = [&](int r) {
+      const int i = r / a.G;
+      return a.q + ((size_t)(gr.first + i) * a.hq + kvh * a.G + (r - i * a.G)) * D;
+    };
+    auto rec_of = [&](int r) {
+      const int i = r / a.G;
+      return (((size_t)(gr.first + i) * a.hkv + kvh) * slots + a.ns_own + part) * (size_t)(a.G * kRec<D>) +
+             (size_t)(r - i * a.G) * kRec<D>;
+    };
+    if (R <= 16)
+      part_narrow<D, false>(row_at(min(lane & 15, R - 1)), R, a.kp + at, a.vp + at, end, end, a.scale_l2,
+                            nullptr, 0, (float*)lds, a.rec, rec_of);
+    else
+      part_wide<D, NR>(a, a.kp + at, a.vp + at, end, t * 64 * NR, R, lds, row_at, rec_of);
+    return;
+  }
+  blk -= n_pre;
+  const int kvh = blk % a.hkv;
+  blk /= a.hkv;
+  const int b = blk % a.batch, part = blk / a.batch;
+  const int len = min(max(a.lens[b], 0), a.max_len);
+  const int start = part * a.chunk_own;
+  if (start >= len) return;
+  const int end = min(a.chunk_own, len - start);
+  const size_t at = (size_t)b * a.b_stride + (size_t)kvh * a.h_stride + (size_t)start * D;
+  const size_t rec = (((size_t)b * a.hkv + kvh) * slots + part) * (size_t)(a.G * kRec<D>);
+  part_narrow<D, false>(a.q + ((size_t)b * a.hq + kvh * a.G + min(lane & 15, a.G - 1)) * D, a.G, a.k + at,
+                        a.v + at, end, end, a.scale_l2, nullptr, 0, (float*)lds, a.rec,
+                        [&](int r) { return rec + (size_t)r * kRec<D>; });
+}
+
+// One wave per (sequence, query head): the records that were written, merged.
+template <int D>
+__global__ __launch_bounds__(256) void prefix_merge_kernel(PrefixArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int i = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+  if (i >= a.batch * a.hq) return;
+  const int b = i / a.hq, h = i - b * a.hq;
+  const int kvh = h / a.G;
+  const int len = min(max(a.lens[b], 0), a.max_len);
+  const int n_own = len > 0 ? (len + a.chunk_own - 1) / a.chunk_own : 0;
+  int n_pre = 0;
+  for (int p0 = 0; p0 < a.n_prefixes; p0 += 64) {
+    const int p = p0 + lane;
+    const bool in = p < a.n_prefixes && cu_at(a, p) <= b && b < cu_at(a, p + 1);
+    const uint64_t who = __ballot(in);
+    if (who != 0) {
+      const int pl = min(max(a.plens[p0 + __builtin_ctzll(who)], 0), a.max_prefix);
+      n_pre = pl > 0 ? (pl + a.chunk_pre - 1) / a.chunk_pre : 0;
+      break;
+    }
+  }
+  const int n = n_own + n_pre, slots = a.ns_own + a.ns_pre;
+  const int slot = lane < n_own ? lane : lane < n ? a.ns_own + lane - n_own : 0;
+  const float* mine = a.rec + ((((size_t)b * a.hkv + kvh) * slots + slot) * a.G + (h - kvh * a.G)) * kRec<D>;
+  float A[D / 64];
+  merge_records<D>(mine, n, lane, A);
+#pragma unroll
+  for (int x = 0; x < D / 64; ++x) {
+    const size_t at = ((size_t)b * a.hq + h) * D + lane + 64 * x;
+    if (a.out) a.out[at] = f32_to_bf16(A[x]);
+    if (a.out_f32) a.out_f32[at] = A[x];
+  }
+}
+
+struct PrefixPlan {
+  int nr, tiles, ns_pre, chunk_pre, ns_own, chunk_own;
+};
+
+static int clamp_int(long long x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : (int)x; }
+
+// How the work is cut. Only bounds are known here (the lengths are on the device).
+static PrefixPlan prefix_plan(int batch, int hq, int hkv, int n_prefixes, int max_prefix, int max_len) {
+  const int G = hq / hkv;
+  const long long rows = (long long)batch * G;
+  PrefixPlan p{};
+  p.nr = rows > 64 ? 2 : 1;
+  const int rt = 64 * p.nr;
+  // every prefix may end inside a tile
+  const long long most = (rows + rt - 1) / rt + (n_prefixes > 0 ? n_prefixes - 1 : 0);
+  p.tiles = (int)(most < batch ? most : batch);
+  if (n_prefixes == 0 || max_prefix == 0) p.tiles = 0;
+  if (p.tiles > 0) {
+    const int unit = rows <= 16 ? kPartRound : 256;
+    p.ns_pre = clamp_int(512 / ((long long)hkv * p.tiles), 1, 32);
+    p.ns_pre = clamp_int((max_prefix + unit - 1) / unit, 1, p.ns_pre);
+    p.chunk_pre = part_chunk(max_prefix, p.ns_pre, 64);
+    p.ns_pre = (max_prefix + p.chunk_pre - 1) / p.chunk_pre;
+  }
+  if (max_len > 0) {
+    p.ns_own = clamp_int(1024 / ((long long)hkv * batch), 1, 32);
+    p.ns_own = clamp_int((max_len + 255) / 256, 1, p.ns_own);
+    p.chunk_own = part_chunk(max_len, p.ns_own, kPartRound);
+    p.ns_own = (max_len + p.chunk_own - 1) / p.chunk_own;
+  }
+  if (p.chunk_pre == 0) p.chunk_pre = 64;
+  if (p.chunk_own == 0) p.chunk_own = kPartRound;
+  return p;
+}
+
+static bool prefix_shape_ok(int batch, int hq, int hkv, int d, int n_prefixes, int max_prefix, int max_len) {
+  return batch >= 1 && batch <= (1 << 20) && hkv >= 1 && hkv <= 1024 && hq >= hkv && hq % hkv == 0 && hq / hkv <= 16 &&
+         (d == 64 || d == 128) && n_prefixes >= 0 && n_prefixes <= batch && max_prefix >= 0 && max_prefix < (1 << 24) &&
+         max_len >= 0 && max_len < (1 << 24) && (long long)batch * hq < (1 << 28);
+}
+
+static size_t prefix_rec_bytes(const PrefixPlan& p, int batch, int hq, int d) {
+  return (size_t)batch * hq * (p.ns_own + p.ns_pre) * (d + 4) * 4;
+}
+
+template <int D>
+static void prefix_launch(const PrefixArgs& a, const PrefixPlan& p, hipStream_t s) {
+  const unsigned grid = (unsigned)(a.hkv * (p.tiles * p.ns_pre + a.batch * p.ns_own));
+  if (grid > 0) {
+    if (p.nr == 1) hipLaunchKernelGGL((prefix_parts_kernel<D, 1>), dim3(grid), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((prefix_parts_kernel<D, 2>), dim3(grid), dim3(256), 0, s, a);
+  }
+  const unsigned wgs = (unsigned)(((long long)a.batch * a.hq + 3) / 4);
+  hipLaunchKernelGGL(prefix_merge_kernel<D>, dim3(wgs), dim3(256), 0, s, a);
+}
+
+}  // namespace q4nx
+
+using namespace q4nx;
+
+extern "C" {
+
+size_t q4nx_gqa_prefix_decode_ws_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim, int n_prefixes,
+                                       int max_prefix, int max_len) {
+  if (!prefix_shape_ok(batch, n_q_heads, n_kv_heads, head_dim, n_prefixes, max_prefix, max_len)) return 0;
+  const PrefixPlan p = prefix_plan(batch, n_q_heads, n_kv_heads, n_prefixes, max_prefix, max_len);
+  return (size_t)Q4NX_WS_COUNTER_BYTES + prefix_rec_bytes(p, batch, n_q_heads, head_dim);
+}
+
+int q4nx_gqa_prefix_decode(const uint16_t* q, const uint16_t* k_prefix, const uint16_t* v_prefix,
+                           int64_t prefix_stride, int64_t prefix_h_stride, const int32_t* prefix_lens,
+                           const int32_t* cu, int n_prefixes, int max_prefix, const uint16_t* k_cache,
+                           const uint16_t* v_cache, int64_t kv_b_stride, int64_t kv_h_stride,
+                           const int32_t* lens, int max_len, uint16_t* out, float* out_f32, int batch,
+                           int n_q_heads, int n_kv_heads, int head_dim, float scale, void* ws, size_t ws_bytes,
+                           void* stream) {
+  const char* what = "q4nx_gqa_prefix_decode";
+  Q4NX_REQUIRE(prefix_shape_ok(batch, n_q_heads, n_kv_heads, head_dim, n_prefixes, max_prefix, max_len),
+               Q4NX_ERR_SHAPE,
+               "%s: batch=%d Hq=%d (a multiple of Hkv, at most 16 times) Hkv=%d head_dim=%d (64, 128) "
+               "n_prefixes=%d (at most batch) max_prefix=%d max_len=%d (below 2^24)",
+               what, batch, n_q_heads, n_kv_heads, head_dim, n_prefixes, max_prefix, max_len);
+  const bool pre = n_prefixes > 0 && max_prefix > 0, own = max_len > 0;
+  Q4NX_REQUIRE(q && lens && (out || out_f32) && (!own || (k_cache && v_cache)) &&
+                   (!pre || (k_prefix && v_prefix && prefix_lens)),
+               Q4NX_ERR_ARG, "%s: q, the caches, their lengths and an output are required", what);
+  Q4NX_REQUIRE(!pre || n_prefixes == 1 || cu, Q4NX_ERR_ARG, "%s: %d prefixes need cu", what, n_prefixes);
+  Q4NX_REQUIRE(Q4NX_ALIGNED(q, 16) && Q4NX_ALIGNED(k_cache, 16) && Q4NX_ALIGNED(v_cache, 16) &&
+                   Q4NX_ALIGNED(k_prefix, 16) && Q4NX_ALIGNED(v_prefix, 16),
+               Q4NX_ERR_ARG, "%s: q and the caches must be 16-byte aligned", what);
+  Q4NX_REQUIRE(!own || (kv_h_stride >= (int64_t)max_len * head_dim && kv_h_stride % 8 == 0 &&
+                        kv_b_stride >= (int64_t)n_kv_heads * kv_h_stride && kv_b_stride % 8 == 0),
+               Q4NX_ERR_SHAPE, "%s: cache strides do not hold [Hkv][max_len][head_dim]", what);
+  Q4NX_REQUIRE(!pre || (prefix_h_stride >= (int64_t)max_prefix * head_dim && prefix_h_stride % 8 == 0 &&
+                        (n_prefixes == 1 || (prefix_stride >= (int64_t)n_kv_heads * prefix_h_stride &&
+                                             prefix_stride % 8 == 0))),
+               Q4NX_ERR_SHAPE, "%s: prefix strides do not hold [Hkv][max_prefix][head_dim]", what);
+  Q4NX_REQUIRE(scale >= 0.f, Q4NX_ERR_ARG, "%s: scale must not be negative", what);
+  const PrefixPlan p = prefix_plan(batch, n_q_heads, n_kv_heads, n_prefixes, max_prefix, max_len);
+  Q4NX_REQUIRE((long long)n_kv_heads * ((long long)p.tiles * p.ns_pre + (long long)batch * p.ns_own) < (1ll << 31),
+               Q4NX_ERR_SHAPE, "%s: more than 2^31 workgroups", what);
+  const size_t need = (size_t)Q4NX_WS_COUNTER_BYTES + prefix_rec_bytes(p, batch, n_q_heads, head_dim);
+  Q4NX_REQUIRE(ws != nullptr && ws_bytes >= need && Q4NX_ALIGNED(ws, 256), Q4NX_ERR_WS,
+               "%s: workspace of %zu bytes (256-aligned) needed, %zu given", what, need, ws_bytes);
+  PrefixArgs a{};
+  a.q = q;
+  a.k = k_cache;
+  a.v = v_cache;
+  a.kp = k_prefix;
+  a.vp = v_prefix;
+  a.lens = lens;
+  a.plens = prefix_lens;
+  a.cu = cu;
+  a.out = out;
+  a.out_f32 = out_f32;
+  a.rec = (float*)((uint8_t*)ws + Q4NX_WS_COUNTER_BYTES);
+  a.b_stride = kv_b_stride;
+  a.h_stride = kv_h_stride;
+  a.pp_stride = n_prefixes > 1 ? prefix_stride : 0;
+  a.ph_stride = prefix_h_stride;
+  a.batch = batch;
+  a.hq = n_q_heads;
+  a.hkv = n_kv_heads;
+  a.G = n_q_heads / n_kv_heads;
+  a.n_prefixes = pre ? n_prefixes : 0;
+  a.max_prefix = max_prefix;
+  a.max_len = max_len;
+  a.ns_pre = p.ns_pre;
+  a.chunk_pre = p.chunk_pre;
+  a.tiles = p.tiles;
+  a.ns_own = p.ns_own;
+  a.chunk_own = p.chunk_own;
+  a.scale_l2 = (float)((double)scale * 1.4426950408889634);
+  hipStream_t s = (hipStream_t)stream;
+  if (head_dim == 64) prefix_launch<64>(a, p, s);
+  else prefix_launch<128>(a, p, s);
+  return check_launch(what);
+}
+
+}  // extern "C"

@@ -588,6 +588,85 @@ def gemv_attn_q4(tiles: torch.Tensor, n_tile_rows: int, records: torch.Tensor,
     return out
 
 
+# ---------------------------------------------------------------- shared prefixes
+
+def _here(t: torch.Tensor, name: str, dtype, shape=None) -> int:
+    """The address of a contiguous tensor of that type (and shape) on the current device."""
+    if t.get_device() != torch.cuda.current_device():
+        raise ValueError(f"{name} must be on the current device, got {t.device}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if not t.is_contiguous() or (shape is not None and t.shape != shape):
+        raise ValueError(f"{name} must be contiguous" + ("" if shape is None else f", {list(shape)}"))
+    return t.data_ptr()
+
+
+def _rows_of(k: torch.Tensor, v: torch.Tensor, name: str, d: int) -> tuple[int, int]:
+    """The sequence and head strides of a pair of caches bf16 [B, Hkv, L, D], rows contiguous (a stride
+    that says nothing, of a dimension with one entry, is what a packed cache has)."""
+    out = []
+    for t, n in ((k, f"k_{name}"), (v, f"v_{name}")):
+        if t.get_device() != torch.cuda.current_device():
+            raise ValueError(f"{n} must be on the current device, got {t.device}")
+        if t.dtype != torch.bfloat16:
+            raise TypeError(f"{n} must be {torch.bfloat16}, got {t.dtype}")
+        shape, st = t.shape, t.stride()
+        if len(shape) != 4 or shape[3] != d or shape[1] == 0 or st[3] != 1 or (shape[2] > 1 and st[2] != d):
+            raise ValueError(f"{n} must be [B, Hkv, L, {d}] with contiguous rows")
+        h = st[1] if shape[1] > 1 else shape[2] * d
+        out.append((st[0] if shape[0] > 1 else shape[1] * h, h))
+    if k.shape != v.shape or out[0] != out[1]:
+        raise ValueError(f"k_{name} and v_{name} must have one shape and one layout")
+    return out[0]
+
+
+def _upto(n: int, most: int | None, name: str) -> int:
+    """The positions a call may read of n."""
+    if most is not None and most < 0:
+        raise ValueError(f"{name} must not be negative")
+    return n if most is None else min(n, most)
+
+
+def gqa_prefix_decode(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor,
+                      prefix_lens: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                      lens: torch.Tensor, cu: torch.Tensor | None = None, scale: float | None = None,
+                      max_prefix: int | None = None, max_len: int | None = None,
+                      out: torch.Tensor | None = None, want_f32: bool = False,
+                      ws: Workspace | None = None):
+    """GQA attention of one token per sequence, q bf16 [B, Hq, D], over a prefix that sequences share
+    (its rows are read once for all of them) and over each one's own cache. k_prefix, v_prefix bf16
+    [P, Hkv, Lp, D] with prefix_lens int32 [P]; sequences cu[p] .. cu[p+1] - 1 (int32 [P + 1]; default:
+    one prefix for all) go on from prefix p, others have none. Own rows bf16 [B, Hkv, L, D], lens int32
+    [B] (without the prefix; 0: none). D 64 or 128, Hq/Hkv at most 16, scale (default D ** -0.5) not
+    negative. max_prefix, max_len: at least the longest lengths (fewer read fewer positions; default the
+    caches'). Returns bf16 [B, Hq, D] (and the fp32 copy when want_f32)."""
+    b, hq, d = q.shape
+    qp = _here(q, "q", torch.bfloat16)
+    ps, ph = _rows_of(k_prefix, v_prefix, "prefix", d)
+    bs, hs = _rows_of(k_cache, v_cache, "cache", d)
+    p, hkv = k_prefix.shape[:2]
+    if k_cache.shape[0] != b or k_cache.shape[1] != hkv:
+        raise ValueError(f"k_cache must be [{b}, {hkv}, L, {d}]")
+    if cu is None and p > 1:
+        raise ValueError(f"{p} prefixes need cu")
+    lp = _here(lens, "lens", torch.int32, (b,))
+    pp = _here(prefix_lens, "prefix_lens", torch.int32, (p,))
+    up = None if cu is None else _here(cu, "cu", torch.int32, (p + 1,))
+    out = torch.empty_like(q) if out is None else out
+    op = _here(out, "out", torch.bfloat16, q.shape)
+    of = torch.empty(q.shape, dtype=torch.float32, device=q.device) if want_f32 else None
+    if b == 0:
+        return (out, of) if want_f32 else out
+    most_p = _upto(k_prefix.shape[2], max_prefix, "max_prefix")
+    most = _upto(k_cache.shape[2], max_len, "max_len")
+    need = _lib.lib().q4nx_gqa_prefix_decode_ws_bytes(b, hq, hkv, d, p, most_p, most)
+    ws, wp, wn, stream = _scratch(ws, need)
+    _lib.call("q4nx_gqa_prefix_decode", qp, k_prefix.data_ptr(), v_prefix.data_ptr(), ps, ph, pp, up, p,
+              most_p, k_cache.data_ptr(), v_cache.data_ptr(), bs, hs, lp, most, op, _ptr(of), b, hq, hkv, d,
+              d ** -0.5 if scale is None else float(scale), wp, wn, stream)
+    return (out, of) if want_f32 else out
+
+
 # ---------------------------------------------------------------- decode helpers
 
 def embed(table: torch.Tensor, kind: str, tokens: torch.Tensor, vocab: int, hidden: int,

@@ -1,0 +1,79 @@
+"""Attention over shared prefixes against float64, and a run of it in a graph."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF16 = 2.0 ** -8   # half a step of bf16
+
+
+def rows(g, *shape):
+    return torch.randn(shape, device="cuda", generator=g).to(torch.bfloat16)
+
+
+def reference(q, kp, vp, plens, k, v, lens, groups, scale):
+    """float64 attention, and the largest sum |p v| of a row's channels (what roundings of p scale with)."""
+    b, hq, d = q.shape
+    hkv = k.shape[1]
+    g = hq // hkv
+    out = torch.zeros((b, hq, d), dtype=torch.float64, device=q.device)
+    mag = torch.zeros_like(out)
+    for i in range(b):
+        p = next((x for x, (lo, hi) in enumerate(groups) if lo <= i < hi), None)
+        for h in range(hkv):
+            n = max(int(lens[i]), 0)
+            kk, vv = k[i, h, :n].double(), v[i, h, :n].double()
+            if p is not None:
+                m = max(int(plens[p]), 0)
+                kk, vv = torch.cat((kp[p, h, :m].double(), kk)), torch.cat((vp[p, h, :m].double(), vv))
+            if len(kk):
+                w = torch.softmax(q[i, h * g:(h + 1) * g].double() @ kk.T * scale, -1)
+                out[i, h * g:(h + 1) * g], mag[i, h * g:(h + 1) * g] = w @ vv, w @ vv.abs()
+    return out, mag
+
+
+def check(got, f32, want, mag):
+    """A weight's rounding to bf16 is off by 2^-8 of it at most, and so is the sum that divides; fp32
+    sums of up to 2^14 terms and 2^-22 of a score's exponent add less than 2^-10 of it together."""
+    err = (f32.double() - want).abs()
+    assert bool((err <= (2 * BF16 + 2.0 ** -10) * mag + 1e-30).all()), float((err / (mag + 1e-30)).max())
+    assert torch.equal(got, f32.to(torch.bfloat16))
+
+
+CASES = [
+    # b, groups, hq, hkv, d, plens, lens
+    (1, [(0, 1)], 8, 8, 64, [1], [0]),
+    (1, [(0, 1)], 16, 1, 128, [130], [1]),
+    (2, [(0, 2)], 40, 8, 64, [513], [33, 1]),
+    (3, [(0, 3)], 10, 2, 64, [64], [0, 129, 64]),
+    (8, [(0, 8)], 40, 8, 64, [2048], [128, 5, 77, 1, 0, 64, 63, 65]),
+    (5, [(0, 2), (2, 2), (2, 5)], 14, 2, 128, [300, 50, 999], [7, 300, 0, 1, 31]),
+    (6, [(1, 4)], 8, 1, 64, [777], [3, 0, 12, 500, 0, 9]),            # sequences without a prefix
+    (4, [(0, 2), (2, 4)], 4, 2, 64, [0, 65], [0, 3, 2, 0]),            # an empty prefix: one row sees nothing
+    (33, [(0, 33)], 7, 1, 64, [4097], [i * 3 for i in range(33)]),
+    (20, [(0, 9), (9, 20)], 32, 4, 128, [1025, 320], [i for i in range(20)]),
+    (70, [(i, i + 1) for i in range(70)], 4, 2, 64, [i * 5 for i in range(70)], [i % 7 for i in range(70)]),
+    (3, [(0, 3)], 16, 1, 64, [40000], [1, 2, 3000]),
+]
+
+
+@pytest.mark.parametrize("case", CASES, ids=[f"b{c[0]}p{len(c[1])}hq{c[2]}_{c[3]}d{c[4]}" for c in CASES])
+def test_prefix_decode(dev, case):
+    from llmnputest_amd import ops
+    b, groups, hq, hkv, d, plens, lens = case
+    g = torch.Generator(device="cuda").manual_seed(len(plens) * 100 + b)
+    lp, lo = max(plens) + 3, max(lens) + 2
+    kp, vp, k, v = (rows(g, n, hkv, m, d) for n, m in ((len(plens), lp), (len(plens), lp), (b, lo), (b, lo)))
+    for i, n in enumerate(plens):   # what lies behind the lengths must not be seen
+        kp[i, :, n:], vp[i, :, n:] = float("nan"), float("inf")
+    for i, n in enumerate(lens):
+        k[i, :, n:], v[i, :, n:] = float("inf"), float("nan")
+    q = rows(g, b, hq, d) * 1.5
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    cu = None if groups == [(0, b)] else ints([groups[0][0]] + [hi for _, hi in groups])
+    out, f32 = ops.gqa_prefix_decode(q, kp, vp, ints(plens), k, v, ints(lens), cu=cu, want_f32=True)
+    want, mag = reference(q, kp, vp, plens, k, v, lens, groups, d ** -0.5)
+    check(out, f32, want, mag)
+    again = ops.gqa_prefix_decode(q, kp, vp, ints(plens), k, v, ints(lens), cu=cu)
+    assert torch.equal(out, again)   # no order of arrival in it
