@@ -322,6 +322,38 @@ int q4nx_gqa_prefix_decode(const uint16_t *q, const uint16_t *k_prefix, const ui
                            uint16_t *out, float *out_f32, int batch, int n_q_heads, int n_kv_heads,
                            int head_dim, float scale, void *ws, size_t ws_bytes, void *stream);
 
+/* ---------------------------------------------------------------- eviction by attention weight
+ * q4nx_gqa_decode that also keeps what each position was given: weights[b][kv_head][l] += the sum over
+ * the group's query heads of the softmax weight of position l, for l < lens[b] (at most max_len); the
+ * newest position's (lens[b] - 1), and with `start` every one's, is set instead. Entries behind are left.
+ * Attention as in q4nx_gqa_prefix_decode without prefixes; weights fp32, strides in elements. No
+ * reference counterpart (its cache never shrinks). */
+size_t q4nx_gqa_decode_weights_ws_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim,
+                                        int max_len);
+int q4nx_gqa_decode_weights(const uint16_t *q, const uint16_t *k_cache, const uint16_t *v_cache,
+                            int64_t kv_b_stride, int64_t kv_h_stride, const int32_t *lens, int max_len,
+                            float *weights, int64_t w_b_stride, int64_t w_h_stride, int start,
+                            uint16_t *out, float *out_f32, int batch, int n_q_heads, int n_kv_heads,
+                            int head_dim, float scale, void *ws, size_t ws_bytes, void *stream);
+/* Every (sequence, kv head) of more than `budget` positions keeps that many: the `recent` last ones and
+ * of the others those of the greatest weights (ties to the lowest position; a NaN is greater than all),
+ * in the order of their positions; shorter ones keep all. Their rows of K and V and their weights go to
+ * the front of the outputs, weights behind them are set to 0 (up to the old length in place, else up to
+ * `room`), rows behind them are left; kept int32 [batch][Hkv][budget]: the positions, -1 behind the last;
+ * lens_out[b] = min(lens[b], budget). rope_tab (optional, as q4nx_rope_table_host writes it for head_dim,
+ * max_pos >= max_len): K is rotated back by the places that a row moves, as if it had been written where
+ * it now stands. In place: the outputs are the inputs (k_out == k_cache, ..), `room` says nothing, lens_out
+ * may be lens. Otherwise they overlap nothing that is read and hold `room` >= min(budget, max_len)
+ * positions a head. lens[b] > max_len counts as max_len. No reference counterpart. */
+size_t q4nx_kv_evict_ws_bytes(int batch, int n_kv_heads);
+int q4nx_kv_evict(const uint16_t *k_cache, const uint16_t *v_cache, int64_t kv_b_stride,
+                  int64_t kv_h_stride, const float *weights, int64_t w_b_stride, int64_t w_h_stride,
+                  const int32_t *lens, int max_len, int budget, int recent, const float *rope_tab,
+                  int max_pos, uint16_t *k_out, uint16_t *v_out, int64_t out_b_stride,
+                  int64_t out_h_stride, float *weights_out, int64_t wout_b_stride,
+                  int64_t wout_h_stride, int room, int32_t *lens_out, int32_t *kept, int batch,
+                  int n_kv_heads, int head_dim, void *ws, size_t ws_bytes, void *stream);
+
 /* ---------------------------------------------------------------- paged 4-bit K/V cache
  * K and V of one layer in pages of 4-bit codes, 10 D bytes per 8 positions and kv head instead of
  * 32 D (bf16). No reference counterpart: its cache is one dense bf16 buffer per sequence
@@ -488,6 +520,35 @@ int q4nx_decode_advance_embed(const uint64_t *keys, int n_slots, int32_t *tokens
                               int32_t *lens, int32_t *history, int32_t *step, int history_len,
                               int batch, int kind, const void *table, int vocab, int hidden,
                               float *h, float *ssq_out, void *stream);
+
+/* Counts of tokens, int32 [batch][count_stride]: how often a sequence's tokens have it each (prompt == 0), or
+ * the sign bit for those the prompt has (prompt != 0). cu (int32 [batch + 1]): sequence b's tokens are
+ * cu[b] .. cu[b+1] - 1 (held to 0 .. n_tokens); NULL: one each. Tokens outside [0, vocab) are skipped.
+ * start: counts of these tokens alone, whatever was there. batch <= 65535. No reference counterpart. */
+int q4nx_count_tokens(int32_t *counts, int64_t count_stride, int vocab, int batch,
+                      const int32_t *tokens, int n_tokens, const int32_t *cu, int prompt, int start,
+                      void *stream);
+/* Rules for the next token. Of logits [batch][stride] (fp32, or bf16 with bf16 != 0), per token in fp32
+ * and rounded after every step:
+ *   count word not 0:    x = x > 0 ? x / repetition[b] : x * repetition[b]
+ *                        x -= frequency[b] * n;  n > 0: x -= presence[b]   (n: the word without its sign bit)
+ *   x += the sequence's biases for it, one after the other
+ *   not allowed:         x = -inf
+ * out (same type; may be logits) [batch][out_stride]; tokens[b] (optional) the greatest x before its
+ * rounding to out's type (NaN above all, ties to the lowest token; all -inf: 0), keys[b] (optional) its
+ * order-preserving key as q4nx_decode_advance takes it with n_slots = 1.
+ * Each of the three penalties may be NULL (none). bias_*: ids (outside [0, vocab): skipped) and values,
+ * sequence b's at bias_cu[b] .. bias_cu[b+1] - 1 (held to 0 .. n_biases). mask [n_mask][mask_stride]: bit
+ * t % 32 of word t / 32 set: token t is allowed; sequence b goes by row mask_rows[b] (negative: all allowed;
+ * n_mask and more: none), without mask_rows by row b. ws: Q4NX_WS_COUNTER_BYTES, batch <= 4096. No
+ * reference counterpart (transformers' generate chooses its tokens, chat.py:74-78). */
+int q4nx_adjust_logits(const void *logits, int bf16, int64_t stride, void *out, int64_t out_stride,
+                       int vocab, int batch, const int32_t *counts, int64_t count_stride,
+                       const float *repetition, const float *presence, const float *frequency,
+                       const int32_t *bias_ids, const float *bias_values, int n_biases,
+                       const int32_t *bias_cu, const uint32_t *mask, int64_t mask_stride, int n_mask,
+                       const int32_t *mask_rows, int32_t *tokens, uint64_t *keys, void *ws,
+                       size_t ws_bytes, void *stream);
 
 #ifdef __cplusplus
 }

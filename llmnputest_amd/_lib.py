@@ -104,6 +104,15 @@ SIGNATURES: dict[str, tuple] = {
     "q4nx_gqa_prefix_decode_ws_bytes": (c_sz, [c_i, c_i, c_i, c_i, c_i, c_i, c_i]),
     "q4nx_gqa_prefix_decode": (c_i, [c_p, c_p, c_p, c_i64, c_i64, c_p, c_p, c_i, c_i, c_p, c_p, c_i64,
                                      c_i64, c_p, c_i, c_p, c_p, c_i, c_i, c_i, c_i, c_f, c_p, c_sz, c_p]),
+    "q4nx_gqa_decode_weights_ws_bytes": (c_sz, [c_i, c_i, c_i, c_i, c_i]),
+    "q4nx_gqa_decode_weights": (c_i, [c_p, c_p, c_p, c_i64, c_i64, c_p, c_i, c_p, c_i64, c_i64, c_i, c_p, c_p,
+                                      c_i, c_i, c_i, c_i, c_f, c_p, c_sz, c_p]),
+    "q4nx_kv_evict_ws_bytes": (c_sz, [c_i, c_i]),
+    "q4nx_kv_evict": (c_i, [c_p, c_p, c_i64, c_i64, c_p, c_i64, c_i64, c_p, c_i, c_i, c_i, c_p, c_i, c_p, c_p,
+                            c_i64, c_i64, c_p, c_i64, c_i64, c_i, c_p, c_p, c_i, c_i, c_i, c_p, c_sz, c_p]),
+    "q4nx_count_tokens": (c_i, [c_p, c_i64, c_i, c_i, c_p, c_i, c_p, c_i, c_i, c_p]),
+    "q4nx_adjust_logits": (c_i, [c_p, c_i, c_i64, c_p, c_i64, c_i, c_i, c_p, c_i64, c_p, c_p, c_p, c_p, c_p, c_i,
+                                 c_p, c_p, c_i64, c_i, c_p, c_p, c_p, c_p, c_sz, c_p]),
     "q4nx_kv4_page_bytes": (c_sz, [c_i, c_i, c_i]),
     "q4nx_kv4_append": (c_i, [c_kv4, c_p, c_p, c_i, c_i64, c_i64, c_i64, c_i64, c_p, c_p, c_i, c_p]),
     "q4nx_kv4_read": (c_i, [c_kv4, c_p, c_p, c_i, c_i64, c_p, c_p, c_i, c_p]),

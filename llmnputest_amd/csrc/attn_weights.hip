@@ -1,0 +1,210 @@
+// Attention of one token per sequence that also sums, per kv head, the weights that its query heads gave
+// each position: what kv_evict.hip decides by. No reference counterpart (its cache never shrinks).
+//
+//   p[h][l]       = softmax over l < len of scale q[h] . K[l]
+//   out[h]        = sum_l p[h][l] V[l]
+//   weights[l]   += sum over the group's heads of p[h][l]      (the newest position's is set)
+//
+// A weight needs the maximum and the sum of the whole row, which a part of it does not know. The parts
+// (part_narrow) therefore also leave their scores, 4 Hq bytes a position beside the 4 D Hkv of K and V, and
+// the second launch turns them into weights once every part's (m, l) is there; its last workgroup of a
+// (sequence, kv head) merges the outputs.
+
+#include "attn_parts.h"
+
+namespace q4nx {
+
+struct WeightArgs {
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
+  const int32_t* lens;
+  uint16_t* out;
+  float* out_f32;
+  float* weights;      // [batch][hkv] rows of w_b_stride, w_h_stride
+  float* rec;          // [batch * hkv][ns][G][kRec<D>]
+  float* scores;       // [batch * hkv][G][score_stride]
+  int64_t b_stride, h_stride, w_b_stride, w_h_stride, score_stride;
+  int batch, hq, hkv, G, max_len, ns, chunk, start;
+  float scale_l2;
+};
+
+template <int D>
+__global__ __launch_bounds__(256) void weight_parts_kernel(WeightArgs a) {
+  __shared__ __attribute__((aligned(16))) float lds[kPartWaves * 16 * D + 8 * 16];
+  int blk = blockIdx.x;
+  const int bk = blk % (a.batch * a.hkv), part = blk / (a.batch * a.hkv);
+  const int b = bk / a.hkv, kvh = bk - b * a.hkv;
+  const int len = min(max(a.lens[b], 0), a.max_len);
+  const int start = part * a.chunk;
+  if (start >= len) return;
+  const int end = min(a.chunk, len - start);
+  const size_t at = (size_t)b * a.b_stride + (size_t)kvh * a.h_stride + (size_t)start * D;
+  const size_t rec = ((size_t)bk * a.ns + part) * (size_t)(a.G * kRec<D>);
+  part_narrow<D, true>(a.q + ((size_t)b * a.hq + kvh * a.G + min((int)(threadIdx.x & 15), a.G - 1)) * D, a.G,
+                       a.k + at, a.v + at, end, end, a.scale_l2,
+                       a.scores + (size_t)bk * a.G * a.score_stride + start, a.score_stride, lds, a.rec,
+                       [&](int r) { return rec + (size_t)r * kRec<D>; });
+}
+
+constexpr int kWeightSpan = 1024;   // positions of a workgroup of the second launch
+
+template <int D>
+__global__ __launch_bounds__(256) void weight_sum_kernel(WeightArgs a, int spans) {
+  __shared__ float s_m[16], s_l[16];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int bk = blockIdx.x / (spans + 1), span = blockIdx.x % (spans + 1);
+  const int b = bk / a.hkv, kvh = bk - b * a.hkv;
+  const int len = min(max(a.lens[b], 0), a.max_len);
+  const int n = (len + a.chunk - 1) / a.chunk;   // parts that were written
+  const float* rec = a.rec + (size_t)bk * a.ns * (size_t)(a.G * kRec<D>);
+  if (span == spans) {
+    for (int h = wave; h < a.G; h += 4) {
+      float A[D / 64];
+      merge_records<D>(rec + ((size_t)min(lane, a.ns - 1) * a.G + h) * kRec<D>, n, lane, A);
+#pragma unroll
+      for (int x = 0; x < D / 64; ++x) {
+        const size_t at = ((size_t)b * a.hq + kvh * a.G + h) * D + lane + 64 * x;
+        if (a.out) a.out[at] = f32_to_bf16(A[x]);
+        if (a.out_f32) a.out_f32[at] = A[x];
+      }
+    }
+    return;
+  }
+  const int p0 = span * kWeightSpan;
+  if (p0 >= len) return;
+  for (int h = wave; h < a.G; h += 4) {
+    const float* mine = rec + ((size_t)min(lane, a.ns - 1) * a.G + h) * kRec<D>;
+    const float2 ml = lane < n ? *(const float2*)(mine + D) : make_float2(-INFINITY, 0.f);
+    const float M = wave_max(ml.x);
+    const float L = wave_sum(ml.x == -INFINITY ? ml.y : exp2_hw(ml.x - M) * ml.y);
+    if (lane == 0) {
+      s_m[h] = M == -INFINITY ? 0.f : M;
+      s_l[h] = L == 0.f ? 0.f : 1.f / L;
+    }
+  }
+  __syncthreads();
+  const float* scores = a.scores + (size_t)bk * a.G * a.score_stride;
+  float w[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int h = 0; h < a.G; ++h) {
+    const float m = s_m[h], li = s_l[h];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int p = p0 + tid + 256 * i;
+      if (p < len) w[i] = fmaf(exp2_hw(scores[h * a.score_stride + p] - m), li, w[i]);
+    }
+  }
+  float* to = a.weights + (size_t)b * a.w_b_stride + (size_t)kvh * a.w_h_stride;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int p = p0 + tid + 256 * i;
+    if (p < len) to[p] = a.start || p == len - 1 ? w[i] : to[p] + w[i];
+  }
+}
+
+struct WeightPlan {
+  int ns, chunk;
+  int64_t score_stride;
+};
+
+static WeightPlan weight_plan(int batch, int hkv, int max_len) {
+  WeightPlan p{};
+  const long long by_grid = 1024 / ((long long)hkv * batch);
+  p.ns = by_grid < 1 ? 1 : by_grid > 32 ? 32 : (int)by_grid;
+  const int by_len = (max_len + 255) / 256;
+  if (p.ns > by_len) p.ns = by_len;
+  p.chunk = part_chunk(max_len, p.ns, kPartRound);
+  p.ns = (max_len + p.chunk - 1) / p.chunk;
+  p.score_stride = (int64_t)p.ns * p.chunk;
+  return p;
+}
+
+static bool weight_shape_ok(int batch, int hq, int hkv, int d, int max_len) {
+  return batch >= 1 && batch <= (1 << 20) && hkv >= 1 && hkv <= 1024 && hq >= hkv && hq % hkv == 0 && hq / hkv <= 16 &&
+         (d == 64 || d == 128) && max_len >= 1 && max_len < (1 << 24) && (long long)batch * hq < (1 << 28);
+}
+
+static size_t weight_rec_bytes(const WeightPlan& p, int batch, int hq, int d) {
+  return (size_t)batch * hq * p.ns * (d + 4) * 4;
+}
+
+static size_t weight_ws(const WeightPlan& p, int batch, int hq, int d) {
+  return (size_t)Q4NX_WS_COUNTER_BYTES + weight_rec_bytes(p, batch, hq, d) + (size_t)batch * hq * p.score_stride * 4;
+}
+
+template <int D>
+static void weight_launch(const WeightArgs& a, hipStream_t s) {
+  const int spans = (a.max_len + kWeightSpan - 1) / kWeightSpan;
+  hipLaunchKernelGGL(weight_parts_kernel<D>, dim3((unsigned)(a.batch * a.hkv * a.ns)), dim3(256), 0, s, a);
+  hipLaunchKernelGGL(weight_sum_kernel<D>, dim3((unsigned)(a.batch * a.hkv * (spans + 1))), dim3(256), 0, s, a, spans);
+}
+
+}  // namespace q4nx
+
+using namespace q4nx;
+
+extern "C" {
+
+size_t q4nx_gqa_decode_weights_ws_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim, int max_len) {
+  if (!weight_shape_ok(batch, n_q_heads, n_kv_heads, head_dim, max_len)) return 0;
+  return weight_ws(weight_plan(batch, n_kv_heads, max_len), batch, n_q_heads, head_dim);
+}
+
+int q4nx_gqa_decode_weights(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache,
+                            int64_t kv_b_stride, int64_t kv_h_stride, const int32_t* lens, int max_len,
+                            float* weights, int64_t w_b_stride, int64_t w_h_stride, int start, uint16_t* out,
+                            float* out_f32, int batch, int n_q_heads, int n_kv_heads, int head_dim, float scale,
+                            void* ws, size_t ws_bytes, void* stream) {
+  const char* what = "q4nx_gqa_decode_weights";
+  Q4NX_REQUIRE(weight_shape_ok(batch, n_q_heads, n_kv_heads, head_dim, max_len), Q4NX_ERR_SHAPE,
+               "%s: batch=%d Hq=%d (a multiple of Hkv, at most 16 times) Hkv=%d head_dim=%d (64, 128) "
+               "max_len=%d (below 2^24)",
+               what, batch, n_q_heads, n_kv_heads, head_dim, max_len);
+  Q4NX_REQUIRE(q && k_cache && v_cache && lens && weights && (out || out_f32), Q4NX_ERR_ARG,
+               "%s: q, caches, lens, weights and an output are required", what);
+  Q4NX_REQUIRE(Q4NX_ALIGNED(q, 16) && Q4NX_ALIGNED(k_cache, 16) && Q4NX_ALIGNED(v_cache, 16), Q4NX_ERR_ARG,
+               "%s: q and caches must be 16-byte aligned", what);
+  Q4NX_REQUIRE(kv_h_stride >= (int64_t)max_len * head_dim && kv_h_stride % 8 == 0 &&
+                   kv_b_stride >= (int64_t)n_kv_heads * kv_h_stride && kv_b_stride % 8 == 0,
+               Q4NX_ERR_SHAPE, "%s: cache strides do not hold [Hkv][max_len][head_dim]", what);
+  Q4NX_REQUIRE(w_h_stride >= max_len && w_b_stride >= (int64_t)n_kv_heads * w_h_stride, Q4NX_ERR_SHAPE,
+               "%s: strides of weights do not hold [Hkv][max_len]", what);
+  Q4NX_REQUIRE(scale >= 0.f, Q4NX_ERR_ARG, "%s: scale must not be negative", what);
+  const WeightPlan p = weight_plan(batch, n_kv_heads, max_len);
+  Q4NX_REQUIRE((long long)n_kv_heads * batch * (max_len / kWeightSpan + 2) < (1ll << 31), Q4NX_ERR_SHAPE,
+               "%s: more than 2^31 workgroups", what);
+  const size_t need = weight_ws(p, batch, n_q_heads, head_dim);
+  Q4NX_REQUIRE(ws != nullptr && ws_bytes >= need && Q4NX_ALIGNED(ws, 256), Q4NX_ERR_WS,
+               "%s: workspace of %zu bytes (256-aligned) needed, %zu given", what, need, ws_bytes);
+  WeightArgs a{};
+  a.q = q;
+  a.k = k_cache;
+  a.v = v_cache;
+  a.lens = lens;
+  a.out = out;
+  a.out_f32 = out_f32;
+  a.weights = weights;
+  a.scores = (float*)((uint8_t*)ws + Q4NX_WS_COUNTER_BYTES);   // rows of whole rounds: 16-byte aligned
+  a.rec = a.scores + (size_t)batch * n_q_heads * p.score_stride;
+  a.b_stride = kv_b_stride;
+  a.h_stride = kv_h_stride;
+  a.w_b_stride = w_b_stride;
+  a.w_h_stride = w_h_stride;
+  a.score_stride = p.score_stride;
+  a.batch = batch;
+  a.hq = n_q_heads;
+  a.hkv = n_kv_heads;
+  a.G = n_q_heads / n_kv_heads;
+  a.max_len = max_len;
+  a.ns = p.ns;
+  a.chunk = p.chunk;
+  a.start = start != 0;
+  a.scale_l2 = (float)((double)scale * 1.4426950408889634);
+  hipStream_t s = (hipStream_t)stream;
+  if (head_dim == 64) weight_launch<64>(a, s);
+  else weight_launch<128>(a, s);
+  return check_launch(what);
+}
+
+}  // extern "C"

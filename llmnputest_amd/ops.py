@@ -667,6 +667,190 @@ def gqa_prefix_decode(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.T
     return (out, of) if want_f32 else out
 
 
+# ---------------------------------------------------------------- eviction by attention weight
+
+def _weight_rows(t: torch.Tensor, name: str, shape: tuple) -> tuple[int, int]:
+    """The sequence and head strides of weights fp32 [B, Hkv, L]."""
+    if t.get_device() != torch.cuda.current_device():
+        raise ValueError(f"{name} must be on the current device, got {t.device}")
+    if t.dtype != torch.float32:
+        raise TypeError(f"{name} must be {torch.float32}, got {t.dtype}")
+    if t.shape != shape or (shape[2] > 1 and t.stride(2) != 1):
+        raise ValueError(f"{name} must be {list(shape)}, positions contiguous")
+    h = t.stride(1) if shape[1] > 1 else shape[2]
+    return (t.stride(0) if shape[0] > 1 else shape[1] * h), h
+
+
+def gqa_decode_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                       lens: torch.Tensor, weights: torch.Tensor, start: bool = False,
+                       scale: float | None = None, max_len: int | None = None,
+                       out: torch.Tensor | None = None, want_f32: bool = False,
+                       ws: Workspace | None = None):
+    """`gqa_decode` (D 64 or 128, Hq/Hkv at most 16, scale by default D ** -0.5) that also adds to
+    weights, fp32 [B, Hkv, L], what the group's query heads gave each position l < lens[b]: the sum over
+    the heads of its softmax weight. The newest position's (lens[b] - 1) is set, not added to, and with
+    `start` every one's; entries behind it are left. What `kv_evict` goes by."""
+    b, hq, d = q.shape
+    qp = _here(q, "q", torch.bfloat16)
+    bs, hs = _rows_of(k_cache, v_cache, "cache", d)
+    hkv, n = k_cache.shape[1:3]
+    if k_cache.shape[0] != b:
+        raise ValueError(f"k_cache must be [{b}, Hkv, L, {d}]")
+    wb, wh = _weight_rows(weights, "weights", (b, hkv, n))
+    lp = _here(lens, "lens", torch.int32, (b,))
+    out = torch.empty_like(q) if out is None else out
+    op = _here(out, "out", torch.bfloat16, q.shape)
+    of = torch.empty(q.shape, dtype=torch.float32, device=q.device) if want_f32 else None
+    most = _upto(n, max_len, "max_len")
+    if b == 0 or most == 0:
+        out.zero_()
+        return (out, of.zero_()) if want_f32 else out
+    need = _lib.lib().q4nx_gqa_decode_weights_ws_bytes(b, hq, hkv, d, most)
+    ws, wp, wn, stream = _scratch(ws, need)
+    _lib.call("q4nx_gqa_decode_weights", qp, k_cache.data_ptr(), v_cache.data_ptr(), bs, hs, lp, most,
+              weights.data_ptr(), wb, wh, int(start), op, _ptr(of), b, hq, hkv, d,
+              d ** -0.5 if scale is None else float(scale), wp, wn, stream)
+    return (out, of) if want_f32 else out
+
+
+def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tensor, lens: torch.Tensor,
+             budget: int, recent: int, rope: torch.Tensor | None = None, into: tuple | None = None,
+             max_len: int | None = None, ws: Workspace | None = None) -> torch.Tensor:
+    """Cuts every (sequence, kv head) of more than `budget` positions down to the `recent` last ones and
+    the heaviest others (ties to the lowest), in their order; the positions that were kept, int32
+    [B, Hkv, budget], -1 behind the last. Caches bf16 [B, Hkv, L, D], weights fp32 [B, Hkv, L], lens int32
+    [B]. The rows, their weights and the lengths go to the front of `into` = (k, v, weights, lens) with
+    room for them, which overlap nothing that is read, or, without it, stay in place. Weights behind them
+    become 0 (in place: up to the old length). rope: a `rope_table` of at least the longest length; K is
+    then turned to its new places, so that what follows goes on from position lens[b]."""
+    b, hkv, n, d = k_cache.shape
+    bs, hs = _rows_of(k_cache, v_cache, "cache", d)
+    wb, wh = _weight_rows(weights, "weights", (b, hkv, n))
+    lp = _here(lens, "lens", torch.int32, (b,))
+    k2, v2, w2, l2 = (k_cache, v_cache, weights, lens) if into is None else into
+    if into is None:
+        obs, ohs, owb, owh, room = bs, hs, wb, wh, n
+    else:
+        if k2.dim() != 4 or k2.shape[:2] != (b, hkv):
+            raise ValueError(f"k of into must be [{b}, {hkv}, room, {d}]")
+        room = k2.shape[2]
+        obs, ohs = _rows_of(k2, v2, "into", d)
+        owb, owh = _weight_rows(w2, "weights of into", (b, hkv, room))
+        _here(l2, "lens of into", torch.int32, (b,))
+        for x, y, name in ((k2, k_cache, "k"), (v2, v_cache, "v"), (w2, weights, "weights")):
+            if x.numel() and x.data_ptr() == y.data_ptr():
+                raise ValueError(f"{name} of into is the input: leave into out to cut down in place")
+    if rope is not None:
+        _here(rope, "rope", torch.float32, (rope.shape[0], 2, d // 2))
+    if budget < 1 or not 0 <= recent <= budget:
+        raise ValueError(f"budget must be positive and recent in 0..budget, got {budget} and {recent}")
+    kept = torch.empty((b, hkv, budget), dtype=torch.int32, device=k_cache.device)
+    most = _upto(n, max_len, "max_len")
+    if b == 0 or most == 0:
+        l2.zero_()
+        if into is not None:
+            w2.zero_()
+        return kept.fill_(-1)
+    need = _lib.lib().q4nx_kv_evict_ws_bytes(b, hkv)
+    ws, wp, wn, stream = _scratch(ws, need)
+    _lib.call("q4nx_kv_evict", k_cache.data_ptr(), v_cache.data_ptr(), bs, hs, weights.data_ptr(), wb, wh, lp,
+              most, budget, recent, _ptr(rope), 0 if rope is None else rope.shape[0], k2.data_ptr(),
+              v2.data_ptr(), obs, ohs, w2.data_ptr(), owb, owh, room, l2.data_ptr(), kept.data_ptr(), b, hkv,
+              d, wp, wn, stream)
+    return kept
+
+
+# ---------------------------------------------------------------- rules for the next token
+
+def _vocab_rows(t: torch.Tensor, name: str, dtype, shape: tuple | None = None) -> int:
+    """The row stride of a tensor [B, V], tokens contiguous."""
+    if t.get_device() != torch.cuda.current_device():
+        raise ValueError(f"{name} must be on the current device, got {t.device}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (shape is not None and t.shape != shape):
+        raise ValueError(f"{name} must be {'[rows, V]' if shape is None else list(shape)}, rows contiguous")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def count_tokens(counts: torch.Tensor, tokens: torch.Tensor, cu: torch.Tensor | None = None,
+                 prompt: bool = False, start: bool = False) -> None:
+    """Counts tokens (int32) for `adjust_logits`: counts int32 [B, V], how often each was generated, and
+    with `prompt` the sign bit of those that the prompt has. One token per sequence, or tokens
+    cu[b] .. cu[b+1] - 1 (int32 [B + 1]); those outside the vocabulary are skipped. start: counts of these
+    alone, whatever was there."""
+    stride = _vocab_rows(counts, "counts", torch.int32)
+    b, v = counts.shape
+    tp = _here(tokens, "tokens", torch.int32)
+    n = tokens.numel()
+    if tokens.dim() != 1 or (cu is None and n != b):
+        raise ValueError(f"tokens must be a list, of {b} without cu")
+    up = None if cu is None else _here(cu, "cu", torch.int32, (b + 1,))
+    if b and v:
+        _lib.call("q4nx_count_tokens", counts.data_ptr(), stride, v, b, tp or None, n, up, int(prompt),
+                  int(start), _stream())
+
+
+def adjust_logits(logits: torch.Tensor, counts: torch.Tensor | None = None,
+                  repetition: torch.Tensor | None = None, presence: torch.Tensor | None = None,
+                  frequency: torch.Tensor | None = None, bias: tuple | None = None,
+                  mask: torch.Tensor | None = None, mask_rows: torch.Tensor | None = None,
+                  out: torch.Tensor | None = None, tokens: torch.Tensor | None = None,
+                  keys: torch.Tensor | None = None, ws: Workspace | None = None):
+    """Rules for the next token on logits [B, V] (fp32 or bf16, any row stride): (out, tokens), out of
+    logits' type (`out=logits` works in place) and the greatest of each row, int32 [B], from the values
+    before their rounding to that type.
+
+    In fp32: tokens in counts (`count_tokens`; not 0): x / repetition where x > 0, else x * repetition;
+    minus frequency times how often it was generated, minus presence if it was (fp32 [B] each, or None);
+    plus the biases (ids int32 [N], values fp32 [N], cu int32 [B + 1]: sequence b's are cu[b] ..
+    cu[b+1] - 1); -inf where the mask (int32 [rows, (V + 31) // 32], bit t % 32 of word t // 32: token t
+    is allowed) has no bit. mask_rows int32 [B]: the row that a sequence goes by, negative: all allowed,
+    behind the last: none; without it row b. keys: int64 [B], the greatest as `decode_advance` takes it
+    (n_slots 1)."""
+    if logits.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"logits must be float32 or bfloat16, got {logits.dtype}")
+    stride = _vocab_rows(logits, "logits", logits.dtype)
+    b, v = logits.shape
+    out = torch.empty((b, v), dtype=logits.dtype, device=logits.device) if out is None else out
+    out_stride = _vocab_rows(out, "out", logits.dtype, logits.shape)
+    cs = 0 if counts is None else _vocab_rows(counts, "counts", torch.int32, logits.shape)
+    pen = []
+    for t, name in ((repetition, "repetition"), (presence, "presence"), (frequency, "frequency")):
+        if t is not None and counts is None:
+            raise ValueError(f"{name} needs counts")
+        pen.append(None if t is None else _here(t, name, torch.float32, (b,)))
+    ids = values = bias_cu = None
+    n_bias = 0
+    if bias is not None:
+        n_bias = bias[0].numel()
+        if n_bias:
+            ids = _here(bias[0], "bias ids", torch.int32, (n_bias,))
+            values = _here(bias[1], "bias values", torch.float32, (n_bias,))
+            bias_cu = _here(bias[2], "bias cu", torch.int32, (b + 1,))
+    ms = n_mask = 0
+    if mask is not None:
+        n_mask = mask.shape[0]
+        ms = _vocab_rows(mask, "mask", torch.int32, (n_mask, (v + 31) // 32))
+        if n_mask == 0 or (mask_rows is None and n_mask != b):
+            raise ValueError(f"mask must have a row for each of {b} sequences, or mask_rows")
+    elif mask_rows is not None:
+        raise ValueError("mask_rows needs mask")
+    rp = None if mask_rows is None else _here(mask_rows, "mask_rows", torch.int32, (b,))
+    if tokens is None:
+        tokens = torch.empty(b, dtype=torch.int32, device=logits.device)
+    tp = _here(tokens, "tokens", torch.int32, (b,))
+    kp = None if keys is None else _here(keys, "keys", torch.int64, (b,))
+    if v == 0:
+        raise ValueError("logits must have at least one token")
+    if b:
+        ws, wp, wn, stream = _scratch(ws, WS_COUNTER_BYTES)
+        _lib.call("q4nx_adjust_logits", logits.data_ptr(), int(logits.dtype == torch.bfloat16), stride,
+                  out.data_ptr(), out_stride, v, b, _ptr(counts), cs, *pen, ids, values, n_bias, bias_cu,
+                  _ptr(mask), ms, n_mask, rp, tp, kp, wp, wn, stream)
+    return out, tokens
+
+
 # ---------------------------------------------------------------- decode helpers
 
 def embed(table: torch.Tensor, kind: str, tokens: torch.Tensor, vocab: int, hidden: int,
