@@ -74,7 +74,8 @@ __device__ __forceinline__ Group find_tile(const PrefixArgs& a, int RT, int lane
 }
 
 // 64 NR query rows (16 NR a wave) over cache rows [0, end): tiles of 64 positions of K and V go through
-// LDS, loaded one tile ahead, read by all four waves. V^T comes out of the transposing LDS read. P is
+// LDS, loaded ahead, read by all four waves; a tile's scores are computed beside the previous tile's
+// exponentials. V^T comes out of the transposing LDS read. P is
 // rounded to bf16 once (2^-9 of a weight; the same rounded weights are summed to l, by a product with
 // ones, so they still add up to one). The running maximum moves only when a row's tile exceeds it by 2^8
 // (weights stay below 2^8 then), which leaves out nearly every rescaling of the accumulators.
@@ -121,67 +122,95 @@ __device__ __forceinline__ void part_wide(const PrefixArgs& a, const uint16_t* k
   }
 
   uint4 gk[LD], gv[LD];
-  auto fetch = [&](int p0) {   // rows past the end: the last one again, whose weight is masked to 0
+  // through buffer resources over the part's rows: those past the end read zeros (their weights are masked
+  // to 0), and the tile's place is a scalar offset
+  const __amdgpu_buffer_rsrc_t kr = make_rsrc(kbase, (uint32_t)end * (2 * D));
+  const __amdgpu_buffer_rsrc_t vr = make_rsrc(vbase, (uint32_t)end * (2 * D));
+  auto fetch = [&](__amdgpu_buffer_rsrc_t r, int p0, uint4 (&x)[LD]) {
 #pragma unroll
     for (int i = 0; i < LD; ++i) {
-      const int id = tid + 256 * i;
-      const size_t at = (size_t)min(p0 + id / C, end - 1) * D + id % C * 8;
-      gk[i] = *(const uint4*)(kbase + at);
-      gv[i] = *(const uint4*)(vbase + at);
+      const v4i_t v = __builtin_amdgcn_raw_buffer_load_b128(r, (tid + 256 * i) * 16, p0 * (2 * D), 0);
+      x[i] = make_uint4((uint32_t)v.x, (uint32_t)v.y, (uint32_t)v.z, (uint32_t)v.w);
     }
   };
-  auto put = [&](int b) {
+  auto put_k = [&](int t) {
 #pragma unroll
-    for (int i = 0; i < LD; ++i) {
-      const int id = tid + 256 * i;
-      sk[b * 64 * C + swz_k<D>(id / C, id % C)] = gk[i];
-      sv[b * 64 * C + swz_v<D>(id / C, id % C)] = gv[i];
-    }
+    for (int i = 0; i < LD; ++i) sk[(t & 1) * 64 * C + swz_k<D>((tid + 256 * i) / C, tid % C)] = gk[i];
+  };
+  auto put_v = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < LD; ++i) sv[(t & 1) * 64 * C + swz_v<D>((tid + 256 * i) / C, tid % C)] = gv[i];
   };
   const bool busy = r0 < R;   // waves without rows only load
   const uint32_t one2 = 0x3F803F80u;
   const u32x4_t ones = {one2, one2, one2, one2};
   const int nt = (end + 63) / 64;
-  fetch(0);
-  put(0);
-  __syncthreads();
-  for (int t = 0; t < nt; ++t) {
-    const int b = t & 1;
-    if (t + 1 < nt) fetch((t + 1) * 64);
+
+  f32x4_t s[NR][4];   // the tile's scores
+  float mx[NR];       // and the greatest of them, scaled
+  // operands read from LDS a step ahead of their products (left to the compiler, every pair of products
+  // waited for its own reads); only arithmetic is moved across
+  u32x4_t kf[2][KC], vf[D / 16];
+  auto hold = [] { __builtin_amdgcn_sched_barrier(0xE); };
+  auto read_k = [&](int t, int x) {
+#pragma unroll
+    for (int c = 0; c < KC; ++c)
+      kf[x & 1][c] = *(const u32x4_t*)(sk + (t & 1) * 64 * C + swz_k<D>(16 * x + j, 4 * c + g));
+    hold();
+  };
+  auto read_v = [&](int t, int x2) {
+#pragma unroll
+    for (int u = 0; u < D / 16; ++u) {
+      uint2 h[2];
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const int row = 32 * x2 + 16 * y + 4 * g + (j >> 2);
+        const char* p = (const char*)(sv + (t & 1) * 64 * C + swz_v<D>(row, 2 * u + ((j & 3) >> 1))) + 8 * (j & 1);
+        h[y] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)p));
+      }
+      vf[u] = u32x4_t{h[0].x, h[0].y, h[1].x, h[1].y};
+    }
+    hold();
+  };
+  auto score = [&](int x) {
+#pragma unroll
+    for (int n = 0; n < NR; ++n) s[n][x] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < KC; ++c)
+#pragma unroll
+      for (int n = 0; n < NR; ++n) s[n][x] = mfma_bf16(kf[x & 1][c], q[n][c], s[n][x]);
+  };
+  // `last`: some positions may lie past the end (apart from the others: as selects in every tile, this made
+  // 120 us of 90 with 256 x 16384)
+  auto scored = [&](int t, auto last) {
+    if constexpr (last) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (t * 64 + 16 * x + 4 * g + e >= end)
+#pragma unroll
+            for (int n = 0; n < NR; ++n) s[n][x][e] = -INFINITY;
+    }
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      float v = s[n][0][0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) v = fmaxf(v, s[n][i >> 2][i & 3]);
+      mx[n] = xor32_max(xor16_max(v)) * a.scale_l2;
+    }
+  };
+  // one tile's weights and their product; as its scores are used up, the next tile's take their place
+  auto tile = [&](int t, auto more, auto last) {
+    if constexpr (more) {
+      fetch(kr, (t + 2) * 64, gk);
+      fetch(vr, (t + 1) * 64, gv);
+    }
     if (busy) {
-      const uint4* const kt = sk + b * 64 * C;
-      const uint4* const vt = sv + b * 64 * C;
-      f32x4_t s[NR][4];
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-#pragma unroll
-        for (int n = 0; n < NR; ++n) s[n][x] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < KC; ++c) {
-          const u32x4_t kk = *(const u32x4_t*)(kt + swz_k<D>(16 * x + j, 4 * c + g));
-#pragma unroll
-          for (int n = 0; n < NR; ++n) s[n][x] = mfma_bf16(kk, q[n][c], s[n][x]);
-        }
-      }
-      if ((t + 1) * 64 > end) {
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (t * 64 + 16 * x + 4 * g + e >= end)
-#pragma unroll
-              for (int n = 0; n < NR; ++n) s[n][x][e] = -INFINITY;
-      }
-      float mx[NR];
+      if constexpr (more) read_k(t + 1, 0);
       bool up = false;
 #pragma unroll
-      for (int n = 0; n < NR; ++n) {
-        float v = s[n][0][0];
-#pragma unroll
-        for (int i = 1; i < 16; ++i) v = fmaxf(v, s[n][i >> 2][i & 3]);
-        mx[n] = xor32_max(xor16_max(v)) * a.scale_l2;
-        up |= mx[n] > m[n] + 8.f;
-      }
+      for (int n = 0; n < NR; ++n) up |= mx[n] > m[n] + 8.f;
       if (__any(up)) {
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
@@ -193,40 +222,60 @@ __device__ __forceinline__ void part_wide(const PrefixArgs& a, const uint16_t* k
           for (int u = 0; u < D / 16; ++u) o[n][u] *= corr;
         }
       }
-      u32x4_t pp[NR][2];
 #pragma unroll
-      for (int n = 0; n < NR; ++n) {
-        const float mb = m[n] == -INFINITY ? 0.f : m[n];
+      for (int x2 = 0; x2 < 2; ++x2) {
+        u32x4_t pp[NR];
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
+        for (int x1 = 0; x1 < 2; ++x1) {
+          const int x = 2 * x2 + x1;
+          if constexpr (more)
+            if (x < 3) read_k(t + 1, x + 1);
+          if (x1 == 1) read_v(t, x2);
 #pragma unroll
-          for (int w = 0; w < 2; ++w)
-            pp[n][x >> 1][2 * (x & 1) + w] =
-                pack_bf16x2_op(exp2_hw(fmaf(s[n][x][2 * w], a.scale_l2, -mb)),
-                               exp2_hw(fmaf(s[n][x][2 * w + 1], a.scale_l2, -mb)));
-      }
+          for (int n = 0; n < NR; ++n) {
+            const float mb = m[n] == -INFINITY ? 0.f : m[n];
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-#pragma unroll
-        for (int n = 0; n < NR; ++n) l[n] = mfma_bf16(ones, pp[n][x], l[n]);
-#pragma unroll
-        for (int u = 0; u < D / 16; ++u) {
-          uint2 h[2];
-#pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            const int row = 32 * x + 16 * y + 4 * g + (j >> 2);
-            const char* p = (const char*)(vt + swz_v<D>(row, 2 * u + ((j & 3) >> 1))) + 8 * (j & 1);
-            h[y] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)p));
+            for (int y = 0; y < 2; ++y)
+              pp[n][2 * x1 + y] = pack_bf16x2_op(exp2_hw(fmaf(s[n][x][2 * y], a.scale_l2, -mb)),
+                                                 exp2_hw(fmaf(s[n][x][2 * y + 1], a.scale_l2, -mb)));
           }
-          const u32x4_t vv = {h[0].x, h[0].y, h[1].x, h[1].y};
-#pragma unroll
-          for (int n = 0; n < NR; ++n) o[n][u] = mfma_bf16(vv, pp[n][x], o[n][u]);
+          if constexpr (more) score(x);
         }
+#pragma unroll
+        for (int n = 0; n < NR; ++n) l[n] = mfma_bf16(ones, pp[n], l[n]);
+#pragma unroll
+        for (int u = 0; u < D / 16; ++u)
+#pragma unroll
+          for (int n = 0; n < NR; ++n) o[n][u] = mfma_bf16(vf[u], pp[n], o[n][u]);
       }
+      if constexpr (more) scored(t + 1, last);
     }
-    if (t + 1 < nt) put(b ^ 1);   // its readers left it before the last barrier
-    __syncthreads();
+    if constexpr (more) {
+      // K of tile t + 2 takes the place of tile t's, V of t + 1 that of t - 1's: both were last read
+      // before the barrier that began this tile
+      put_k(t + 2);
+      put_v(t + 1);
+      __syncthreads();
+    }
+  };
+  fetch(kr, 0, gk);
+  fetch(vr, 0, gv);
+  put_k(0);
+  put_v(0);
+  fetch(kr, 64, gk);
+  put_k(1);
+  __syncthreads();
+  if (busy) {
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      read_k(0, x);
+      score(x);
+    }
+    scored(0, std::true_type{});
   }
+  for (int t = 0; t + 2 < nt; ++t) tile(t, std::true_type{}, std::false_type{});
+  if (nt > 1) tile(nt - 2, std::true_type{}, std::true_type{});
+  tile(nt - 1, std::false_type{}, std::false_type{});
 #pragma unroll
   for (int n = 0; n < NR; ++n) {
     const int r = r0 + 16 * n + j;
@@ -334,11 +383,12 @@ struct PrefixPlan {
 static int clamp_int(long long x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : (int)x; }
 
 // How the work is cut. Only bounds are known here (the lengths are on the device).
-static PrefixPlan prefix_plan(int batch, int hq, int hkv, int n_prefixes, int max_prefix, int max_len) {
+static PrefixPlan prefix_plan(int batch, int hq, int hkv, int d, int n_prefixes, int max_prefix, int max_len) {
   const int G = hq / hkv;
   const long long rows = (long long)batch * G;
   PrefixPlan p{};
-  p.nr = rows > 64 ? 2 : 1;
+  // 32 rows a wave where prefixes have more than 64 of them on average and the registers hold it
+  p.nr = d == 64 && rows > 64ll * (n_prefixes > 1 ? n_prefixes : 1) ? 2 : 1;
   const int rt = 64 * p.nr;
   // every prefix may end inside a tile
   const long long most = (rows + rt - 1) / rt + (n_prefixes > 0 ? n_prefixes - 1 : 0);
@@ -376,8 +426,8 @@ template <int D>
 static void prefix_launch(const PrefixArgs& a, const PrefixPlan& p, hipStream_t s) {
   const unsigned grid = (unsigned)(a.hkv * (p.tiles * p.ns_pre + a.batch * p.ns_own));
   if (grid > 0) {
-    if (p.nr == 1) hipLaunchKernelGGL((prefix_parts_kernel<D, 1>), dim3(grid), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((prefix_parts_kernel<D, 2>), dim3(grid), dim3(256), 0, s, a);
+    if (D == 64 && p.nr == 2) hipLaunchKernelGGL((prefix_parts_kernel<64, 2>), dim3(grid), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((prefix_parts_kernel<D, 1>), dim3(grid), dim3(256), 0, s, a);
   }
   const unsigned wgs = (unsigned)(((long long)a.batch * a.hq + 3) / 4);
   hipLaunchKernelGGL(prefix_merge_kernel<D>, dim3(wgs), dim3(256), 0, s, a);
@@ -392,7 +442,7 @@ extern "C" {
 size_t q4nx_gqa_prefix_decode_ws_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim, int n_prefixes,
                                        int max_prefix, int max_len) {
   if (!prefix_shape_ok(batch, n_q_heads, n_kv_heads, head_dim, n_prefixes, max_prefix, max_len)) return 0;
-  const PrefixPlan p = prefix_plan(batch, n_q_heads, n_kv_heads, n_prefixes, max_prefix, max_len);
+  const PrefixPlan p = prefix_plan(batch, n_q_heads, n_kv_heads, head_dim, n_prefixes, max_prefix, max_len);
   return (size_t)Q4NX_WS_COUNTER_BYTES + prefix_rec_bytes(p, batch, n_q_heads, head_dim);
 }
 
@@ -425,7 +475,7 @@ int q4nx_gqa_prefix_decode(const uint16_t* q, const uint16_t* k_prefix, const ui
                                              prefix_stride % 8 == 0))),
                Q4NX_ERR_SHAPE, "%s: prefix strides do not hold [Hkv][max_prefix][head_dim]", what);
   Q4NX_REQUIRE(scale >= 0.f, Q4NX_ERR_ARG, "%s: scale must not be negative", what);
-  const PrefixPlan p = prefix_plan(batch, n_q_heads, n_kv_heads, n_prefixes, max_prefix, max_len);
+  const PrefixPlan p = prefix_plan(batch, n_q_heads, n_kv_heads, head_dim, n_prefixes, max_prefix, max_len);
   Q4NX_REQUIRE((long long)n_kv_heads * ((long long)p.tiles * p.ns_pre + (long long)batch * p.ns_own) < (1ll << 31),
                Q4NX_ERR_SHAPE, "%s: more than 2^31 workgroups", what);
   const size_t need = (size_t)Q4NX_WS_COUNTER_BYTES + prefix_rec_bytes(p, batch, n_q_heads, head_dim);
