@@ -191,29 +191,57 @@ __device__ __forceinline__ void part_narrow(const uint16_t* qrow, int R, const u
   }
 }
 
-// The merge of a (sequence, query head)'s records by one wave: lane r < n holds the address of record r.
-// Channel lane + 64 i of the answer in A[i]; 0 where the records hold nothing.
-template <int D>
-__device__ __forceinline__ void merge_records(const float* mine, int n, int lane, float (&A)[D / 64]) {
-  const bool have = lane < n;
-  const float2 ml = have ? *(const float2*)(mine + D) : make_float2(-INFINITY, 0.f);
-  const float M = wave_max(ml.x);
-  const float f = ml.x == -INFINITY ? 0.f : exp2_hw(ml.x - M);
-  const float L = wave_sum(f * ml.y);   // a NaN of any record reaches L
-  const uint64_t at = (uint64_t)(uintptr_t)mine;
+// The merge of a (sequence, query head)'s records by one wave: record r < slots at rec + r * stride, those
+// with valid(r) count. Groups of D/4 lanes take a record each, four channels a lane; nothing is waited for
+// before all records are on their way (valid() may wait for lengths), stale ones of earlier launches among
+// them. Channels 4 c .. 4 c + 3 (c = lane % (D/4)) of the answer in every group; 0 where nothing was seen.
+template <int D, typename Valid>
+__device__ __forceinline__ float4 merge_records(const float* rec, size_t stride, int slots, int lane, Valid valid) {
+  constexpr int LR = D / 4, GR = 64 / LR, U = 4;   // lanes of a record, records at once, and in flight
+  const int q = lane / LR, c = lane % LR;
+  const float2 head = *(const float2*)(rec + (size_t)min(lane, slots - 1) * stride + D);
+  float4 x[U];
 #pragma unroll
-  for (int i = 0; i < D / 64; ++i) A[i] = 0.f;
-#pragma unroll 4
-  for (int r = 0; r < n; ++r) {
-    const uint64_t a = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)at, r) |
-                       (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(at >> 32), r) << 32;
-    const float* p = (const float*)(uintptr_t)a;
-    const float w = lane_f(f, r);
+  for (int i = 0; i < U; ++i) x[i] = *(const float4*)(rec + (size_t)min(GR * i + q, slots - 1) * stride + 4 * c);
+  const bool counts = valid(lane);   // by all lanes: it may vote
+  const bool ok = lane < slots && counts;
+  const uint64_t who = __ballot(ok);
+  const float m = ok ? head.x : -INFINITY, l = ok ? head.y : 0.f;
+  const float M = wave_max(m);
+  const float f = m == -INFINITY ? 0.f : exp2_hw(m - M);
+  const float L = wave_sum(m == -INFINITY ? l : f * l);   // a NaN of any record reaches L
+  float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int r0 = 0; r0 < slots; r0 += U * GR) {
+    if (r0 > 0) {
 #pragma unroll
-    for (int i = 0; i < D / 64; ++i) A[i] = fmaf(p[lane + 64 * i], w, A[i]);
+      for (int i = 0; i < U; ++i)
+        x[i] = *(const float4*)(rec + (size_t)min(r0 + GR * i + q, slots - 1) * stride + 4 * c);
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int r = r0 + GR * i + q;
+      const float w = __shfl(f, r & 63);
+      if (r < slots && (who >> (r & 63) & 1)) {
+        A.x = fmaf(x[i].x, w, A.x);
+        A.y = fmaf(x[i].y, w, A.y);
+        A.z = fmaf(x[i].z, w, A.z);
+        A.w = fmaf(x[i].w, w, A.w);
+      }
+    }
   }
+  float* const a = (float*)&A;
 #pragma unroll
-  for (int i = 0; i < D / 64; ++i) A[i] = L == 0.f ? 0.f : attn_div(A[i], L);
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (GR == 4) a[i] = xor16_sum(a[i]);
+    a[i] = L == 0.f ? 0.f : attn_div(xor32_sum(a[i]), L);
+  }
+  return A;
+}
+
+// Its four channels of the answer at `at` of the outputs that are wanted.
+__device__ __forceinline__ void put_channels(uint16_t* out, float* out_f32, size_t at, const float4& A) {
+  if (out) *(uint2*)(out + at) = make_uint2(pack_bf16x2(A.x, A.y), pack_bf16x2(A.z, A.w));
+  if (out_f32) *(float4*)(out_f32 + at) = A;
 }
 
 // Positions a part takes when `len` is cut in ns, a multiple of `unit`.

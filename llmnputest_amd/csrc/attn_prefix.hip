@@ -349,31 +349,32 @@ __global__ __launch_bounds__(256) void prefix_merge_kernel(PrefixArgs a) {
   const int i = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
   if (i >= a.batch * a.hq) return;
   const int b = i / a.hq, h = i - b * a.hq;
-  const int kvh = h / a.G;
-  const int len = min(max(a.lens[b], 0), a.max_len);
-  const int n_own = len > 0 ? (len + a.chunk_own - 1) / a.chunk_own : 0;
-  int n_pre = 0;
-  for (int p0 = 0; p0 < a.n_prefixes; p0 += 64) {
-    const int p = p0 + lane;
-    const bool in = p < a.n_prefixes && cu_at(a, p) <= b && b < cu_at(a, p + 1);
-    const uint64_t who = __ballot(in);
-    if (who != 0) {
-      const int pl = min(max(a.plens[p0 + __builtin_ctzll(who)], 0), a.max_prefix);
-      n_pre = pl > 0 ? (pl + a.chunk_pre - 1) / a.chunk_pre : 0;
-      break;
+  const int kvh = h / a.G, slots = a.ns_own + a.ns_pre;
+  if (slots == 0) {
+    if (lane < D / 4) put_channels(a.out, a.out_f32, (size_t)i * D + 4 * lane, make_float4(0.f, 0.f, 0.f, 0.f));
+    return;
+  }
+  const float* rec = a.rec + (((size_t)b * a.hkv + kvh) * slots * a.G + (h - kvh * a.G)) * kRec<D>;
+  const float4 A = merge_records<D>(rec, (size_t)a.G * kRec<D>, slots, lane, [&](int r) {
+    const int len = min(max(a.lens[b], 0), a.max_len);
+    int pl = 0;
+    for (int p0 = 0; p0 < a.n_prefixes; p0 += 64) {
+      const int p = p0 + lane;
+      bool in = false;
+      int n = 0;
+      if (p < a.n_prefixes) {
+        in = cu_at(a, p) <= b && b < cu_at(a, p + 1);
+        n = a.plens[p];
+      }
+      const uint64_t who = __ballot(in);
+      if (who != 0) {
+        pl = min(max(__builtin_amdgcn_readlane(n, __builtin_ctzll(who)), 0), a.max_prefix);
+        break;
+      }
     }
-  }
-  const int n = n_own + n_pre, slots = a.ns_own + a.ns_pre;
-  const int slot = lane < n_own ? lane : lane < n ? a.ns_own + lane - n_own : 0;
-  const float* mine = a.rec + ((((size_t)b * a.hkv + kvh) * slots + slot) * a.G + (h - kvh * a.G)) * kRec<D>;
-  float A[D / 64];
-  merge_records<D>(mine, n, lane, A);
-#pragma unroll
-  for (int x = 0; x < D / 64; ++x) {
-    const size_t at = ((size_t)b * a.hq + h) * D + lane + 64 * x;
-    if (a.out) a.out[at] = f32_to_bf16(A[x]);
-    if (a.out_f32) a.out_f32[at] = A[x];
-  }
+    return r < a.ns_own ? r * a.chunk_own < len : (r - a.ns_own) * a.chunk_pre < pl;
+  });
+  if (lane < D / 4) put_channels(a.out, a.out_f32, (size_t)i * D + 4 * lane, A);
 }
 
 struct PrefixPlan {
@@ -467,6 +468,8 @@ int q4nx_gqa_prefix_decode(const uint16_t* q, const uint16_t* k_prefix, const ui
   Q4NX_REQUIRE(Q4NX_ALIGNED(q, 16) && Q4NX_ALIGNED(k_cache, 16) && Q4NX_ALIGNED(v_cache, 16) &&
                    Q4NX_ALIGNED(k_prefix, 16) && Q4NX_ALIGNED(v_prefix, 16),
                Q4NX_ERR_ARG, "%s: q and the caches must be 16-byte aligned", what);
+  Q4NX_REQUIRE(Q4NX_ALIGNED(out, 8) && Q4NX_ALIGNED(out_f32, 16), Q4NX_ERR_ARG,
+               "%s: out must be 8-byte, out_f32 16-byte aligned", what);
   Q4NX_REQUIRE(!own || (kv_h_stride >= (int64_t)max_len * head_dim && kv_h_stride % 8 == 0 &&
                         kv_b_stride >= (int64_t)n_kv_heads * kv_h_stride && kv_b_stride % 8 == 0),
                Q4NX_ERR_SHAPE, "%s: cache strides do not hold [Hkv][max_len][head_dim]", what);

@@ -51,55 +51,67 @@ constexpr int kWeightSpan = 1024;   // positions of a workgroup of the second la
 
 template <int D>
 __global__ __launch_bounds__(256) void weight_sum_kernel(WeightArgs a, int spans) {
+  constexpr int GH = 8, P = kWeightSpan / 256;   // heads in flight, positions a thread
   __shared__ float s_m[16], s_l[16];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int bk = blockIdx.x / (spans + 1), span = blockIdx.x % (spans + 1);
   const int b = bk / a.hkv, kvh = bk - b * a.hkv;
   const int len = min(max(a.lens[b], 0), a.max_len);
-  const int n = (len + a.chunk - 1) / a.chunk;   // parts that were written
   const float* rec = a.rec + (size_t)bk * a.ns * (size_t)(a.G * kRec<D>);
   if (span == spans) {
     for (int h = wave; h < a.G; h += 4) {
-      float A[D / 64];
-      merge_records<D>(rec + ((size_t)min(lane, a.ns - 1) * a.G + h) * kRec<D>, n, lane, A);
-#pragma unroll
-      for (int x = 0; x < D / 64; ++x) {
-        const size_t at = ((size_t)b * a.hq + kvh * a.G + h) * D + lane + 64 * x;
-        if (a.out) a.out[at] = f32_to_bf16(A[x]);
-        if (a.out_f32) a.out_f32[at] = A[x];
-      }
+      const float4 A = merge_records<D>(rec + (size_t)h * kRec<D>, (size_t)a.G * kRec<D>, a.ns, lane,
+                                        [&](int r) { return r * a.chunk < len; });
+      if (lane < D / 4) put_channels(a.out, a.out_f32, ((size_t)b * a.hq + kvh * a.G + h) * D + 4 * lane, A);
     }
     return;
   }
-  const int p0 = span * kWeightSpan;
-  if (p0 >= len) return;
+  const int p0 = span * kWeightSpan + tid;
+  // scores and old weights are on their way before the length is known (within the buffers; those behind
+  // it are left out)
+  const float* scores = a.scores + (size_t)bk * a.G * a.score_stride;
+  float* to = a.weights + (size_t)b * a.w_b_stride + (size_t)kvh * a.w_h_stride;
+  float s[GH][P], w[P], old[P];
+  auto load = [&](int h0) {
+#pragma unroll
+    for (int g = 0; g < GH; ++g)
+#pragma unroll
+      for (int i = 0; i < P; ++i)
+        s[g][i] = h0 + g < a.G ? scores[(h0 + g) * a.score_stride + min(p0 + 256 * i, a.max_len - 1)] : 0.f;
+  };
+  load(0);
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    w[i] = 0.f;
+    old[i] = a.start ? 0.f : to[min(p0 + 256 * i, a.max_len - 1)];
+  }
   for (int h = wave; h < a.G; h += 4) {
-    const float* mine = rec + ((size_t)min(lane, a.ns - 1) * a.G + h) * kRec<D>;
-    const float2 ml = lane < n ? *(const float2*)(mine + D) : make_float2(-INFINITY, 0.f);
-    const float M = wave_max(ml.x);
-    const float L = wave_sum(ml.x == -INFINITY ? ml.y : exp2_hw(ml.x - M) * ml.y);
+    const float2 head = *(const float2*)(rec + ((size_t)min(lane, a.ns - 1) * a.G + h) * kRec<D> + D);
+    const bool ok = lane < a.ns && lane * a.chunk < len;
+    const float m = ok ? head.x : -INFINITY, l = ok ? head.y : 0.f;
+    const float M = wave_max(m);
+    const float L = wave_sum(m == -INFINITY ? l : exp2_hw(m - M) * l);
     if (lane == 0) {
       s_m[h] = M == -INFINITY ? 0.f : M;
       s_l[h] = L == 0.f ? 0.f : 1.f / L;
     }
   }
   __syncthreads();
-  const float* scores = a.scores + (size_t)bk * a.G * a.score_stride;
-  float w[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int h = 0; h < a.G; ++h) {
-    const float m = s_m[h], li = s_l[h];
+  for (int h0 = 0; h0 < a.G; h0 += GH) {
+    if (h0 > 0) load(h0);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int p = p0 + tid + 256 * i;
-      if (p < len) w[i] = fmaf(exp2_hw(scores[h * a.score_stride + p] - m), li, w[i]);
+    for (int g = 0; g < GH; ++g) {
+      if (h0 + g >= a.G) break;
+      const float m = s_m[h0 + g], li = s_l[h0 + g];
+#pragma unroll
+      for (int i = 0; i < P; ++i) w[i] = fmaf(exp2_hw(s[g][i] - m), li, w[i]);
     }
   }
-  float* to = a.weights + (size_t)b * a.w_b_stride + (size_t)kvh * a.w_h_stride;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int p = p0 + tid + 256 * i;
-    if (p < len) to[p] = a.start || p == len - 1 ? w[i] : to[p] + w[i];
+  for (int i = 0; i < P; ++i) {
+    const int p = p0 + 256 * i;
+    if (p < len) to[p] = p == len - 1 ? w[i] : old[i] + w[i];
   }
 }
 
@@ -165,6 +177,8 @@ int q4nx_gqa_decode_weights(const uint16_t* q, const uint16_t* k_cache, const ui
                "%s: q, caches, lens, weights and an output are required", what);
   Q4NX_REQUIRE(Q4NX_ALIGNED(q, 16) && Q4NX_ALIGNED(k_cache, 16) && Q4NX_ALIGNED(v_cache, 16), Q4NX_ERR_ARG,
                "%s: q and caches must be 16-byte aligned", what);
+  Q4NX_REQUIRE(Q4NX_ALIGNED(out, 8) && Q4NX_ALIGNED(out_f32, 16), Q4NX_ERR_ARG,
+               "%s: out must be 8-byte, out_f32 16-byte aligned", what);
   Q4NX_REQUIRE(kv_h_stride >= (int64_t)max_len * head_dim && kv_h_stride % 8 == 0 &&
                    kv_b_stride >= (int64_t)n_kv_heads * kv_h_stride && kv_b_stride % 8 == 0,
                Q4NX_ERR_SHAPE, "%s: cache strides do not hold [Hkv][max_len][head_dim]", what);

@@ -48,8 +48,21 @@ __device__ __forceinline__ uint32_t weight_key(float x) {
 constexpr int kPickThreads = 1024;
 constexpr int kPickWaves = kPickThreads / 64;
 constexpr int kPickBins = 2048;    // 11 bits a pass: 32 bits in three
-constexpr int kPickLoads = 8;      // in flight per thread
 
+// Sum over the lanes up to and with this one.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);   // row_shr:1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);   // row_bcast:15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);   // row_bcast:31 into rows 2 and 3
+  return v;
+}
+
+// A wave takes KPT * 64 positions in a row (of every KPT * 1024). HELD: that is all of them, and their keys
+// stay in registers; otherwise each pass reads the weights again.
+template <int KPT, bool HELD>
 __global__ __launch_bounds__(kPickThreads) void evict_pick_kernel(EvictArgs a) {
   __shared__ int s_hist[kPickBins];
   __shared__ int s_sum[kPickWaves], s_gt[kPickWaves], s_eq[kPickWaves];
@@ -70,6 +83,30 @@ __global__ __launch_bounds__(kPickThreads) void evict_pick_kernel(EvictArgs a) {
   if (want == 0) return;
   const float* w = a.weights + (size_t)b * a.w_b_stride + (size_t)h * a.w_h_stride;
 
+  uint32_t key[KPT];
+  auto load = [&](int p0) {   // key 0 (below that of every weight) past the end
+    float x[KPT];
+#pragma unroll
+    for (int i = 0; i < KPT; ++i) {
+      const int p = p0 + 64 * i + lane;
+      x[i] = p < old ? w[p] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < KPT; ++i) key[i] = p0 + 64 * i + lane < old ? weight_key(x[i]) : 0u;
+  };
+  const int first = wave * KPT * 64;
+  auto each = [&](auto f) {
+    if constexpr (HELD) {
+      f(first);
+    } else {
+      for (int p0 = first; p0 < old; p0 += KPT * kPickThreads) {
+        load(p0);
+        f(p0);
+      }
+    }
+  };
+  if constexpr (HELD) load(first);
+
   // ---- the key of the want-th greatest, 11, 11 and 10 bits at a time; `left`: how many of the keys that
   // share the bits found so far are wanted
   uint32_t found = 0;
@@ -77,93 +114,71 @@ __global__ __launch_bounds__(kPickThreads) void evict_pick_kernel(EvictArgs a) {
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
     const uint32_t mask = pass < 2 ? 2047u : 1023u;
-    const int above = pass == 0 ? 32 : pass == 1 ? 21 : 10;   // bits from here on are known
+    const uint32_t known = pass == 0 ? 0u : pass == 1 ? ~0u << 21 : ~0u << 10;
     for (int i = tid; i < kPickBins; i += kPickThreads) s_hist[i] = 0;
     __syncthreads();
-    for (int p0 = 0; p0 < old; p0 += kPickThreads * kPickLoads) {
-      float x[kPickLoads];
+    each([&](int) {
 #pragma unroll
-      for (int i = 0; i < kPickLoads; ++i) {
-        const int p = p0 + tid + i * kPickThreads;
-        x[i] = p < old ? w[p] : 0.f;
-      }
-#pragma unroll
-      for (int i = 0; i < kPickLoads; ++i) {
-        const int p = p0 + tid + i * kPickThreads;
-        const uint32_t key = weight_key(x[i]);
-        if (p < old && (above == 32 || (key >> above) == (found >> above)))
-          atomicAdd(&s_hist[(key >> shift) & mask], 1);
-      }
-    }
+      for (int i = 0; i < KPT; ++i)
+        if (key[i] != 0 && (key[i] & known) == found) atomicAdd(&s_hist[(key[i] >> shift) & mask], 1);
+    });
     __syncthreads();
-    // the bin where the sum from the greatest on reaches `left`: thread t holds bins 2 t', 2 t' + 1 of the
-    // reversed order
+    // the bin where the sum from the greatest on reaches `left`: two bins a thread, the greatest first
     const int hi = kPickBins - 1 - 2 * tid;
     const int c0 = s_hist[hi], c1 = s_hist[hi - 1];
-    int upto = c0 + c1;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const int x = __shfl_up(upto, d);
-      if (lane >= d) upto += x;
-    }
+    const int upto = wave_scan(c0 + c1);
     if (lane == 63) s_sum[wave] = upto;
     __syncthreads();
     int before = 0;
-    for (int i = 0; i < wave; ++i) before += s_sum[i];
+#pragma unroll
+    for (int i = 0; i < kPickWaves; ++i) before += i < wave ? s_sum[i] : 0;
     const int from = before + upto - c0 - c1;   // keys above this thread's bins
     if (from < left && left <= from + c0 + c1) {
-      const bool first = left <= from + c0;
-      s_key = found | (uint32_t)(first ? hi : hi - 1) << shift;
-      s_left = left - (first ? from : from + c0);
+      const bool one = left <= from + c0;
+      s_key = found | (uint32_t)(one ? hi : hi - 1) << shift;
+      s_left = left - (one ? from : from + c0);
     }
     __syncthreads();
     found = s_key;
     left = s_left;
-    __syncthreads();
   }
 
-  // ---- positions in order: a wave counts its share, then writes it
-  const int share = ((old + kPickWaves - 1) / kPickWaves + 63) / 64 * 64;
-  const int lo = min(old, wave * share), up = min(old, lo + share);
-  int gt = 0, eq = 0;
-  for (int p0 = lo; p0 < up; p0 += 64 * kPickLoads) {
-    float x[kPickLoads];
-#pragma unroll
-    for (int i = 0; i < kPickLoads; ++i) x[i] = p0 + lane + 64 * i < up ? w[p0 + lane + 64 * i] : 0.f;
-#pragma unroll
-    for (int i = 0; i < kPickLoads; ++i) {
-      const bool in = p0 + lane + 64 * i < up;
-      const uint32_t key = weight_key(x[i]);
-      gt += __popcll(__ballot(in && key > found));
-      eq += __popcll(__ballot(in && key == found));
-    }
-  }
-  if (lane == 0) {
-    s_gt[wave] = gt;
-    s_eq[wave] = eq;
-  }
-  __syncthreads();
-  int at = 0, ties = 0;   // written before this wave's share, and equal keys before it
-  for (int i = 0; i < wave; ++i) {
-    at += s_gt[i] + min(s_eq[i], max(left - ties, 0));
-    ties += s_eq[i];
-  }
+  // ---- positions in order: the waves count theirs, then write them
+  int done = 0, ties = 0;   // written, and equal keys seen, before the block of positions at hand
   const uint64_t below = (1ull << lane) - 1;
-  for (int p0 = lo; p0 < up; p0 += 64 * kPickLoads) {
-    float x[kPickLoads];
+  for (int p0 = 0; p0 < old; p0 += KPT * kPickThreads) {
+    if constexpr (!HELD) load(p0 + first);
+    int gt = 0, eq = 0;
 #pragma unroll
-    for (int i = 0; i < kPickLoads; ++i) x[i] = p0 + lane + 64 * i < up ? w[p0 + lane + 64 * i] : 0.f;
+    for (int i = 0; i < KPT; ++i) {
+      gt += __popcll(__ballot(key[i] > found));
+      eq += __popcll(__ballot(key[i] == found));
+    }
+    __syncthreads();
+    if (lane == 0) {
+      s_gt[wave] = gt;
+      s_eq[wave] = eq;
+    }
+    __syncthreads();
+    int at = done, seen = ties;
 #pragma unroll
-    for (int i = 0; i < kPickLoads; ++i) {
-      const int p = p0 + lane + 64 * i;
-      const bool in = p < up;
-      const uint32_t key = weight_key(x[i]);
-      const uint64_t same = __ballot(in && key == found);
-      const bool take = in && (key > found || (key == found && ties + __popcll(same & below) < left));
+    for (int i = 0; i < kPickWaves; ++i) {
+      const int g = s_gt[i], e = s_eq[i], t = min(e, max(left - ties, 0));
+      done += g + t;
+      ties += e;
+      if (i < wave) {
+        at = done;
+        seen = ties;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < KPT; ++i) {
+      const uint64_t same = __ballot(key[i] == found);
+      const bool take = key[i] > found || (key[i] == found && seen + __popcll(same & below) < left);
       const uint64_t who = __ballot(take);
-      if (take) kept[at + __popcll(who & below)] = p;
+      if (take) kept[at + __popcll(who & below)] = p0 + first + 64 * i + lane;
       at += __popcll(who);
-      ties += __popcll(same);
+      seen += __popcll(same);
     }
   }
 }
@@ -349,7 +364,11 @@ int q4nx_kv_evict(const uint16_t* k_cache, const uint16_t* v_cache, int64_t kv_b
   if (a.blocks > 4096) a.blocks = 4096;
   Q4NX_REQUIRE(2ll * bh * a.blocks < (1ll << 31), Q4NX_ERR_SHAPE, "%s: more than 2^31 workgroups", what);
   hipStream_t s = (hipStream_t)stream;
-  hipLaunchKernelGGL(evict_pick_kernel, dim3((unsigned)bh), dim3(kPickThreads), 0, s, a);
+  const dim3 heads((unsigned)bh), threads(kPickThreads);
+  if (max_len <= 4 * kPickThreads) hipLaunchKernelGGL((evict_pick_kernel<4, true>), heads, threads, 0, s, a);
+  else if (max_len <= 16 * kPickThreads) hipLaunchKernelGGL((evict_pick_kernel<16, true>), heads, threads, 0, s, a);
+  else if (max_len <= 48 * kPickThreads) hipLaunchKernelGGL((evict_pick_kernel<48, true>), heads, threads, 0, s, a);
+  else hipLaunchKernelGGL((evict_pick_kernel<16, false>), heads, threads, 0, s, a);
   const dim3 grid((unsigned)(2 * bh * a.blocks));
   if (head_dim == 64) hipLaunchKernelGGL(evict_move_kernel<64>, grid, dim3(kMoveThreads), 0, s, a);
   else hipLaunchKernelGGL(evict_move_kernel<128>, grid, dim3(kMoveThreads), 0, s, a);

@@ -27,9 +27,9 @@ struct LogitArgs {
   const int32_t* mask_rows;
   int32_t* tokens;
   unsigned long long* keys;
-  unsigned* slots;          // 4 words a row: arrivals, -, the greatest key
+  unsigned* slots;          // a row's arrivals, an unused word, its greatest key
   int64_t stride, out_stride, count_stride, mask_stride;
-  int vocab, batch, n_mask, n_bias, parts;
+  int vocab, batch, n_mask, n_bias, parts, slot_words;
 };
 
 constexpr int kLogitThreads = 256;
@@ -164,7 +164,7 @@ __global__ __launch_bounds__(kLogitThreads) void adjust_logits_kernel(LogitArgs 
 #pragma unroll
   for (int w = 1; w < kLogitThreads / 64; ++w) best = s_key[w] > best ? s_key[w] : best;
   if (a.parts > 1) {
-    unsigned* const slot = a.slots + 4 * (size_t)b;
+    unsigned* const slot = a.slots + (size_t)b * a.slot_words;
     unsigned long long* const top = (unsigned long long*)(slot + 2);
     atomicMax(top, best);
     wait_vm();
@@ -287,16 +287,27 @@ int q4nx_adjust_logits(const void* logits, int bf16, int64_t stride, void* out, 
   a.batch = batch;
   a.n_mask = n_mask;
   a.n_bias = n_biases;
-  const bool few = (long long)batch * vocab < (1 << 22);
-  const int span = logit_span(bf16, few ? 1 : 4);
+  // rows' words on lines of their own as far as the counters go: with all of 8 rows' on one line, 122
+  // workgroups a row took 19 us, most of them for the atomics
+  a.slot_words = Q4NX_WS_COUNTER_BYTES / 4 / batch / 4 * 4;
+  if (a.slot_words > 64) a.slot_words = 64;
+  // 16-byte loads a thread: more of them, and fewer workgroups that meet at a row's word, as soon as about
+  // 512 workgroups remain
+  int u = 4;
+  while (u > 1 && (long long)batch * ((vocab + logit_span(bf16, u) - 1) / logit_span(bf16, u)) < 512) u /= 2;
+  const int span = logit_span(bf16, u);
   a.parts = (vocab + span - 1) / span;
   Q4NX_REQUIRE((long long)a.parts * batch < (1ll << 31), Q4NX_ERR_SHAPE, "%s: more than 2^31 workgroups", what);
   hipStream_t s = (hipStream_t)stream;
-  const dim3 grid((unsigned)(a.parts * batch));
-  if (bf16 && few) hipLaunchKernelGGL((adjust_logits_kernel<uint16_t, 1>), grid, dim3(kLogitThreads), 0, s, a);
-  else if (bf16) hipLaunchKernelGGL((adjust_logits_kernel<uint16_t, 4>), grid, dim3(kLogitThreads), 0, s, a);
-  else if (few) hipLaunchKernelGGL((adjust_logits_kernel<float, 1>), grid, dim3(kLogitThreads), 0, s, a);
-  else hipLaunchKernelGGL((adjust_logits_kernel<float, 4>), grid, dim3(kLogitThreads), 0, s, a);
+  const dim3 grid((unsigned)(a.parts * batch)), threads(kLogitThreads);
+  switch (u + (bf16 ? 8 : 0)) {
+    case 1: hipLaunchKernelGGL((adjust_logits_kernel<float, 1>), grid, threads, 0, s, a); break;
+    case 2: hipLaunchKernelGGL((adjust_logits_kernel<float, 2>), grid, threads, 0, s, a); break;
+    case 4: hipLaunchKernelGGL((adjust_logits_kernel<float, 4>), grid, threads, 0, s, a); break;
+    case 9: hipLaunchKernelGGL((adjust_logits_kernel<uint16_t, 1>), grid, threads, 0, s, a); break;
+    case 10: hipLaunchKernelGGL((adjust_logits_kernel<uint16_t, 2>), grid, threads, 0, s, a); break;
+    default: hipLaunchKernelGGL((adjust_logits_kernel<uint16_t, 4>), grid, threads, 0, s, a); break;
+  }
   return check_launch(what);
 }
 
