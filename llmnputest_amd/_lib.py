@@ -171,4 +171,6 @@ def check(rc: int) -> None:
 
 
 def call(name: str, *args) -> None:
-    check(getattr(lib(), name)(*args))
+    rc = getattr(_lib if _lib is not None else lib(), name)(*args)
+    if rc:
+        check(rc)

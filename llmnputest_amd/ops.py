@@ -136,10 +136,11 @@ def default_workspace() -> Workspace:
     return _defaults.get(s.device_index, s.cuda_stream)
 
 
-def _scratch(ws: Workspace | None, nbytes: int) -> tuple[Workspace, int, int, int]:
-    """The workspace of a call that needs nbytes, its address and size, and the current stream.
-    The caller holds the workspace until its launches are queued."""
-    device, stream = _device_stream()
+def _scratch(ws: Workspace | None, nbytes: int, at: tuple | None = None) -> tuple[Workspace, int, int, int]:
+    """The workspace of a call that needs nbytes, its address and size, and the current stream (`at`:
+    the device and stream, where the caller has them). The caller holds the workspace until its
+    launches are queued."""
+    device, stream = at or _device_stream()
     if ws is None:
         ws = _defaults.get(device, stream)
         if nbytes > max(DEFAULT_WS_BYTES, ws.buf.numel()):
@@ -590,41 +591,59 @@ def gemv_attn_q4(tiles: torch.Tensor, n_tile_rows: int, records: torch.Tensor,
 
 # ---------------------------------------------------------------- shared prefixes
 
-def _here(t: torch.Tensor, name: str, dtype, shape=None) -> int:
-    """The address of a contiguous tensor of that type (and shape) on the current device."""
-    if t.get_device() != torch.cuda.current_device():
-        raise ValueError(f"{name} must be on the current device, got {t.device}")
-    if t.dtype != dtype:
-        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if not t.is_contiguous() or (shape is not None and t.shape != shape):
+def _here(t: torch.Tensor, name: str, dtype, dev: int, shape=None) -> int:
+    """The address of a contiguous tensor of that type (and shape) on device `dev`, the current one."""
+    if t.get_device() != dev or t.dtype != dtype or not t.is_contiguous() \
+            or (shape is not None and t.shape != shape):
+        _refuse(t, name, dtype, dev)
         raise ValueError(f"{name} must be contiguous" + ("" if shape is None else f", {list(shape)}"))
     return t.data_ptr()
 
 
-def _rows_of(k: torch.Tensor, v: torch.Tensor, name: str, d: int) -> tuple[int, int]:
-    """The sequence and head strides of a pair of caches bf16 [B, Hkv, L, D], rows contiguous (a stride
-    that says nothing, of a dimension with one entry, is what a packed cache has)."""
-    out = []
-    for t, n in ((k, f"k_{name}"), (v, f"v_{name}")):
-        if t.get_device() != torch.cuda.current_device():
-            raise ValueError(f"{n} must be on the current device, got {t.device}")
-        if t.dtype != torch.bfloat16:
-            raise TypeError(f"{n} must be {torch.bfloat16}, got {t.dtype}")
-        shape, st = t.shape, t.stride()
-        if len(shape) != 4 or shape[3] != d or shape[1] == 0 or st[3] != 1 or (shape[2] > 1 and st[2] != d):
-            raise ValueError(f"{n} must be [B, Hkv, L, {d}] with contiguous rows")
-        h = st[1] if shape[1] > 1 else shape[2] * d
-        out.append((st[0] if shape[0] > 1 else shape[1] * h, h))
-    if k.shape != v.shape or out[0] != out[1]:
+def _refuse(t: torch.Tensor, name: str, dtype, dev: int) -> None:
+    if t.get_device() != dev:
+        raise ValueError(f"{name} must be on the current device, cuda:{dev}, got {t.device}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+
+
+def _rows_of(k: torch.Tensor, v: torch.Tensor, name: str, d: int, dev: int) -> tuple:
+    """The shape and the sequence and head strides of a pair of caches bf16 [B, Hkv, L, D], rows
+    contiguous (a stride that says nothing, of a dimension with one entry, is what a packed cache has)."""
+    if k.get_device() != dev or v.get_device() != dev or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
+        _refuse(k, f"k_{name}", torch.bfloat16, dev)
+        _refuse(v, f"v_{name}", torch.bfloat16, dev)
+    shape, st = k.shape, k.stride()
+    if len(shape) != 4 or shape[3] != d or shape[1] == 0 or st[3] != 1 or (shape[2] > 1 and st[2] != d):
+        raise ValueError(f"k_{name} must be [B, Hkv, L, {d}] with contiguous rows")
+    b, hkv, n, _ = shape
+    sv = v.stride()
+    if v.shape != shape or (sv != st and any(x > 1 and s != t for x, s, t in zip(shape, st, sv))):
         raise ValueError(f"k_{name} and v_{name} must have one shape and one layout")
-    return out[0]
+    h = st[1] if hkv > 1 else n * d
+    return b, hkv, n, (st[0] if b > 1 else hkv * h), h
 
 
 def _upto(n: int, most: int | None, name: str) -> int:
     """The positions a call may read of n."""
-    if most is not None and most < 0:
+    if most is None:
+        return n
+    if most < 0:
         raise ValueError(f"{name} must not be negative")
-    return n if most is None else min(n, most)
+    return min(n, most)
+
+
+_needs: dict = {}   # workspace bytes by the sizes that set them
+
+
+def _need(fn: str, *sizes) -> int:
+    key = (fn, *sizes)
+    n = _needs.get(key)
+    if n is None:
+        if len(_needs) > 4096:   # lengths that change from call to call
+            _needs.clear()
+        n = _needs[key] = int(getattr(_lib.lib(), fn)(*sizes))
+    return n
 
 
 def gqa_prefix_decode(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor,
@@ -640,45 +659,42 @@ def gqa_prefix_decode(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.T
     [B] (without the prefix; 0: none). D 64 or 128, Hq/Hkv at most 16, scale (default D ** -0.5) not
     negative. max_prefix, max_len: at least the longest lengths (fewer read fewer positions; default the
     caches'). Returns bf16 [B, Hq, D] (and the fp32 copy when want_f32)."""
-    b, hq, d = q.shape
-    qp = _here(q, "q", torch.bfloat16)
-    ps, ph = _rows_of(k_prefix, v_prefix, "prefix", d)
-    bs, hs = _rows_of(k_cache, v_cache, "cache", d)
-    p, hkv = k_prefix.shape[:2]
-    if k_cache.shape[0] != b or k_cache.shape[1] != hkv:
+    at = dev, _ = _device_stream()
+    b, hq, d = shape = q.shape
+    qp = _here(q, "q", torch.bfloat16, dev)
+    p, hkv, n_pre, ps, ph = _rows_of(k_prefix, v_prefix, "prefix", d, dev)
+    bk, hk, n, bs, hs = _rows_of(k_cache, v_cache, "cache", d, dev)
+    if bk != b or hk != hkv:
         raise ValueError(f"k_cache must be [{b}, {hkv}, L, {d}]")
     if cu is None and p > 1:
         raise ValueError(f"{p} prefixes need cu")
-    lp = _here(lens, "lens", torch.int32, (b,))
-    pp = _here(prefix_lens, "prefix_lens", torch.int32, (p,))
-    up = None if cu is None else _here(cu, "cu", torch.int32, (p + 1,))
+    lp = _here(lens, "lens", torch.int32, dev, (b,))
+    pp = _here(prefix_lens, "prefix_lens", torch.int32, dev, (p,))
+    up = None if cu is None else _here(cu, "cu", torch.int32, dev, (p + 1,))
     out = torch.empty_like(q) if out is None else out
-    op = _here(out, "out", torch.bfloat16, q.shape)
-    of = torch.empty(q.shape, dtype=torch.float32, device=q.device) if want_f32 else None
+    op = _here(out, "out", torch.bfloat16, dev, shape)
+    of = torch.empty(shape, dtype=torch.float32, device=q.device) if want_f32 else None
     if b == 0:
         return (out, of) if want_f32 else out
-    most_p = _upto(k_prefix.shape[2], max_prefix, "max_prefix")
-    most = _upto(k_cache.shape[2], max_len, "max_len")
-    need = _lib.lib().q4nx_gqa_prefix_decode_ws_bytes(b, hq, hkv, d, p, most_p, most)
-    ws, wp, wn, stream = _scratch(ws, need)
+    most_p, most = _upto(n_pre, max_prefix, "max_prefix"), _upto(n, max_len, "max_len")
+    need = _need("q4nx_gqa_prefix_decode_ws_bytes", b, hq, hkv, d, p, most_p, most)
+    ws, wp, wn, stream = _scratch(ws, need, at)
     _lib.call("q4nx_gqa_prefix_decode", qp, k_prefix.data_ptr(), v_prefix.data_ptr(), ps, ph, pp, up, p,
               most_p, k_cache.data_ptr(), v_cache.data_ptr(), bs, hs, lp, most, op, _ptr(of), b, hq, hkv, d,
-              d ** -0.5 if scale is None else float(scale), wp, wn, stream)
+              d ** -0.5 if scale is None else scale, wp, wn, stream)
     return (out, of) if want_f32 else out
 
 
 # ---------------------------------------------------------------- eviction by attention weight
 
-def _weight_rows(t: torch.Tensor, name: str, shape: tuple) -> tuple[int, int]:
+def _weight_rows(t: torch.Tensor, name: str, shape: tuple, dev: int) -> tuple[int, int]:
     """The sequence and head strides of weights fp32 [B, Hkv, L]."""
-    if t.get_device() != torch.cuda.current_device():
-        raise ValueError(f"{name} must be on the current device, got {t.device}")
-    if t.dtype != torch.float32:
-        raise TypeError(f"{name} must be {torch.float32}, got {t.dtype}")
-    if t.shape != shape or (shape[2] > 1 and t.stride(2) != 1):
+    _refuse(t, name, torch.float32, dev)
+    st = t.stride()
+    if t.shape != shape or (shape[2] > 1 and st[2] != 1):
         raise ValueError(f"{name} must be {list(shape)}, positions contiguous")
-    h = t.stride(1) if shape[1] > 1 else shape[2]
-    return (t.stride(0) if shape[0] > 1 else shape[1] * h), h
+    h = st[1] if shape[1] > 1 else shape[2]
+    return (st[0] if shape[0] > 1 else shape[1] * h), h
 
 
 def gqa_decode_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -690,26 +706,26 @@ def gqa_decode_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
     weights, fp32 [B, Hkv, L], what the group's query heads gave each position l < lens[b]: the sum over
     the heads of its softmax weight. The newest position's (lens[b] - 1) is set, not added to, and with
     `start` every one's; entries behind it are left. What `kv_evict` goes by."""
-    b, hq, d = q.shape
-    qp = _here(q, "q", torch.bfloat16)
-    bs, hs = _rows_of(k_cache, v_cache, "cache", d)
-    hkv, n = k_cache.shape[1:3]
-    if k_cache.shape[0] != b:
+    at = dev, _ = _device_stream()
+    b, hq, d = shape = q.shape
+    qp = _here(q, "q", torch.bfloat16, dev)
+    bk, hkv, n, bs, hs = _rows_of(k_cache, v_cache, "cache", d, dev)
+    if bk != b:
         raise ValueError(f"k_cache must be [{b}, Hkv, L, {d}]")
-    wb, wh = _weight_rows(weights, "weights", (b, hkv, n))
-    lp = _here(lens, "lens", torch.int32, (b,))
+    wb, wh = _weight_rows(weights, "weights", (b, hkv, n), dev)
+    lp = _here(lens, "lens", torch.int32, dev, (b,))
     out = torch.empty_like(q) if out is None else out
-    op = _here(out, "out", torch.bfloat16, q.shape)
-    of = torch.empty(q.shape, dtype=torch.float32, device=q.device) if want_f32 else None
+    op = _here(out, "out", torch.bfloat16, dev, shape)
+    of = torch.empty(shape, dtype=torch.float32, device=q.device) if want_f32 else None
     most = _upto(n, max_len, "max_len")
     if b == 0 or most == 0:
         out.zero_()
         return (out, of.zero_()) if want_f32 else out
-    need = _lib.lib().q4nx_gqa_decode_weights_ws_bytes(b, hq, hkv, d, most)
-    ws, wp, wn, stream = _scratch(ws, need)
+    need = _need("q4nx_gqa_decode_weights_ws_bytes", b, hq, hkv, d, most)
+    ws, wp, wn, stream = _scratch(ws, need, at)
     _lib.call("q4nx_gqa_decode_weights", qp, k_cache.data_ptr(), v_cache.data_ptr(), bs, hs, lp, most,
-              weights.data_ptr(), wb, wh, int(start), op, _ptr(of), b, hq, hkv, d,
-              d ** -0.5 if scale is None else float(scale), wp, wn, stream)
+              weights.data_ptr(), wb, wh, bool(start), op, _ptr(of), b, hq, hkv, d,
+              d ** -0.5 if scale is None else scale, wp, wn, stream)
     return (out, of) if want_f32 else out
 
 
@@ -723,25 +739,25 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tensor
     room for them, which overlap nothing that is read, or, without it, stay in place. Weights behind them
     become 0 (in place: up to the old length). rope: a `rope_table` of at least the longest length; K is
     then turned to its new places, so that what follows goes on from position lens[b]."""
-    b, hkv, n, d = k_cache.shape
-    bs, hs = _rows_of(k_cache, v_cache, "cache", d)
-    wb, wh = _weight_rows(weights, "weights", (b, hkv, n))
-    lp = _here(lens, "lens", torch.int32, (b,))
+    at = dev, _ = _device_stream()
+    d = k_cache.shape[-1]
+    b, hkv, n, bs, hs = _rows_of(k_cache, v_cache, "cache", d, dev)
+    wb, wh = _weight_rows(weights, "weights", (b, hkv, n), dev)
+    lp = _here(lens, "lens", torch.int32, dev, (b,))
     k2, v2, w2, l2 = (k_cache, v_cache, weights, lens) if into is None else into
     if into is None:
         obs, ohs, owb, owh, room = bs, hs, wb, wh, n
     else:
-        if k2.dim() != 4 or k2.shape[:2] != (b, hkv):
+        ob, oh, room, obs, ohs = _rows_of(k2, v2, "into", d, dev)
+        if ob != b or oh != hkv:
             raise ValueError(f"k of into must be [{b}, {hkv}, room, {d}]")
-        room = k2.shape[2]
-        obs, ohs = _rows_of(k2, v2, "into", d)
-        owb, owh = _weight_rows(w2, "weights of into", (b, hkv, room))
-        _here(l2, "lens of into", torch.int32, (b,))
+        owb, owh = _weight_rows(w2, "weights of into", (b, hkv, room), dev)
+        _here(l2, "lens of into", torch.int32, dev, (b,))
         for x, y, name in ((k2, k_cache, "k"), (v2, v_cache, "v"), (w2, weights, "weights")):
             if x.numel() and x.data_ptr() == y.data_ptr():
                 raise ValueError(f"{name} of into is the input: leave into out to cut down in place")
     if rope is not None:
-        _here(rope, "rope", torch.float32, (rope.shape[0], 2, d // 2))
+        _here(rope, "rope", torch.float32, dev, (rope.shape[0], 2, d // 2))
     if budget < 1 or not 0 <= recent <= budget:
         raise ValueError(f"budget must be positive and recent in 0..budget, got {budget} and {recent}")
     kept = torch.empty((b, hkv, budget), dtype=torch.int32, device=k_cache.device)
@@ -751,8 +767,8 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tensor
         if into is not None:
             w2.zero_()
         return kept.fill_(-1)
-    need = _lib.lib().q4nx_kv_evict_ws_bytes(b, hkv)
-    ws, wp, wn, stream = _scratch(ws, need)
+    need = _need("q4nx_kv_evict_ws_bytes", b, hkv)
+    ws, wp, wn, stream = _scratch(ws, need, at)
     _lib.call("q4nx_kv_evict", k_cache.data_ptr(), v_cache.data_ptr(), bs, hs, weights.data_ptr(), wb, wh, lp,
               most, budget, recent, _ptr(rope), 0 if rope is None else rope.shape[0], k2.data_ptr(),
               v2.data_ptr(), obs, ohs, w2.data_ptr(), owb, owh, room, l2.data_ptr(), kept.data_ptr(), b, hkv,
@@ -762,15 +778,14 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tensor
 
 # ---------------------------------------------------------------- rules for the next token
 
-def _vocab_rows(t: torch.Tensor, name: str, dtype, shape: tuple | None = None) -> int:
+def _vocab_rows(t: torch.Tensor, name: str, dtype, dev: int, shape: tuple | None = None) -> int:
     """The row stride of a tensor [B, V], tokens contiguous."""
-    if t.get_device() != torch.cuda.current_device():
-        raise ValueError(f"{name} must be on the current device, got {t.device}")
-    if t.dtype != dtype:
-        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (shape is not None and t.shape != shape):
+    if t.get_device() != dev or t.dtype != dtype:
+        _refuse(t, name, dtype, dev)
+    got, st = t.shape, t.stride()
+    if len(got) != 2 or (got[1] > 1 and st[1] != 1) or (shape is not None and got != shape):
         raise ValueError(f"{name} must be {'[rows, V]' if shape is None else list(shape)}, rows contiguous")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    return st[0] if got[0] > 1 else got[1]
 
 
 def count_tokens(counts: torch.Tensor, tokens: torch.Tensor, cu: torch.Tensor | None = None,
@@ -779,16 +794,17 @@ def count_tokens(counts: torch.Tensor, tokens: torch.Tensor, cu: torch.Tensor | 
     with `prompt` the sign bit of those that the prompt has. One token per sequence, or tokens
     cu[b] .. cu[b+1] - 1 (int32 [B + 1]); those outside the vocabulary are skipped. start: counts of these
     alone, whatever was there."""
-    stride = _vocab_rows(counts, "counts", torch.int32)
+    dev, stream = _device_stream()
+    stride = _vocab_rows(counts, "counts", torch.int32, dev)
     b, v = counts.shape
-    tp = _here(tokens, "tokens", torch.int32)
+    tp = _here(tokens, "tokens", torch.int32, dev)
     n = tokens.numel()
     if tokens.dim() != 1 or (cu is None and n != b):
         raise ValueError(f"tokens must be a list, of {b} without cu")
-    up = None if cu is None else _here(cu, "cu", torch.int32, (b + 1,))
+    up = None if cu is None else _here(cu, "cu", torch.int32, dev, (b + 1,))
     if b and v:
-        _lib.call("q4nx_count_tokens", counts.data_ptr(), stride, v, b, tp or None, n, up, int(prompt),
-                  int(start), _stream())
+        _lib.call("q4nx_count_tokens", counts.data_ptr(), stride, v, b, tp or None, n, up, bool(prompt),
+                  bool(start), stream)
 
 
 def adjust_logits(logits: torch.Tensor, counts: torch.Tensor | None = None,
@@ -810,44 +826,46 @@ def adjust_logits(logits: torch.Tensor, counts: torch.Tensor | None = None,
     (n_slots 1)."""
     if logits.dtype not in (torch.float32, torch.bfloat16):
         raise TypeError(f"logits must be float32 or bfloat16, got {logits.dtype}")
-    stride = _vocab_rows(logits, "logits", logits.dtype)
-    b, v = logits.shape
-    out = torch.empty((b, v), dtype=logits.dtype, device=logits.device) if out is None else out
-    out_stride = _vocab_rows(out, "out", logits.dtype, logits.shape)
-    cs = 0 if counts is None else _vocab_rows(counts, "counts", torch.int32, logits.shape)
+    at = dev, _ = _device_stream()
+    dtype = logits.dtype
+    stride = _vocab_rows(logits, "logits", dtype, dev)
+    b, v = shape = logits.shape
+    if v == 0:
+        raise ValueError("logits must have at least one token")
+    out = torch.empty(shape, dtype=dtype, device=logits.device) if out is None else out
+    out_stride = _vocab_rows(out, "out", dtype, dev, shape)
+    cp, cs = (None, 0) if counts is None else (counts.data_ptr(), _vocab_rows(counts, "counts", torch.int32, dev, shape))
     pen = []
     for t, name in ((repetition, "repetition"), (presence, "presence"), (frequency, "frequency")):
         if t is not None and counts is None:
             raise ValueError(f"{name} needs counts")
-        pen.append(None if t is None else _here(t, name, torch.float32, (b,)))
+        pen.append(None if t is None else _here(t, name, torch.float32, dev, (b,)))
     ids = values = bias_cu = None
-    n_bias = 0
-    if bias is not None:
-        n_bias = bias[0].numel()
-        if n_bias:
-            ids = _here(bias[0], "bias ids", torch.int32, (n_bias,))
-            values = _here(bias[1], "bias values", torch.float32, (n_bias,))
-            bias_cu = _here(bias[2], "bias cu", torch.int32, (b + 1,))
+    n_bias = 0 if bias is None else bias[0].numel()
+    if n_bias:
+        ids = _here(bias[0], "bias ids", torch.int32, dev, (n_bias,))
+        values = _here(bias[1], "bias values", torch.float32, dev, (n_bias,))
+        bias_cu = _here(bias[2], "bias cu", torch.int32, dev, (b + 1,))
+    mp = rp = None
     ms = n_mask = 0
     if mask is not None:
-        n_mask = mask.shape[0]
-        ms = _vocab_rows(mask, "mask", torch.int32, (n_mask, (v + 31) // 32))
+        n_mask, mp = mask.shape[0], mask.data_ptr()
+        ms = _vocab_rows(mask, "mask", torch.int32, dev, (n_mask, (v + 31) // 32))
         if n_mask == 0 or (mask_rows is None and n_mask != b):
             raise ValueError(f"mask must have a row for each of {b} sequences, or mask_rows")
+        if mask_rows is not None:
+            rp = _here(mask_rows, "mask_rows", torch.int32, dev, (b,))
     elif mask_rows is not None:
         raise ValueError("mask_rows needs mask")
-    rp = None if mask_rows is None else _here(mask_rows, "mask_rows", torch.int32, (b,))
     if tokens is None:
         tokens = torch.empty(b, dtype=torch.int32, device=logits.device)
-    tp = _here(tokens, "tokens", torch.int32, (b,))
-    kp = None if keys is None else _here(keys, "keys", torch.int64, (b,))
-    if v == 0:
-        raise ValueError("logits must have at least one token")
+    tp = _here(tokens, "tokens", torch.int32, dev, (b,))
+    kp = None if keys is None else _here(keys, "keys", torch.int64, dev, (b,))
     if b:
-        ws, wp, wn, stream = _scratch(ws, WS_COUNTER_BYTES)
-        _lib.call("q4nx_adjust_logits", logits.data_ptr(), int(logits.dtype == torch.bfloat16), stride,
-                  out.data_ptr(), out_stride, v, b, _ptr(counts), cs, *pen, ids, values, n_bias, bias_cu,
-                  _ptr(mask), ms, n_mask, rp, tp, kp, wp, wn, stream)
+        ws, wp, wn, stream = _scratch(ws, WS_COUNTER_BYTES, at)
+        _lib.call("q4nx_adjust_logits", logits.data_ptr(), dtype == torch.bfloat16, stride, out.data_ptr(),
+                  out_stride, v, b, cp, cs, *pen, ids, values, n_bias, bias_cu, mp, ms, n_mask, rp, tp, kp,
+                  wp, wn, stream)
     return out, tokens
 
 
