@@ -307,8 +307,8 @@ int q4nx_gqa_decode_records(const uint16_t *q, const uint16_t *k_cache,
  * Own rows as in q4nx_qkv_rope, l < lens[b] (at most max_len; 0: none, the caches may be NULL). Query
  * head h reads kv head h / (Hq/Hkv), Hq/Hkv <= 16; head_dim 64 or 128; scale >= 0. A sequence that sees
  * nothing gives zeros. q, out: [batch][Hq][head_dim]; caches bf16, 16-byte aligned, strides in elements,
- * multiples of 8. Softmax weights of a prefix with more than 16 rows (members * Hq/Hkv) enter the product
- * rounded to bf16 (their sum is that of the rounded ones), all others with 17 bits. |v| times the
+ * multiples of 8. Softmax weights enter the products as two
+ * bf16 terms (2^-15 of a weight may be lost). |v| times the
  * positions seen has to stay below 2^112. No reference counterpart: its attention reads one sequence's cache
  * (designs/granite_gemv/granite_attention.h:221-237).
  * ws: q4nx_gqa_prefix_decode_ws_bytes(...) bytes (0: a shape that is not taken). */

@@ -8,6 +8,9 @@ decoded on the device and the reference's report line is printed.
 
     python -m llmnputest_amd.chat [--layers 40] [--ctx 2048] [--new 128] [--batch 1]
     python -m llmnputest_amd.chat --q4nx model.q4nx ...     # a real granite q4nx file
+    python -m llmnputest_amd.chat --batch 8 --prefix 1024   # the first 1024 positions held once
+    python -m llmnputest_amd.chat --repetition 1.2 --frequency 0.3    # penalties for what was said
+    python -m llmnputest_amd.chat --keep 512 --recent 64    # the context cut down after half of the tokens
     python -m llmnputest_amd.chat --hf-tiny                 # chat.py's own flow (below)
 
 `--hf-tiny` runs chat.py's flow itself (chat.py:36-42, 80-94): a transformers causal LM whose
@@ -83,6 +86,7 @@ def hf_tiny(new_tokens: int, seed: int) -> int:
 
 def main(argv: list[str]) -> int:
     from .granite import GraniteConfig, GraniteDecoder, GraniteWeights
+    from .rules import TokenRules
 
     ap = argparse.ArgumentParser(prog="llmnputest_amd.chat")
     ap.add_argument("--layers", type=int, default=40)
@@ -91,6 +95,13 @@ def main(argv: list[str]) -> int:
     ap.add_argument("--batch", type=int, default=1)
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--q4nx", default=None, help="load weights from a granite .q4nx file")
+    ap.add_argument("--prefix", type=int, default=0, help="positions of the context that all sequences share")
+    ap.add_argument("--repetition", type=float, default=1.0)
+    ap.add_argument("--presence", type=float, default=0.0)
+    ap.add_argument("--frequency", type=float, default=0.0)
+    ap.add_argument("--keep", type=int, default=0,
+                    help="positions kept, those that attention gave most, after half of the new tokens")
+    ap.add_argument("--recent", type=int, default=32, help="the last ones that --keep always keeps")
     ap.add_argument("--hf-tiny", action="store_true",
                     help="transformers generate with the GPU lm_head (chat.py's flow)")
     ap.add_argument("prompt_ids", nargs="*", type=int)
@@ -102,19 +113,33 @@ def main(argv: list[str]) -> int:
     cfg = GraniteConfig(n_layers=a.layers)
     w = (GraniteWeights.from_q4nx(a.q4nx, cfg) if a.q4nx
          else GraniteWeights.synthetic(cfg, seed=a.seed))
-    dec = GraniteDecoder(w, max_batch=a.batch, max_len=a.ctx + a.new)
-    dec.seed_cache(a.ctx, seed=a.seed + 1)
     rng = np.random.default_rng(a.seed)
     prompt = a.prompt_ids or rng.integers(0, cfg.vocab, a.batch).tolist()
     first = (prompt + prompt * a.batch)[:a.batch]
+    rules = None
+    if a.repetition != 1.0 or a.presence or a.frequency:
+        rules = TokenRules(a.batch, cfg.vocab, a.repetition, a.presence, a.frequency)
+        rules.begin([[x] for x in first])
+    dec = GraniteDecoder(w, max_batch=a.batch, max_len=a.ctx + a.new, prefix_len=a.prefix,
+                         track_weights=a.keep > 0, rules=rules)
+    dec.seed_cache(a.ctx, seed=a.seed + 1)
     print(f"gpu      granite-3B shape, {cfg.n_layers} layers, lm_head q8 {cfg.vocab} x "
           f"{cfg.hidden}, batch {a.batch}, context {a.ctx}")
-    dec.generate(first, [a.ctx] * a.batch, 2)          # capture the step graph
+    dec.generate(first, [a.ctx] * a.batch, min(2, a.new))   # capture the step graph
+    if rules is not None:
+        rules.begin([[x] for x in first])
     print(f"ready    {time.time() - t0:.1f}s\n")
 
     torch.cuda.synchronize()
     t = time.time()
-    toks, _ = dec.generate(first, [a.ctx] * a.batch, a.new)
+    at, half = [a.ctx] * a.batch, a.new // 2 if a.keep else 0
+    toks = np.empty((a.batch, 0), np.int32)
+    if half:
+        toks, _ = dec.generate(first, at, half)
+        at = dec.evict([x + half for x in at], a.keep, min(a.recent, a.keep))
+        first = toks[:, -1].tolist()
+    if a.new > half:
+        toks = np.concatenate((toks, dec.generate(first, at, a.new - half)[0]), 1)
     dt = time.time() - t
     for b in range(a.batch):
         print(" ".join(str(int(x)) for x in toks[b]))

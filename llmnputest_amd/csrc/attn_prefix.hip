@@ -75,9 +75,9 @@ __device__ __forceinline__ Group find_tile(const PrefixArgs& a, int RT, int lane
 
 // 64 NR query rows (16 NR a wave) over cache rows [0, end): tiles of 64 positions of K and V go through
 // LDS, loaded ahead, read by all four waves; a tile's scores are computed beside the previous tile's
-// exponentials. V^T comes out of the transposing LDS read. P is
-// rounded to bf16 once (2^-9 of a weight; the same rounded weights are summed to l, by a product with
-// ones, so they still add up to one). The running maximum moves only when a row's tile exceeds it by 2^8
+// exponentials. V^T comes out of the transposing LDS read. P enters
+// as two bf16 terms, its upper half and what that leaves (2^-15 of it is lost); l is their sum, by a product
+// with ones. The running maximum moves only when a row's tile exceeds it by 2^8
 // (weights stay below 2^8 then), which leaves out nearly every rescaling of the accumulators.
 // 16-byte pieces of a row are swizzled by the row, so that 16 rows' pieces lie in different banks.
 template <int D>
@@ -224,7 +224,7 @@ __device__ __forceinline__ void part_wide(const PrefixArgs& a, const uint16_t* k
       }
 #pragma unroll
       for (int x2 = 0; x2 < 2; ++x2) {
-        u32x4_t pp[NR];
+        u32x4_t pp[NR], pr[NR];
 #pragma unroll
         for (int x1 = 0; x1 < 2; ++x1) {
           const int x = 2 * x2 + x1;
@@ -235,18 +235,28 @@ __device__ __forceinline__ void part_wide(const PrefixArgs& a, const uint16_t* k
           for (int n = 0; n < NR; ++n) {
             const float mb = m[n] == -INFINITY ? 0.f : m[n];
 #pragma unroll
-            for (int y = 0; y < 2; ++y)
-              pp[n][2 * x1 + y] = pack_bf16x2_op(exp2_hw(fmaf(s[n][x][2 * y], a.scale_l2, -mb)),
-                                                 exp2_hw(fmaf(s[n][x][2 * y + 1], a.scale_l2, -mb)));
+            for (int y = 0; y < 2; ++y) {
+              const float a0 = exp2_hw(fmaf(s[n][x][2 * y], a.scale_l2, -mb));
+              const float a1 = exp2_hw(fmaf(s[n][x][2 * y + 1], a.scale_l2, -mb));
+              const uint32_t hi = perm(__float_as_uint(a1), __float_as_uint(a0), 0x07060302u);
+              pp[n][2 * x1 + y] = hi;
+              pr[n][2 * x1 + y] = pack_bf16x2_op(a0 - bf16lo(hi), a1 - bf16hi(hi));
+            }
           }
           if constexpr (more) score(x);
         }
 #pragma unroll
-        for (int n = 0; n < NR; ++n) l[n] = mfma_bf16(ones, pp[n], l[n]);
+        for (int n = 0; n < NR; ++n) {
+          l[n] = mfma_bf16(ones, pp[n], l[n]);
+          l[n] = mfma_bf16(ones, pr[n], l[n]);
+        }
 #pragma unroll
         for (int u = 0; u < D / 16; ++u)
 #pragma unroll
-          for (int n = 0; n < NR; ++n) o[n][u] = mfma_bf16(vf[u], pp[n], o[n][u]);
+          for (int n = 0; n < NR; ++n) {
+            o[n][u] = mfma_bf16(vf[u], pp[n], o[n][u]);
+            o[n][u] = mfma_bf16(vf[u], pr[n], o[n][u]);
+          }
       }
       if constexpr (more) scored(t + 1, last);
     }

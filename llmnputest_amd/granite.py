@@ -39,6 +39,7 @@ import torch
 from . import ops
 from .kv4 import Kv4Cache
 from .ops import Policy
+from .rules import TokenRules
 from .q4nx import Q4_TILE_BYTES, Q8_TILE_BYTES, Q4NX, TILE_BYTES, check_stored_shape, projection_shape
 
 # greedy steps per replay of the multi-step decode graph
@@ -210,12 +211,19 @@ class GraniteDecoder:
     of every sequence): 2048 bytes a layer and position of 8 kv heads become 672. The fused q/k/v
     launch then writes a bf16 row into one cache that all layers share, from where it is quantised;
     two launches more a layer than kv="bf16". sparse_pages > 0: attention reads that many pages of
-    each (sequence, kv head), chosen by every token's query, the first and the newest among them."""
+    each (sequence, kv head), chosen by every token's query, the first and the newest among them.
+
+    prefix_len > 0 (kv="bf16"): the first prefix_len positions are one prefix that all sequences share,
+    held once and read once a step for all of them (`load_prefix`); sequences write from there on.
+    track_weights (kv="bf16"): attention sums what each position was given (`weights`, fp32 [B, Hkv, L] a
+    layer), by which `evict` cuts the caches down. rules: a TokenRules for max_batch sequences, applied to
+    every step's logits; generate() chooses by them and counts what it says."""
 
     def __init__(self, weights: GraniteWeights, max_batch: int = 1, max_len: int = 4096,
                  device="cuda", fused_attn_o: bool = True, attn_splits: int = 0,
                  policy: Policy | None = None, kv: str = "bf16", page_len: int = 64,
-                 sparse_pages: int = 0):
+                 sparse_pages: int = 0, prefix_len: int = 0, track_weights: bool = False,
+                 rules: TokenRules | None = None):
         c = weights.cfg
         self.cfg, self.w = c, weights
         # the launch policy of every kernel this decoder issues (its own copy: other
@@ -227,13 +235,24 @@ class GraniteDecoder:
         self.attn_splits = attn_splits   # 0: the library's choice for the path taken
         self.dev = torch.device(device)
         self.max_batch = max_batch
-        self.max_len = (max_len + 63) // 64 * 64
+        if prefix_len < 0 or (prefix_len and prefix_len >= max_len):
+            raise ValueError(f"prefix_len must be in [0, {max_len})")
+        if kv != "bf16" and (prefix_len or track_weights):
+            raise ValueError('prefix_len and track_weights need kv="bf16"')
+        if prefix_len and track_weights:
+            raise ValueError("track_weights needs every position in the sequences' own caches: no prefix_len")
+        if rules is not None and (rules.n_seqs != max_batch or rules.vocab != c.vocab):
+            raise ValueError(f"rules must be for {max_batch} sequences of {c.vocab} tokens")
+        # positions from prefix_len on are the sequences' own: pos, lens and the caches' rows count from there
+        self.prefix_len = prefix_len
+        self.own_len = (max_len - prefix_len + 63) // 64 * 64
+        self.max_len = prefix_len + self.own_len
         b, dev = max_batch, self.dev
         if kv not in ("bf16", "q4"):
             raise ValueError(f'kv must be "bf16" or "q4", not {kv!r}')
         if sparse_pages and (kv != "q4" or sparse_pages < 2):
             raise ValueError('sparse_pages needs kv="q4" and at least 2 pages')
-        kv_shape = (b, c.n_kv, self.max_len, c.head_dim)
+        kv_shape = (b, c.n_kv, self.own_len, c.head_dim)
         # kv="q4": the rows of one layer at a time, on their way into its pages
         own = c.n_layers if kv == "bf16" else 1
         self.k_cache, self.v_cache = (
@@ -249,6 +268,16 @@ class GraniteDecoder:
         # per sequence, where pages begin that no other one can have (on a page's border)
         self._own_from = [0] * b
         self.rope = ops.rope_table(self.max_len, c.head_dim, c.theta, device=dev)
+        self._rope_own = self.rope[prefix_len:]
+        if prefix_len:
+            self.k_prefix, self.v_prefix = (
+                [torch.zeros((1, c.n_kv, prefix_len, c.head_dim), dtype=torch.bfloat16, device=dev)
+                 for _ in range(c.n_layers)] for _ in range(2))
+            self.prefix_lens = torch.full((1,), prefix_len, dtype=torch.int32, device=dev)
+        self.weights = ([torch.zeros((b, c.n_kv, self.own_len), dtype=torch.float32, device=dev)
+                         for _ in range(c.n_layers)] if track_weights else None)
+        self.rules = rules
+        self.rule_keys = torch.zeros(b, dtype=torch.int64, device=dev)   # the rules' choice, one key a row
         self.h = torch.zeros((b, c.hidden), dtype=torch.float32, device=dev)
         # sums of h^2 per 16 entries, written by each producer of h for the next RMSNorm
         self.ssq = torch.zeros((b, c.hidden // 16), dtype=torch.float32, device=dev)
@@ -301,7 +330,7 @@ class GraniteDecoder:
         pol = self.policy
         n_split = self.attn_splits or ops.gqa_decode_records_splits(b, c.n_q, c.n_kv,
                                                                     self.max_len, policy=pol)
-        fuse_o = self.fuses_attn_o(b, n_split)
+        fuse_o = self.fuses_attn_o(b, n_split) and not self.prefix_len and self.weights is None
         if embed:
             self._embed(b)
         tr = None
@@ -316,7 +345,7 @@ class GraniteDecoder:
             pos_host = self.pos[:b].cpu().numpy()
         for li, L in enumerate(w.layers):
             kc, vc = self.k_cache[li], self.v_cache[li]
-            ops.qkv_rope(L["q"], L["k"], L["v"], c.n_q, c.n_kv, kt_h, h, self.pos[:b], self.rope,
+            ops.qkv_rope(L["q"], L["k"], L["v"], c.n_q, c.n_kv, kt_h, h, self.pos[:b], self._rope_own,
                          kc, vc, q_out=q, norm_w=L["norm_in"], eps=c.eps, ws=self.ws,
                          ssq_in=ssq, policy=pol, raw_out=tr and tr["raw"], xn_out=tr and tr["xn"])
             if self.kv is not None:
@@ -335,9 +364,16 @@ class GraniteDecoder:
                                    max_len=self.max_len, n_split=n_split, out=tr["attn"],
                                    ws=self.ws, policy=pol)
             else:
-                ops.gqa_decode(q.view(b, c.n_q, c.head_dim), kc, vc, self.lens[:b], c.scale,
-                               max_len=self.max_len, n_split=self.attn_splits, out=attn,
-                               ws=self.ws, policy=pol)
+                q3 = q.view(b, c.n_q, c.head_dim)
+                if self.prefix_len:
+                    ops.gqa_prefix_decode(q3, self.k_prefix[li], self.v_prefix[li], self.prefix_lens, kc[:b],
+                                          vc[:b], self.lens[:b], scale=c.scale, out=attn, ws=self.ws)
+                elif self.weights is not None:
+                    ops.gqa_decode_weights(q3, kc[:b], vc[:b], self.lens[:b], self.weights[li][:b],
+                                           scale=c.scale, out=attn, ws=self.ws)
+                else:
+                    ops.gqa_decode(q3, kc, vc, self.lens[:b], c.scale, max_len=self.max_len,
+                                   n_split=self.attn_splits, out=attn, ws=self.ws, policy=pol)
                 ops.gemv_ex(L["o"], "q4", attn.view(b, c.q_dim), c.hidden // 32, kt_q,
                             residual=h, out=h, ssq_out=ssq, ws=self.ws, policy=pol)
                 if tr is not None:
@@ -349,10 +385,12 @@ class GraniteDecoder:
                 trace.append(self._trace_layer(tr, li, b, pos_host, mlp))
             ops.gemv_ex(L["down"], "q4", mlp, c.hidden // 32, kt_i, residual=h, out=h,
                         ssq_out=ssq, ws=self.ws, policy=pol)
-        # final RMSNorm fused into the lm_head prologue, greedy argmax into its epilogue
+        # final RMSNorm fused into the lm_head prologue, greedy argmax into its epilogue (or the rules')
         ops.gemv_ex(w.lm_head, w.lm_head_kind, h, c.vocab // 32, kt_h, norm_w=w.norm_final,
-                    eps=c.eps, out=self.logits[:b], argmax_keys=self.keys[:b], ssq_in=ssq,
-                    ws=self.ws, policy=pol)
+                    eps=c.eps, out=self.logits[:b], ssq_in=ssq, ws=self.ws, policy=pol,
+                    argmax_keys=self.keys[:b] if self.rules is None else None)
+        if self.rules is not None:
+            self.rules.apply(self.logits[:b], out=self.logits[:b], keys=self.rule_keys[:b], ws=self.ws)
 
     def _attn_q4(self, li: int, b: int, q: torch.Tensor, attn: torch.Tensor) -> None:
         """The layer's new rows into its pages, then attention over them."""
@@ -412,6 +450,36 @@ class GraniteDecoder:
         if int(self.kv.status):
             raise RuntimeError("the pool has no pages left for the sequences")
 
+    def load_prefix(self, source: "GraniteDecoder", seq: int = 0) -> None:
+        """The shared prefix: the first prefix_len positions of a sequence of another decoder of the same
+        model (kv="bf16", no prefix of its own), which has run the prompt."""
+        if not self.prefix_len:
+            raise ValueError("load_prefix needs prefix_len")
+        if source.kv is not None or source.prefix_len or source.cfg != self.cfg \
+                or source.own_len < self.prefix_len or not 0 <= seq < source.max_batch:
+            raise ValueError(f"the source must hold {self.prefix_len} positions of this model, in bf16")
+        for mine, its in ((self.k_prefix, source.k_cache), (self.v_prefix, source.v_cache)):
+            for to, rows in zip(mine, its):
+                to[0].copy_(rows[seq, :, :self.prefix_len])
+
+    def evict(self, lens, budget: int, recent: int) -> list[int]:
+        """Cuts the first lens[b] positions of every sequence down to `budget`, in every layer and kv head
+        to the `recent` last and those that attention gave most (track_weights). Keys are turned to their
+        new places: sequence b goes on at position min(lens[b], budget), which is what is returned."""
+        if self.weights is None:
+            raise ValueError("evict needs track_weights")
+        lens = [int(x) for x in lens]
+        if len(lens) != self.max_batch or not all(0 <= x <= self.own_len for x in lens):
+            raise ValueError(f"{self.max_batch} lengths in [0, {self.own_len}]")
+        if budget < 1 or not 0 <= recent <= budget:
+            raise ValueError("budget must be positive and recent in 0..budget")
+        held = torch.tensor(lens, dtype=torch.int32, device=self.dev)
+        left = torch.empty_like(held)
+        for k, v, w in zip(self.k_cache, self.v_cache, self.weights):
+            left.copy_(held)
+            ops.kv_evict(k, v, w, left, budget, recent, rope=self.rope, ws=self.ws)
+        return [min(x, budget) for x in lens]
+
     def _check_own(self, positions, n: int = 1) -> None:
         """Refuses n positions from positions[i] of sequence i on where a page of them is another's too.
         Only sequences that were forked, and only positions before that, look at the device."""
@@ -462,9 +530,10 @@ class GraniteDecoder:
         b = tokens.numel()
         if b > self.max_batch or positions.numel() != b:
             raise ValueError("batch exceeds max_batch or positions do not match tokens")
-        if int(positions.max()) >= self.max_len or int(positions.min()) < 0:
-            raise ValueError(f"positions must be in [0, {self.max_len})")
+        if int(positions.max()) >= self.max_len or int(positions.min()) < self.prefix_len:
+            raise ValueError(f"positions must be in [{self.prefix_len}, {self.max_len})")
         self._check_own(positions.tolist())
+        positions = positions - self.prefix_len
         self.tokens[:b].copy_(tokens)
         self.pos[:b].copy_(positions)
         self.lens[:b].copy_(positions + 1)
@@ -476,11 +545,14 @@ class GraniteDecoder:
         """The next token from the argmax keys, positions and history advanced, and the
         token's embedding row into h for the next step: one launch."""
         table, kind = self._embed_table()
-        ops.decode_advance_embed(self.keys[:b], self.cfg.vocab // 16, self.tokens[:b],
+        keys, slots = (self.keys[:b], self.cfg.vocab // 16) if self.rules is None else (self.rule_keys[:b], 1)
+        ops.decode_advance_embed(keys, slots, self.tokens[:b],
                                  self.pos[:b], self.lens[:b], self.step_ctr,
                                  self.history[:, :b] if b == self.max_batch else None,
                                  table, kind, self.cfg.vocab, self.cfg.hidden, self.h[:b],
                                  self.ssq[:b])
+        if self.rules is not None:
+            self.rules.count(self.tokens[:b])
 
     def capture(self, b: int) -> None:
         """Capture one greedy step for b sequences: the step's kernels from h, then one launch
@@ -491,7 +563,12 @@ class GraniteDecoder:
         first."""
         if self.kv is not None and any(self._own_from):
             self._check_own(self.pos[:b].tolist())   # the warm step below writes there
-        snap = (self.tokens.clone(), self.pos.clone(), self.lens.clone(), self.step_ctr.clone())
+        state = [self.tokens, self.pos, self.lens, self.step_ctr]
+        if self.rules is not None:
+            state.append(self.rules.counts)
+        if self.weights is not None:
+            state += self.weights
+        snap = [x.clone() for x in state]
         self._launch_step(b)                       # warm: sizes every workspace
         self._advance(b)
         torch.cuda.synchronize()
@@ -505,7 +582,7 @@ class GraniteDecoder:
             graphs.append(g)
         self.graph, self.graph_steps = graphs
         self.graph_batch = b
-        for t, s0 in zip((self.tokens, self.pos, self.lens, self.step_ctr), snap):
+        for t, s0 in zip(state, snap):
             t.copy_(s0)
 
     def generate(self, first_tokens, start_pos, n_new: int, record_logits: bool = False):
@@ -516,11 +593,12 @@ class GraniteDecoder:
         b = first.numel()
         if int(start.max()) + n_new > self.max_len:
             raise ValueError("max_len too small for this many new tokens")
-        if int(start.min()) < 0 or start.numel() != b:
-            raise ValueError("start positions must be >= 0, one per sequence")
+        if int(start.min()) < self.prefix_len or start.numel() != b:
+            raise ValueError(f"start positions must be >= {self.prefix_len}, one per sequence")
         if b != self.max_batch:
             raise ValueError("generate() runs all max_batch sequences; size the decoder to them")
         self._check_own(start.tolist(), n_new)
+        start = start - self.prefix_len
         # tokens, positions, lengths and the step counter in one copy: four of them, three waited
         # for, added 15 to 30 us to a one-token call
         state = torch.zeros(self._state.shape, dtype=torch.int32, device=first.device)
@@ -549,11 +627,20 @@ class GraniteDecoder:
 
     def seed_cache(self, ctx: int, seed: int = 0) -> None:
         """Fill positions [0, ctx) of every layer's K/V cache with bf16 N(0,1) (a synthetic
-        context; no prefill runs through the model)."""
+        context; no prefill runs through the model), the shared prefix among them."""
         if self.kv is not None:   # every sequence writes its own rows
             self.reset(range(self.max_batch))
         g = torch.Generator(device=self.dev)
         g.manual_seed(seed)
+        if self.prefix_len:
+            if ctx < self.prefix_len:
+                raise ValueError(f"the context must reach behind the prefix of {self.prefix_len} positions")
+            for t in (*self.k_prefix, *self.v_prefix):
+                t.copy_(torch.randn(t.shape, device=self.dev, generator=g))
+            ctx -= self.prefix_len
+        if self.weights is not None:
+            for t in self.weights:
+                t.zero_()
         rows = torch.arange(self.max_batch + 1, dtype=torch.int32, device=self.dev) * ctx
         for li, (kc, vc) in enumerate(zip(self.k_cache, self.v_cache)):
             for t in (kc, vc):
