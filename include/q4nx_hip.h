@@ -345,7 +345,7 @@ int q4nx_gqa_decode_weights(const uint16_t *q, const uint16_t *k_cache, const ui
  * it now stands. In place: the outputs are the inputs (k_out == k_cache, ..), `room` says nothing, lens_out
  * may be lens. Otherwise they overlap nothing that is read and hold `room` >= min(budget, max_len)
  * positions a head. lens[b] > max_len counts as max_len. No reference counterpart. */
-size_t q4nx_kv_evict_ws_bytes(int batch, int n_kv_heads);
+size_t q4nx_kv_evict_ws_bytes(int batch, int n_kv_heads, int max_len);
 int q4nx_kv_evict(const uint16_t *k_cache, const uint16_t *v_cache, int64_t kv_b_stride,
                   int64_t kv_h_stride, const float *weights, int64_t w_b_stride, int64_t w_h_stride,
                   const int32_t *lens, int max_len, int budget, int recent, const float *rope_tab,

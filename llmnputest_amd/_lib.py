@@ -107,7 +107,7 @@ SIGNATURES: dict[str, tuple] = {
     "q4nx_gqa_decode_weights_ws_bytes": (c_sz, [c_i, c_i, c_i, c_i, c_i]),
     "q4nx_gqa_decode_weights": (c_i, [c_p, c_p, c_p, c_i64, c_i64, c_p, c_i, c_p, c_i64, c_i64, c_i, c_p, c_p,
                                       c_i, c_i, c_i, c_i, c_f, c_p, c_sz, c_p]),
-    "q4nx_kv_evict_ws_bytes": (c_sz, [c_i, c_i]),
+    "q4nx_kv_evict_ws_bytes": (c_sz, [c_i, c_i, c_i]),
     "q4nx_kv_evict": (c_i, [c_p, c_p, c_i64, c_i64, c_p, c_i64, c_i64, c_p, c_i, c_i, c_i, c_p, c_i, c_p, c_p,
                             c_i64, c_i64, c_p, c_i64, c_i64, c_i, c_p, c_p, c_i, c_i, c_i, c_p, c_sz, c_p]),
     "q4nx_count_tokens": (c_i, [c_p, c_i64, c_i, c_i, c_p, c_i, c_p, c_i, c_i, c_p]),

@@ -3,8 +3,11 @@
 //
 // Per (sequence, kv head) with n = lens[b] > budget positions: of the first n - recent those budget - recent
 // of the greatest weights (ties to the lowest position), then the `recent` last, in the order of their
-// positions. Two launches: which ones (a radix selection by one workgroup), then the rows. With n <= budget
-// all are kept.
+// positions. With n <= budget all are kept. First which ones, by a radix selection of the weights' keys, then
+// the rows. Up to 4096 positions the selection is one workgroup's for a (sequence, kv head). Beyond, that was
+// bound by its own instructions on a quarter of the chip (8 sequences of 32771: 44 us), so parts of 4096 share
+// it: histograms of the keys' upper 11 bits; where the wanted number is reached, and the keys of that bin,
+// among which the last part to arrive looks for the rest; then the positions, in order.
 //
 // Rows move towards the front. Into other memory they move all at once. In place, row i comes from a
 // position >= i, so a workgroup that takes rows in order, a block at a time, only overwrites rows that it
@@ -31,10 +34,16 @@ struct EvictArgs {
   float* weights_out;
   int32_t* lens_out;
   int32_t* kept;           // [batch][hkv][budget]
-  int32_t* n_old;          // [batch * hkv]: lengths, for the second launch
+  int32_t* n_old;          // [batch * hkv]: lengths, for the later launches
+  unsigned* counters;      // the next five: selection by parts, index bk * parts + part
+  uint16_t* hist;          // [..][kPickBins]
+  uint32_t* cand;          // [..][kPickPart]: keys in the bin where the wanted number is reached
+  int32_t* part_info;      // [..][4]: keys above the bin, keys in it; then its first place, equal keys before it
+  uint32_t* cut;           // [batch * hkv][2]: the last wanted key, and how many of its like
   int64_t b_stride, h_stride, w_b_stride, w_h_stride;
   int64_t ob_stride, oh_stride, ow_b_stride, ow_h_stride;
   int batch, hkv, max_len, budget, recent, room;
+  int parts;               // of 4096 positions
   int in_place, blocks;    // blocks: workgroups for a (sequence, kv head)'s rows
 };
 
@@ -48,6 +57,7 @@ __device__ __forceinline__ uint32_t weight_key(float x) {
 constexpr int kPickThreads = 1024;
 constexpr int kPickWaves = kPickThreads / 64;
 constexpr int kPickBins = 2048;    // 11 bits a pass: 32 bits in three
+constexpr int kPickCopies = 4;     // of the histogram, by lane: weights crowd in few bins
 
 // Sum over the lanes up to and with this one.
 __device__ __forceinline__ int wave_scan(int v) {
@@ -60,11 +70,11 @@ __device__ __forceinline__ int wave_scan(int v) {
   return v;
 }
 
-// A wave takes KPT * 64 positions in a row (of every KPT * 1024). HELD: that is all of them, and their keys
-// stay in registers; otherwise each pass reads the weights again.
+// The waves take equal shares of the positions in a row, at most KPT * 64 each. HELD: that is all of them,
+// and their keys stay in registers; otherwise each pass reads the weights again, KPT * 1024 at a time.
 template <int KPT, bool HELD>
 __global__ __launch_bounds__(kPickThreads) void evict_pick_kernel(EvictArgs a) {
-  __shared__ int s_hist[kPickBins];
+  __shared__ __attribute__((aligned(16))) int s_hist[kPickBins * kPickCopies];
   __shared__ int s_sum[kPickWaves], s_gt[kPickWaves], s_eq[kPickWaves];
   __shared__ uint32_t s_key;
   __shared__ int s_left;
@@ -84,24 +94,25 @@ __global__ __launch_bounds__(kPickThreads) void evict_pick_kernel(EvictArgs a) {
   const float* w = a.weights + (size_t)b * a.w_b_stride + (size_t)h * a.w_h_stride;
 
   uint32_t key[KPT];
+  const int share = HELD ? (old + kPickThreads - 1) / kPickThreads * 64 : KPT * 64;   // a wave's
+  const int first = wave * share;
   auto load = [&](int p0) {   // key 0 (below that of every weight) past the end
     float x[KPT];
 #pragma unroll
     for (int i = 0; i < KPT; ++i) {
       const int p = p0 + 64 * i + lane;
-      x[i] = p < old ? w[p] : 0.f;
+      x[i] = 64 * i < share && p < old ? w[p] : 0.f;
     }
 #pragma unroll
-    for (int i = 0; i < KPT; ++i) key[i] = p0 + 64 * i + lane < old ? weight_key(x[i]) : 0u;
+    for (int i = 0; i < KPT; ++i) key[i] = 64 * i < share && p0 + 64 * i + lane < old ? weight_key(x[i]) : 0u;
   };
-  const int first = wave * KPT * 64;
   auto each = [&](auto f) {
     if constexpr (HELD) {
-      f(first);
+      f();
     } else {
-      for (int p0 = first; p0 < old; p0 += KPT * kPickThreads) {
-        load(p0);
-        f(p0);
+      for (int p0 = 0; p0 < old; p0 += KPT * kPickThreads) {
+        load(p0 + first);
+        f();
       }
     }
   };
@@ -115,17 +126,18 @@ __global__ __launch_bounds__(kPickThreads) void evict_pick_kernel(EvictArgs a) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
     const uint32_t mask = pass < 2 ? 2047u : 1023u;
     const uint32_t known = pass == 0 ? 0u : pass == 1 ? ~0u << 21 : ~0u << 10;
-    for (int i = tid; i < kPickBins; i += kPickThreads) s_hist[i] = 0;
+    for (int i = tid; i < kPickBins * kPickCopies; i += kPickThreads) s_hist[i] = 0;
     __syncthreads();
-    each([&](int) {
+    each([&] {
 #pragma unroll
       for (int i = 0; i < KPT; ++i)
-        if (key[i] != 0 && (key[i] & known) == found) atomicAdd(&s_hist[(key[i] >> shift) & mask], 1);
+        if (64 * i < share && key[i] != 0 && (key[i] & known) == found) atomicAdd(&s_hist[((key[i] >> shift) & mask) * kPickCopies + lane % kPickCopies], 1);
     });
     __syncthreads();
     // the bin where the sum from the greatest on reaches `left`: two bins a thread, the greatest first
     const int hi = kPickBins - 1 - 2 * tid;
-    const int c0 = s_hist[hi], c1 = s_hist[hi - 1];
+    const int4 h0 = *(const int4*)(s_hist + 4 * hi), h1 = *(const int4*)(s_hist + 4 * hi - 4);
+    const int c0 = h0.x + h0.y + h0.z + h0.w, c1 = h1.x + h1.y + h1.z + h1.w;
     const int upto = wave_scan(c0 + c1);
     if (lane == 63) s_sum[wave] = upto;
     __syncthreads();
@@ -146,14 +158,15 @@ __global__ __launch_bounds__(kPickThreads) void evict_pick_kernel(EvictArgs a) {
   // ---- positions in order: the waves count theirs, then write them
   int done = 0, ties = 0;   // written, and equal keys seen, before the block of positions at hand
   const uint64_t below = (1ull << lane) - 1;
-  for (int p0 = 0; p0 < old; p0 += KPT * kPickThreads) {
+  for (int p0 = 0; p0 < old; p0 += kPickWaves * share) {
     if constexpr (!HELD) load(p0 + first);
     int gt = 0, eq = 0;
 #pragma unroll
-    for (int i = 0; i < KPT; ++i) {
-      gt += __popcll(__ballot(key[i] > found));
-      eq += __popcll(__ballot(key[i] == found));
-    }
+    for (int i = 0; i < KPT; ++i)
+      if (64 * i < share) {
+        gt += __popcll(__ballot(key[i] > found));
+        eq += __popcll(__ballot(key[i] == found));
+      }
     __syncthreads();
     if (lane == 0) {
       s_gt[wave] = gt;
@@ -173,6 +186,7 @@ __global__ __launch_bounds__(kPickThreads) void evict_pick_kernel(EvictArgs a) {
     }
 #pragma unroll
     for (int i = 0; i < KPT; ++i) {
+      if (64 * i >= share) break;
       const uint64_t same = __ballot(key[i] == found);
       const bool take = key[i] > found || (key[i] == found && seen + __popcll(same & below) < left);
       const uint64_t who = __ballot(take);
@@ -180,6 +194,250 @@ __global__ __launch_bounds__(kPickThreads) void evict_pick_kernel(EvictArgs a) {
       at += __popcll(who);
       seen += __popcll(same);
     }
+  }
+}
+
+// ---- by parts of 4096 positions, 256 threads each: a wave holds 1024 of them in a row
+constexpr int kPickPart = 4096;
+constexpr int kPartThreads = 256;
+constexpr int kPartKeys = kPickPart / kPartThreads;
+
+struct PartJob {
+  int bk, part, n, old, want, p0;   // p0: the wave's first position
+  const float* w;
+};
+__device__ __forceinline__ PartJob part_job(const EvictArgs& a) {
+  PartJob j;
+  j.bk = blockIdx.x / a.parts;
+  j.part = blockIdx.x % a.parts;
+  const int b = j.bk / a.hkv, h = j.bk - b * a.hkv;
+  j.n = min(max(a.lens[b], 0), a.max_len);
+  j.old = j.n - a.recent;
+  j.want = a.budget - a.recent;
+  j.p0 = j.part * kPickPart + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 64 * kPartKeys;
+  j.w = a.weights + (size_t)b * a.w_b_stride + (size_t)h * a.w_h_stride;
+  return j;
+}
+// Whether there is a choice to make, and this part has some of it.
+__device__ __forceinline__ bool part_chooses(const EvictArgs& a, const PartJob& j) {
+  return j.n > a.budget && j.want > 0 && j.part * kPickPart < j.old;
+}
+__device__ __forceinline__ void part_keys(const PartJob& j, int lane, uint32_t (&key)[kPartKeys]) {
+  float x[kPartKeys];
+#pragma unroll
+  for (int i = 0; i < kPartKeys; ++i) x[i] = j.w[min(j.p0 + 64 * i + lane, j.old - 1)];
+#pragma unroll
+  for (int i = 0; i < kPartKeys; ++i) key[i] = j.p0 + 64 * i + lane < j.old ? weight_key(x[i]) : 0u;
+}
+
+__global__ __launch_bounds__(kPartThreads) void evict_hist_kernel(EvictArgs a) {
+  __shared__ __attribute__((aligned(16))) int s_hist[kPickBins];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const PartJob j = part_job(a);
+  if (j.part == 0 && tid == 0) a.n_old[j.bk] = j.n;
+  if (!part_chooses(a, j)) return;
+  uint32_t key[kPartKeys];
+  part_keys(j, lane, key);
+  for (int i = tid; i < kPickBins; i += kPartThreads) s_hist[i] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kPartKeys; ++i)
+    if (key[i] != 0) atomicAdd(&s_hist[key[i] >> 21], 1);
+  __syncthreads();
+  uint32_t* const to = (uint32_t*)(a.hist + (size_t)blockIdx.x * kPickBins);
+  for (int i = tid; i < kPickBins / 2; i += kPartThreads)
+    to[i] = (uint32_t)s_hist[2 * i] | (uint32_t)s_hist[2 * i + 1] << 16;
+}
+
+// With eight bins' counts a thread (c[0] the lowest bin's; thread t has bins 8 (255 - t) ..): the bin where the
+// sum from the greatest on reaches `left`, and what is left of it there.
+__device__ __forceinline__ void find_bin(const int (&c)[8], int left, int* s_sum, int* s_found) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int total = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) total += c[i];
+  const int upto = wave_scan(total);
+  if (lane == 63) s_sum[wave] = upto;
+  __syncthreads();
+  int from = upto - total;
+#pragma unroll
+  for (int i = 0; i < kPartThreads / 64; ++i) from += i < wave ? s_sum[i] : 0;
+#pragma unroll
+  for (int i = 7; i >= 0; --i) {
+    if (from < left && left <= from + c[i]) {
+      s_found[0] = 8 * (kPartThreads - 1 - tid) + i;
+      s_found[1] = left - from;
+    }
+    from += c[i];
+  }
+  __syncthreads();
+}
+
+__global__ __launch_bounds__(kPartThreads) void evict_cut_kernel(EvictArgs a) {
+  __shared__ __attribute__((aligned(16))) int s_hist[kPickBins];
+  __shared__ int s_sum[kPartThreads / 64], s_found[2], s_gt, s_eq, s_last;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const PartJob j = part_job(a);
+  if (!part_chooses(a, j)) return;
+  const int parts = (j.old + kPickPart - 1) / kPickPart;   // that take part
+  const size_t row0 = (size_t)j.bk * a.parts;
+  uint32_t key[kPartKeys];
+  part_keys(j, lane, key);
+  if (tid == 0) s_gt = s_eq = 0;
+  int c[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll 4
+  for (int p = 0; p < parts; ++p) {
+    const uint4 h = *(const uint4*)(a.hist + (row0 + p) * kPickBins + 8 * (kPartThreads - 1 - tid));
+    const uint32_t x[4] = {h.x, h.y, h.z, h.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      c[2 * i] += (int)(x[i] & 0xffffu);
+      c[2 * i + 1] += (int)(x[i] >> 16);
+    }
+  }
+  find_bin(c, j.want, s_sum, s_found);
+  const uint32_t bin = (uint32_t)s_found[0];
+  int left = s_found[1];
+
+  // ---- this part's keys above the bin, and those in it (in any order), for whoever arrives last
+  uint32_t* const mine = a.cand + (row0 + j.part) * kPickPart;
+  int gt = 0;
+#pragma unroll
+  for (int i = 0; i < kPartKeys; ++i) {
+    gt += __popcll(__ballot(key[i] >> 21 > bin));
+    const bool in = key[i] != 0 && key[i] >> 21 == bin;
+    const uint64_t who = __ballot(in);
+    if (who == 0) continue;
+    int at = 0;
+    if (lane == 0) at = atomicAdd(&s_eq, __popcll(who));
+    at = __builtin_amdgcn_readfirstlane(at);
+    if (in)
+      __hip_atomic_store(mine + at + __popcll(who & ((1ull << lane) - 1)), key[i], __ATOMIC_RELAXED,
+                         __HIP_MEMORY_SCOPE_SYSTEM);
+  }
+  if (lane == 0) atomicAdd(&s_gt, gt);
+  __syncthreads();
+  int32_t* const info = a.part_info + row0 * 4;
+  if (tid == 0) {
+    __hip_atomic_store(info + 4 * j.part, s_gt, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+    __hip_atomic_store(info + 4 * j.part + 1, s_eq, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+  }
+  wait_vm();
+  __syncthreads();
+  if (tid == 0) s_last = ticket(a.counters + j.bk, parts) ? 1 : 0;
+  __syncthreads();
+  if (!s_last) return;
+
+  // ---- the last: the wanted key's lower 21 bits, from the keys of the bin
+  uint32_t found = bin << 21;
+  const uint32_t* const all = a.cand + row0 * kPickPart;
+  auto load = [&](const uint32_t* p) {
+    return __hip_atomic_load(const_cast<uint32_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+  };
+  auto load_i = [&](const int32_t* p) {
+    return __hip_atomic_load(const_cast<int32_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+  };
+  for (int pass = 0; pass < 2; ++pass) {
+    const int shift = pass == 0 ? 10 : 0;
+    const uint32_t mask = pass == 0 ? 2047u : 1023u, known = pass == 0 ? ~0u << 21 : ~0u << 10;
+    for (int i = tid; i < kPickBins; i += kPartThreads) s_hist[i] = 0;
+    __syncthreads();
+    for (int p = wave; p < parts; p += kPartThreads / 64) {
+      const int m = load_i(info + 4 * p + 1);
+#pragma unroll 4
+      for (int i = lane; i < m; i += 64) {
+        const uint32_t k = load(all + (size_t)p * kPickPart + i);
+        if ((k & known) == found) atomicAdd(&s_hist[k >> shift & mask], 1);
+      }
+    }
+    __syncthreads();
+    int d[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) d[i] = s_hist[8 * (kPartThreads - 1 - tid) + i];
+    find_bin(d, left, s_sum, s_found);
+    found |= (uint32_t)s_found[0] << shift;
+    left = s_found[1];
+    __syncthreads();
+  }
+  // ---- how many each part writes, and from where on
+  for (int p = wave; p < parts; p += kPartThreads / 64) {
+    const int m = load_i(info + 4 * p + 1);
+    int above = 0, same = 0;
+#pragma unroll 4
+    for (int i = lane; i < m; i += 64) {
+      const uint32_t k = load(all + (size_t)p * kPickPart + i);
+      above += k > found;
+      same += k == found;
+    }
+    above = wave_scan(above);
+    same = wave_scan(same);
+    if (lane == 63) {
+      info[4 * p + 2] = load_i(info + 4 * p) + above;
+      info[4 * p + 3] = same;
+    }
+  }
+  wait_vm();
+  __syncthreads();
+  if (tid == 0) {
+    int at = 0, ties = 0;
+    for (int p = 0; p < parts; ++p) {
+      const int g = info[4 * p + 2], e = info[4 * p + 3];
+      info[4 * p + 2] = at;
+      info[4 * p + 3] = ties;
+      at += g + min(e, max(left - ties, 0));
+      ties += e;
+    }
+    a.cut[2 * j.bk] = found;
+    a.cut[2 * j.bk + 1] = (uint32_t)left;
+  }
+}
+
+__global__ __launch_bounds__(kPartThreads) void evict_list_kernel(EvictArgs a) {
+  __shared__ int s_gt[kPartThreads / 64], s_eq[kPartThreads / 64];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const PartJob j = part_job(a);
+  int32_t* const kept = a.kept + (size_t)j.bk * a.budget;
+  const int stride = a.parts * kPartThreads;
+  if (j.n <= a.budget) {
+    for (int i = j.part * kPartThreads + tid; i < a.budget; i += stride) kept[i] = i < j.n ? i : -1;
+    return;
+  }
+  for (int i = j.part * kPartThreads + tid; i < a.recent; i += stride) kept[j.want + i] = j.old + i;
+  if (!part_chooses(a, j)) return;
+  const uint32_t found = a.cut[2 * j.bk];
+  const int left = (int)a.cut[2 * j.bk + 1];
+  const int32_t* const info = a.part_info + ((size_t)j.bk * a.parts + j.part) * 4;
+  int at = info[2], ties = info[3];
+  uint32_t key[kPartKeys];
+  part_keys(j, lane, key);
+  int gt = 0, eq = 0;
+#pragma unroll
+  for (int i = 0; i < kPartKeys; ++i) {
+    gt += __popcll(__ballot(key[i] > found));
+    eq += __popcll(__ballot(key[i] == found));
+  }
+  if (lane == 0) {
+    s_gt[wave] = gt;
+    s_eq[wave] = eq;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kPartThreads / 64; ++i)
+    if (i < wave) {
+      at += s_gt[i] + min(s_eq[i], max(left - ties, 0));
+      ties += s_eq[i];
+    }
+  const uint64_t below = (1ull << lane) - 1;
+#pragma unroll
+  for (int i = 0; i < kPartKeys; ++i) {
+    const uint64_t same = __ballot(key[i] == found);
+    const bool take = key[i] > found || (key[i] == found && ties + __popcll(same & below) < left);
+    const uint64_t who = __ballot(take);
+    if (take) kept[at + __popcll(who & below)] = j.p0 + 64 * i + lane;
+    at += __popcll(who);
+    ties += __popcll(same);
   }
 }
 
@@ -283,15 +541,25 @@ static bool evict_shape_ok(int batch, int hkv, int d, int max_len, int budget, i
          max_len < (1 << 24) && budget >= 1 && recent >= 0 && recent <= budget;
 }
 
+// Parts of a (sequence, kv head)'s selection; 0: one workgroup's, with few positions and where there are more
+// (sequence, kv head)s than counters.
+static int evict_parts(size_t bh, int max_len) {
+  return max_len <= kPickPart || bh > Q4NX_WS_COUNTER_BYTES / 4 ? 0 : (max_len + kPickPart - 1) / kPickPart;
+}
+// Lengths and cuts, before the parts' memory.
+static size_t evict_head_bytes(size_t bh) { return (bh * 12 + 255) / 256 * 256; }
+
 }  // namespace q4nx
 
 using namespace q4nx;
 
 extern "C" {
 
-size_t q4nx_kv_evict_ws_bytes(int batch, int n_kv_heads) {
-  if (batch < 1 || n_kv_heads < 1 || (long long)batch * n_kv_heads > (1 << 24)) return 0;
-  return (size_t)Q4NX_WS_COUNTER_BYTES + (size_t)batch * n_kv_heads * 4;
+size_t q4nx_kv_evict_ws_bytes(int batch, int n_kv_heads, int max_len) {
+  if (!evict_shape_ok(batch, n_kv_heads, 64, max_len, 1, 0)) return 0;
+  const size_t bh = (size_t)batch * n_kv_heads;
+  return (size_t)Q4NX_WS_COUNTER_BYTES + evict_head_bytes(bh) +
+         bh * evict_parts(bh, max_len) * (kPickPart * 4 + kPickBins * 2 + 16);
 }
 
 int q4nx_kv_evict(const uint16_t* k_cache, const uint16_t* v_cache, int64_t kv_b_stride, int64_t kv_h_stride,
@@ -328,7 +596,7 @@ int q4nx_kv_evict(const uint16_t* k_cache, const uint16_t* v_cache, int64_t kv_b
                Q4NX_ERR_SHAPE, "%s: the outputs' room of %d does not hold the %d positions kept", what, room, most);
   Q4NX_REQUIRE(rope_tab == nullptr || max_pos >= max_len, Q4NX_ERR_SHAPE,
                "%s: the table's %d positions are fewer than max_len=%d", what, max_pos, max_len);
-  const size_t need = q4nx_kv_evict_ws_bytes(batch, n_kv_heads);
+  const size_t need = q4nx_kv_evict_ws_bytes(batch, n_kv_heads, max_len);
   Q4NX_REQUIRE(ws != nullptr && ws_bytes >= need && Q4NX_ALIGNED(ws, 256), Q4NX_ERR_WS,
                "%s: workspace of %zu bytes (256-aligned) needed, %zu given", what, need, ws_bytes);
   EvictArgs a{};
@@ -342,7 +610,14 @@ int q4nx_kv_evict(const uint16_t* k_cache, const uint16_t* v_cache, int64_t kv_b
   a.weights_out = weights_out;
   a.lens_out = lens_out;
   a.kept = kept;
+  const int bh = batch * n_kv_heads, parts = evict_parts(bh, max_len);
+  a.parts = parts;
+  a.counters = (unsigned*)ws;
   a.n_old = (int32_t*)((uint8_t*)ws + Q4NX_WS_COUNTER_BYTES);
+  a.cut = (uint32_t*)(a.n_old + bh);
+  a.cand = (uint32_t*)((uint8_t*)a.n_old + evict_head_bytes(bh));
+  a.hist = (uint16_t*)(a.cand + (size_t)bh * parts * kPickPart);
+  a.part_info = (int32_t*)(a.hist + (size_t)bh * parts * kPickBins);
   a.b_stride = kv_b_stride;
   a.h_stride = kv_h_stride;
   a.w_b_stride = w_b_stride;
@@ -358,17 +633,21 @@ int q4nx_kv_evict(const uint16_t* k_cache, const uint16_t* v_cache, int64_t kv_b
   a.recent = recent;
   a.room = room;
   a.in_place = in_place;
-  const int bh = batch * n_kv_heads;
   const int step = kMoveThreads / (head_dim / 16);
   a.blocks = in_place ? 1 : (most + step - 1) / step;
   if (a.blocks > 4096) a.blocks = 4096;
-  Q4NX_REQUIRE(2ll * bh * a.blocks < (1ll << 31), Q4NX_ERR_SHAPE, "%s: more than 2^31 workgroups", what);
+  Q4NX_REQUIRE(2ll * bh * a.blocks < (1ll << 31) && (long long)bh * parts < (1ll << 31), Q4NX_ERR_SHAPE, "%s: more than 2^31 workgroups", what);
   hipStream_t s = (hipStream_t)stream;
-  const dim3 heads((unsigned)bh), threads(kPickThreads);
-  if (max_len <= 4 * kPickThreads) hipLaunchKernelGGL((evict_pick_kernel<4, true>), heads, threads, 0, s, a);
-  else if (max_len <= 16 * kPickThreads) hipLaunchKernelGGL((evict_pick_kernel<16, true>), heads, threads, 0, s, a);
-  else if (max_len <= 48 * kPickThreads) hipLaunchKernelGGL((evict_pick_kernel<48, true>), heads, threads, 0, s, a);
-  else hipLaunchKernelGGL((evict_pick_kernel<16, false>), heads, threads, 0, s, a);
+  if (parts > 0) {
+    const dim3 all((unsigned)(bh * parts)), threads(kPartThreads);
+    hipLaunchKernelGGL(evict_hist_kernel, all, threads, 0, s, a);
+    hipLaunchKernelGGL(evict_cut_kernel, all, threads, 0, s, a);
+    hipLaunchKernelGGL(evict_list_kernel, all, threads, 0, s, a);
+  } else if (max_len <= kPickPart) {
+    hipLaunchKernelGGL((evict_pick_kernel<4, true>), dim3((unsigned)bh), dim3(kPickThreads), 0, s, a);
+  } else {
+    hipLaunchKernelGGL((evict_pick_kernel<16, false>), dim3((unsigned)bh), dim3(kPickThreads), 0, s, a);
+  }
   const dim3 grid((unsigned)(2 * bh * a.blocks));
   if (head_dim == 64) hipLaunchKernelGGL(evict_move_kernel<64>, grid, dim3(kMoveThreads), 0, s, a);
   else hipLaunchKernelGGL(evict_move_kernel<128>, grid, dim3(kMoveThreads), 0, s, a);

@@ -767,7 +767,7 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tensor
         if into is not None:
             w2.zero_()
         return kept.fill_(-1)
-    need = _need("q4nx_kv_evict_ws_bytes", b, hkv)
+    need = _need("q4nx_kv_evict_ws_bytes", b, hkv, most)
     ws, wp, wn, stream = _scratch(ws, need, at)
     _lib.call("q4nx_kv_evict", k_cache.data_ptr(), v_cache.data_ptr(), bs, hs, weights.data_ptr(), wb, wh, lp,
               most, budget, recent, _ptr(rope), 0 if rope is None else rope.shape[0], k2.data_ptr(),
