@@ -10,9 +10,11 @@
 //
 // Parts, all in one grid (the prefix's first, which take longest; the own cache's, which wait for memory,
 // run beside them):
-//   own caches      (sequence, kv head, part): part_narrow
+//   own caches      (sequence, kv head, part): Narrow
 //   prefix, R > 16  (kv head, 64 NR rows, part): part_wide below
-//   prefix, R <= 16 (kv head, part): part_narrow over the members' rows
+//   prefix, R <= 16 (kv head, part): Narrow over the members' rows
+// Short calls of few sequences are one launch: a workgroup a (sequence, kv head) takes the prefix's rows, then
+// its own.
 
 #include "attn_parts.h"
 
@@ -330,10 +332,14 @@ __global__ __launch_bounds__(256, 2) void prefix_parts_kernel(PrefixArgs a) {
       return (((size_t)(gr.first + i) * a.hkv + kvh) * slots + a.ns_own + part) * (size_t)(a.G * kRec<D>) +
              (size_t)(r - i * a.G) * kRec<D>;
     };
-    if (R <= 16)
-      part_narrow<D, false>(row_at(min(lane & 15, R - 1)), R, a.kp + at, a.vp + at, end, end, a.scale_l2,
-                            nullptr, 0, (float*)lds, a.rec, rec_of);
-    else
+    if (R <= 16) {
+      Narrow<D> st;
+      st.init(row_at(min(lane & 15, R - 1)), R);
+      st.template run<false>(a.kp + at, a.vp + at, end, a.scale_l2, R, nullptr, 0);
+      st.finish(R, (float*)lds, [&](int r, int d, const float4& A, float m, float l) {
+        put_record<D>(a.rec + rec_of(r), d, A, m, l);
+      });
+    } else
       part_wide<D, NR>(a, a.kp + at, a.vp + at, end, t * 64 * NR, R, lds, row_at, rec_of);
     return;
   }
@@ -347,9 +353,52 @@ __global__ __launch_bounds__(256, 2) void prefix_parts_kernel(PrefixArgs a) {
   const int end = min(a.chunk_own, len - start);
   const size_t at = (size_t)b * a.b_stride + (size_t)kvh * a.h_stride + (size_t)start * D;
   const size_t rec = (((size_t)b * a.hkv + kvh) * slots + part) * (size_t)(a.G * kRec<D>);
-  part_narrow<D, false>(a.q + ((size_t)b * a.hq + kvh * a.G + min(lane & 15, a.G - 1)) * D, a.G, a.k + at,
-                        a.v + at, end, end, a.scale_l2, nullptr, 0, (float*)lds, a.rec,
-                        [&](int r) { return rec + (size_t)r * kRec<D>; });
+  Narrow<D> st;
+  st.init(a.q + ((size_t)b * a.hq + kvh * a.G + min(lane & 15, a.G - 1)) * D, a.G);
+  st.template run<false>(a.k + at, a.v + at, end, a.scale_l2, a.G, nullptr, 0);
+  st.finish(a.G, (float*)lds, [&](int r, int d, const float4& A, float m, float l) {
+    put_record<D>(a.rec + rec + (size_t)r * kRec<D>, d, A, m, l);
+  });
+}
+
+// The prefix of sequence b (-1: none) and its length, by all lanes of a wave; one round of loads for 64
+// prefixes.
+struct Prefix {
+  int p, len;
+};
+__device__ __forceinline__ Prefix prefix_of(const PrefixArgs& a, int b, int lane) {
+  for (int p0 = 0; p0 < a.n_prefixes; p0 += 64) {
+    const int p = min(p0 + lane, a.n_prefixes - 1);
+    const int n = a.plens[p];
+    const uint64_t who = __ballot(p == p0 + lane && cu_at(a, p) <= b && b < cu_at(a, p + 1));
+    if (who != 0) {
+      const int w = __builtin_ctzll(who);
+      return {p0 + w, min(max(__builtin_amdgcn_readlane(n, w), 0), a.max_prefix)};
+    }
+  }
+  return {-1, 0};
+}
+
+// One workgroup per (sequence, kv head): everything.
+template <int D>
+__global__ __launch_bounds__(kPartWaves * 64) void prefix_whole_kernel(PrefixArgs a) {
+  extern __shared__ __attribute__((aligned(16))) float lds[];   // kPartWaves * G * (D + 2)
+  const int lane = threadIdx.x & 63;
+  const int b = blockIdx.x / a.hkv, kvh = blockIdx.x - b * a.hkv;
+  const size_t row = (size_t)b * a.hq + kvh * a.G;
+  Narrow<D> st;
+  st.init(a.q + (row + min(lane & 15, a.G - 1)) * D, a.G);
+  const int len = min(max(a.lens[b], 0), a.max_len);
+  const Prefix p = prefix_of(a, b, lane);
+  if (p.len > 0) {
+    const size_t at = (size_t)p.p * a.pp_stride + (size_t)kvh * a.ph_stride;
+    st.template run<false>(a.kp + at, a.vp + at, p.len, a.scale_l2, a.G, nullptr, 0);
+  }
+  const size_t at = (size_t)b * a.b_stride + (size_t)kvh * a.h_stride;
+  if (len > 0) st.template run<false>(a.k + at, a.v + at, len, a.scale_l2, a.G, nullptr, 0);
+  st.finish(a.G, lds, [&](int r, int d, const float4& A, float, float l) {
+    put_channels(a.out, a.out_f32, (row + r) * D + d, whole(A, l));
+  });
 }
 
 // One wave per (sequence, query head): the records that were written, merged.
@@ -367,37 +416,26 @@ __global__ __launch_bounds__(256) void prefix_merge_kernel(PrefixArgs a) {
   const float* rec = a.rec + (((size_t)b * a.hkv + kvh) * slots * a.G + (h - kvh * a.G)) * kRec<D>;
   const float4 A = merge_records<D>(rec, (size_t)a.G * kRec<D>, slots, lane, [&](int r) {
     const int len = min(max(a.lens[b], 0), a.max_len);
-    int pl = 0;
-    for (int p0 = 0; p0 < a.n_prefixes; p0 += 64) {
-      const int p = p0 + lane;
-      bool in = false;
-      int n = 0;
-      if (p < a.n_prefixes) {
-        in = cu_at(a, p) <= b && b < cu_at(a, p + 1);
-        n = a.plens[p];
-      }
-      const uint64_t who = __ballot(in);
-      if (who != 0) {
-        pl = min(max(__builtin_amdgcn_readlane(n, __builtin_ctzll(who)), 0), a.max_prefix);
-        break;
-      }
-    }
+    const int pl = prefix_of(a, b, lane).len;
     return r < a.ns_own ? r * a.chunk_own < len : (r - a.ns_own) * a.chunk_pre < pl;
   });
   if (lane < D / 4) put_channels(a.out, a.out_f32, (size_t)i * D + 4 * lane, A);
 }
 
 struct PrefixPlan {
+  bool whole;   // one launch
   int nr, tiles, ns_pre, chunk_pre, ns_own, chunk_own;
 };
-
-static int clamp_int(long long x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : (int)x; }
 
 // How the work is cut. Only bounds are known here (the lengths are on the device).
 static PrefixPlan prefix_plan(int batch, int hq, int hkv, int d, int n_prefixes, int max_prefix, int max_len) {
   const int G = hq / hkv;
   const long long rows = (long long)batch * G;
   PrefixPlan p{};
+  // Up to 1024 positions on a compute unit each (2 x 513 + 33, 40 q / 8 kv heads: 7.8 us, 5.0 and 3.7
+  // in two launches, of which the second costs the host 3.5 us)
+  p.whole = (long long)batch * hkv <= 256 && max_prefix + max_len <= 1024 && kPartWaves * G * (d + 2) <= 16384;
+  if (p.whole) return p;
   // 32 rows a wave where prefixes have more than 64 of them on average and the registers hold it
   p.nr = d == 64 && rows > 64ll * (n_prefixes > 1 ? n_prefixes : 1) ? 2 : 1;
   const int rt = 64 * p.nr;
@@ -405,19 +443,10 @@ static PrefixPlan prefix_plan(int batch, int hq, int hkv, int d, int n_prefixes,
   const long long most = (rows + rt - 1) / rt + (n_prefixes > 0 ? n_prefixes - 1 : 0);
   p.tiles = (int)(most < batch ? most : batch);
   if (n_prefixes == 0 || max_prefix == 0) p.tiles = 0;
-  if (p.tiles > 0) {
-    const int unit = rows <= 16 ? kPartRound : 256;
-    p.ns_pre = clamp_int(512 / ((long long)hkv * p.tiles), 1, 32);
-    p.ns_pre = clamp_int((max_prefix + unit - 1) / unit, 1, p.ns_pre);
-    p.chunk_pre = part_chunk(max_prefix, p.ns_pre, 64);
-    p.ns_pre = (max_prefix + p.chunk_pre - 1) / p.chunk_pre;
-  }
-  if (max_len > 0) {
-    p.ns_own = clamp_int(1024 / ((long long)hkv * batch), 1, 32);
-    p.ns_own = clamp_int((max_len + 255) / 256, 1, p.ns_own);
-    p.chunk_own = part_chunk(max_len, p.ns_own, kPartRound);
-    p.ns_own = (max_len + p.chunk_own - 1) / p.chunk_own;
-  }
+  if (p.tiles > 0)
+    cut_parts(max_prefix, 512 / ((long long)hkv * p.tiles), rows <= 16 ? kPartRound : 256, 64, &p.ns_pre, &p.chunk_pre);
+  if (max_len > 0)
+    cut_parts(max_len, 1024 / ((long long)hkv * batch), 256, kPartRound, &p.ns_own, &p.chunk_own);
   if (p.chunk_pre == 0) p.chunk_pre = 64;
   if (p.chunk_own == 0) p.chunk_own = kPartRound;
   return p;
@@ -435,6 +464,11 @@ static size_t prefix_rec_bytes(const PrefixPlan& p, int batch, int hq, int d) {
 
 template <int D>
 static void prefix_launch(const PrefixArgs& a, const PrefixPlan& p, hipStream_t s) {
+  if (p.whole) {
+    const size_t lds = (size_t)kPartWaves * a.G * (D + 2) * 4;
+    hipLaunchKernelGGL(prefix_whole_kernel<D>, dim3((unsigned)(a.batch * a.hkv)), dim3(kPartWaves * 64), lds, s, a);
+    return;
+  }
   const unsigned grid = (unsigned)(a.hkv * (p.tiles * p.ns_pre + a.batch * p.ns_own));
   if (grid > 0) {
     if (D == 64 && p.nr == 2) hipLaunchKernelGGL((prefix_parts_kernel<64, 2>), dim3(grid), dim3(256), 0, s, a);

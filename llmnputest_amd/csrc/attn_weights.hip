@@ -6,9 +6,9 @@
 //   weights[l]   += sum over the group's heads of p[h][l]      (the newest position's is set)
 //
 // A weight needs the maximum and the sum of the whole row, which a part of it does not know. The parts
-// (part_narrow) therefore also leave their scores, 4 Hq bytes a position beside the 4 D Hkv of K and V, and
+// (Narrow) therefore also leave their scores, 4 Hq bytes a position beside the 4 D Hkv of K and V, and
 // the second launch turns them into weights once every part's (m, l) is there; its last workgroup of a
-// (sequence, kv head) merges the outputs.
+// (sequence, kv head) merges the outputs. Short rows of few sequences are one launch.
 
 #include "attn_parts.h"
 
@@ -41,10 +41,44 @@ __global__ __launch_bounds__(256) void weight_parts_kernel(WeightArgs a) {
   const int end = min(a.chunk, len - start);
   const size_t at = (size_t)b * a.b_stride + (size_t)kvh * a.h_stride + (size_t)start * D;
   const size_t rec = ((size_t)bk * a.ns + part) * (size_t)(a.G * kRec<D>);
-  part_narrow<D, true>(a.q + ((size_t)b * a.hq + kvh * a.G + min((int)(threadIdx.x & 15), a.G - 1)) * D, a.G,
-                       a.k + at, a.v + at, end, end, a.scale_l2,
-                       a.scores + (size_t)bk * a.G * a.score_stride + start, a.score_stride, lds, a.rec,
-                       [&](int r) { return rec + (size_t)r * kRec<D>; });
+  Narrow<D> st;
+  st.init(a.q + ((size_t)b * a.hq + kvh * a.G + min((int)(threadIdx.x & 15), a.G - 1)) * D, a.G);
+  st.template run<true>(a.k + at, a.v + at, end, a.scale_l2, a.G,
+                        a.scores + (size_t)bk * a.G * a.score_stride + start, a.score_stride);
+  st.finish(a.G, lds, [&](int r, int d, const float4& A, float m, float l) {
+    put_record<D>(a.rec + rec + (size_t)r * kRec<D>, d, A, m, l);
+  });
+}
+
+// One workgroup per (sequence, kv head): everything, the scores in LDS.
+template <int D>
+__global__ __launch_bounds__(kPartWaves * 64) void weight_whole_kernel(WeightArgs a, int score_stride) {
+  extern __shared__ __attribute__((aligned(16))) float lds[];   // scores [G][score_stride], then states
+  __shared__ float s_m[16], s_l[16];
+  const int tid = threadIdx.x;
+  const int b = blockIdx.x / a.hkv, kvh = blockIdx.x - b * a.hkv;
+  const int len = min(max(a.lens[b], 0), a.max_len);
+  const size_t at = (size_t)b * a.b_stride + (size_t)kvh * a.h_stride;
+  const size_t row = (size_t)b * a.hq + kvh * a.G;
+  float* const scores = lds;
+  float* const to = a.weights + (size_t)b * a.w_b_stride + (size_t)kvh * a.w_h_stride;
+  Narrow<D> st;
+  st.init(a.q + (row + min(tid & 15, a.G - 1)) * D, a.G);
+  st.template run<true>(a.k + at, a.v + at, len, a.scale_l2, a.G, scores, score_stride);
+  st.finish(a.G, lds + a.G * score_stride, [&](int r, int d, const float4& A, float m, float l) {
+    put_channels(a.out, a.out_f32, (row + r) * D + d, whole(A, l));
+    if (d == 0) {
+      s_m[r] = m == -INFINITY ? 0.f : m;
+      s_l[r] = l == 0.f ? 0.f : 1.f / l;
+    }
+  });
+  __syncthreads();
+  for (int p = tid; p < len; p += kPartWaves * 64) {
+    const float old = a.start || p == len - 1 ? 0.f : to[p];
+    float w = 0.f;
+    for (int h = 0; h < a.G; ++h) w = fmaf(exp2_hw(scores[h * score_stride + p] - s_m[h]), s_l[h], w);
+    to[p] = old + w;
+  }
 }
 
 constexpr int kWeightSpan = 1024;   // positions of a workgroup of the second launch
@@ -116,18 +150,23 @@ __global__ __launch_bounds__(256) void weight_sum_kernel(WeightArgs a, int spans
 }
 
 struct WeightPlan {
-  int ns, chunk;
+  int ns, chunk;         // ns 0: one launch
   int64_t score_stride;
 };
 
-static WeightPlan weight_plan(int batch, int hkv, int max_len) {
+// Bytes of LDS that a workgroup with a whole row takes.
+static size_t whole_lds(int G, int d, int64_t score_stride) {
+  return (size_t)G * (score_stride + kPartWaves * (d + 2)) * 4;
+}
+
+static WeightPlan weight_plan(int batch, int hq, int hkv, int d, int max_len) {
   WeightPlan p{};
-  const long long by_grid = 1024 / ((long long)hkv * batch);
-  p.ns = by_grid < 1 ? 1 : by_grid > 32 ? 32 : (int)by_grid;
-  const int by_len = (max_len + 255) / 256;
-  if (p.ns > by_len) p.ns = by_len;
-  p.chunk = part_chunk(max_len, p.ns, kPartRound);
-  p.ns = (max_len + p.chunk - 1) / p.chunk;
+  // Up to 1024 positions on a compute unit each, as far as LDS holds their scores (1 x 513, 40 q / 8 kv heads:
+  // 8.0 us, 5.2 and 4.4 in two launches, of which the second costs the host 3.5 us)
+  const int round = 32 * kPartWaves;
+  p.score_stride = (max_len + round - 1) / round * round;
+  if ((long long)batch * hkv <= 256 && max_len <= 1024 && whole_lds(hq / hkv, d, p.score_stride) <= 65024) return p;
+  cut_parts(max_len, 1024 / ((long long)hkv * batch), 256, kPartRound, &p.ns, &p.chunk);
   p.score_stride = (int64_t)p.ns * p.chunk;
   return p;
 }
@@ -142,11 +181,17 @@ static size_t weight_rec_bytes(const WeightPlan& p, int batch, int hq, int d) {
 }
 
 static size_t weight_ws(const WeightPlan& p, int batch, int hq, int d) {
-  return (size_t)Q4NX_WS_COUNTER_BYTES + weight_rec_bytes(p, batch, hq, d) + (size_t)batch * hq * p.score_stride * 4;
+  return (size_t)Q4NX_WS_COUNTER_BYTES +
+         (p.ns == 0 ? 0 : weight_rec_bytes(p, batch, hq, d) + (size_t)batch * hq * p.score_stride * 4);
 }
 
 template <int D>
 static void weight_launch(const WeightArgs& a, hipStream_t s) {
+  if (a.ns == 0) {
+    hipLaunchKernelGGL(weight_whole_kernel<D>, dim3((unsigned)(a.batch * a.hkv)), dim3(kPartWaves * 64),
+                       whole_lds(a.G, D, a.score_stride), s, a, (int)a.score_stride);
+    return;
+  }
   const int spans = (a.max_len + kWeightSpan - 1) / kWeightSpan;
   hipLaunchKernelGGL(weight_parts_kernel<D>, dim3((unsigned)(a.batch * a.hkv * a.ns)), dim3(256), 0, s, a);
   hipLaunchKernelGGL(weight_sum_kernel<D>, dim3((unsigned)(a.batch * a.hkv * (spans + 1))), dim3(256), 0, s, a, spans);
@@ -160,7 +205,7 @@ extern "C" {
 
 size_t q4nx_gqa_decode_weights_ws_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim, int max_len) {
   if (!weight_shape_ok(batch, n_q_heads, n_kv_heads, head_dim, max_len)) return 0;
-  return weight_ws(weight_plan(batch, n_kv_heads, max_len), batch, n_q_heads, head_dim);
+  return weight_ws(weight_plan(batch, n_q_heads, n_kv_heads, head_dim, max_len), batch, n_q_heads, head_dim);
 }
 
 int q4nx_gqa_decode_weights(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache,
@@ -185,7 +230,7 @@ int q4nx_gqa_decode_weights(const uint16_t* q, const uint16_t* k_cache, const ui
   Q4NX_REQUIRE(w_h_stride >= max_len && w_b_stride >= (int64_t)n_kv_heads * w_h_stride, Q4NX_ERR_SHAPE,
                "%s: strides of weights do not hold [Hkv][max_len]", what);
   Q4NX_REQUIRE(scale >= 0.f, Q4NX_ERR_ARG, "%s: scale must not be negative", what);
-  const WeightPlan p = weight_plan(batch, n_kv_heads, max_len);
+  const WeightPlan p = weight_plan(batch, n_q_heads, n_kv_heads, head_dim, max_len);
   Q4NX_REQUIRE((long long)n_kv_heads * batch * (max_len / kWeightSpan + 2) < (1ll << 31), Q4NX_ERR_SHAPE,
                "%s: more than 2^31 workgroups", what);
   const size_t need = weight_ws(p, batch, n_q_heads, head_dim);

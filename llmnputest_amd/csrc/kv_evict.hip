@@ -44,7 +44,7 @@ struct EvictArgs {
   int64_t ob_stride, oh_stride, ow_b_stride, ow_h_stride;
   int batch, hkv, max_len, budget, recent, room;
   int parts;               // of 4096 positions
-  int in_place, blocks;    // blocks: workgroups for a (sequence, kv head)'s rows
+  int blocks;              // workgroups for a (sequence, kv head)'s rows of K, and of V
 };
 
 // Greater weights have greater keys; a NaN's is the greatest; -0 and 0 are one value.
@@ -273,9 +273,11 @@ __device__ __forceinline__ void find_bin(const int (&c)[8], int left, int* s_sum
   __syncthreads();
 }
 
+constexpr int kHeldKeys = 4096;
 __global__ __launch_bounds__(kPartThreads) void evict_cut_kernel(EvictArgs a) {
   __shared__ __attribute__((aligned(16))) int s_hist[kPickBins];
-  __shared__ int s_sum[kPartThreads / 64], s_found[2], s_gt, s_eq, s_last;
+  __shared__ int s_sum[kPartThreads / 64], s_found[2], s_gt, s_eq, s_last, s_end[kPartThreads];
+  __shared__ uint32_t s_held[kHeldKeys];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const PartJob j = part_job(a);
@@ -329,7 +331,9 @@ __global__ __launch_bounds__(kPartThreads) void evict_cut_kernel(EvictArgs a) {
   __syncthreads();
   if (!s_last) return;
 
-  // ---- the last: the wanted key's lower 21 bits, from the keys of the bin
+  // ---- the last: the wanted key's lower 21 bits, from the keys of the bin. They are few unless weights are
+  // much alike: then they are held in LDS, where they are looked at three times (131072 positions of one
+  // sequence: 30 to 25 us)
   uint32_t found = bin << 21;
   const uint32_t* const all = a.cand + row0 * kPickPart;
   auto load = [&](const uint32_t* p) {
@@ -338,19 +342,44 @@ __global__ __launch_bounds__(kPartThreads) void evict_cut_kernel(EvictArgs a) {
   auto load_i = [&](const int32_t* p) {
     return __hip_atomic_load(const_cast<int32_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
   };
+  // thread p has part p's count, and where its keys begin
+  const int many = tid < parts ? load_i(info + 4 * tid + 1) : 0;
+  const int above_bin = tid < parts ? load_i(info + 4 * tid) : 0;
+  int upto = wave_scan(many);
+  if (lane == 63) s_sum[wave] = upto;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kPartThreads / 64; ++i) upto += i < wave ? s_sum[i] : 0;
+  s_end[tid] = upto;
+  __syncthreads();
+  const bool held = parts <= kPartThreads && s_end[kPartThreads - 1] <= kHeldKeys;
+  if (held) {
+    for (int p = wave; p < parts; p += kPartThreads / 64) {
+      const int end = s_end[p], begin = p > 0 ? s_end[p - 1] : 0;
+      for (int i = begin + lane; i < end; i += 64) s_held[i] = load(all + (size_t)p * kPickPart + (i - begin));
+    }
+    __syncthreads();
+  }
+  // f(key) of part p's keys, by a wave
+  auto keys_of = [&](int p, auto f) {
+    if (held) {
+      const int end = s_end[p], begin = p > 0 ? s_end[p - 1] : 0;
+      for (int i = begin + lane; i < end; i += 64) f(s_held[i]);
+    } else {
+      const int m = load_i(info + 4 * p + 1);
+#pragma unroll 4
+      for (int i = lane; i < m; i += 64) f(load(all + (size_t)p * kPickPart + i));
+    }
+  };
   for (int pass = 0; pass < 2; ++pass) {
     const int shift = pass == 0 ? 10 : 0;
     const uint32_t mask = pass == 0 ? 2047u : 1023u, known = pass == 0 ? ~0u << 21 : ~0u << 10;
     for (int i = tid; i < kPickBins; i += kPartThreads) s_hist[i] = 0;
     __syncthreads();
-    for (int p = wave; p < parts; p += kPartThreads / 64) {
-      const int m = load_i(info + 4 * p + 1);
-#pragma unroll 4
-      for (int i = lane; i < m; i += 64) {
-        const uint32_t k = load(all + (size_t)p * kPickPart + i);
+    for (int p = wave; p < parts; p += kPartThreads / 64)
+      keys_of(p, [&](uint32_t k) {
         if ((k & known) == found) atomicAdd(&s_hist[k >> shift & mask], 1);
-      }
-    }
+      });
     __syncthreads();
     int d[8];
 #pragma unroll
@@ -360,34 +389,60 @@ __global__ __launch_bounds__(kPartThreads) void evict_cut_kernel(EvictArgs a) {
     left = s_found[1];
     __syncthreads();
   }
-  // ---- how many each part writes, and from where on
+  // ---- how many each part writes, and from where on: its first place, and the equal keys before it
   for (int p = wave; p < parts; p += kPartThreads / 64) {
-    const int m = load_i(info + 4 * p + 1);
     int above = 0, same = 0;
-#pragma unroll 4
-    for (int i = lane; i < m; i += 64) {
-      const uint32_t k = load(all + (size_t)p * kPickPart + i);
+    keys_of(p, [&](uint32_t k) {
       above += k > found;
       same += k == found;
-    }
+    });
     above = wave_scan(above);
     same = wave_scan(same);
     if (lane == 63) {
-      info[4 * p + 2] = load_i(info + 4 * p) + above;
+      info[4 * p + 2] = above;
       info[4 * p + 3] = same;
     }
   }
   wait_vm();
   __syncthreads();
-  if (tid == 0) {
-    int at = 0, ties = 0;
-    for (int p = 0; p < parts; ++p) {
-      const int g = info[4 * p + 2], e = info[4 * p + 3];
-      info[4 * p + 2] = at;
-      info[4 * p + 3] = ties;
-      at += g + min(e, max(left - ties, 0));
-      ties += e;
+  int at = 0, ties = 0;   // before the parts at hand
+  for (int p0 = 0; p0 < parts; p0 += kPartThreads) {
+    const int p = p0 + tid;
+    int g = 0, e = 0;
+    if (p < parts) {
+      g = (p0 == 0 ? above_bin : load_i(info + 4 * p)) + info[4 * p + 2];
+      e = info[4 * p + 3];
     }
+    int eq_upto = wave_scan(e);
+    if (lane == 63) s_sum[wave] = eq_upto;
+    __syncthreads();
+    int eq_all = 0;
+#pragma unroll
+    for (int i = 0; i < kPartThreads / 64; ++i) {
+      eq_upto += i < wave ? s_sum[i] : 0;
+      eq_all += s_sum[i];
+    }
+    __syncthreads();
+    const int before = ties + eq_upto - e;
+    const int n = g + min(e, max(left - before, 0));
+    int n_upto = wave_scan(n);
+    if (lane == 63) s_sum[wave] = n_upto;
+    __syncthreads();
+    int n_all = 0;
+#pragma unroll
+    for (int i = 0; i < kPartThreads / 64; ++i) {
+      n_upto += i < wave ? s_sum[i] : 0;
+      n_all += s_sum[i];
+    }
+    __syncthreads();
+    if (p < parts) {
+      info[4 * p + 2] = at + n_upto - n;
+      info[4 * p + 3] = before;
+    }
+    at += n_all;
+    ties += eq_all;
+  }
+  if (tid == 0) {
     a.cut[2 * j.bk] = found;
     a.cut[2 * j.bk + 1] = (uint32_t)left;
   }
@@ -463,7 +518,7 @@ __device__ __forceinline__ void turn_back(uint4& a, uint4& z, const float* cs, i
 constexpr int kMoveThreads = 512;
 
 // kMoveThreads / (D / 16) rows of K (`which` 0) or V (1) a step: two 16-byte pieces a thread.
-template <int D>
+template <int D, bool IN_PLACE>
 __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a) {
   constexpr int L = D / 16, STEP = kMoveThreads / L;   // threads of a row, rows of a step
   const int tid = threadIdx.x, c = tid % L, sub = tid / L;
@@ -474,11 +529,8 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a) {
   const int b = bk / a.hkv, h = bk - b * a.hkv;
   const int n = a.n_old[bk], m = min(n, a.budget);
   const int32_t* kept = a.kept + (size_t)bk * a.budget;
-  if (which == 1) {
-    // the weights go with V's rows, by the first wave's threads ... of the same blocks
-    if (block == 0 && h == 0 && tid == 0) a.lens_out[b] = m;
-  }
-  if (a.in_place && n <= a.budget) return;
+  if (which == 1 && block == 0 && h == 0 && tid == 0) a.lens_out[b] = m;
+  if (IN_PLACE && n <= a.budget) return;
   const uint16_t* from = (which ? a.v : a.k) + (size_t)b * a.b_stride + (size_t)h * a.h_stride;
   uint16_t* to = (which ? a.v_out : a.k_out) + (size_t)b * a.ob_stride + (size_t)h * a.oh_stride;
   const float* w = a.weights + (size_t)b * a.w_b_stride + (size_t)h * a.w_h_stride;
@@ -487,8 +539,8 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a) {
   // K's second piece is half a row on (its partner of a rotation), V's the next sixteen bytes
   const int e0 = which ? 16 * c : 8 * c, e1 = which ? 16 * c + 8 : D / 2 + 8 * c;
 
-  uint4 x[2], y[2];
-  float ws = 0.f, ws2 = 0.f;
+  uint4 x[2];
+  float ws = 0.f;
   int src = 0;
   auto load = [&](int i0, int& s_, uint4 (&r)[2], float& wv) {
     const int i = i0 + sub;
@@ -507,7 +559,7 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a) {
     *(uint4*)(to + (size_t)i * D + e1) = r[1];
     if (which && c == 0) w_to[i] = wv;
   };
-  if (!a.in_place) {
+  if constexpr (!IN_PLACE) {
     for (int i0 = block * STEP; i0 < m; i0 += a.blocks * STEP) {
       load(i0, src, x, ws);
       store(i0, src, x, ws);
@@ -517,6 +569,8 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a) {
     return;
   }
   // in place, one workgroup for all rows: the next step's rows are read before this step's are written
+  uint4 y[2];
+  float ws2 = 0.f;
   int src2 = 0;
   load(0, src, x, ws);
   for (int i0 = 0; i0 < m; i0 += STEP) {
@@ -632,7 +686,6 @@ int q4nx_kv_evict(const uint16_t* k_cache, const uint16_t* v_cache, int64_t kv_b
   a.budget = budget;
   a.recent = recent;
   a.room = room;
-  a.in_place = in_place;
   const int step = kMoveThreads / (head_dim / 16);
   a.blocks = in_place ? 1 : (most + step - 1) / step;
   if (a.blocks > 4096) a.blocks = 4096;
@@ -649,8 +702,11 @@ int q4nx_kv_evict(const uint16_t* k_cache, const uint16_t* v_cache, int64_t kv_b
     hipLaunchKernelGGL((evict_pick_kernel<16, false>), dim3((unsigned)bh), dim3(kPickThreads), 0, s, a);
   }
   const dim3 grid((unsigned)(2 * bh * a.blocks));
-  if (head_dim == 64) hipLaunchKernelGGL(evict_move_kernel<64>, grid, dim3(kMoveThreads), 0, s, a);
-  else hipLaunchKernelGGL(evict_move_kernel<128>, grid, dim3(kMoveThreads), 0, s, a);
+  const dim3 threads(kMoveThreads);
+  if (head_dim == 64 && in_place) hipLaunchKernelGGL((evict_move_kernel<64, true>), grid, threads, 0, s, a);
+  else if (head_dim == 64) hipLaunchKernelGGL((evict_move_kernel<64, false>), grid, threads, 0, s, a);
+  else if (in_place) hipLaunchKernelGGL((evict_move_kernel<128, true>), grid, threads, 0, s, a);
+  else hipLaunchKernelGGL((evict_move_kernel<128, false>), grid, threads, 0, s, a);
   return check_launch(what);
 }
 

@@ -671,8 +671,11 @@ def gqa_prefix_decode(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.T
     lp = _here(lens, "lens", torch.int32, dev, (b,))
     pp = _here(prefix_lens, "prefix_lens", torch.int32, dev, (p,))
     up = None if cu is None else _here(cu, "cu", torch.int32, dev, (p + 1,))
-    out = torch.empty_like(q) if out is None else out
-    op = _here(out, "out", torch.bfloat16, dev, shape)
+    if out is None:
+        out = torch.empty_like(q)
+        op = out.data_ptr()
+    else:
+        op = _here(out, "out", torch.bfloat16, dev, shape)
     of = torch.empty(shape, dtype=torch.float32, device=q.device) if want_f32 else None
     if b == 0:
         return (out, of) if want_f32 else out
@@ -714,8 +717,11 @@ def gqa_decode_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
         raise ValueError(f"k_cache must be [{b}, Hkv, L, {d}]")
     wb, wh = _weight_rows(weights, "weights", (b, hkv, n), dev)
     lp = _here(lens, "lens", torch.int32, dev, (b,))
-    out = torch.empty_like(q) if out is None else out
-    op = _here(out, "out", torch.bfloat16, dev, shape)
+    if out is None:
+        out = torch.empty_like(q)
+        op = out.data_ptr()
+    else:
+        op = _here(out, "out", torch.bfloat16, dev, shape)
     of = torch.empty(shape, dtype=torch.float32, device=q.device) if want_f32 else None
     most = _upto(n, max_len, "max_len")
     if b == 0 or most == 0:
@@ -760,7 +766,7 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tensor
         _here(rope, "rope", torch.float32, dev, (rope.shape[0], 2, d // 2))
     if budget < 1 or not 0 <= recent <= budget:
         raise ValueError(f"budget must be positive and recent in 0..budget, got {budget} and {recent}")
-    kept = torch.empty((b, hkv, budget), dtype=torch.int32, device=k_cache.device)
+    kept = lens.new_empty((b, hkv, budget))
     most = _upto(n, max_len, "max_len")
     if b == 0 or most == 0:
         l2.zero_()
@@ -832,14 +838,21 @@ def adjust_logits(logits: torch.Tensor, counts: torch.Tensor | None = None,
     b, v = shape = logits.shape
     if v == 0:
         raise ValueError("logits must have at least one token")
-    out = torch.empty(shape, dtype=dtype, device=logits.device) if out is None else out
-    out_stride = _vocab_rows(out, "out", dtype, dev, shape)
-    cp, cs = (None, 0) if counts is None else (counts.data_ptr(), _vocab_rows(counts, "counts", torch.int32, dev, shape))
-    pen = []
-    for t, name in ((repetition, "repetition"), (presence, "presence"), (frequency, "frequency")):
-        if t is not None and counts is None:
-            raise ValueError(f"{name} needs counts")
-        pen.append(None if t is None else _here(t, name, torch.float32, dev, (b,)))
+    if out is None:
+        out = logits.new_empty(shape)
+        out_stride = v
+    else:
+        out_stride = _vocab_rows(out, "out", dtype, dev, shape)
+    one = (b,)
+    cp = rep = pres = freq = None
+    cs = 0
+    if counts is not None:
+        cp, cs = counts.data_ptr(), _vocab_rows(counts, "counts", torch.int32, dev, shape)
+        rep = None if repetition is None else _here(repetition, "repetition", torch.float32, dev, one)
+        pres = None if presence is None else _here(presence, "presence", torch.float32, dev, one)
+        freq = None if frequency is None else _here(frequency, "frequency", torch.float32, dev, one)
+    elif not (repetition is presence is frequency is None):
+        raise ValueError("penalties need counts")
     ids = values = bias_cu = None
     n_bias = 0 if bias is None else bias[0].numel()
     if n_bias:
@@ -854,17 +867,19 @@ def adjust_logits(logits: torch.Tensor, counts: torch.Tensor | None = None,
         if n_mask == 0 or (mask_rows is None and n_mask != b):
             raise ValueError(f"mask must have a row for each of {b} sequences, or mask_rows")
         if mask_rows is not None:
-            rp = _here(mask_rows, "mask_rows", torch.int32, dev, (b,))
+            rp = _here(mask_rows, "mask_rows", torch.int32, dev, one)
     elif mask_rows is not None:
         raise ValueError("mask_rows needs mask")
     if tokens is None:
-        tokens = torch.empty(b, dtype=torch.int32, device=logits.device)
-    tp = _here(tokens, "tokens", torch.int32, dev, (b,))
-    kp = None if keys is None else _here(keys, "keys", torch.int64, dev, (b,))
+        tokens = logits.new_empty(one, dtype=torch.int32)
+        tp = tokens.data_ptr()
+    else:
+        tp = _here(tokens, "tokens", torch.int32, dev, one)
+    kp = None if keys is None else _here(keys, "keys", torch.int64, dev, one)
     if b:
         ws, wp, wn, stream = _scratch(ws, WS_COUNTER_BYTES, at)
         _lib.call("q4nx_adjust_logits", logits.data_ptr(), dtype == torch.bfloat16, stride, out.data_ptr(),
-                  out_stride, v, b, cp, cs, *pen, ids, values, n_bias, bias_cu, mp, ms, n_mask, rp, tp, kp,
+                  out_stride, v, b, cp, cs, rep, pres, freq, ids, values, n_bias, bias_cu, mp, ms, n_mask, rp, tp, kp,
                   wp, wn, stream)
     return out, tokens
 

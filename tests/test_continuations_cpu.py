@@ -54,7 +54,7 @@ def test_prefix_refusals(change, code):
     (dict(q=None), ERR_ARG), (dict(w=None), ERR_ARG), (dict(out=None), ERR_ARG), (dict(k=AT + 8), ERR_ARG),
     (dict(out=AT + 4), ERR_ARG), (dict(scale=-1.0), ERR_ARG), (dict(hq=7), ERR_SHAPE), (dict(d=32), ERR_SHAPE),
     (dict(most=0), ERR_SHAPE), (dict(most=51), ERR_SHAPE), (dict(wh=49), ERR_SHAPE), (dict(wb=8 * 49), ERR_SHAPE),
-    (dict(hs=50 * 64 + 2), ERR_SHAPE), (dict(ws=None), ERR_WS), (dict(wn=70000), ERR_WS)])
+    (dict(hs=50 * 64 + 2), ERR_SHAPE), (dict(ws=None), ERR_WS), (dict(wn=65535), ERR_WS)])
 def test_weights_refusals(change, code):
     rc, msg = refused("q4nx_gqa_decode_weights", WEIGHTS, **change)
     assert rc == code and msg.startswith("q4nx_gqa_decode_weights"), msg
@@ -95,8 +95,8 @@ def test_logits_refusals(change, code):
 def test_workspaces():
     lib = _lib.lib()
     size = lib.q4nx_gqa_prefix_decode_ws_bytes
-    assert size(4, 40, 8, 64, 2, 100, 50) >= 65536 + 4 * 40 * 2 * 68 * 4      # a part of each kind
-    assert size(4, 40, 8, 64, 0, 0, 0) == 65536 and size(1, 8, 8, 128, 1, 1, 0) == 65536 + 8 * 132 * 4
+    assert size(4, 40, 8, 64, 2, 1000, 500) >= 65536 + 4 * 40 * 2 * 68 * 4      # a part of each kind
+    assert size(4, 40, 8, 64, 0, 0, 0) == 65536 and size(1, 8, 8, 128, 1, 1024, 0) == 65536   # one launch
     for bad in ((0, 40, 8, 64, 1, 1, 1), (4, 40, 7, 64, 1, 1, 1), (4, 40, 8, 65, 1, 1, 1), (4, 40, 8, 64, 5, 1, 1)):
         assert size(*bad) == 0
     size = lib.q4nx_gqa_decode_weights_ws_bytes
@@ -111,7 +111,7 @@ def test_more_parts_than_a_wave_has_lanes_never():
     """A wave's lanes hold a (sequence, head)'s records: 32 parts of a prefix and 32 of an own cache."""
     lib = _lib.lib()
     for b in (1, 2, 3, 16, 64, 200):
-        for most in (1, 300, 5000, 70000, (1 << 24) - 1):
+        for most in (1025, 5000, 70000, (1 << 24) - 1):
             n = (lib.q4nx_gqa_prefix_decode_ws_bytes(b, 8, 4, 64, 1, most, most) - 65536) // (b * 8 * 68 * 4)
             assert 2 <= n <= 64
             one = lib.q4nx_gqa_prefix_decode_ws_bytes(b, 8, 4, 64, 0, 0, most) - 65536
