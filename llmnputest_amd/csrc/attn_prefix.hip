@@ -79,8 +79,8 @@ __device__ __forceinline__ Group find_tile(const PrefixArgs& a, int RT, int lane
 // LDS, loaded ahead, read by all four waves; a tile's scores are computed beside the previous tile's
 // exponentials. V^T comes out of the transposing LDS read. P enters
 // as two bf16 terms, its upper half and what that leaves (2^-15 of it is lost); l is their sum, by a product
-// with ones. The running maximum moves only when a row's tile exceeds it by 2^8
-// (weights stay below 2^8 then), which leaves out nearly every rescaling of the accumulators.
+// with ones. The running maximum is the first tile's and moves only when a weight against it
+// exceeds 2^8, which leaves out nearly every search for it and every rescaling of the accumulators.
 // 16-byte pieces of a row are swizzled by the row, so that 16 rows' pieces lie in different banks.
 template <int D>
 __device__ __forceinline__ int swz_k(int row, int c) {
@@ -89,6 +89,13 @@ __device__ __forceinline__ int swz_k(int row, int c) {
 template <int D>
 __device__ __forceinline__ int swz_v(int row, int c) {
   return row * (D / 8) + (c ^ (D == 64 ? row & 7 : (row & 7) * 2));
+}
+
+// 16 bytes a lane from base + voff to LDS at lds + 16 lane. No register receives them; who reads them waits
+// for the count of loads first. (The builtin makes the compiler wait before every later read of LDS.)
+__device__ __forceinline__ void lds16(const void* base, uint32_t voff, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :: "s"(lds), "v"(voff), "s"(base) : "memory");
 }
 
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
@@ -123,33 +130,27 @@ __device__ __forceinline__ void part_wide(const PrefixArgs& a, const uint16_t* k
     for (int u = 0; u < D / 16; ++u) o[n][u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
 
-  uint4 gk[LD], gv[LD];
-  // through buffer resources over the part's rows: those past the end read zeros (their weights are masked
-  // to 0), and the tile's place is a scalar offset
-  const __amdgpu_buffer_rsrc_t kr = make_rsrc(kbase, (uint32_t)end * (2 * D));
-  const __amdgpu_buffer_rsrc_t vr = make_rsrc(vbase, (uint32_t)end * (2 * D));
-  auto fetch = [&](__amdgpu_buffer_rsrc_t r, int p0, uint4 (&x)[LD]) {
+  // Tile t of K or V straight into its LDS buffer, 16 bytes a lane; a lane fetches what the swizzle puts in
+  // its place. Rows past the end: the last one again, whose weight is masked to 0.
+  const uint32_t k0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint4*)sk;
+  const uint32_t v0 = k0 + 2 * 64 * C * 16;
+  const int nt = (end + 63) / 64;
+  const int row_of = tid / C;   // of this lane's first piece; the others are 256 / C rows on each
+  const uint32_t ck = (uint32_t)((swz_k<D>(row_of, tid % C) % C) * 16), cv = (uint32_t)((swz_v<D>(row_of, tid % C) % C) * 16);
+  auto fetch = [&](const uint16_t* base, uint32_t lds0, uint32_t c, int t) {
+    if (t >= nt) return;
+    const uint16_t* const from = base + (size_t)t * 64 * D;
+    const int lim = min(63, end - 1 - t * 64);
 #pragma unroll
-    for (int i = 0; i < LD; ++i) {
-      const v4i_t v = __builtin_amdgcn_raw_buffer_load_b128(r, (tid + 256 * i) * 16, p0 * (2 * D), 0);
-      x[i] = make_uint4((uint32_t)v.x, (uint32_t)v.y, (uint32_t)v.z, (uint32_t)v.w);
-    }
-  };
-  auto put_k = [&](int t) {
-#pragma unroll
-    for (int i = 0; i < LD; ++i) sk[(t & 1) * 64 * C + swz_k<D>((tid + 256 * i) / C, tid % C)] = gk[i];
-  };
-  auto put_v = [&](int t) {
-#pragma unroll
-    for (int i = 0; i < LD; ++i) sv[(t & 1) * 64 * C + swz_v<D>((tid + 256 * i) / C, tid % C)] = gv[i];
+    for (int i = 0; i < LD; ++i)
+      lds16(from, (uint32_t)min(row_of + i * (256 / C), lim) * (2 * D) + c,
+            lds0 + (uint32_t)((t & 1) * 64 * C + wave * 64 + 256 * i) * 16);
   };
   const bool busy = r0 < R;   // waves without rows only load
   const uint32_t one2 = 0x3F803F80u;
   const u32x4_t ones = {one2, one2, one2, one2};
-  const int nt = (end + 63) / 64;
 
   f32x4_t s[NR][4];   // the tile's scores
-  float mx[NR];       // and the greatest of them, scaled
   // operands read from LDS a step ahead of their products (left to the compiler, every pair of products
   // waited for its own reads); only arithmetic is moved across
   u32x4_t kf[2][KC], vf[D / 16];
@@ -184,7 +185,7 @@ __device__ __forceinline__ void part_wide(const PrefixArgs& a, const uint16_t* k
   };
   // `last`: some positions may lie past the end (apart from the others: as selects in every tile, this made
   // 120 us of 90 with 256 x 16384)
-  auto scored = [&](int t, auto last) {
+  auto mask = [&](int t, auto last) {
     if constexpr (last) {
 #pragma unroll
       for (int x = 0; x < 4; ++x)
@@ -194,58 +195,74 @@ __device__ __forceinline__ void part_wide(const PrefixArgs& a, const uint16_t* k
 #pragma unroll
             for (int n = 0; n < NR; ++n) s[n][x][e] = -INFINITY;
     }
+  };
+  // The greatest scaled score of subtiles x0 .. x1 - 1, per row.
+  auto greatest = [&](int n, int x0, int x1) {
+    float v = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      if (x >= x0 && x < x1)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v = fmaxf(v, s[n][x][e]);
+    return xor32_max(xor16_max(v)) * a.scale_l2;
+  };
+  // Weights of half a tile against the maximum as it stands, and whether one is above 2^8 (or a NaN; positive
+  // floats and NaNs, compared as whole numbers) or there is no maximum yet (every score so far was -inf).
+  float w[NR][8];
+  auto weigh = [&](int x2) {
+    uint32_t top = 0;
+    bool none = false;
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
-      float v = s[n][0][0];
+      none |= m[n] == -INFINITY;
+      const float mb = m[n] == -INFINITY ? 0.f : m[n];
 #pragma unroll
-      for (int i = 1; i < 16; ++i) v = fmaxf(v, s[n][i >> 2][i & 3]);
-      mx[n] = xor32_max(xor16_max(v)) * a.scale_l2;
+      for (int i = 0; i < 8; ++i) {
+        w[n][i] = exp2_hw(fmaf(s[n][2 * x2 + (i >> 2)][i & 3], a.scale_l2, -mb));
+        top = max(top, __float_as_uint(w[n][i]));
+      }
     }
+    return __any(top > 0x43800000u || none);
   };
   // one tile's weights and their product; as its scores are used up, the next tile's take their place
   auto tile = [&](int t, auto more, auto last) {
     if constexpr (more) {
-      fetch(kr, (t + 2) * 64, gk);
-      fetch(vr, (t + 1) * 64, gv);
+      // K of tile t + 2 takes the place of tile t's, V of t + 1 that of t - 1's: both were last read
+      // before the barrier that began this tile
+      fetch(kbase, k0, ck, t + 2);
+      fetch(vbase, v0, cv, t + 1);
     }
     if (busy) {
       if constexpr (more) read_k(t + 1, 0);
-      bool up = false;
-#pragma unroll
-      for (int n = 0; n < NR; ++n) up |= mx[n] > m[n] + 8.f;
-      if (__any(up)) {
-#pragma unroll
-        for (int n = 0; n < NR; ++n) {
-          const float mn = fmaxf(m[n], mx[n]);
-          const float corr = mn == -INFINITY ? 0.f : exp2_hw(m[n] - mn);
-          m[n] = mn;
-          l[n] *= corr;
-#pragma unroll
-          for (int u = 0; u < D / 16; ++u) o[n][u] *= corr;
-        }
-      }
 #pragma unroll
       for (int x2 = 0; x2 < 2; ++x2) {
-        u32x4_t pp[NR], pr[NR];
-#pragma unroll
-        for (int x1 = 0; x1 < 2; ++x1) {
-          const int x = 2 * x2 + x1;
-          if constexpr (more)
-            if (x < 3) read_k(t + 1, x + 1);
-          if (x1 == 1) read_v(t, x2);
+        if (weigh(x2)) {   // the maximum moves, and what was summed against it
 #pragma unroll
           for (int n = 0; n < NR; ++n) {
-            const float mb = m[n] == -INFINITY ? 0.f : m[n];
+            const float mn = fmaxf(m[n], greatest(n, 2 * x2, 2 * x2 + 2));
+            const float corr = mn == -INFINITY ? 0.f : exp2_hw(m[n] - mn);
+            m[n] = mn;
+            l[n] *= corr;
 #pragma unroll
-            for (int y = 0; y < 2; ++y) {
-              const float a0 = exp2_hw(fmaf(s[n][x][2 * y], a.scale_l2, -mb));
-              const float a1 = exp2_hw(fmaf(s[n][x][2 * y + 1], a.scale_l2, -mb));
-              const uint32_t hi = perm(__float_as_uint(a1), __float_as_uint(a0), 0x07060302u);
-              pp[n][2 * x1 + y] = hi;
-              pr[n][2 * x1 + y] = pack_bf16x2_op(a0 - bf16lo(hi), a1 - bf16hi(hi));
-            }
+            for (int u = 0; u < D / 16; ++u) o[n][u] *= corr;
           }
-          if constexpr (more) score(x);
+          weigh(x2);
+        }
+        if constexpr (more) read_k(t + 1, 2 * x2 + 1);
+        read_v(t, x2);
+        u32x4_t pp[NR], pr[NR];
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const uint32_t hi = perm(__float_as_uint(w[n][2 * y + 1]), __float_as_uint(w[n][2 * y]), 0x07060302u);
+            pp[n][y] = hi;
+            pr[n][y] = pack_bf16x2_op(w[n][2 * y] - bf16lo(hi), w[n][2 * y + 1] - bf16hi(hi));
+          }
+        if constexpr (more) {
+          score(2 * x2);
+          if (x2 == 0) read_k(t + 1, 2);
+          score(2 * x2 + 1);
         }
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
@@ -260,22 +277,17 @@ __device__ __forceinline__ void part_wide(const PrefixArgs& a, const uint16_t* k
             o[n][u] = mfma_bf16(vf[u], pr[n], o[n][u]);
           }
       }
-      if constexpr (more) scored(t + 1, last);
+      if constexpr (more) mask(t + 1, last);
     }
     if constexpr (more) {
-      // K of tile t + 2 takes the place of tile t's, V of t + 1 that of t - 1's: both were last read
-      // before the barrier that began this tile
-      put_k(t + 2);
-      put_v(t + 1);
+      wait_vm();
       __syncthreads();
     }
   };
-  fetch(kr, 0, gk);
-  fetch(vr, 0, gv);
-  put_k(0);
-  put_v(0);
-  fetch(kr, 64, gk);
-  put_k(1);
+  fetch(kbase, k0, ck, 0);
+  fetch(vbase, v0, cv, 0);
+  fetch(kbase, k0, ck, 1);
+  wait_vm();
   __syncthreads();
   if (busy) {
 #pragma unroll
@@ -283,7 +295,9 @@ __device__ __forceinline__ void part_wide(const PrefixArgs& a, const uint16_t* k
       read_k(0, x);
       score(x);
     }
-    scored(0, std::true_type{});
+    mask(0, std::true_type{});
+#pragma unroll
+    for (int n = 0; n < NR; ++n) m[n] = greatest(n, 0, 4);
   }
   for (int t = 0; t + 2 < nt; ++t) tile(t, std::true_type{}, std::false_type{});
   if (nt > 1) tile(nt - 2, std::true_type{}, std::true_type{});
@@ -301,7 +315,7 @@ __device__ __forceinline__ void part_wide(const PrefixArgs& a, const uint16_t* k
 }
 
 template <int D, int NR>
-__global__ __launch_bounds__(256, 2) void prefix_parts_kernel(PrefixArgs a) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void prefix_parts_kernel(PrefixArgs a) {
   constexpr int kNarrow = (kPartWaves * 16 * D + 8 * 16) * 4;
   constexpr int kWide = 4 * 64 * D * 2;
   __shared__ __attribute__((aligned(16))) uint4 lds[(kNarrow > kWide ? kNarrow : kWide) / 16];
@@ -444,7 +458,9 @@ static PrefixPlan prefix_plan(int batch, int hq, int hkv, int d, int n_prefixes,
   p.tiles = (int)(most < batch ? most : batch);
   if (n_prefixes == 0 || max_prefix == 0) p.tiles = 0;
   if (p.tiles > 0)
-    cut_parts(max_prefix, 512 / ((long long)hkv * p.tiles), rows <= 16 ? kPartRound : 256, 64, &p.ns_pre, &p.chunk_pre);
+    // what the chip holds at once: three workgroups a compute unit with D = 64, two with 128
+    cut_parts(max_prefix, (d == 64 ? 768 : 512) / ((long long)hkv * p.tiles), rows <= 16 ? kPartRound : 256, 64,
+              &p.ns_pre, &p.chunk_pre);
   if (max_len > 0)
     cut_parts(max_len, 1024 / ((long long)hkv * batch), 256, kPartRound, &p.ns_own, &p.chunk_own);
   if (p.chunk_pre == 0) p.chunk_pre = 64;

@@ -76,3 +76,43 @@ def test_prefix_decode(dev, case):
     check(out, f32, want, mag)
     again = ops.gqa_prefix_decode(q, kp, vp, ints(plens), k, v, ints(lens), cu=cu)
     assert torch.equal(out, again)   # no order of arrival in it
+
+
+@pytest.mark.parametrize("b", [2, 20])
+def test_scores_that_rise(dev, b):
+    """Maxima that move late and far, by more than 2^8 at once and by little; scores of -inf and then far below
+    zero; rows of one workgroup that differ in all of that."""
+    from llmnputest_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(b)
+    n, d = 3000, 64
+    kp, vp = rows(g, 1, 2, n, d), rows(g, 1, 2, n, d)
+    kp[0, 0] *= torch.linspace(0.1, 3, n, device="cuda")[:, None]
+    kp[0, 0, 2500] *= 8
+    kp[0, 1, :200, 0] = float("-inf")          # -inf for every q whose first channel is positive
+    kp[0, 1, 200:, 0] = -300.0
+    q = rows(g, b, 8, d)
+    q[..., 0] = q[..., 0].abs() + 0.5
+    q[1] *= 0.01
+    none = torch.zeros((b, 2, 0, d), dtype=torch.bfloat16, device="cuda")
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    out, f32 = ops.gqa_prefix_decode(q, kp, vp, ints([n]), none, none, ints([0] * b), want_f32=True)
+    want, mag = reference(q, kp, vp, [n], none, none, [0] * b, [(0, b)], d ** -0.5)
+    # scores reach 2^9 here: 2^-24 of that, a few times, in the exponent
+    assert bool(((f32.double() - want).abs() <= 2.0 ** -11 * mag + 1e-30).all())
+    assert torch.equal(out, f32.to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("b", [1, 30])
+def test_nan_stays(dev, b):
+    """A NaN or an infinity of a key or a value that a row sees shows in it, and in no other group's rows."""
+    from llmnputest_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(7)
+    kp, vp = rows(g, 2, 1, 1500, 64), rows(g, 2, 1, 1500, 64)
+    kp[0, 0, 900, 3] = float("nan")
+    vp[1, 0, 1400, 5] = float("inf")
+    q, k, v = rows(g, 2 * b, 4, 64), rows(g, 2 * b, 1, 3, 64), rows(g, 2 * b, 1, 3, 64)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    out = ops.gqa_prefix_decode(q, kp, vp, ints([1500, 1500]), k, v, ints([3] * (2 * b)), cu=ints([0, b, 2 * b]))
+    assert bool(out[:b].isnan().all())
+    bad = ~out[b:].isfinite()
+    assert bool(bad[..., 5].all()) and not bool(bad[..., :5].any()) and not bool(bad[..., 6:].any())
