@@ -46,6 +46,13 @@ __device__ __forceinline__ float penalised(float x, float repetition, float freq
 // Rows need no alignment beyond their type's: 16-byte accesses of any address are single instructions here.
 typedef uint32_t u32x4_any_t __attribute__((ext_vector_type(4), aligned(2)));
 
+// Long calls (U = 4) stream past the caches (64 x 100353: 21.1 to 18.9 us).
+template <bool STREAM>
+__device__ __forceinline__ u32x4_any_t logit_load(const u32x4_any_t* p) {
+  if constexpr (STREAM) return __builtin_nontemporal_load(p);
+  else return *p;
+}
+
 // VEC values a load (16 bytes), U loads a thread, in flight together.
 template <typename T, int U>
 __global__ __launch_bounds__(kLogitThreads) void adjust_logits_kernel(LogitArgs a) {
@@ -67,7 +74,7 @@ __global__ __launch_bounds__(kLogitThreads) void adjust_logits_kernel(LogitArgs 
   for (int u = 0; u < U; ++u) {
     const int v = v0 + (u * kLogitThreads + tid) * VEC;
     if (v + VEC <= a.vocab) {
-      x[u].v = *(const u32x4_any_t*)(in + v);
+      x[u].v = logit_load<U == 4>((const u32x4_any_t*)(in + v));
     } else {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) x[u].e[i] = v + i < a.vocab ? in[v + i] : (T)0;
@@ -75,7 +82,7 @@ __global__ __launch_bounds__(kLogitThreads) void adjust_logits_kernel(LogitArgs 
 #pragma unroll
     for (int i = 0; i < VEC; i += 4) {
       if (cnt != nullptr && v + i + 4 <= a.vocab) {
-        const u32x4_any_t c = *(const u32x4_any_t*)(cnt + v + i);
+        const u32x4_any_t c = logit_load<U == 4>((const u32x4_any_t*)(cnt + v + i));
 #pragma unroll
         for (int k = 0; k < 4; ++k) n[u][i + k] = (int32_t)c[k];
       } else {
@@ -125,24 +132,28 @@ __global__ __launch_bounds__(kLogitThreads) void adjust_logits_kernel(LogitArgs 
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int at = (u * kLogitThreads + tid) * VEC, v = v0 + at;
+    float f[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      float f;
-      if constexpr (sizeof(T) == 2) f = bf16_to_f32(x[u].e[i]);
-      else f = x[u].e[i];
+      if constexpr (sizeof(T) == 2) f[i] = bf16_to_f32(x[u].e[i]);
+      else f[i] = x[u].e[i];
       const int32_t c = n[u][i];
-      if (c != 0) f = penalised(f, rep, freq, pres, c & 0x7fffffff);
-      if (biased) f += s_bias[at + i];
-      if (row >= 0 && !(may[u] >> i & 1u)) f = -INFINITY;
+      if (c != 0) f[i] = penalised(f[i], rep, freq, pres, c & 0x7fffffff);
+      if (biased) f[i] += s_bias[at + i];
+      if (row >= 0 && !(may[u] >> i & 1u)) f[i] = -INFINITY;
       if (v + i < a.vocab) {
-        const unsigned long long k = argmax_key(f, (uint32_t)(v + i));
+        const unsigned long long k = argmax_key(f[i], (uint32_t)(v + i));
         best = k > best ? k : best;
       }
-      if constexpr (sizeof(T) == 2) x[u].e[i] = f32_to_bf16(f);
-      else x[u].e[i] = f;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 2) x[u].v[i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
+      else x[u].v[i] = __float_as_uint(f[i]);
     }
     if (v + VEC <= a.vocab) {
-      *(u32x4_any_t*)(to + v) = x[u].v;
+      if constexpr (U == 4) __builtin_nontemporal_store(x[u].v, (u32x4_any_t*)(to + v));
+      else *(u32x4_any_t*)(to + v) = x[u].v;
     } else {
 #pragma unroll
       for (int i = 0; i < VEC; ++i)
@@ -202,11 +213,17 @@ __global__ __launch_bounds__(kCountThreads) void count_fresh_kernel(int32_t* cou
   const int span = min(kCountSpan, vocab - v0);
   for (int i = threadIdx.x; i < kCountSpan; i += kCountThreads) s[i] = 0;
   __syncthreads();
-  for (int i = from + (int)threadIdx.x; i < to; i += kCountThreads) {
-    const int t = tokens[i];
-    if (t < v0 || t - v0 >= span) continue;
-    if (prompt) atomicOr((unsigned*)s + (t - v0), 0x80000000u);
-    else atomicAdd(s + (t - v0), 1);
+  constexpr int U = 8;   // in flight (one at a time, 8 lists of 4096 took 8.1 us of 6.9)
+  for (int i0 = from + (int)threadIdx.x; i0 < to; i0 += U * kCountThreads) {
+    int t[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) t[u] = i0 + u * kCountThreads < to ? tokens[i0 + u * kCountThreads] : -1;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (t[u] < v0 || t[u] - v0 >= span) continue;
+      if (prompt) atomicOr((unsigned*)s + (t[u] - v0), 0x80000000u);
+      else atomicAdd(s + (t[u] - v0), 1);
+    }
   }
   __syncthreads();
   int32_t* const row = counts + (int64_t)b * stride + v0;
