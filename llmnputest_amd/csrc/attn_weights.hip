@@ -104,15 +104,17 @@ __global__ __launch_bounds__(256) void weight_sum_kernel(WeightArgs a, int spans
   const int p0 = span * kWeightSpan + tid;
   // scores and old weights are on their way before the length is known (within the buffers; those behind
   // it are left out)
-  const float* scores = a.scores + (size_t)bk * a.G * a.score_stride;
+  const __amdgpu_buffer_rsrc_t scores =
+      make_rsrc(a.scores + (size_t)bk * a.G * a.score_stride, (uint32_t)(a.G * a.score_stride * 4));
   float* to = a.weights + (size_t)b * a.w_b_stride + (size_t)kvh * a.w_h_stride;
   float s[GH][P], w[P], old[P];
-  auto load = [&](int h0) {
+  auto load = [&](int h0) {   // heads that are none read zeros, outside the buffer
 #pragma unroll
     for (int g = 0; g < GH; ++g)
 #pragma unroll
       for (int i = 0; i < P; ++i)
-        s[g][i] = h0 + g < a.G ? scores[(h0 + g) * a.score_stride + min(p0 + 256 * i, a.max_len - 1)] : 0.f;
+        s[g][i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
+                                                scores, ((h0 + g) * (int)a.score_stride + p0 + 256 * i) * 4, 0, 0));
   };
   load(0);
 #pragma unroll
