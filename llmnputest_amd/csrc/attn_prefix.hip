@@ -458,8 +458,10 @@ static PrefixPlan prefix_plan(int batch, int hq, int hkv, int d, int n_prefixes,
   p.tiles = (int)(most < batch ? most : batch);
   if (n_prefixes == 0 || max_prefix == 0) p.tiles = 0;
   if (p.tiles > 0)
-    // what the chip holds at once: three workgroups a compute unit with D = 64, two with 128
-    cut_parts(max_prefix, (d == 64 ? 768 : 512) / ((long long)hkv * p.tiles), rows <= 16 ? kPartRound : 256, 64,
+    // D = 64: what the chip holds at once, three workgroups a compute unit (256 x 16384: 384 / 512 / 640 / 768 /
+    // 1024 took 119 / 94 / 96 / 91 / 95 us). D = 128: less, beside the own caches' parts (48 x 5003: 384 / 512 /
+    // 768 / 1024 took 30.4 / 32.0 / 32.3 / 34.2)
+    cut_parts(max_prefix, (d == 64 ? 768 : 384) / ((long long)hkv * p.tiles), rows <= 16 ? kPartRound : 256, 64,
               &p.ns_pre, &p.chunk_pre);
   if (max_len > 0)
     cut_parts(max_len, 1024 / ((long long)hkv * batch), 256, kPartRound, &p.ns_own, &p.chunk_own);

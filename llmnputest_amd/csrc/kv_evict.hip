@@ -72,24 +72,22 @@ __device__ __forceinline__ int wave_scan(int v) {
 
 // The waves take equal shares of the positions in a row, at most KPT * 64 each. HELD: that is all of them,
 // and their keys stay in registers; otherwise each pass reads the weights again, KPT * 1024 at a time.
-template <int KPT, bool HELD>
-__global__ __launch_bounds__(kPickThreads) void evict_pick_kernel(EvictArgs a) {
+// put(i, p): kept position i is p.
+template <int KPT, bool HELD, typename Put>
+__device__ __forceinline__ void evict_pick(const EvictArgs& a, int bk, int n, Put put) {
   __shared__ __attribute__((aligned(16))) int s_hist[kPickBins * kPickCopies];
   __shared__ int s_sum[kPickWaves], s_gt[kPickWaves], s_eq[kPickWaves];
   __shared__ uint32_t s_key;
   __shared__ int s_left;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int bk = blockIdx.x, b = bk / a.hkv, h = bk - b * a.hkv;
-  const int n = min(max(a.lens[b], 0), a.max_len);
-  int32_t* kept = a.kept + (size_t)bk * a.budget;
-  if (tid == 0) a.n_old[bk] = n;
+  const int b = bk / a.hkv, h = bk - b * a.hkv;
   if (n <= a.budget) {
-    for (int i = tid; i < a.budget; i += kPickThreads) kept[i] = i < n ? i : -1;
+    for (int i = tid; i < a.budget; i += kPickThreads) put(i, i < n ? i : -1);
     return;
   }
   const int old = n - a.recent, want = a.budget - a.recent;   // want < old
-  for (int i = tid; i < a.recent; i += kPickThreads) kept[want + i] = old + i;
+  for (int i = tid; i < a.recent; i += kPickThreads) put(want + i, old + i);
   if (want == 0) return;
   const float* w = a.weights + (size_t)b * a.w_b_stride + (size_t)h * a.w_h_stride;
 
@@ -190,11 +188,20 @@ __global__ __launch_bounds__(kPickThreads) void evict_pick_kernel(EvictArgs a) {
       const uint64_t same = __ballot(key[i] == found);
       const bool take = key[i] > found || (key[i] == found && seen + __popcll(same & below) < left);
       const uint64_t who = __ballot(take);
-      if (take) kept[at + __popcll(who & below)] = p0 + first + 64 * i + lane;
+      if (take) put(at + __popcll(who & below), p0 + first + 64 * i + lane);
       at += __popcll(who);
       seen += __popcll(same);
     }
   }
+}
+
+template <int KPT, bool HELD>
+__global__ __launch_bounds__(kPickThreads) void evict_pick_kernel(EvictArgs a) {
+  const int bk = blockIdx.x;
+  const int n = min(max(a.lens[bk / a.hkv], 0), a.max_len);
+  if (threadIdx.x == 0) a.n_old[bk] = n;
+  int32_t* const kept = a.kept + (size_t)bk * a.budget;
+  evict_pick<KPT, HELD>(a, bk, n, [&](int i, int p) { kept[i] = p; });
 }
 
 // ---- by parts of 4096 positions, 256 threads each: a wave holds 1024 of them in a row
@@ -517,19 +524,15 @@ __device__ __forceinline__ void turn_back(uint4& a, uint4& z, const float* cs, i
 
 constexpr int kMoveThreads = 512;
 
-// kMoveThreads / (D / 16) rows of K (`which` 0) or V (1) a step: two 16-byte pieces a thread.
-template <int D, bool IN_PLACE>
-__global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a) {
-  constexpr int L = D / 16, STEP = kMoveThreads / L;   // threads of a row, rows of a step
+// The rows of K (`which` 0) or V (1) and with V's the weights, TH / (D / 16) of them a step, two 16-byte pieces
+// a thread; workgroup `block` of `blocks`, in place one for all. n: the old length.
+template <int D, bool IN_PLACE, int TH>
+__device__ __forceinline__ void evict_move(const EvictArgs& a, int bk, int n, int which, int block, int blocks,
+                                           const int32_t* kept) {
+  constexpr int L = D / 16, STEP = TH / L;   // threads of a row, rows of a step
   const int tid = threadIdx.x, c = tid % L, sub = tid / L;
-  int blk = blockIdx.x;
-  const int which = blk & 1;
-  blk >>= 1;
-  const int bk = blk / a.blocks, block = blk % a.blocks;
   const int b = bk / a.hkv, h = bk - b * a.hkv;
-  const int n = a.n_old[bk], m = min(n, a.budget);
-  const int32_t* kept = a.kept + (size_t)bk * a.budget;
-  if (which == 1 && block == 0 && h == 0 && tid == 0) a.lens_out[b] = m;
+  const int m = min(n, a.budget);
   if (IN_PLACE && n <= a.budget) return;
   const uint16_t* from = (which ? a.v : a.k) + (size_t)b * a.b_stride + (size_t)h * a.h_stride;
   uint16_t* to = (which ? a.v_out : a.k_out) + (size_t)b * a.ob_stride + (size_t)h * a.oh_stride;
@@ -539,55 +542,84 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a) {
   // K's second piece is half a row on (its partner of a rotation), V's the next sixteen bytes
   const int e0 = which ? 16 * c : 8 * c, e1 = which ? 16 * c + 8 : D / 2 + 8 * c;
 
-  uint4 x[2];
-  float ws = 0.f;
-  int src = 0;
-  auto load = [&](int i0, int& s_, uint4 (&r)[2], float& wv) {
+  struct Row {
+    int src;
+    uint4 x[2];
+    float w;
+  };
+  auto load = [&](int i0, Row& r) {
     const int i = i0 + sub;
-    s_ = i < m ? kept[i] : -1;
-    if (s_ >= 0) {
-      r[0] = *(const uint4*)(from + (size_t)s_ * D + e0);
-      r[1] = *(const uint4*)(from + (size_t)s_ * D + e1);
-      if (which && c == 0) wv = w[s_];
+    r.src = i < m ? kept[i] : -1;
+    if (r.src >= 0) {
+      r.x[0] = *(const uint4*)(from + (size_t)r.src * D + e0);
+      r.x[1] = *(const uint4*)(from + (size_t)r.src * D + e1);
+      if (which && c == 0) r.w = w[r.src];
     }
   };
-  auto store = [&](int i0, int s_, uint4 (&r)[2], float wv) {
+  auto store = [&](int i0, Row& r) {
     const int i = i0 + sub;
-    if (s_ < 0) return;
-    if (turn && s_ != i) turn_back(r[0], r[1], a.tab + (size_t)(s_ - i) * D, D / 2, c);
-    *(uint4*)(to + (size_t)i * D + e0) = r[0];
-    *(uint4*)(to + (size_t)i * D + e1) = r[1];
-    if (which && c == 0) w_to[i] = wv;
+    if (r.src < 0) return;
+    if (turn && r.src != i) turn_back(r.x[0], r.x[1], a.tab + (size_t)(r.src - i) * D, D / 2, c);
+    *(uint4*)(to + (size_t)i * D + e0) = r.x[0];
+    *(uint4*)(to + (size_t)i * D + e1) = r.x[1];
+    if (which && c == 0) w_to[i] = r.w;
   };
+  Row r;
   if constexpr (!IN_PLACE) {
-    for (int i0 = block * STEP; i0 < m; i0 += a.blocks * STEP) {
-      load(i0, src, x, ws);
-      store(i0, src, x, ws);
+    for (int i0 = block * STEP; i0 < m; i0 += blocks * STEP) {
+      load(i0, r);
+      store(i0, r);
     }
     if (which)
-      for (int i = m + block * kMoveThreads + tid; i < a.room; i += a.blocks * kMoveThreads) w_to[i] = 0.f;
-    return;
+      for (int i = m + block * TH + tid; i < a.room; i += blocks * TH) w_to[i] = 0.f;
+  } else {
+    // the next step's rows are read before this step's are written
+    Row next;
+    load(0, r);
+    for (int i0 = 0; i0 < m; i0 += STEP) {
+      next.src = -1;
+      if (i0 + STEP < m) load(i0 + STEP, next);
+      wait_vm();          // this step's rows have been read by every thread before any is written
+      __syncthreads();
+      store(i0, r);
+      r = next;
+    }
+    if (which) {
+      wait_vm();
+      __syncthreads();
+      for (int i = m + tid; i < n; i += TH) w_to[i] = 0.f;
+    }
   }
-  // in place, one workgroup for all rows: the next step's rows are read before this step's are written
-  uint4 y[2];
-  float ws2 = 0.f;
-  int src2 = 0;
-  load(0, src, x, ws);
-  for (int i0 = 0; i0 < m; i0 += STEP) {
-    if (i0 + STEP < m) load(i0 + STEP, src2, y, ws2);
-    wait_vm();          // this step's rows have been read by every thread before any is written
-    __syncthreads();
-    store(i0, src, x, ws);
-    src = src2;
-    x[0] = y[0];
-    x[1] = y[1];
-    ws = ws2;
-  }
-  if (which) {
-    wait_vm();
-    __syncthreads();
-    for (int i = m + tid; i < n; i += kMoveThreads) w_to[i] = 0.f;
-  }
+}
+
+template <int D, bool IN_PLACE>
+__global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a) {
+  int blk = blockIdx.x;
+  const int which = blk & 1;
+  blk >>= 1;
+  const int bk = blk / a.blocks, block = blk % a.blocks;
+  const int n = a.n_old[bk];
+  if (which == 1 && block == 0 && bk % a.hkv == 0 && threadIdx.x == 0) a.lens_out[bk / a.hkv] = min(n, a.budget);
+  evict_move<D, IN_PLACE, kMoveThreads>(a, bk, n, which, block, a.blocks, a.kept + (size_t)bk * a.budget);
+}
+
+// Short caches cut down to few rows: a workgroup picks its (sequence, kv head)'s and moves them. The lengths
+// stay as they are until the last workgroup of a sequence has read its own.
+constexpr int kWholeRows = 1024;
+template <int D, bool IN_PLACE>
+__global__ __launch_bounds__(kPickThreads) void evict_whole_kernel(EvictArgs a) {
+  __shared__ int32_t s_kept[kWholeRows];
+  const int bk = blockIdx.x, b = bk / a.hkv;
+  const int n = min(max(a.lens[b], 0), a.max_len);
+  int32_t* const kept = a.kept + (size_t)bk * a.budget;
+  evict_pick<4, true>(a, bk, n, [&](int i, int p) {
+    kept[i] = p;
+    if (i < kWholeRows) s_kept[i] = p;
+  });
+  __syncthreads();
+  if (threadIdx.x == 0 && ticket(a.counters + b, a.hkv)) a.lens_out[b] = min(n, a.budget);
+  evict_move<D, IN_PLACE, kPickThreads>(a, bk, n, 0, 0, 1, s_kept);
+  evict_move<D, IN_PLACE, kPickThreads>(a, bk, n, 1, 0, 1, s_kept);
 }
 
 static bool evict_shape_ok(int batch, int hkv, int d, int max_len, int budget, int recent) {
@@ -686,11 +718,20 @@ int q4nx_kv_evict(const uint16_t* k_cache, const uint16_t* v_cache, int64_t kv_b
   a.budget = budget;
   a.recent = recent;
   a.room = room;
+  hipStream_t s = (hipStream_t)stream;
+  // 1 x 1000 to 512 in one launch: 13.3 us a pass, 16.2 in two; more rows go faster by more workgroups than one
+  if (max_len <= kPickPart && most <= kWholeRows && batch <= Q4NX_WS_COUNTER_BYTES / 4) {
+    const dim3 grid((unsigned)bh), threads(kPickThreads);
+    if (head_dim == 64 && in_place) hipLaunchKernelGGL((evict_whole_kernel<64, true>), grid, threads, 0, s, a);
+    else if (head_dim == 64) hipLaunchKernelGGL((evict_whole_kernel<64, false>), grid, threads, 0, s, a);
+    else if (in_place) hipLaunchKernelGGL((evict_whole_kernel<128, true>), grid, threads, 0, s, a);
+    else hipLaunchKernelGGL((evict_whole_kernel<128, false>), grid, threads, 0, s, a);
+    return check_launch(what);
+  }
   const int step = kMoveThreads / (head_dim / 16);
   a.blocks = in_place ? 1 : (most + step - 1) / step;
   if (a.blocks > 4096) a.blocks = 4096;
   Q4NX_REQUIRE(2ll * bh * a.blocks < (1ll << 31) && (long long)bh * parts < (1ll << 31), Q4NX_ERR_SHAPE, "%s: more than 2^31 workgroups", what);
-  hipStream_t s = (hipStream_t)stream;
   if (parts > 0) {
     const dim3 all((unsigned)(bh * parts)), threads(kPartThreads);
     hipLaunchKernelGGL(evict_hist_kernel, all, threads, 0, s, a);
