@@ -327,3 +327,73 @@ def test_empty_and_bounded(dev):
     counts = torch.ones((2, 9), dtype=torch.int32, device="cuda")
     ops.count_tokens(counts, n(), n(0, 0, 0))
     assert bool((counts == 1).all())
+
+
+def test_rules_on_the_q4_cache(weights):
+    """The rules go with either cache."""
+    rules = TokenRules(2, CFG.vocab, frequency=100.0)
+    dec = GraniteDecoder(weights, 2, 128, kv="q4", rules=rules)
+    dec.seed_cache(40, seed=1)
+    toks, _ = dec.generate([1, 2], [40, 30], 30)
+    assert all(len(set(t)) == 30 for t in toks.tolist())     # nothing is said twice
+
+
+def test_a_table_of_masks(dev):
+    """Sequences that move through a grammar's states between calls."""
+    v = 100
+    table = torch.zeros((3, 4), dtype=torch.int32, device="cuda")
+    table[0, 0], table[1, 1], table[2, 3] = 1 << 5, 1 << 3, 1 << 2      # tokens 5, 35, 98
+    rules = TokenRules(2, v, masks=table)
+    x = torch.randn((2, v), device="cuda")
+    for a, b, want in ((0, 1, [5, 35]), (2, 0, [98, 5]), (-1, 2, [int(x[0].argmax()), 98])):
+        rules.mask_rows.copy_(ints([a, b]))
+        assert rules.apply(x)[1].tolist() == want
+
+
+LONG = 16_000_000   # positions: rows behind 2^31 bytes, 3907 parts of a selection
+
+
+def test_long_attention(dev):
+    """Equal scores over a cache of 4 GiB: every position is given the same, and the answer is V's mean."""
+    k = torch.zeros((1, 2, LONG, 64), dtype=torch.bfloat16, device="cuda")
+    v = torch.zeros_like(k)
+    v[:, 0], v[:, 1, LONG // 2:] = 2.0, 1.0
+    k[:, 1, LONG - 7:] = 0
+    q = torch.ones((1, 4, 64), dtype=torch.bfloat16, device="cuda")
+    n = LONG - 5
+    v[:, :, n:] = float("nan")
+    want = torch.tensor([2.0, (n - LONG // 2) / n], device="cuda").repeat_interleave(2)[None, :, None].expand(1, 4, 64)
+    w = torch.full((1, 2, LONG), 9.0, device="cuda")
+    out = ops.gqa_decode_weights(q, k, v, ints([n]), w, start=True, want_f32=True)[1]
+    # fp32 sums of 2^19 equal terms a part and wave: a relative 2^-24 for each of up to 2^14 additions
+    assert torch.allclose(out, want, rtol=2.0 ** -10, atol=0)
+    assert torch.allclose(w[..., :n], torch.full_like(w[..., :n], 2 / n), rtol=2.0 ** -10, atol=0)
+    assert bool((w[..., n:] == 9).all())
+    none = torch.zeros((3, 2, 0, 64), dtype=torch.bfloat16, device="cuda")
+    out = ops.gqa_prefix_decode(q.expand(3, 4, 64).contiguous(), k, v, ints([n]), none, none, ints([0, 0, 0]), want_f32=True)[1]
+    assert torch.allclose(out, want.expand(3, 4, 64), rtol=2.0 ** -10, atol=0)
+    many = ops.gqa_prefix_decode(q.expand(30, 4, 64).contiguous(), k, v, ints([n]), none[:1].expand(30, 2, 0, 64).contiguous(),
+                                 none[:1].expand(30, 2, 0, 64).contiguous(), torch.zeros(30, dtype=torch.int32, device="cuda"),
+                                 want_f32=True)[1]
+    assert torch.allclose(many, want.expand(30, 4, 64), rtol=2.0 ** -10, atol=0)
+
+
+@pytest.mark.parametrize("kind", ["random", "few values"])
+def test_long_eviction(dev, kind):
+    """A selection by 3907 parts, weights apart and much alike, and rows from behind 2^31 bytes."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    k = torch.zeros((1, 2, LONG, 64), dtype=torch.bfloat16, device="cuda")
+    k[0, 0, :, 0] = torch.arange(LONG, device="cuda") % 251
+    k[0, 1, :, 1] = torch.arange(LONG, device="cuda") % 241
+    w = torch.rand((1, 2, LONG), device="cuda", generator=g)
+    if kind == "few values":
+        w = (w * 3).floor()
+    n, budget, recent = LONG - 9, 5000, 77
+    into = tuple(torch.zeros(s, dtype=t, device="cuda") for s, t in (
+        ((1, 2, budget, 64), torch.bfloat16), ((1, 2, budget, 64), torch.bfloat16), ((1, 2, budget), torch.float32), ((1,), torch.int32)))
+    kept = ops.kv_evict(k, k.view_as(k), w, ints([n]), budget, recent, into=into).long()
+    for h in range(2):
+        order = torch.sort(w[0, h, :n - recent], descending=True, stable=True).indices[:budget - recent].sort().values
+        want = torch.cat((order, torch.arange(n - recent, n, device="cuda")))
+        assert torch.equal(kept[0, h], want)
+        assert torch.equal(into[0][0, h], k[0, h, want]) and torch.equal(into[2][0, h], w[0, h, want])
