@@ -303,14 +303,14 @@ int q4nx_gqa_decode_records(const uint16_t *q, const uint16_t *k_cache,
  * out[b][h] = softmax(scale * [Kpre; Kown] q) [Vpre; Vown]. Prefix p's rows are
  * k_prefix + p * prefix_stride + kv_head * prefix_h_stride + l * head_dim for l < prefix_lens[p]
  * (at most max_prefix); they are read once for all sequences cu[p] .. cu[p+1] - 1 (int32
- * [n_prefixes + 1], not falling; NULL: one prefix for all). A sequence in no such range has no prefix.
+ * [n_prefixes + 1], not falling, taken as at most batch; NULL: one prefix for all). A prefix may have no
+ * sequence; a sequence in no such range has no prefix.
  * Own rows as in q4nx_qkv_rope, l < lens[b] (at most max_len; 0: none, the caches may be NULL). Query
  * head h reads kv head h / (Hq/Hkv), Hq/Hkv <= 16; head_dim 64 or 128; scale >= 0. A sequence that sees
  * nothing gives zeros. q, out: [batch][Hq][head_dim]; caches bf16, 16-byte aligned, strides in elements,
- * multiples of 8. Softmax weights enter the products as two
- * bf16 terms (2^-15 of a weight may be lost). |v| times the
- * positions seen has to stay below 2^112. No reference counterpart: its attention reads one sequence's cache
- * (designs/granite_gemv/granite_attention.h:221-237).
+ * multiples of 8. Softmax weights enter the products as two bf16 terms (2^-15 of a weight may be lost).
+ * |v| times the positions seen has to stay below 2^112. No reference counterpart: its attention reads one
+ * sequence's cache (designs/granite_gemv/granite_attention.h:221-237).
  * ws: q4nx_gqa_prefix_decode_ws_bytes(...) bytes (0: a shape that is not taken). */
 size_t q4nx_gqa_prefix_decode_ws_bytes(int batch, int n_q_heads, int n_kv_heads, int head_dim,
                                        int n_prefixes, int max_prefix, int max_len);

@@ -128,6 +128,8 @@ def main(argv: list[str]) -> int:
     dec.generate(first, [a.ctx] * a.batch, min(2, a.new))   # capture the step graph
     if rules is not None:
         rules.begin([[x] for x in first])
+    for t in dec.weights or ():                         # nor do its tokens count here
+        t.zero_()
     print(f"ready    {time.time() - t0:.1f}s\n")
 
     torch.cuda.synchronize()

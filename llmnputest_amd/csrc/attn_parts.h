@@ -258,7 +258,8 @@ __device__ __forceinline__ void put_channels(uint16_t* out, float* out_f32, size
   if (out_f32) *(float4*)(out_f32 + at) = A;
 }
 
-// Parts of at least `unit` positions that len (< 2^24) is cut in, about `want` of them, and the positions of one, a multiple of `step`.
+// Parts of at least `unit` positions that len (< 2^24) is cut in, about `want` of them, and the positions of
+// one, a multiple of `step`.
 static inline void cut_parts(int len, long long want, int unit, int step, int* ns, int* chunk) {
   int n = want < 1 ? 1 : want > kMaxParts ? kMaxParts : (int)want;
   if (n > (len + unit - 1) / unit) n = (len + unit - 1) / unit;

@@ -136,7 +136,8 @@ __device__ __forceinline__ void part_wide(const PrefixArgs& a, const uint16_t* k
   const uint32_t v0 = k0 + 2 * 64 * C * 16;
   const int nt = (end + 63) / 64;
   const int row_of = tid / C;   // of this lane's first piece; the others are 256 / C rows on each
-  const uint32_t ck = (uint32_t)((swz_k<D>(row_of, tid % C) % C) * 16), cv = (uint32_t)((swz_v<D>(row_of, tid % C) % C) * 16);
+  const uint32_t ck = (uint32_t)((swz_k<D>(row_of, tid % C) % C) * 16);
+  const uint32_t cv = (uint32_t)((swz_v<D>(row_of, tid % C) % C) * 16);
   auto fetch = [&](const uint16_t* base, uint32_t lds0, uint32_t c, int t) {
     if (t >= nt) return;
     const uint16_t* const from = base + (size_t)t * 64 * D;
@@ -453,7 +454,7 @@ static PrefixPlan prefix_plan(int batch, int hq, int hkv, int d, int n_prefixes,
   // 32 rows a wave where prefixes have more than 64 of them on average and the registers hold it
   p.nr = d == 64 && rows > 64ll * (n_prefixes > 1 ? n_prefixes : 1) ? 2 : 1;
   const int rt = 64 * p.nr;
-  // every prefix may end inside a tile
+  // every prefix may end inside a tile; a tile has a member at least (prefixes may have none)
   const long long most = (rows + rt - 1) / rt + (n_prefixes > 0 ? n_prefixes - 1 : 0);
   p.tiles = (int)(most < batch ? most : batch);
   if (n_prefixes == 0 || max_prefix == 0) p.tiles = 0;
@@ -472,8 +473,8 @@ static PrefixPlan prefix_plan(int batch, int hq, int hkv, int d, int n_prefixes,
 
 static bool prefix_shape_ok(int batch, int hq, int hkv, int d, int n_prefixes, int max_prefix, int max_len) {
   return batch >= 1 && batch <= (1 << 20) && hkv >= 1 && hkv <= 1024 && hq >= hkv && hq % hkv == 0 && hq / hkv <= 16 &&
-         (d == 64 || d == 128) && n_prefixes >= 0 && n_prefixes <= batch && max_prefix >= 0 && max_prefix < (1 << 24) &&
-         max_len >= 0 && max_len < (1 << 24) && (long long)batch * hq < (1 << 28);
+         (d == 64 || d == 128) && n_prefixes >= 0 && n_prefixes <= (1 << 20) && max_prefix >= 0 &&
+         max_prefix < (1 << 24) && max_len >= 0 && max_len < (1 << 24) && (long long)batch * hq < (1 << 28);
 }
 
 static size_t prefix_rec_bytes(const PrefixPlan& p, int batch, int hq, int d) {
@@ -520,7 +521,7 @@ int q4nx_gqa_prefix_decode(const uint16_t* q, const uint16_t* k_prefix, const ui
   Q4NX_REQUIRE(prefix_shape_ok(batch, n_q_heads, n_kv_heads, head_dim, n_prefixes, max_prefix, max_len),
                Q4NX_ERR_SHAPE,
                "%s: batch=%d Hq=%d (a multiple of Hkv, at most 16 times) Hkv=%d head_dim=%d (64, 128) "
-               "n_prefixes=%d (at most batch) max_prefix=%d max_len=%d (below 2^24)",
+               "n_prefixes=%d (at most 2^20) max_prefix=%d max_len=%d (below 2^24)",
                what, batch, n_q_heads, n_kv_heads, head_dim, n_prefixes, max_prefix, max_len);
   const bool pre = n_prefixes > 0 && max_prefix > 0, own = max_len > 0;
   Q4NX_REQUIRE(q && lens && (out || out_f32) && (!own || (k_cache && v_cache)) &&

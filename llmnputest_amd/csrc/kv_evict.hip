@@ -129,7 +129,8 @@ __device__ __forceinline__ void evict_pick(const EvictArgs& a, int bk, int n, Pu
     each([&] {
 #pragma unroll
       for (int i = 0; i < KPT; ++i)
-        if (64 * i < share && key[i] != 0 && (key[i] & known) == found) atomicAdd(&s_hist[((key[i] >> shift) & mask) * kPickCopies + lane % kPickCopies], 1);
+        if (64 * i < share && key[i] != 0 && (key[i] & known) == found)
+          atomicAdd(&s_hist[((key[i] >> shift) & mask) * kPickCopies + lane % kPickCopies], 1);
     });
     __syncthreads();
     // the bin where the sum from the greatest on reaches `left`: two bins a thread, the greatest first
@@ -731,7 +732,8 @@ int q4nx_kv_evict(const uint16_t* k_cache, const uint16_t* v_cache, int64_t kv_b
   const int step = kMoveThreads / (head_dim / 16);
   a.blocks = in_place ? 1 : (most + step - 1) / step;
   if (a.blocks > 4096) a.blocks = 4096;
-  Q4NX_REQUIRE(2ll * bh * a.blocks < (1ll << 31) && (long long)bh * parts < (1ll << 31), Q4NX_ERR_SHAPE, "%s: more than 2^31 workgroups", what);
+  Q4NX_REQUIRE(2ll * bh * a.blocks < (1ll << 31) && (long long)bh * parts < (1ll << 31), Q4NX_ERR_SHAPE,
+               "%s: more than 2^31 workgroups", what);
   if (parts > 0) {
     const dim3 all((unsigned)(bh * parts)), threads(kPartThreads);
     hipLaunchKernelGGL(evict_hist_kernel, all, threads, 0, s, a);

@@ -263,9 +263,9 @@ int q4nx_count_tokens(int32_t* counts, int64_t count_stride, int vocab, int batc
 int q4nx_adjust_logits(const void* logits, int bf16, int64_t stride, void* out, int64_t out_stride, int vocab,
                        int batch, const int32_t* counts, int64_t count_stride, const float* repetition,
                        const float* presence, const float* frequency, const int32_t* bias_ids,
-                       const float* bias_values, int n_biases, const int32_t* bias_cu, const uint32_t* mask, int64_t mask_stride,
-                       int n_mask, const int32_t* mask_rows, int32_t* tokens, uint64_t* keys, void* ws,
-                       size_t ws_bytes, void* stream) {
+                       const float* bias_values, int n_biases, const int32_t* bias_cu, const uint32_t* mask,
+                       int64_t mask_stride, int n_mask, const int32_t* mask_rows, int32_t* tokens,
+                       uint64_t* keys, void* ws, size_t ws_bytes, void* stream) {
   const char* what = "q4nx_adjust_logits";
   Q4NX_REQUIRE(logits && out, Q4NX_ERR_ARG, "%s: logits and out are required", what);
   Q4NX_REQUIRE(vocab >= 1 && vocab <= (1 << 28) && batch >= 1 && batch <= Q4NX_WS_COUNTER_BYTES / 16 &&

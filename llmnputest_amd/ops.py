@@ -654,8 +654,8 @@ def gqa_prefix_decode(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.T
                       ws: Workspace | None = None):
     """GQA attention of one token per sequence, q bf16 [B, Hq, D], over a prefix that sequences share
     (its rows are read once for all of them) and over each one's own cache. k_prefix, v_prefix bf16
-    [P, Hkv, Lp, D] with prefix_lens int32 [P]; sequences cu[p] .. cu[p+1] - 1 (int32 [P + 1]; default:
-    one prefix for all) go on from prefix p, others have none. Own rows bf16 [B, Hkv, L, D], lens int32
+    [P, Hkv, Lp, D] with prefix_lens int32 [P]; sequences cu[p] .. cu[p+1] - 1 (int32 [P + 1], not
+    falling, beyond B as B; default: one prefix for all) go on from prefix p, others have none. Own rows bf16 [B, Hkv, L, D], lens int32
     [B] (without the prefix; 0: none). D 64 or 128, Hq/Hkv at most 16, scale (default D ** -0.5) not
     negative. max_prefix, max_len: at least the longest lengths (fewer read fewer positions; default the
     caches'). Returns bf16 [B, Hq, D] (and the fp32 copy when want_f32)."""

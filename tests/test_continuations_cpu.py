@@ -41,7 +41,7 @@ LOGITS = dict(x=AT, bf16=0, stride=100, out=AT, os=100, vocab=100, b=4, counts=A
     (dict(v=None), ERR_ARG), (dict(plens=None), ERR_ARG), (dict(cu=None), ERR_ARG), (dict(q=AT + 8), ERR_ARG),
     (dict(k=AT + 8), ERR_ARG), (dict(vp=AT + 2), ERR_ARG), (dict(out=AT + 4), ERR_ARG), (dict(of=AT + 8), ERR_ARG),
     (dict(scale=-0.1), ERR_ARG), (dict(scale=float("nan")), ERR_ARG), (dict(b=0), ERR_SHAPE), (dict(hq=41), ERR_SHAPE),
-    (dict(hq=136), ERR_SHAPE), (dict(hkv=0), ERR_SHAPE), (dict(d=96), ERR_SHAPE), (dict(p=5), ERR_SHAPE),
+    (dict(hq=136), ERR_SHAPE), (dict(hkv=0), ERR_SHAPE), (dict(d=96), ERR_SHAPE), (dict(p=(1 << 20) + 1), ERR_SHAPE),
     (dict(p=-1), ERR_SHAPE), (dict(most_p=-1), ERR_SHAPE), (dict(most=1 << 24), ERR_SHAPE), (dict(most=51), ERR_SHAPE),
     (dict(most_p=101), ERR_SHAPE), (dict(hs=50 * 64 + 4), ERR_SHAPE), (dict(bs=50 * 64), ERR_SHAPE),
     (dict(ps=100 * 64), ERR_SHAPE), (dict(ws=None), ERR_WS), (dict(wn=1000), ERR_WS), (dict(ws=AT + 16), ERR_WS)])
@@ -97,7 +97,7 @@ def test_workspaces():
     size = lib.q4nx_gqa_prefix_decode_ws_bytes
     assert size(4, 40, 8, 64, 2, 1000, 500) >= 65536 + 4 * 40 * 2 * 68 * 4      # a part of each kind
     assert size(4, 40, 8, 64, 0, 0, 0) == 65536 and size(1, 8, 8, 128, 1, 1024, 0) == 65536   # one launch
-    for bad in ((0, 40, 8, 64, 1, 1, 1), (4, 40, 7, 64, 1, 1, 1), (4, 40, 8, 65, 1, 1, 1), (4, 40, 8, 64, 5, 1, 1)):
+    for bad in ((0, 40, 8, 64, 1, 1, 1), (4, 40, 7, 64, 1, 1, 1), (4, 40, 8, 65, 1, 1, 1), (4, 40, 8, 64, -1, 1, 1)):
         assert size(*bad) == 0
     size = lib.q4nx_gqa_decode_weights_ws_bytes
     # scores of the longest length, and records

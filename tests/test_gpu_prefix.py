@@ -116,3 +116,20 @@ def test_nan_stays(dev, b):
     assert bool(out[:b].isnan().all())
     bad = ~out[b:].isfinite()
     assert bool(bad[..., 5].all()) and not bool(bad[..., :5].any()) and not bool(bad[..., 6:].any())
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_more_prefixes_than_sequences(dev, d):
+    """The first sequences of a larger batch: prefixes without members, before, between and behind theirs."""
+    from llmnputest_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(d)
+    plens, edges = [1100 + 7 * i for i in range(70)], [0, 0, 0, 2] + [2] * 60 + [6, 9, 30, 31, 32, 33, 40]
+    kp, vp = rows(g, 70, 2, max(plens), d), rows(g, 70, 2, max(plens), d)
+    lens = [0, 3, 9, 140, 1, 2, 5]
+    k, v, q = rows(g, 7, 2, 140, d), rows(g, 7, 2, 140, d), rows(g, 7, 8, d)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    want, mag = reference(q, kp, vp, plens, k, v, lens, list(zip(edges, edges[1:])), d ** -0.5)
+    for b in (7, 1):
+        out, f32 = ops.gqa_prefix_decode(q[:b], kp, vp, ints(plens), k[:b], v[:b], ints(lens[:b]), cu=ints(edges),
+                                         want_f32=True)
+        check(out, f32, want[:b], mag[:b])
