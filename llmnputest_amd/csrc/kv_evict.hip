@@ -4,10 +4,11 @@
 // Per (sequence, kv head) with n = lens[b] > budget positions: of the first n - recent those budget - recent
 // of the greatest weights (ties to the lowest position), then the `recent` last, in the order of their
 // positions. With n <= budget all are kept. First which ones, by a radix selection of the weights' keys, then
-// the rows. Up to 4096 positions the selection is one workgroup's for a (sequence, kv head). Beyond, that was
-// bound by its own instructions on a quarter of the chip (8 sequences of 32771: 44 us), so parts of 4096 share
-// it: histograms of the keys' upper 11 bits; where the wanted number is reached, and the keys of that bin,
-// among which the last part to arrive looks for the rest; then the positions, in order.
+// the rows. Up to 16384 positions the selection is one workgroup's for a (sequence, kv head), the keys in
+// registers (8 sequences of 5000 / 16384: 13.2 / 19.7 us, by parts 21.7 / 22.6 and two launches more). Beyond,
+// that is bound by its own instructions on a quarter of the chip (8 sequences of 32771: 33.7 us of 25.6), so
+// parts of 4096 share it: histograms of the keys' upper 11 bits; where the wanted number is reached, and the
+// keys of that bin, among which the last part to arrive looks for the rest; then the positions, in order.
 //
 // Rows move towards the front. Into other memory they move all at once. In place, row i comes from a
 // position >= i, so a workgroup that takes rows in order, a block at a time, only overwrites rows that it
@@ -50,13 +51,17 @@ struct EvictArgs {
 // Greater weights have greater keys; a NaN's is the greatest; -0 and 0 are one value.
 __device__ __forceinline__ uint32_t weight_key(float x) {
   const uint32_t u = __float_as_uint(x + 0.f);
-  if ((u & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
-  return (u >> 31) ? ~u : (u | 0x80000000u);
+  const uint32_t key = u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+  return (u & 0x7fffffffu) > 0x7f800000u ? 0xffffffffu : key;
+}
+__device__ __forceinline__ float weight_at(const float* w, int p) {   // p below 2^24: a base and 32 bits
+  return *(const float*)((const char*)w + (uint32_t)p * 4u);
 }
 
 constexpr int kPickThreads = 1024;
 constexpr int kPickWaves = kPickThreads / 64;
 constexpr int kPickBins = 2048;    // 11 bits a pass: 32 bits in three
+constexpr int kPickFew = 4 * kPickThreads, kPickHeld = 16 * kPickThreads;   // positions held in 4, in 16 registers
 constexpr int kPickCopies = 4;     // of the histogram, by lane: weights crowd in few bins
 
 // Sum over the lanes up to and with this one.
@@ -98,8 +103,7 @@ __device__ __forceinline__ void evict_pick(const EvictArgs& a, int bk, int n, Pu
     float x[KPT];
 #pragma unroll
     for (int i = 0; i < KPT; ++i) {
-      const int p = p0 + 64 * i + lane;
-      x[i] = 64 * i < share && p < old ? w[p] : 0.f;
+      x[i] = 64 * i < share ? weight_at(w, min(p0 + 64 * i + lane, old - 1)) : 0.f;
     }
 #pragma unroll
     for (int i = 0; i < KPT; ++i) key[i] = 64 * i < share && p0 + 64 * i + lane < old ? weight_key(x[i]) : 0u;
@@ -129,7 +133,7 @@ __device__ __forceinline__ void evict_pick(const EvictArgs& a, int bk, int n, Pu
     each([&] {
 #pragma unroll
       for (int i = 0; i < KPT; ++i)
-        if (64 * i < share && key[i] != 0 && (key[i] & known) == found)
+        if (64 * i < share && (key[i] & known) == found)   // (no weight's key is in key 0's bin)
           atomicAdd(&s_hist[((key[i] >> shift) & mask) * kPickCopies + lane % kPickCopies], 1);
     });
     __syncthreads();
@@ -233,7 +237,7 @@ __device__ __forceinline__ bool part_chooses(const EvictArgs& a, const PartJob& 
 __device__ __forceinline__ void part_keys(const PartJob& j, int lane, uint32_t (&key)[kPartKeys]) {
   float x[kPartKeys];
 #pragma unroll
-  for (int i = 0; i < kPartKeys; ++i) x[i] = j.w[min(j.p0 + 64 * i + lane, j.old - 1)];
+  for (int i = 0; i < kPartKeys; ++i) x[i] = weight_at(j.w, min(j.p0 + 64 * i + lane, j.old - 1));
 #pragma unroll
   for (int i = 0; i < kPartKeys; ++i) key[i] = j.p0 + 64 * i + lane < j.old ? weight_key(x[i]) : 0u;
 }
@@ -285,6 +289,7 @@ constexpr int kHeldKeys = 4096;
 __global__ __launch_bounds__(kPartThreads) void evict_cut_kernel(EvictArgs a) {
   __shared__ __attribute__((aligned(16))) int s_hist[kPickBins];
   __shared__ int s_sum[kPartThreads / 64], s_found[2], s_gt, s_eq, s_last, s_end[kPartThreads];
+  __shared__ int s_above[kPartThreads], s_same[kPartThreads];   // the first parts' (the others' go through memory)
   __shared__ uint32_t s_held[kHeldKeys];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -309,6 +314,8 @@ __global__ __launch_bounds__(kPartThreads) void evict_cut_kernel(EvictArgs a) {
   find_bin(c, j.want, s_sum, s_found);
   const uint32_t bin = (uint32_t)s_found[0];
   int left = s_found[1];
+  // thread p: part p's keys in the bin, on its way beside the arrivals
+  const int many = tid < parts ? a.hist[(row0 + tid) * kPickBins + bin] : 0;
 
   // ---- this part's keys above the bin, and those in it (in any order), for whoever arrives last
   uint32_t* const mine = a.cand + (row0 + j.part) * kPickPart;
@@ -350,8 +357,7 @@ __global__ __launch_bounds__(kPartThreads) void evict_cut_kernel(EvictArgs a) {
   auto load_i = [&](const int32_t* p) {
     return __hip_atomic_load(const_cast<int32_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
   };
-  // thread p has part p's count, and where its keys begin
-  const int many = tid < parts ? load_i(info + 4 * tid + 1) : 0;
+  // where part p's keys end
   const int above_bin = tid < parts ? load_i(info + 4 * tid) : 0;
   int upto = wave_scan(many);
   if (lane == 63) s_sum[wave] = upto;
@@ -407,8 +413,8 @@ __global__ __launch_bounds__(kPartThreads) void evict_cut_kernel(EvictArgs a) {
     above = wave_scan(above);
     same = wave_scan(same);
     if (lane == 63) {
-      info[4 * p + 2] = above;
-      info[4 * p + 3] = same;
+      (p < kPartThreads ? s_above[p] : info[4 * p + 2]) = above;
+      (p < kPartThreads ? s_same[p] : info[4 * p + 3]) = same;
     }
   }
   wait_vm();
@@ -418,8 +424,8 @@ __global__ __launch_bounds__(kPartThreads) void evict_cut_kernel(EvictArgs a) {
     const int p = p0 + tid;
     int g = 0, e = 0;
     if (p < parts) {
-      g = (p0 == 0 ? above_bin : load_i(info + 4 * p)) + info[4 * p + 2];
-      e = info[4 * p + 3];
+      g = p0 == 0 ? above_bin + s_above[p] : load_i(info + 4 * p) + info[4 * p + 2];
+      e = p0 == 0 ? s_same[p] : info[4 * p + 3];
     }
     int eq_upto = wave_scan(e);
     if (lane == 63) s_sum[wave] = eq_upto;
@@ -595,9 +601,11 @@ __device__ __forceinline__ void evict_move(const EvictArgs& a, int bk, int n, in
 
 template <int D, bool IN_PLACE>
 __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a) {
-  int blk = blockIdx.x;
-  const int which = blk & 1;
-  blk >>= 1;
+  // K first, which takes longer with a table; with 8 blocks or more an XCD has the same blocks of every (sequence,
+  // kv head), and so about the same rows of the table (8 sequences, 4096 rows: 33 to 31 us)
+  const int per = gridDim.x / 2;
+  const int which = (int)blockIdx.x < per ? 0 : 1;
+  const int blk = blockIdx.x - which * per;
   const int bk = blk / a.blocks, block = blk % a.blocks;
   const int n = a.n_old[bk];
   if (which == 1 && block == 0 && bk % a.hkv == 0 && threadIdx.x == 0) a.lens_out[bk / a.hkv] = min(n, a.budget);
@@ -607,13 +615,13 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a) {
 // Short caches cut down to few rows: a workgroup picks its (sequence, kv head)'s and moves them. The lengths
 // stay as they are until the last workgroup of a sequence has read its own.
 constexpr int kWholeRows = 1024;
-template <int D, bool IN_PLACE>
+template <int D, bool IN_PLACE, int KPT>
 __global__ __launch_bounds__(kPickThreads) void evict_whole_kernel(EvictArgs a) {
   __shared__ int32_t s_kept[kWholeRows];
   const int bk = blockIdx.x, b = bk / a.hkv;
   const int n = min(max(a.lens[b], 0), a.max_len);
   int32_t* const kept = a.kept + (size_t)bk * a.budget;
-  evict_pick<4, true>(a, bk, n, [&](int i, int p) {
+  evict_pick<KPT, true>(a, bk, n, [&](int i, int p) {
     kept[i] = p;
     if (i < kWholeRows) s_kept[i] = p;
   });
@@ -621,6 +629,13 @@ __global__ __launch_bounds__(kPickThreads) void evict_whole_kernel(EvictArgs a) 
   if (threadIdx.x == 0 && ticket(a.counters + b, a.hkv)) a.lens_out[b] = min(n, a.budget);
   evict_move<D, IN_PLACE, kPickThreads>(a, bk, n, 0, 0, 1, s_kept);
   evict_move<D, IN_PLACE, kPickThreads>(a, bk, n, 1, 0, 1, s_kept);
+}
+
+template <int D, bool IN_PLACE>
+static void whole_launch(const EvictArgs& a, hipStream_t s) {
+  const dim3 grid((unsigned)(a.batch * a.hkv)), threads(kPickThreads);
+  if (a.max_len <= kPickFew) hipLaunchKernelGGL((evict_whole_kernel<D, IN_PLACE, 4>), grid, threads, 0, s, a);
+  else hipLaunchKernelGGL((evict_whole_kernel<D, IN_PLACE, 16>), grid, threads, 0, s, a);
 }
 
 static bool evict_shape_ok(int batch, int hkv, int d, int max_len, int budget, int recent) {
@@ -631,7 +646,7 @@ static bool evict_shape_ok(int batch, int hkv, int d, int max_len, int budget, i
 // Parts of a (sequence, kv head)'s selection; 0: one workgroup's, with few positions and where there are more
 // (sequence, kv head)s than counters.
 static int evict_parts(size_t bh, int max_len) {
-  return max_len <= kPickPart || bh > Q4NX_WS_COUNTER_BYTES / 4 ? 0 : (max_len + kPickPart - 1) / kPickPart;
+  return max_len <= kPickHeld || bh > Q4NX_WS_COUNTER_BYTES / 4 ? 0 : (max_len + kPickPart - 1) / kPickPart;
 }
 // Lengths and cuts, before the parts' memory.
 static size_t evict_head_bytes(size_t bh) { return (bh * 12 + 255) / 256 * 256; }
@@ -721,12 +736,11 @@ int q4nx_kv_evict(const uint16_t* k_cache, const uint16_t* v_cache, int64_t kv_b
   a.room = room;
   hipStream_t s = (hipStream_t)stream;
   // 1 x 1000 to 512 in one launch: 13.3 us a pass, 16.2 in two; more rows go faster by more workgroups than one
-  if (max_len <= kPickPart && most <= kWholeRows && batch <= Q4NX_WS_COUNTER_BYTES / 4) {
-    const dim3 grid((unsigned)bh), threads(kPickThreads);
-    if (head_dim == 64 && in_place) hipLaunchKernelGGL((evict_whole_kernel<64, true>), grid, threads, 0, s, a);
-    else if (head_dim == 64) hipLaunchKernelGGL((evict_whole_kernel<64, false>), grid, threads, 0, s, a);
-    else if (in_place) hipLaunchKernelGGL((evict_whole_kernel<128, true>), grid, threads, 0, s, a);
-    else hipLaunchKernelGGL((evict_whole_kernel<128, false>), grid, threads, 0, s, a);
+  if (max_len <= kPickHeld && most <= kWholeRows && batch <= Q4NX_WS_COUNTER_BYTES / 4) {
+    if (head_dim == 64 && in_place) whole_launch<64, true>(a, s);
+    else if (head_dim == 64) whole_launch<64, false>(a, s);
+    else if (in_place) whole_launch<128, true>(a, s);
+    else whole_launch<128, false>(a, s);
     return check_launch(what);
   }
   const int step = kMoveThreads / (head_dim / 16);
@@ -739,8 +753,10 @@ int q4nx_kv_evict(const uint16_t* k_cache, const uint16_t* v_cache, int64_t kv_b
     hipLaunchKernelGGL(evict_hist_kernel, all, threads, 0, s, a);
     hipLaunchKernelGGL(evict_cut_kernel, all, threads, 0, s, a);
     hipLaunchKernelGGL(evict_list_kernel, all, threads, 0, s, a);
-  } else if (max_len <= kPickPart) {
+  } else if (max_len <= kPickFew) {
     hipLaunchKernelGGL((evict_pick_kernel<4, true>), dim3((unsigned)bh), dim3(kPickThreads), 0, s, a);
+  } else if (max_len <= kPickHeld) {
+    hipLaunchKernelGGL((evict_pick_kernel<16, true>), dim3((unsigned)bh), dim3(kPickThreads), 0, s, a);
   } else {
     hipLaunchKernelGGL((evict_pick_kernel<16, false>), dim3((unsigned)bh), dim3(kPickThreads), 0, s, a);
   }

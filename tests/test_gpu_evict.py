@@ -116,6 +116,13 @@ EVICT = [
     (2, 1, 64, [4097, 1025], 1024, 100, True, "special"),
     (1, 2, 128, [40000], 5000, 333, True, "random"),
     (4, 2, 64, [2049, 2048, 2047, 1], 2048, 5, True, "steps"),
+    # around the most positions whose keys one workgroup holds (room for two more than the longest)
+    (2, 2, 64, [16382, 9000], 3000, 100, True, "steps"),
+    (1, 2, 64, [16382], 700, 50, False, "special"),
+    (2, 2, 128, [6001, 4098], 1000, 3, True, "equal"),
+    (2, 2, 128, [16383, 50], 1000, 77, True, "random"),
+    (3, 1, 64, [20000, 4096, 300], 600, 17, True, "special"),
+    (2, 2, 64, [30000, 12289], 9000, 0, False, "equal"),
 ]
 
 
