@@ -103,6 +103,10 @@ DEFAULT_WS_BYTES = 256 << 20
 DEFAULT_WS_STREAMS = 16
 
 
+# torch.cuda.is_current_stream_capturing without the call around it
+_capturing = torch._C._cuda_isCurrentStreamCapturing
+
+
 class _Defaults(threading.local):
     """A host thread's default workspaces, by device and stream: given back when the thread ends.
     A stream that records a graph has one of its own for that capture, which lies in the graph's
@@ -114,7 +118,7 @@ class _Defaults(threading.local):
 
     def get(self, device: int, stream: int) -> Workspace:
         key, capture = (device, stream), 0
-        if torch.cuda.is_current_stream_capturing():
+        if _capturing():
             capture = _lib.lib().q4nx_stream_capture_id(stream)
             key = (device, stream, "capture")
         held = self.by_stream.get(key)
@@ -143,7 +147,7 @@ def _scratch(ws: Workspace | None, nbytes: int, at: tuple | None = None) -> tupl
     device, stream = at or _device_stream()
     if ws is None:
         ws = _defaults.get(device, stream)
-        if nbytes > max(DEFAULT_WS_BYTES, ws.buf.numel()):
+        if nbytes > DEFAULT_WS_BYTES and nbytes > ws.buf.numel():
             ws = Workspace(device=ws.device)       # for this call alone: only its counters zeroed
             ws.buf = torch.empty(nbytes, dtype=torch.uint8, device=ws.device)
             ws.buf[:WS_COUNTER_BYTES].zero_()
@@ -614,14 +618,17 @@ def _rows_of(k: torch.Tensor, v: torch.Tensor, name: str, d: int, dev: int) -> t
         _refuse(k, f"k_{name}", torch.bfloat16, dev)
         _refuse(v, f"v_{name}", torch.bfloat16, dev)
     shape, st = k.shape, k.stride()
-    if len(shape) != 4 or shape[3] != d or shape[1] == 0 or st[3] != 1 or (shape[2] > 1 and st[2] != d):
+    if len(shape) != 4:
         raise ValueError(f"k_{name} must be [B, Hkv, L, {d}] with contiguous rows")
-    b, hkv, n, _ = shape
+    b, hkv, n, dk = shape
+    sb, sh, sl, sd = st
+    if dk != d or hkv == 0 or sd != 1 or (sl != d and n > 1):
+        raise ValueError(f"k_{name} must be [B, Hkv, L, {d}] with contiguous rows")
     sv = v.stride()
     if v.shape != shape or (sv != st and any(x > 1 and s != t for x, s, t in zip(shape, st, sv))):
         raise ValueError(f"k_{name} and v_{name} must have one shape and one layout")
-    h = st[1] if hkv > 1 else n * d
-    return b, hkv, n, (st[0] if b > 1 else hkv * h), h
+    h = sh if hkv > 1 else n * d
+    return b, hkv, n, (sb if b > 1 else hkv * h), h
 
 
 def _upto(n: int, most: int | None, name: str) -> int:
@@ -839,7 +846,7 @@ def adjust_logits(logits: torch.Tensor, counts: torch.Tensor | None = None,
     if v == 0:
         raise ValueError("logits must have at least one token")
     if out is None:
-        out = logits.new_empty(shape)
+        out = torch.empty_like(logits)   # rows of V, packed
         out_stride = v
     else:
         out_stride = _vocab_rows(out, "out", dtype, dev, shape)
