@@ -13,7 +13,7 @@
 //   own caches      (sequence, kv head, part): Narrow
 //   prefix, R > 16  (kv head, 64 NR rows, part): part_wide below
 //   prefix, R <= 16 (kv head, part): Narrow over the members' rows
-// Short calls of few sequences are one launch: a workgroup a (sequence, kv head) takes the prefix's rows, then
+// Short calls are one launch: a workgroup a (sequence, kv head) takes the prefix's rows, then
 // its own.
 
 #include "attn_parts.h"
@@ -424,10 +424,6 @@ __global__ __launch_bounds__(256) void prefix_merge_kernel(PrefixArgs a) {
   if (i >= a.batch * a.hq) return;
   const int b = i / a.hq, h = i - b * a.hq;
   const int kvh = h / a.G, slots = a.ns_own + a.ns_pre;
-  if (slots == 0) {
-    if (lane < D / 4) put_channels(a.out, a.out_f32, (size_t)i * D + 4 * lane, make_float4(0.f, 0.f, 0.f, 0.f));
-    return;
-  }
   const float* rec = a.rec + (((size_t)b * a.hkv + kvh) * slots * a.G + (h - kvh * a.G)) * kRec<D>;
   const float4 A = merge_records<D>(rec, (size_t)a.G * kRec<D>, slots, lane, [&](int r) {
     const int len = min(max(a.lens[b], 0), a.max_len);
@@ -447,9 +443,12 @@ static PrefixPlan prefix_plan(int batch, int hq, int hkv, int d, int n_prefixes,
   const int G = hq / hkv;
   const long long rows = (long long)batch * G;
   PrefixPlan p{};
-  // Up to 1024 positions on a compute unit each (2 x 513 + 33, 40 q / 8 kv heads: 7.8 us, 5.0 and 3.7
-  // in two launches, of which the second costs the host 3.5 us)
-  p.whole = (long long)batch * hkv <= 256 && max_prefix + max_len <= 1024 && kPartWaves * G * (d + 2) <= 16384;
+  if (n_prefixes == 0) max_prefix = 0;
+  // One launch up to 256 KB of K and V for each compute unit, which takes 1024 positions of D = 64 in 5 us
+  // (eager / in a graph, two launches: 8 x 500 10.6 / 7.1, 13.4 / 9.2; 8 x 900 10.7 / 9.3, 13.3 / 9.3; 64 x 300
+  // 10.4 / 8.8, 13.4 / 12.5; 1 x 900 10.5 / 9.1, 13.2 / 7.1; D = 128, 8 x 900 14.5 / 14.7, 13.3 / 10.4)
+  const long long each = ((long long)batch * hkv + 255) / 256;   // a compute unit's workgroups
+  p.whole = each * (max_prefix + max_len) <= 65536 / d;
   if (p.whole) return p;
   // 32 rows a wave where prefixes have more than 64 of them on average and the registers hold it
   p.nr = d == 64 && rows > 64ll * (n_prefixes > 1 ? n_prefixes : 1) ? 2 : 1;
@@ -457,7 +456,7 @@ static PrefixPlan prefix_plan(int batch, int hq, int hkv, int d, int n_prefixes,
   // every prefix may end inside a tile; a tile has a member at least (prefixes may have none)
   const long long most = (rows + rt - 1) / rt + (n_prefixes > 0 ? n_prefixes - 1 : 0);
   p.tiles = (int)(most < batch ? most : batch);
-  if (n_prefixes == 0 || max_prefix == 0) p.tiles = 0;
+  if (max_prefix == 0) p.tiles = 0;
   if (p.tiles > 0)
     // D = 64: what the chip holds at once, three workgroups a compute unit (256 x 16384: 384 / 512 / 640 / 768 /
     // 1024 took 119 / 94 / 96 / 91 / 95 us). D = 128: less, beside the own caches' parts (48 x 5003: 384 / 512 /
@@ -489,10 +488,8 @@ static void prefix_launch(const PrefixArgs& a, const PrefixPlan& p, hipStream_t 
     return;
   }
   const unsigned grid = (unsigned)(a.hkv * (p.tiles * p.ns_pre + a.batch * p.ns_own));
-  if (grid > 0) {
-    if (D == 64 && p.nr == 2) hipLaunchKernelGGL((prefix_parts_kernel<64, 2>), dim3(grid), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((prefix_parts_kernel<D, 1>), dim3(grid), dim3(256), 0, s, a);
-  }
+  if (D == 64 && p.nr == 2) hipLaunchKernelGGL((prefix_parts_kernel<64, 2>), dim3(grid), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((prefix_parts_kernel<D, 1>), dim3(grid), dim3(256), 0, s, a);
   const unsigned wgs = (unsigned)(((long long)a.batch * a.hq + 3) / 4);
   hipLaunchKernelGGL(prefix_merge_kernel<D>, dim3(wgs), dim3(256), 0, s, a);
 }

@@ -8,7 +8,8 @@
 // A weight needs the maximum and the sum of the whole row, which a part of it does not know. The parts
 // (Narrow) therefore also leave their scores, 4 Hq bytes a position beside the 4 D Hkv of K and V, and
 // the second launch turns them into weights once every part's (m, l) is there; its last workgroup of a
-// (sequence, kv head) merges the outputs. Short rows of few sequences are one launch.
+// (sequence, kv head) merges the outputs. Short rows, and those of
+// many sequences whose scores LDS holds, are one launch.
 
 #include "attn_parts.h"
 
@@ -163,11 +164,13 @@ static size_t whole_lds(int G, int d, int64_t score_stride) {
 
 static WeightPlan weight_plan(int batch, int hq, int hkv, int d, int max_len) {
   WeightPlan p{};
-  // Up to 1024 positions on a compute unit each, as far as LDS holds their scores (1 x 513, 40 q / 8 kv heads:
-  // 8.0 us, 5.2 and 4.4 in two launches, of which the second costs the host 3.5 us)
+  // One launch, as far as LDS holds a row's scores: for any length where rows fill most of the chip (64 x 1024,
+  // 40 q / 8 kv heads: 26.1 us, 35.2 in two launches; 64 x 2100 51.6, 66.4; 20 x 2100 19.1, 22.5; 16 x 2100 18.3,
+  // 18.9), else up to 256 KB of K and V for a compute unit (12 x 1024 10.5, 12.4; D = 128, 1 x 900 14.7, 12.3)
   const int round = 32 * kPartWaves;
   p.score_stride = (max_len + round - 1) / round * round;
-  if ((long long)batch * hkv <= 256 && max_len <= 1024 && whole_lds(hq / hkv, d, p.score_stride) <= 65024) return p;
+  const bool fits = whole_lds(hq / hkv, d, p.score_stride) <= 65024;
+  if (fits && ((long long)batch * hkv >= 160 || max_len <= 65536 / d)) return p;
   cut_parts(max_len, 1024 / ((long long)hkv * batch), 256, kPartRound, &p.ns, &p.chunk);
   p.score_stride = (int64_t)p.ns * p.chunk;
   return p;

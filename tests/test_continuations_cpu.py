@@ -96,7 +96,7 @@ def test_workspaces():
     lib = _lib.lib()
     size = lib.q4nx_gqa_prefix_decode_ws_bytes
     assert size(4, 40, 8, 64, 2, 1000, 500) >= 65536 + 4 * 40 * 2 * 68 * 4      # a part of each kind
-    assert size(4, 40, 8, 64, 0, 0, 0) == 65536 and size(1, 8, 8, 128, 1, 1024, 0) == 65536   # one launch
+    assert size(4, 40, 8, 64, 0, 0, 0) == 65536 and size(1, 8, 8, 128, 1, 512, 0) == 65536   # one launch
     for bad in ((0, 40, 8, 64, 1, 1, 1), (4, 40, 7, 64, 1, 1, 1), (4, 40, 8, 65, 1, 1, 1), (4, 40, 8, 64, -1, 1, 1)):
         assert size(*bad) == 0
     size = lib.q4nx_gqa_decode_weights_ws_bytes

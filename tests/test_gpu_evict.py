@@ -48,6 +48,11 @@ CASES = [
     (2, 14, 2, 128, [9000, 8191]),
     (1, 5, 1, 64, [70000]),
     (300, 4, 4, 64, [i * 2 for i in range(300)]),
+    # many rows: with their scores in LDS as far as it holds them, in memory beyond
+    (24, 40, 8, 64, [max(2500 - 113 * i, 0) for i in range(24)]),
+    (160, 3, 1, 128, [(i * 37) % 1100 for i in range(160)]),
+    (40, 64, 4, 64, [(i * 101) % 900 for i in range(40)]),
+    (12, 4, 2, 128, [600 - 50 * i for i in range(12)]),
 ]
 
 

@@ -54,6 +54,9 @@ CASES = [
     (20, [(0, 9), (9, 20)], 32, 4, 128, [1025, 320], [i for i in range(20)]),
     (70, [(i, i + 1) for i in range(70)], 4, 2, 64, [i * 5 for i in range(70)], [i % 7 for i in range(70)]),
     (3, [(0, 3)], 16, 1, 64, [40000], [1, 2, 3000]),
+    # two and five workgroups a compute unit
+    (64, [(0, 20), (20, 64)], 40, 8, 64, [300, 401], [i % 41 for i in range(64)]),
+    (300, [(0, 300)], 16, 4, 128, [60], [i % 40 for i in range(300)]),
 ]
 
 
