@@ -229,7 +229,7 @@ __device__ __forceinline__ void part_wide(const PrefixArgs& a, const uint16_t* k
   auto tile = [&](int t, auto more, auto last) {
     if constexpr (more) {
       // K of tile t + 2 takes the place of tile t's, V of t + 1 that of t - 1's: both were last read
-      // before the barrier that began this tile
+      // before the barrier that began this tile (the first tile's K, in front of the loop)
       fetch(kbase, k0, ck, t + 2);
       fetch(vbase, v0, cv, t + 1);
     }
@@ -300,6 +300,9 @@ __device__ __forceinline__ void part_wide(const PrefixArgs& a, const uint16_t* k
 #pragma unroll
     for (int n = 0; n < NR; ++n) m[n] = greatest(n, 0, 4);
   }
+  // every wave has read the first tile of K before any fetches the third into its place (waves without rows
+  // read nothing and would be far ahead)
+  if (nt > 2) __syncthreads();
   for (int t = 0; t + 2 < nt; ++t) tile(t, std::true_type{}, std::false_type{});
   if (nt > 1) tile(nt - 2, std::true_type{}, std::true_type{});
   tile(nt - 1, std::false_type{}, std::false_type{});

@@ -1,0 +1,36 @@
+"""Several continuations of a prompt, at the edges: what workgroups' waves share in LDS, scales of nothing,
+signs of zero, and lengths that need another path than the usual ones."""
+
+import pytest
+import torch
+
+from tests.test_gpu_prefix import check, reference, rows
+
+pytestmark = pytest.mark.gpu
+
+
+def ints(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("b", [5, 8, 13, 40])
+def test_first_tile_of_a_prefix_part(dev, b, d):
+    """Parts of four tiles of 64 positions, the first of which has nearly all of the weight and the third, whose
+    rows of K take its place in LDS, none of it; waves without query rows among those with some."""
+    from llmnputest_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(b)
+    hq, hkv, n = 40, 8, 3001
+    u = torch.randn((hkv, 1, d), device="cuda", generator=g).sign()
+    toward = torch.tensor([2.0, 0.0, -2.0, 0.0], device="cuda")[torch.arange(n, device="cuda") // 64 % 4]
+    kp = (toward[:, None] * u + 0.1 * torch.randn((1, hkv, n, d), device="cuda", generator=g)).to(torch.bfloat16)
+    vp = rows(g, 1, hkv, n, d)
+    q = (u.expand(hkv, hq // hkv, d).reshape(hq, d) + 0.1 * torch.randn((b, hq, d), device="cuda", generator=g)).to(torch.bfloat16)
+    k, v, lens = rows(g, b, hkv, 3, d), rows(g, b, hkv, 3, d), [i % 4 for i in range(b)]
+    want, mag = reference(q, kp, vp, [n], k, v, lens, [(0, b)], d ** -0.5)
+    first = None
+    for _ in range(10):
+        out, f32 = ops.gqa_prefix_decode(q, kp, vp, ints([n]), k, v, ints(lens), want_f32=True)
+        check(out, f32, want, mag)
+        first = f32 if first is None else first
+        assert torch.equal(f32, first)
