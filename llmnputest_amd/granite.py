@@ -296,6 +296,7 @@ class GraniteDecoder:
         self.graph: torch.cuda.CUDAGraph | None = None         # one greedy step
         self.graph_steps: torch.cuda.CUDAGraph | None = None   # GRAPH_STEPS greedy steps
         self.graph_batch = 0
+        self._graph_ws: torch.Tensor | None = None
         self.calls = 0
         self.seconds = 0.0
 
@@ -477,7 +478,8 @@ class GraniteDecoder:
         left = torch.empty_like(held)
         for k, v, w in zip(self.k_cache, self.v_cache, self.weights):
             left.copy_(held)
-            ops.kv_evict(k, v, w, left, budget, recent, rope=self.rope, ws=self.ws)
+            # not in self.ws, whose address the step's graphs hold: long caches need more here than a step does
+            ops.kv_evict(k, v, w, left, budget, recent, rope=self.rope)
         return [min(x, budget) for x in lens]
 
     def _check_own(self, positions, n: int = 1) -> None:
@@ -582,6 +584,7 @@ class GraniteDecoder:
             graphs.append(g)
         self.graph, self.graph_steps = graphs
         self.graph_batch = b
+        self._graph_ws = self.ws.buf               # where the graphs' scratch lies, also if self.ws grows later
         for t, s0 in zip(state, snap):
             t.copy_(s0)
 

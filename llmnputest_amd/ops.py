@@ -84,7 +84,8 @@ class Workspace:
 
     Kernels that use it leave its counters at zero, so they are zeroed only on (re)allocation. An
     op of two launches keeps its operands there between them: two threads, or two streams, need a
-    workspace each.
+    workspace each. A call that needs more than there is gets a larger `buf` in its place; a graph
+    keeps the one that it was captured with, which has to live as long as the graph.
     """
 
     def __init__(self, nbytes: int = 0, device=None):

@@ -4,6 +4,7 @@ signs of zero, and lengths that need another path than the usual ones."""
 import pytest
 import torch
 
+from llmnputest_amd.granite import GraniteConfig, GraniteDecoder, GraniteWeights
 from tests.test_gpu_prefix import check, reference, rows
 
 pytestmark = pytest.mark.gpu
@@ -34,3 +35,20 @@ def test_first_tile_of_a_prefix_part(dev, b, d):
         check(out, f32, want, mag)
         first = f32 if first is None else first
         assert torch.equal(f32, first)
+
+
+def test_graphs_keep_their_workspace(dev):
+    """A decoder's graphs go on in the memory they were captured with, also when its workspace has grown since."""
+    cfg = GraniteConfig(n_layers=2, vocab=4096)
+    dec = GraniteDecoder(GraniteWeights.synthetic(cfg, seed=3, device="cuda"), 2, 256, track_weights=True)
+    dec.seed_cache(150, seed=9)
+    want, _ = dec.generate([3, 4], [150, 90], 20)
+    size = dec.ws.buf.numel()
+    dec.ws.get(2 * size)
+    others = [torch.full((size,), 0x5A, dtype=torch.uint8, device="cuda") for _ in range(3)]
+    dec.seed_cache(150, seed=9)
+    got, _ = dec.generate([3, 4], [150, 90], 20)
+    assert (got == want).all() and all(bool((x == 0x5A).all()) for x in others)
+    assert dec.evict([170, 110], 100, 16) == [100, 100]
+    got, _ = dec.generate([5, 6], [100, 100], 20)
+    assert got.shape == (2, 20) and all(bool((x == 0x5A).all()) for x in others)
