@@ -131,7 +131,7 @@ __device__ __forceinline__ void part_wide(const PrefixArgs& a, const uint16_t* k
   }
 
   // Tile t of K or V straight into its LDS buffer, 16 bytes a lane; a lane fetches what the swizzle puts in
-  // its place. Rows past the end: the last one again, whose weight is masked to 0.
+  // its place. Rows past the end: the last one again, which moves no maximum, with a weight of 0 (`weigh`).
   const uint32_t k0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint4*)sk;
   const uint32_t v0 = k0 + 2 * 64 * C * 16;
   const int nt = (end + 63) / 64;
@@ -184,19 +184,6 @@ __device__ __forceinline__ void part_wide(const PrefixArgs& a, const uint16_t* k
 #pragma unroll
       for (int n = 0; n < NR; ++n) s[n][x] = mfma_bf16(kf[x & 1][c], q[n][c], s[n][x]);
   };
-  // `last`: some positions may lie past the end (apart from the others: as selects in every tile, this made
-  // 120 us of 90 with 256 x 16384)
-  auto mask = [&](int t, auto last) {
-    if constexpr (last) {
-#pragma unroll
-      for (int x = 0; x < 4; ++x)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (t * 64 + 16 * x + 4 * g + e >= end)
-#pragma unroll
-            for (int n = 0; n < NR; ++n) s[n][x][e] = -INFINITY;
-    }
-  };
   // The greatest scaled score of subtiles x0 .. x1 - 1, per row.
   auto greatest = [&](int n, int x0, int x1) {
     float v = -INFINITY;
@@ -209,8 +196,11 @@ __device__ __forceinline__ void part_wide(const PrefixArgs& a, const uint16_t* k
   };
   // Weights of half a tile against the maximum as it stands, and whether one is above 2^8 (or a NaN; positive
   // floats and NaNs, compared as whole numbers) or there is no maximum yet (every score so far was -inf).
+  // `last`: some positions may lie past the end; theirs are 0, whatever the scale (scores of -inf would be NaN
+  // with a scale of 0). Apart from the other tiles: as selects in every one, this made 120 us of 90 with
+  // 256 x 16384.
   float w[NR][8];
-  auto weigh = [&](int x2) {
+  auto weigh = [&](int x2, auto last) {
     uint32_t top = 0;
     bool none = false;
 #pragma unroll
@@ -220,13 +210,16 @@ __device__ __forceinline__ void part_wide(const PrefixArgs& a, const uint16_t* k
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         w[n][i] = exp2_hw(fmaf(s[n][2 * x2 + (i >> 2)][i & 3], a.scale_l2, -mb));
+        if constexpr (last)
+          if ((nt - 1) * 64 + 32 * x2 + 16 * (i >> 2) + 4 * g + (i & 3) >= end) w[n][i] = 0.f;
         top = max(top, __float_as_uint(w[n][i]));
       }
     }
     return __any(top > 0x43800000u || none);
   };
   // one tile's weights and their product; as its scores are used up, the next tile's take their place
-  auto tile = [&](int t, auto more, auto last) {
+  auto tile = [&](int t, auto more) {
+    constexpr std::integral_constant<bool, !more> last{};
     if constexpr (more) {
       // K of tile t + 2 takes the place of tile t's, V of t + 1 that of t - 1's: both were last read
       // before the barrier that began this tile (the first tile's K, in front of the loop)
@@ -237,7 +230,7 @@ __device__ __forceinline__ void part_wide(const PrefixArgs& a, const uint16_t* k
       if constexpr (more) read_k(t + 1, 0);
 #pragma unroll
       for (int x2 = 0; x2 < 2; ++x2) {
-        if (weigh(x2)) {   // the maximum moves, and what was summed against it
+        if (weigh(x2, last)) {   // the maximum moves, and what was summed against it
 #pragma unroll
           for (int n = 0; n < NR; ++n) {
             const float mn = fmaxf(m[n], greatest(n, 2 * x2, 2 * x2 + 2));
@@ -247,7 +240,7 @@ __device__ __forceinline__ void part_wide(const PrefixArgs& a, const uint16_t* k
 #pragma unroll
             for (int u = 0; u < D / 16; ++u) o[n][u] *= corr;
           }
-          weigh(x2);
+          weigh(x2, last);
         }
         if constexpr (more) read_k(t + 1, 2 * x2 + 1);
         read_v(t, x2);
@@ -278,7 +271,6 @@ __device__ __forceinline__ void part_wide(const PrefixArgs& a, const uint16_t* k
             o[n][u] = mfma_bf16(vf[u], pr[n], o[n][u]);
           }
       }
-      if constexpr (more) mask(t + 1, last);
     }
     if constexpr (more) {
       wait_vm();
@@ -296,16 +288,14 @@ __device__ __forceinline__ void part_wide(const PrefixArgs& a, const uint16_t* k
       read_k(0, x);
       score(x);
     }
-    mask(0, std::true_type{});
 #pragma unroll
     for (int n = 0; n < NR; ++n) m[n] = greatest(n, 0, 4);
   }
   // every wave has read the first tile of K before any fetches the third into its place (waves without rows
   // read nothing and would be far ahead)
   if (nt > 2) __syncthreads();
-  for (int t = 0; t + 2 < nt; ++t) tile(t, std::true_type{}, std::false_type{});
-  if (nt > 1) tile(nt - 2, std::true_type{}, std::true_type{});
-  tile(nt - 1, std::false_type{}, std::false_type{});
+  for (int t = 0; t + 1 < nt; ++t) tile(t, std::true_type{});
+  tile(nt - 1, std::false_type{});
 #pragma unroll
   for (int n = 0; n < NR; ++n) {
     const int r = r0 + 16 * n + j;

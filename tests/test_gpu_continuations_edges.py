@@ -52,3 +52,39 @@ def test_graphs_keep_their_workspace(dev):
     assert dec.evict([170, 110], 100, 16) == [100, 100]
     got, _ = dec.generate([5, 6], [100, 100], 20)
     assert got.shape == (2, 20) and all(bool((x == 0x5A).all()) for x in others)
+
+
+@pytest.mark.parametrize("scale", [0.0, 1e-46, 0.05])
+@pytest.mark.parametrize("d", [64, 128])
+def test_ends_of_prefixes(dev, d, scale):
+    """Prefixes that end at every place of a tile, as rows of a wide product, and own rows; with a scale of nothing
+    (or one that is nothing in fp32) the answer is the mean of what is seen."""
+    from llmnputest_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(d)
+    plens = [1, 5, 31, 32, 33, 47, 63, 64, 65, 95, 96, 97, 128, 129, 160, 193, 700, 1101]
+    b = 2 * len(plens)
+    groups = [(2 * i, 2 * i + 2) for i in range(len(plens))]
+    lens = [(0, 3, 129, 40)[i % 4] for i in range(b)]
+    kp, vp = rows(g, len(plens), 1, 1104, d), rows(g, len(plens), 1, 1104, d)
+    k, v, q = rows(g, b, 1, 130, d), rows(g, b, 1, 130, d), rows(g, b, 16, d)
+    for i, n in enumerate(plens):
+        kp[i, :, n:], vp[i, :, n:] = float("nan"), float("inf")
+    cu = ints([0] + [hi for _, hi in groups])
+    out, f32 = ops.gqa_prefix_decode(q, kp, vp, ints(plens), k, v, ints(lens), cu=cu, scale=scale, want_f32=True)
+    want, mag = reference(q, kp, vp, plens, k, v, lens, groups, scale)
+    check(out, f32, want, mag)
+
+
+def test_weights_without_a_scale(dev):
+    """A scale of 0: every position is given the same."""
+    from llmnputest_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(1)
+    lens = [3000, 1, 77]
+    k, v, q = rows(g, 3, 2, 3000, 64), rows(g, 3, 2, 3000, 64), rows(g, 3, 10, 64)
+    w = torch.zeros((3, 2, 3000), device="cuda")
+    out = ops.gqa_decode_weights(q, k, v, ints(lens), w, start=True, scale=0.0, want_f32=True)[1]
+    for i, n in enumerate(lens):
+        mean = v[i, :, :n].double().mean(1).repeat_interleave(5, 0)
+        # equal weights are exact; sums of n terms and a quotient in fp32
+        assert bool(((out[i].double() - mean).abs() <= 2.0 ** -15 * v[i, :, :n].double().abs().mean(1).repeat_interleave(5, 0)).all())
+        assert torch.allclose(w[i, :, :n], torch.full_like(w[i, :, :n], 5 / n), rtol=2.0 ** -20, atol=0)
