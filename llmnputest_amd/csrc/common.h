@@ -96,9 +96,9 @@ __device__ __forceinline__ uint32_t perm(uint32_t s0, uint32_t s1, uint32_t sel)
 }
 
 // 64-bit key whose unsigned order is numpy's argmax order: larger value first, NaN above
-// everything, and on ties the smaller index (stored inverted in the low word).
+// everything, and on ties (-0 and 0 among them) the smaller index (stored inverted in the low word).
 __device__ __forceinline__ unsigned long long argmax_key(float v, uint32_t idx) {
-  const uint32_t u = __float_as_uint(v);
+  const uint32_t u = __float_as_uint(v + 0.f);   // -0 becomes 0
   uint32_t ord;
   if ((u & 0x7fffffffu) > 0x7f800000u) ord = 0xffffffffu;
   else ord = (u & 0x80000000u) ? ~u : (u | 0x80000000u);

@@ -88,3 +88,20 @@ def test_weights_without_a_scale(dev):
         # equal weights are exact; sums of n terms and a quotient in fp32
         assert bool(((out[i].double() - mean).abs() <= 2.0 ** -15 * v[i, :, :n].double().abs().mean(1).repeat_interleave(5, 0)).all())
         assert torch.allclose(w[i, :, :n], torch.full_like(w[i, :, :n], 5 / n), rtol=2.0 ** -20, atol=0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("v", [9, 5000, 100352])
+def test_zeros_are_one_value(dev, v, dtype):
+    """0 and -0 tie, and the lowest token takes it, within a thread's tokens and across workgroups."""
+    from llmnputest_amd import ops
+    x = torch.full((4, v), -1.0, dtype=dtype, device="cuda")
+    x[0, 3], x[0, v - 1] = -0.0, 0.0
+    x[1, 3], x[1, v - 1] = 0.0, -0.0
+    x[2, 5], x[2, 6], x[2, 7] = -0.0, -0.0, 0.0
+    x[3, v - 2], x[3, v - 1] = -0.0, 2.0 ** -126
+    keys = torch.empty(4, dtype=torch.int64, device="cuda")
+    out, token = ops.adjust_logits(x, keys=keys)
+    assert token.tolist() == [3, 3, 5, v - 1]
+    assert (0xFFFFFFFF - (keys & 0xFFFFFFFF)).tolist() == token.tolist()
+    assert torch.equal(out.view(torch.int16), x.view(torch.int16))   # the logits' own zeros stay as they are
