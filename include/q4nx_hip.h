@@ -532,7 +532,7 @@ int q4nx_count_tokens(int32_t *counts, int64_t count_stride, int vocab, int batc
  * and rounded after every step:
  *   count word not 0:    x = x > 0 ? x / repetition[b] : x * repetition[b]
  *                        x -= frequency[b] * n;  n > 0: x -= presence[b]   (n: the word without its sign bit)
- *   x += the sequence's biases for it, one after the other
+ *   x += the sum of the sequence's biases for it (fp32, added up from 0 in the order of the list)
  *   not allowed:         x = -inf
  * out (same type; may be logits) [batch][out_stride]; tokens[b] (optional) the greatest x before its
  * rounding to out's type (NaN above all, ties to the lowest token; all -inf: 0), keys[b] (optional) its

@@ -6,6 +6,7 @@
 // written):
 //   seen (count word not 0):  x = x > 0 ? x / repetition : x * repetition
 //   x -= frequency * count;   count > 0: x -= presence;   x += bias;   not allowed: x = -inf
+// (a token that is listed several times: the sum of its biases, in the order of the list)
 // A count word holds how often a token was generated and, in the sign bit, whether the prompt has it.
 // Bound by memory: logits, counts and masks are read once, what comes of the logits is written once.
 

@@ -105,3 +105,15 @@ def test_zeros_are_one_value(dev, v, dtype):
     assert token.tolist() == [3, 3, 5, v - 1]
     assert (0xFFFFFFFF - (keys & 0xFFFFFFFF)).tolist() == token.tolist()
     assert torch.equal(out.view(torch.int16), x.view(torch.int16))   # the logits' own zeros stay as they are
+
+
+def test_biases_are_summed_first(dev):
+    """A token that is listed twice gets the sum of its biases: 1 + (2^24 - 2^24), not (1 + 2^24) - 2^24."""
+    from llmnputest_amd import ops
+    big = 2.0 ** 24
+    x = torch.ones((2, 40), device="cuda")
+    bias = (ints([7, 9, 7, 39, 39, 39]), torch.tensor([big, 0.5, -big, big, 1.0, -big], device="cuda"), ints([0, 3, 6]))
+    out, token = ops.adjust_logits(x, bias=bias)
+    want = torch.ones((2, 40), device="cuda")
+    want[0, 9] = 1.5                  # 39: big + 1 is big in fp32, so its sum is 0
+    assert torch.equal(out, want) and token.tolist() == [9, 0]
