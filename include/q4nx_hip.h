@@ -538,10 +538,12 @@ int q4nx_count_tokens(int32_t *counts, int64_t count_stride, int vocab, int batc
  * rounding to out's type (NaN above all, ties to the lowest token; all -inf: 0), keys[b] (optional) its
  * order-preserving key as q4nx_decode_advance takes it with n_slots = 1.
  * Each of the three penalties may be NULL (none). bias_*: ids (outside [0, vocab): skipped) and values,
- * sequence b's at bias_cu[b] .. bias_cu[b+1] - 1 (held to 0 .. n_biases). mask [n_mask][mask_stride]: bit
- * t % 32 of word t / 32 set: token t is allowed; sequence b goes by row mask_rows[b] (negative: all allowed;
- * n_mask and more: none), without mask_rows by row b. ws: Q4NX_WS_COUNTER_BYTES, batch <= 4096. No
- * reference counterpart (transformers' generate chooses its tokens, chat.py:74-78). */
+ * sequence b's at bias_cu[b] .. bias_cu[b+1] - 1 (held to 0 .. n_biases); every workgroup of a row walks the
+ * row's list, which is meant for hundreds (300 neighbouring tokens: 26 us a call, none 10; all of 100352: 331).
+ * mask [n_mask][mask_stride]: bit t % 32 of word t / 32 set: token t is allowed; sequence b goes by row
+ * mask_rows[b] (negative: all allowed; n_mask and more: none), without mask_rows by row b.
+ * ws: Q4NX_WS_COUNTER_BYTES, batch <= 4096. No reference counterpart (transformers' generate chooses its
+ * tokens, chat.py:74-78). */
 int q4nx_adjust_logits(const void *logits, int bf16, int64_t stride, void *out, int64_t out_stride,
                        int vocab, int batch, const int32_t *counts, int64_t count_stride,
                        const float *repetition, const float *presence, const float *frequency,

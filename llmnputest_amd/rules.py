@@ -22,7 +22,8 @@ from . import ops
 class TokenRules:
     """`counts` int32 [n_seqs, vocab] (`ops.count_tokens`), `repetition`, `presence`, `frequency` fp32
     [n_seqs]; `mask` int32 [rows, (vocab + 31) // 32] with `mask_rows` int32 [n_seqs], the row that a
-    sequence goes by (-1: all allowed); at most max_biases biases in all.
+    sequence goes by (-1: all allowed); at most max_biases biases in all, lists of up to hundreds a sequence
+    (of 1 x 100352 logits, 10 us without: 300 neighbouring tokens 26 us, 4096 88, all 331).
 
     masks: a table of masks, int32 [rows, words], that sequences go by as `mask_rows` says (a grammar's
     states, say); without it every sequence has a row of its own, which `allow` sets."""
