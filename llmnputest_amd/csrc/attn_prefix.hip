@@ -45,7 +45,7 @@ struct Group {
 __device__ __forceinline__ int cu_at(const PrefixArgs& a, int p) {
   return a.cu == nullptr ? (p > 0 ? a.batch : 0) : min(max(a.cu[p], 0), a.batch);
 }
-// 16-row-tile counting for a prefix of so many members: tiles of RT rows.
+// Tiles of RT rows (64 or 128) of a prefix with so many members.
 __device__ __forceinline__ int tiles_of(int members, int G, int RT) { return (members * G + RT - 1) / RT; }
 
 // Which prefix row tile t belongs to, 64 prefixes at a time; t becomes its index there. p = -1: none.
@@ -92,7 +92,8 @@ __device__ __forceinline__ int swz_v(int row, int c) {
 }
 
 // 16 bytes a lane from base + voff to LDS at lds + 16 lane. No register receives them; who reads them waits
-// for the count of loads first. (The builtin makes the compiler wait before every later read of LDS.)
+// for the count of loads first. (The builtin makes the compiler wait before every later read of LDS.) m0 is a
+// register that the compiler reserves, and warns about as one that is changed; it has no other use of it here.
 __device__ __forceinline__ void lds16(const void* base, uint32_t voff, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                :: "s"(lds), "v"(voff), "s"(base) : "memory");
