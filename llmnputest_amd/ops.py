@@ -104,10 +104,6 @@ DEFAULT_WS_BYTES = 256 << 20
 DEFAULT_WS_STREAMS = 16
 
 
-# torch.cuda.is_current_stream_capturing without the call around it
-_capturing = torch._C._cuda_isCurrentStreamCapturing
-
-
 class _Defaults(threading.local):
     """A host thread's default workspaces, by device and stream: given back when the thread ends.
     A stream that records a graph has one of its own for that capture, which lies in the graph's
@@ -119,7 +115,7 @@ class _Defaults(threading.local):
 
     def get(self, device: int, stream: int) -> Workspace:
         key, capture = (device, stream), 0
-        if _capturing():
+        if torch.cuda.is_current_stream_capturing():
             capture = _lib.lib().q4nx_stream_capture_id(stream)
             key = (device, stream, "capture")
         held = self.by_stream.get(key)

@@ -1,6 +1,8 @@
 """Several continuations of a prompt without a GPU: what the kernels' sources have to say about memory that
 waves share, and what the decoder and the rules do on the host."""
 
+import subprocess
+import sys
 from pathlib import Path
 
 from llmnputest_amd import _lib, ops
@@ -35,3 +37,9 @@ def test_eviction_leaves_the_steps_workspace(monkeypatch):
     monkeypatch.setattr(ops, "kv_evict", kv_evict)
     assert dec.evict([16400, 9], 100, 10) == [100, 9]
     assert calls == [[16400, 9]] * 2 and dec.ws.buf is held
+
+
+def test_import_needs_no_private_names():
+    """The package is imported also where torch's own name for the question whether a stream captures is gone."""
+    code = "import torch; del torch._C._cuda_isCurrentStreamCapturing; import llmnputest_amd.ops"
+    assert subprocess.run([sys.executable, "-c", code], cwd=CSRC.parents[1]).returncode == 0
