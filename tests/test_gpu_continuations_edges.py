@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from llmnputest_amd.granite import GraniteConfig, GraniteDecoder, GraniteWeights
+from tests.test_gpu_evict import CASES as EVICT_CASES, WEIGHT
 from tests.test_gpu_prefix import check, reference, rows
 
 pytestmark = pytest.mark.gpu
@@ -117,3 +118,27 @@ def test_biases_are_summed_first(dev):
     want = torch.ones((2, 40), device="cuda")
     want[0, 9] = 1.5                  # 39: big + 1 is big in fp32, so its sum is 0
     assert torch.equal(out, want) and token.tolist() == [9, 0]
+
+
+@pytest.mark.parametrize("case", EVICT_CASES, ids=[f"b{c[0]}hq{c[1]}_{c[2]}d{c[3]}l{max(c[4])}" for c in EVICT_CASES])
+def test_weights_add_up(dev, case):
+    """What a step gives the positions of a kv head is one for each of its query heads, all together; what lies
+    behind the newest is no part of it."""
+    from llmnputest_amd import ops
+    b, hq, hkv, d, lens = case
+    g = torch.Generator(device="cuda").manual_seed(hq)
+    n = max(lens) + 3
+    k, v = rows(g, b, hkv, n, d), rows(g, b, hkv, n, d)
+    weights = torch.full((b, hkv, n), 7.0, device="cuda")
+    seen = torch.arange(n, device="cuda") < ints(lens)[:, None, None]
+    for step in range(3):
+        # the last position is the newest each time: what it was given before is gone
+        before = weights.double()
+        ops.gqa_decode_weights(rows(g, b, hq, d), k, v, ints(lens), weights, start=step == 0)
+        newest = torch.stack([before[i, :, max(m - 1, 0)] * (m > 0) for i, m in enumerate(lens)])
+        was = torch.where(seen, before, 0.0).sum(-1) - newest if step else torch.zeros_like(newest)
+        now = torch.where(seen, weights.double(), 0.0).sum(-1)
+        want = hq // hkv * (ints(lens)[:, None] > 0).double().expand_as(now)
+        # each weight within WEIGHT of itself; what was there before is rounded once more by the addition
+        assert bool(((now - was - want).abs() <= WEIGHT * want + 2.0 ** -24 * was).all())
+        assert bool((weights == 7.0)[~seen.expand_as(weights)].all())
