@@ -13,7 +13,8 @@
 // Rows move towards the front. Into other memory they move all at once. In place, row i comes from a
 // position >= i, so a workgroup that takes rows in order, a block at a time, only overwrites rows that it
 // has read: a block's sources lie at or behind the block's own first row, and every later block's behind it.
-// K and V have a workgroup each.
+// K and V have a workgroup each, a chain of blocks: for one sequence of 8 kv heads, 4096 of 16384 rows of 64,
+// turned, 28.5 us (into other memory 5.0), for 8 of 32771 66.5 (33.4).
 //
 // With a RoPE table K is turned to its new place: a key that was rotated by position o and now stands at i
 // is rotated back by o - i places, in fp32, rounded once.
@@ -586,7 +587,7 @@ __device__ __forceinline__ void evict_move(const EvictArgs& a, int bk, int n, in
     for (int i0 = 0; i0 < m; i0 += STEP) {
       next.src = -1;
       if (i0 + STEP < m) load(i0 + STEP, next);
-      wait_vm();          // this step's rows have been read by every thread before any is written
+      wait_vm();          // this step's rows (with those read ahead) are there for every thread before any is written
       __syncthreads();
       store(i0, r);
       r = next;
