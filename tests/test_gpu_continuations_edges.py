@@ -142,3 +142,28 @@ def test_weights_add_up(dev, case):
         # each weight within WEIGHT of itself; what was there before is rounded once more by the addition
         assert bool(((now - was - want).abs() <= WEIGHT * want + 2.0 ** -24 * was).all())
         assert bool((weights == 7.0)[~seen.expand_as(weights)].all())
+
+
+@pytest.mark.parametrize("b,hkv,n,budget,recent", [(16400, 1, 21, 9, 2), (2050, 8, 16390, 40, 7)])
+def test_more_caches_than_counters(dev, b, hkv, n, budget, recent):
+    """More sequences, or (sequence, kv head)s, than a workspace has counters: a workgroup selects alone, also from
+    more positions than its registers hold."""
+    from llmnputest_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(n)
+    k = torch.empty((b, hkv, n, 64), dtype=torch.bfloat16, device="cuda")
+    k.copy_((torch.arange(n, device="cuda") % 251)[:, None].expand(n, 64).to(torch.bfloat16))
+    w = torch.randint(0, 1000, (b, hkv, n), device="cuda", generator=g).float()
+    lens = [n - 3 * (i % 5) for i in range(b)]
+    into = tuple(torch.zeros(s, dtype=t, device="cuda") for s, t in (
+        ((b, hkv, budget, 64), torch.bfloat16), ((b, hkv, budget, 64), torch.bfloat16), ((b, hkv, budget), torch.float32), ((b,), torch.int32)))
+    kept = ops.kv_evict(k, k.view_as(k), w, ints(lens), budget, recent, into=into).long()
+    assert into[3].tolist() == [budget] * b
+    index = torch.arange(n, device="cuda")
+    for i0 in range(0, b, 512):
+        m, x = ints(lens[i0:i0 + 512])[:, None, None], w[i0:i0 + 512]
+        x = torch.where(index < m - recent, x, torch.where(index < m, float("inf"), float("-inf")))
+        want = torch.sort(x, descending=True, stable=True).indices[..., :budget].sort(-1).values
+        assert torch.equal(kept[i0:i0 + 512], want)
+        assert torch.equal(into[2][i0:i0 + 512], torch.gather(w[i0:i0 + 512], 2, want))
+        for to in into[:2]:
+            assert torch.equal(to[i0:i0 + 512], (want % 251).to(torch.bfloat16)[..., None].expand(*want.shape, 64))
