@@ -827,14 +827,14 @@ def adjust_logits(logits: torch.Tensor, counts: torch.Tensor | None = None,
     logits' type (`out=logits` works in place) and the greatest of each row, int32 [B], from the values
     before their rounding to that type.
 
-    In fp32: tokens in counts (`count_tokens`; not 0): x / repetition where x > 0, else x * repetition;
-    minus frequency times how often it was generated, minus presence if it was (fp32 [B] each, or None);
-    plus the sum of the biases for it, in their order (ids int32 [N], values fp32 [N], cu int32 [B + 1]:
-    sequence b's are cu[b] .. cu[b+1] - 1; lists of up to hundreds, every workgroup of a row walks the row's:
-    what holds for much of the vocabulary is better added to the logits); -inf where the mask (int32 [rows, (V + 31) // 32], bit t % 32 of word t // 32: token t
-    is allowed) has no bit. mask_rows int32 [B]: the row that a sequence goes by, negative: all allowed,
-    behind the last: none; without it row b. keys: int64 [B], the greatest as `decode_advance` takes it
-    (n_slots 1)."""
+    In fp32: tokens in counts (`count_tokens`; not 0): x / repetition where x > 0, else x * repetition; minus
+    frequency times how often it was generated, minus presence if it was (fp32 [B] each, or None); plus the
+    sum of the biases for it, in their order (ids int32 [N], values fp32 [N], cu int32 [B + 1]: sequence b's
+    are cu[b] .. cu[b+1] - 1; lists of up to hundreds, every workgroup of a row walks the row's: what holds
+    for much of the vocabulary is better added to the logits); -inf where the mask (int32 [rows, (V + 31) //
+    32], bit t % 32 of word t // 32: token t is allowed) has no bit. mask_rows int32 [B]: the row that a
+    sequence goes by, negative: all allowed, behind the last: none; without it row b. keys: int64 [B], the
+    greatest as `decode_advance` takes it (n_slots 1)."""
     if logits.dtype not in (torch.float32, torch.bfloat16):
         raise TypeError(f"logits must be float32 or bfloat16, got {logits.dtype}")
     at = dev, _ = _device_stream()
